@@ -14,8 +14,16 @@ from .attention import (
     paged_attention_decode_b200,
     paged_attention_prefill_b200,
 )
+from .eviction import accumulate_key_weights, evict_by_weight
 from .integration import install_into_reference
 from .decoder import FusedDecodeExecutor, FusedDecoder
+from .kv4 import (
+    Kv4BlockPool,
+    kv4_append,
+    kv4_read,
+    paged_attention_decode_kv4,
+    paged_attention_prefill_kv4,
+)
 from .step import DecodeGraph, DecodeStep, SharedStepMetadata
 from .serving import ContinuousBatchingRank, LeastOutstandingTokensRouter, ServeResult, gather_request_times, serve
 from .paged_kv import (
@@ -39,17 +47,24 @@ __all__ = [
     "ServeResult",
     "gather_request_times",
     "serve",
+    "Kv4BlockPool",
     "LayerBlockPool",
     "PagedKVCacheState",
     "SUPPORTED_BACKENDS",
+    "accumulate_key_weights",
     "clear_status",
     "device_metadata",
+    "evict_by_weight",
     "flush_pending",
     "install_into_reference",
+    "kv4_append",
+    "kv4_read",
     "load_library",
     "paged_attention",
     "paged_attention_decode_b200",
+    "paged_attention_decode_kv4",
     "paged_attention_prefill_b200",
+    "paged_attention_prefill_kv4",
     "raise_on_device_status",
     "read_status",
     "set_fused_append",

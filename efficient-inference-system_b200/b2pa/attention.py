@@ -22,6 +22,8 @@ import torch
 
 from . import _lib
 from ._metadata import block_table_and_lengths
+from .eviction import accumulate_from
+from .kv4 import _attend as _attend_kv4
 from .paged_kv import _kv_append, flush_pending, take_pending
 from .step import _StepPending
 
@@ -99,7 +101,6 @@ def paged_attention(backend: str, q: torch.Tensor, kv_cache, current_lengths) ->
     if not q.is_cuda:
         raise RuntimeError("b2pa: q must be a CUDA tensor (this package has no CPU path)")
     B, _, T, _ = q.shape
-    dev = q.device
     # host-side current lengths as one int32 metadata row (a scalar stands for
     # a row of equal values)
     host_cur = None
@@ -120,6 +121,16 @@ def paged_attention(backend: str, q: torch.Tensor, kv_cache, current_lengths) ->
         step.layer_of(kv_cache)
         pool._b2pa_pending = None
         return step.attend(q, kv_cache, pend)
+    out = _attention_now(q, kv_cache, current_lengths, host_cur, pool, pend)
+    if getattr(pool, "key_weights", None) is not None:
+        accumulate_from(kv_cache, q, current_lengths)
+    return out
+
+
+def _attention_now(q: torch.Tensor, kv_cache, current_lengths, host_cur, pool, pend) -> torch.Tensor:
+    """paged_attention outside a DecodeStep."""
+    dev = q.device
+    T = q.shape[2]
     if pend is not None:
         if (pend.cache is kv_cache and pend.k_new.shape[2] == T and pend.k_new.device == dev
                 and pool.k_blocks.dtype == q.dtype):
@@ -136,6 +147,9 @@ def paged_attention(backend: str, q: torch.Tensor, kv_cache, current_lengths) ->
     else:
         page_table, seq_lens, max_pages = block_table_and_lengths(kv_cache, dev, transient=True)
         cur = current_lengths.to(dtype=torch.int32)
+    if pool.k_blocks.dtype == torch.uint8:
+        name = "paged_attention_decode_kv4" if T == 1 else "paged_attention_prefill_kv4"
+        return _attend_kv4(name, q, pool.k_blocks, pool.v_blocks, page_table, seq_lens, cur, max_pages)
     fn = "decode" if T == 1 else "prefill"
     return _attn_call(fn, q, pool.k_blocks, pool.v_blocks, page_table, seq_lens, cur, max_pages)
 

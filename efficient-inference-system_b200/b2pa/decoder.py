@@ -146,9 +146,21 @@ class FusedDecodeExecutor:
     sides, host work included).  The requests' KV caches must exist (their
     prompt was prefilled).  Per-request bookkeeping follows the reference:
     start time and batch id on first service, the new token appended, phase
-    and finish time updated, completed requests returned."""
+    and finish time updated, completed requests returned.
 
-    def __init__(self, model, device, max_batch: int = 16):
+    With ``evict_keep`` every request's cache is bounded: after a step, the
+    layers of each request that holds ``evict_keep + evict_slack`` tokens or
+    more are cut to ``evict_keep`` by accumulated attention weight, the
+    ``evict_recent`` last tokens always kept (the pools must track key
+    weights: ``track_key_weights``).  The slack lets one cut serve that many
+    steps."""
+
+    def __init__(self, model, device, max_batch: int = 16, evict_keep: int | None = None, evict_recent: int = 0,
+                 evict_slack: int = 32):
+        if evict_keep is not None and (evict_keep < 1 or evict_recent < 0 or evict_slack < 1):
+            raise ValueError("b2pa.FusedDecodeExecutor: evict_keep and evict_slack must be at least 1, "
+                             "evict_recent not negative")
+        self.evict_keep, self.evict_recent, self.evict_slack = evict_keep, evict_recent, evict_slack
         self.model = model
         self.device = torch.device(device)
         self.decoder = FusedDecoder(model, max_batch=max_batch)
@@ -181,6 +193,10 @@ class FusedDecodeExecutor:
         with step:
             _, nxt = self.decoder.step(self.ids[:M], self.pos[:M], batches)
         self.meta = step.meta
+        if self.evict_keep is not None:
+            full = [i for i, s in enumerate(layer_states[0]) if s.seq_len >= self.evict_keep + self.evict_slack]
+            for states in layer_states if full else ():
+                BatchedPagedKVCache([states[i] for i in full], states[0].pool).evict(self.evict_keep, self.evict_recent)
         next_tokens = nxt.tolist()
         torch.cuda.synchronize(self.device)
         elapsed_ms = (time.perf_counter() - t0) * 1000.0

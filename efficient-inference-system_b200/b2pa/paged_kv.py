@@ -53,6 +53,30 @@ class LayerBlockPool:
         self.free_block_ids: list[int] = []
         self.capacity_blocks = 0
         self._b2pa_pending = None  # a deferred decode append (set_fused_append)
+        self.key_weights: torch.Tensor | None = None  # fp32 [blocks, H, block_size], see track_key_weights
+        self.key_weight_window: int | None = None
+        self._tracks_weights = False
+
+    def track_key_weights(self, window: int | None = None) -> None:
+        """From now on each ``paged_attention`` on this pool adds its queries'
+        attention weights to ``key_weights``, one running sum per head and
+        cached token, which ``BatchedPagedKVCache.evict`` goes by.  With
+        ``window`` only the last ``window`` queries of each call count."""
+        if window is not None and window < 1:
+            raise ValueError(f"b2pa: window {window} < 1")
+        if self._b2pa_pending is not None or getattr(self, "_b2pa_step", None) is not None:
+            raise RuntimeError("b2pa: track_key_weights between an append and its attention")
+        self.key_weight_window = window
+        self._tracks_weights = True
+        if self.k_blocks is not None and self.key_weights is None:
+            self.key_weights = self._new_weights(self.capacity_blocks)
+
+    def _new_blocks(self, count: int) -> torch.Tensor:
+        return torch.zeros(count, self.num_heads, self.block_size, self.head_dim, dtype=self.dtype,
+                           device=self.device)
+
+    def _new_weights(self, count: int) -> torch.Tensor:
+        return torch.zeros(count, self.num_heads, self.block_size, dtype=torch.float32, device=self.device)
 
     def ensure_initialized(self, num_heads: int, head_dim: int, dtype: torch.dtype, device: torch.device) -> None:
         """Lazily allocates the pool on first use (paged_kv.py:28-42)."""
@@ -79,8 +103,7 @@ class LayerBlockPool:
             else int(math.ceil(self.capacity_blocks * (self.growth_factor - 1.0))),
         )
         grow_by = max(grow_by, 1)
-        new_k = torch.zeros(grow_by, self.num_heads, self.block_size, self.head_dim, dtype=self.dtype,
-                            device=self.device)
+        new_k = self._new_blocks(grow_by)
         new_v = torch.zeros_like(new_k)
         if self.k_blocks is None:
             self.k_blocks = new_k
@@ -88,6 +111,9 @@ class LayerBlockPool:
         else:
             self.k_blocks = torch.cat([self.k_blocks, new_k], dim=0)
             self.v_blocks = torch.cat([self.v_blocks, new_v], dim=0)
+        if self._tracks_weights:
+            new_w = self._new_weights(grow_by)
+            self.key_weights = new_w if self.key_weights is None else torch.cat([self.key_weights, new_w], dim=0)
         start = self.capacity_blocks
         self.capacity_blocks += grow_by
         self.free_block_ids.extend(range(start, self.capacity_blocks))
@@ -192,6 +218,17 @@ class BatchedPagedKVCache:
         """Writes each request's new tokens into its blocks; returns the new
         sequence lengths as int64 (paged_kv.py:151-172)."""
         return append_batch_into(self, k_new, v_new, current_lengths)
+
+    def evict(self, keep: int, recent: int = 0) -> torch.Tensor:
+        """Cuts every sequence of more than ``keep`` tokens to ``keep``: the
+        ``recent`` last ones and, per head, those of the others with the
+        largest accumulated attention weight (the pool must track them:
+        ``track_key_weights``).  The kept tokens move together in order and
+        the freed blocks return to the pool.  Returns the kept positions,
+        int32 [B, H, keep], -1 behind a shorter sequence's last."""
+        from .eviction import evict_batch
+
+        return evict_batch(self, keep, recent)
 
     def page_table_array(self) -> np.ndarray:
         """int32 ``[B, max_pages]`` block table, -1 padded (paged_kv.py:174-193)."""
@@ -338,6 +375,8 @@ def append_batch_into(cache, k_new: torch.Tensor, v_new: torch.Tensor, current_l
         flush_pending(pool)  # an earlier deferred append goes first
     starts = plan_append(cache, k_new, clamped, as_array=True)
     if any_new and k_new.device.type == "cuda":
+        if pool.k_blocks.dtype == torch.uint8:  # 4-bit pages: quantised here, fused append or not
+            return _kv4_append(cache, k_new, v_new, starts, clamped)
         if _fused_append and k_new.stride(3) == 1 and v_new.stride(3) == 1:
             seq_out = torch.empty(B, dtype=torch.long, device=k_new.device)
             try:
@@ -448,12 +487,38 @@ def _kv_append(cache, k_new: torch.Tensor, v_new: torch.Tensor, starts: list[int
     return seq_lens
 
 
+def _kv4_append(cache, k_new: torch.Tensor, v_new: torch.Tensor, starts, lengths) -> torch.Tensor:
+    """b2pa_kv4_append of a batch; returns the lengths after it (int64)."""
+    from .kv4 import kv4_append
+
+    pool = cache.pool
+    _require_cuda(v_new, "v_new")
+    dev = k_new.device
+    if pool.k_blocks.device != dev:
+        raise ValueError(f"pool on {pool.k_blocks.device} but k_new on {dev}")
+    table, _, start_t, len_t, max_pages = block_table_and_lengths(cache, dev, [starts, lengths], transient=True)
+    seq_out = torch.empty(k_new.shape[0], dtype=torch.long, device=dev)
+    kv4_append(k_new, v_new, pool.k_blocks, pool.v_blocks, table[:, :max_pages], start_t, len_t, seq_out)
+    return seq_out
+
+
 def _zero_blocks(pool: LayerBlockPool, block_ids: list[int]) -> None:
     kb, vb = pool.k_blocks, pool.v_blocks
     dev = kb.device
     ids = stage_int32(np.asarray(block_ids, dtype=np.int32), dev, transient=True)
     lib = _lib.load()
-    rc = lib.b2pa_zero_blocks(kb.data_ptr(), vb.data_ptr(), _lib.strides4(kb), kb.shape[0], ids.data_ptr(),
-                              len(block_ids), kb.shape[1], kb.shape[3], kb.shape[2], _lib.dtype_code(kb.dtype),
-                              _lib.status_buffer(dev).data_ptr(), _lib.stream_handle(dev))
-    _lib.check(rc, "b2pa_zero_blocks")
+
+    def zero(k: torch.Tensor, v: torch.Tensor, H: int, D: int, block_size: int, dtype: int) -> None:
+        strides = (ctypes.c_int64 * 4)(H * block_size * D, block_size * D, D, 1)
+        rc = lib.b2pa_zero_blocks(k.data_ptr(), v.data_ptr(), strides, k.shape[0], ids.data_ptr(), len(block_ids), H,
+                                  D, block_size, dtype, _lib.status_buffer(dev).data_ptr(), _lib.stream_handle(dev))
+        _lib.check(rc, "b2pa_zero_blocks")
+
+    H, bs = kb.shape[1], kb.shape[2]
+    if kb.dtype == torch.uint8:  # whole pages of 32-bit words
+        zero(kb, vb, H, kb.shape[3] // 4, bs, _lib.DTYPE_F32)
+    else:
+        zero(kb, vb, H, kb.shape[3], bs, _lib.dtype_code(kb.dtype))
+    weights = getattr(pool, "key_weights", None)
+    if weights is not None:
+        zero(weights, weights, H, 1, bs, _lib.DTYPE_F32)

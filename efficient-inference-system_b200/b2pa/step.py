@@ -122,16 +122,31 @@ class SharedStepMetadata:
         _rt_check(rt.cudaEventRecord(self.events[i], stream), "cudaEventRecord")
         self.recorded[i] = True
 
-    def ensure_workspace(self, H: int, D: int, block_size: int, dtype: torch.dtype) -> torch.Tensor:
-        key = (H, D, block_size, dtype)
+    def ensure_workspace(self, H: int, D: int, block_size: int, dtype: torch.dtype,
+                         kv4: bool = False, weights: bool = False) -> torch.Tensor:
+        """Scratch for the decode of every layer (and, with ``weights``, for
+        the key weights' accumulation behind it); ``kv4``: 4-bit pools of rows
+        of ``dtype``."""
+        key = (H, D, block_size, dtype, kv4, weights)
         if key == self._ws_key:
             return self.workspace
         self._ws_key = key
         lib = _lib.load()
+        code = _lib.dtype_code(dtype)
+
+        def need_of(b: int) -> int:
+            if kv4:
+                n = lib.b2pa_paged_decode_kv4_workspace_size(b, H, D, self.width, block_size)
+            else:
+                n = lib.b2pa_paged_decode_workspace_size(b, H, D, self.width, block_size, code)
+            if weights:
+                n = max(n, lib.b2pa_key_weights_workspace_size(b, H, 1, D, self.width, block_size, code,
+                                                               _lib.DTYPE_KV4 if kv4 else code))
+            return n
+
         # enough for every batch size the buffers serve (the split plan is not
         # monotone in B)
-        need = max(lib.b2pa_paged_decode_workspace_size(b, H, D, self.width, block_size, _lib.dtype_code(dtype))
-                   for b in range(1, self.capacity + 1))
+        need = max(need_of(b) for b in range(1, self.capacity + 1))
         if self.workspace is None or self.workspace.numel() < need:
             self.workspace = torch.empty(max(need, 256), dtype=torch.uint8, device=self.device)
         return self.workspace
@@ -198,8 +213,12 @@ class DecodeStep:
         starts = reserve_lockstep(self.layer_states, self.pools)
         first = self.layer_states[0]
         self.meta.upload([s.block_ids for s in first], [s.seq_len for s in first], starts)
-        kb = self.pools[0].k_blocks
-        self.meta.ensure_workspace(kb.shape[1], kb.shape[3], kb.shape[2], kb.dtype)
+        pool = self.pools[0]
+        kb = pool.k_blocks
+        kv4 = kb.dtype == torch.uint8
+        self.meta.ensure_workspace(kb.shape[1], pool.head_dim if kv4 else kb.shape[3], kb.shape[2],
+                                   pool.dtype if kv4 else kb.dtype, kv4,
+                                   any(getattr(p, "key_weights", None) is not None for p in self.pools))
         for pool in self.pools:
             pool._b2pa_step = self
         self.open = True
@@ -253,8 +272,30 @@ class DecodeStep:
 
     def attend(self, q: torch.Tensor, cache, pend: _StepPending) -> torch.Tensor:
         """b2pa_paged_decode_append on the shared metadata (no host work
-        beyond the launch)."""
+        beyond the launches); a pool that tracks key weights adds its own."""
         pool = cache.pool
+        out = self._attend_kv4(q, pool, pend) if pool.k_blocks.dtype == torch.uint8 else self._attend_plain(q, pool, pend)
+        weights = getattr(pool, "key_weights", None)
+        if weights is not None:
+            from .eviction import launch_key_weights
+            from .kv4 import aligned_rows
+
+            m, kb = self.meta, pool.k_blocks
+            code = _lib.DTYPE_KV4 if kb.dtype == torch.uint8 else _lib.dtype_code(kb.dtype)
+            launch_key_weights(aligned_rows(q), kb, code, weights, weights, m.table, m.width, m.width, m.seq_lens,
+                               m.ones, pool.key_weight_window, m.workspace)
+        return out
+
+    def _attend_kv4(self, q: torch.Tensor, pool, pend: _StepPending) -> torch.Tensor:
+        from .kv4 import _attend, kv4_append
+
+        m = self.meta
+        table = m.table.view(m.capacity, m.width)[: self.B]
+        starts, ones, lens = (t[: self.B] for t in (m.start_pos, m.ones, m.seq_lens))
+        kv4_append(pend.k_new, pend.v_new, pool.k_blocks, pool.v_blocks, table, starts, ones, m.seq_out[: self.B])
+        return _attend("paged_attention_decode_kv4", q, pool.k_blocks, pool.v_blocks, table, lens, ones, ws=m.workspace)
+
+    def _attend_plain(self, q: torch.Tensor, pool, pend: _StepPending) -> torch.Tensor:
         kb, vb = pool.k_blocks, pool.v_blocks
         B, H, _, D = q.shape
         m = self.meta
@@ -276,7 +317,9 @@ class DecodeStep:
         """Every address and size a captured step bakes in."""
         m = self.meta
         return (self.B, m.width, m.dev.data_ptr(), m.workspace.data_ptr(),
-                tuple((p.k_blocks.data_ptr(), p.v_blocks.data_ptr(), p.k_blocks.shape[0]) for p in self.pools))
+                tuple((p.k_blocks.data_ptr(), p.v_blocks.data_ptr(), p.k_blocks.shape[0]) for p in self.pools),
+                tuple((w.data_ptr(), p.key_weight_window) if (w := getattr(p, "key_weights", None)) is not None else None
+                      for p in self.pools))
 
 
 def reserve_lockstep(layer_states: list[list], pools: list) -> list[int]:

@@ -159,6 +159,79 @@ int launch_paged_prefill_f32(const AttnArgs& a, cudaStream_t s);
 int launch_paged_prefill_bf16(const AttnArgs& a, cudaStream_t s);
 int launch_paged_prefill_f16(const AttnArgs& a, cudaStream_t s);
 
+// ---- 4-bit cache (kv4.cuh) and eviction by accumulated attention weight ----
+struct Kv4ReadArgs {
+  const void* k_pool;
+  const void* v_pool;
+  int64_t num_blocks;
+  const int32_t* page_table;
+  int64_t pt_stride;
+  int max_pages;
+  const int32_t* start_pos;
+  const int32_t* lengths;
+  void* k_out;
+  void* v_out;
+  int64_t sk[4], sv[4];  // element strides of [B,H,T,D], unit D stride
+  int B, H, T, D, block_size, dtype;
+  int32_t* status;
+};
+
+struct KeyWeightArgs {
+  const void* q;
+  int64_t sq[4];
+  const void* k_pool;
+  int64_t num_blocks;
+  const int32_t* page_table;
+  int64_t pt_stride;
+  int max_pages;
+  const int32_t* seq_lens;
+  const int32_t* cur_lens;
+  const float* w_in;
+  float* w_out;
+  int window;  // 0: every query counts
+  int B, H, T, D, block_size, dtype, pool_dtype;
+  float scale;
+  void* workspace;
+  float* lse;
+  int32_t* status;
+};
+
+struct EvictArgs {
+  void* k_pool;
+  void* v_pool;
+  float* weights;
+  int64_t num_blocks;
+  const int32_t* page_table;
+  int64_t pt_stride;
+  int max_pages;
+  const int32_t* out_table;  // null: in place
+  int64_t out_stride;
+  const int32_t* seq_lens;
+  int keep, recent;
+  int32_t* kept;
+  int B, H, D, block_size, dtype;
+  int elem;  // bytes per element of a plain pool
+  int32_t* status;
+};
+
+int launch_kv4_append(const AppendArgs& a, int64_t* seq_lens_out, cudaStream_t s);
+int launch_kv4_read(const Kv4ReadArgs& a, cudaStream_t s);
+
+size_t kv4_decode_workspace(int B, int H, int D, int max_pages, int block_size);
+int launch_kv4_decode(const AttnArgs& a, cudaStream_t s);
+
+struct Kv4PrefillPlan {
+  size_t off_k, off_v, off_table, off_inner, inner_bytes, bytes;
+};
+Kv4PrefillPlan make_kv4_prefill_plan(int B, int H, int T, int D, int max_pages, int block_size, int dtype);
+int launch_kv4_prefill(const AttnArgs& a, const Kv4PrefillPlan& plan, cudaStream_t s);
+
+size_t key_weights_workspace(int B, int H, int T, int D, int max_pages, int block_size, int dtype, int pool_dtype);
+int launch_key_weights(const KeyWeightArgs& a, cudaStream_t s);
+int launch_evict(const EvictArgs& a, cudaStream_t s);
+
+inline bool kv4_head_dim_supported(int D) { return D == 64 || D == 128 || D == 256; }
+
 inline int dtype_size(int dtype) {
   return dtype == B2PA_DTYPE_F32 ? 4 : (dtype == B2PA_DTYPE_BF16 || dtype == B2PA_DTYPE_F16) ? 2 : 0;
 }

@@ -1,0 +1,105 @@
+// kv4_prefill.cu -- chunked prefill over a 4-bit cache (format: kv4.cuh).
+//
+// A prompt chunk of T queries makes 4 T L D operations of every L keys, so
+// its time is the tensor cores' and not the cache's.  The pages the call
+// reads are first written out in the type of q in the workspace, as a pool of
+// B * max_pages blocks with a table of their own (exact: a stored value has 7
+// significant bits), and the prefill kernels of the plain pools run on it.
+// Rows past a sequence's length are written as zeros.
+#include "common.cuh"
+#include "kernels.h"
+#include "kv4.cuh"
+
+namespace b2pa {
+
+// One CTA per (page, sequence): dequantises every head's K and V page.
+template <typename T>
+__global__ void __launch_bounds__(256) kv4_unpack_kernel(AttnArgs a, T* k_out, T* v_out, int32_t* table) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int p = blockIdx.x, b = blockIdx.y;
+  const int64_t slot = (int64_t)b * a.max_pages + p;
+  const int BS = a.block_size, D = a.D;
+  const int64_t first = (int64_t)p * BS;
+  const int64_t L = a.seq_lens[b];
+  const bool used = first < L;
+  int32_t blk = used ? a.page_table[(int64_t)b * a.pt_stride + p] : -1;
+  if (used && (blk < 0 || blk >= a.num_blocks)) {
+    if (threadIdx.x == 0 && blk >= a.num_blocks) set_status(a.status, B2PA_ERR_BAD_BLOCK_ID);
+    blk = -1;
+  }
+  if (threadIdx.x == 0) table[slot] = blk >= 0 ? (int32_t)slot : -1;
+  if (blk < 0) return;
+  const int page_bytes = kv4_page_bytes(BS, D), codes = BS * (D / 2);
+  const int wpr = D / 8, per_head = BS * wpr, total = a.H * per_head;
+  constexpr int N = 16 / (int)sizeof(T);
+  for (int i = threadIdx.x; i < total; i += blockDim.x) {
+    const int h = i / per_head, r = i - h * per_head;
+    const int row = r / wpr, w = r - row * wpr;
+    const uint8_t* kh = static_cast<const uint8_t*>(a.k_pool) + ((int64_t)blk * a.H + h) * page_bytes;
+    const uint8_t* vh = static_cast<const uint8_t*>(a.v_pool) + ((int64_t)blk * a.H + h) * page_bytes;
+    float xk[8] = {}, xv[8] = {};
+    if (first + row < L) {
+      kv4_unpack8(*reinterpret_cast<const uint32_t*>(kh + 4 * r), kv4_scale(kh[codes + row * (D / 16) + w / 2]), xk);
+      kv4_unpack8(*reinterpret_cast<const uint32_t*>(vh + 4 * r), kv4_scale(vh[codes + (w / 2) * BS + row]), xv);
+    }
+    const int64_t o = (slot * a.H * per_head + i) * 8;
+#pragma unroll
+    for (int c = 0; c < 8; c += N) {
+      Vec<T, N> k, v;
+      k.from_float(xk + c);
+      v.from_float(xv + c);
+      *reinterpret_cast<uint4*>(k_out + o + c) = k.w;
+      *reinterpret_cast<uint4*>(v_out + o + c) = v.w;
+    }
+  }
+}
+
+static size_t up256(size_t x) { return (x + 255) / 256 * 256; }
+
+Kv4PrefillPlan make_kv4_prefill_plan(int B, int H, int T, int D, int max_pages, int block_size, int dtype) {
+  Kv4PrefillPlan pl;
+  const size_t pool = up256((size_t)B * max_pages * H * block_size * D * dtype_size(dtype));
+  pl.off_k = 0;
+  pl.off_v = pool;
+  pl.off_table = 2 * pool;
+  pl.off_inner = up256(2 * pool + 4 * (size_t)B * max_pages);
+  pl.inner_bytes = make_prefill_plan(B, H, T, D, max_pages, block_size, dtype).bytes;
+  pl.bytes = pl.off_inner + pl.inner_bytes;
+  return pl;
+}
+
+template <typename T>
+static cudaError_t unpack_as(const AttnArgs& a, char* ws, const Kv4PrefillPlan& pl, cudaStream_t s) {
+  return launch_pdl(kv4_unpack_kernel<T>, dim3((unsigned)a.max_pages, (unsigned)a.B), dim3(256), 0, s, a,
+                    reinterpret_cast<T*>(ws + pl.off_k), reinterpret_cast<T*>(ws + pl.off_v),
+                    reinterpret_cast<int32_t*>(ws + pl.off_table));
+}
+
+int launch_kv4_prefill(const AttnArgs& a, const Kv4PrefillPlan& pl, cudaStream_t s) {
+  char* ws = static_cast<char*>(a.workspace);
+  AttnArgs in = a;
+  if (a.max_pages > 0) {
+    cudaError_t e;
+    switch (a.dtype) {
+      case B2PA_DTYPE_F32: e = unpack_as<float>(a, ws, pl, s); break;
+      case B2PA_DTYPE_BF16: e = unpack_as<__nv_bfloat16>(a, ws, pl, s); break;
+      default: e = unpack_as<__half>(a, ws, pl, s); break;
+    }
+    if (e != cudaSuccess) return set_error(B2PA_ERR_CUDA, "paged_prefill_kv4 launch: %s", cudaGetErrorString(e));
+  }
+  in.k_pool = ws + pl.off_k;
+  in.v_pool = ws + pl.off_v;
+  in.num_blocks = (int64_t)a.B * a.max_pages;
+  in.page_table = reinterpret_cast<const int32_t*>(ws + pl.off_table);
+  in.pt_stride = a.max_pages;
+  in.workspace = ws + pl.off_inner;
+  in.workspace_bytes = pl.inner_bytes;
+  switch (a.dtype) {
+    case B2PA_DTYPE_F32: return launch_paged_prefill_f32(in, s);
+    case B2PA_DTYPE_BF16: return launch_paged_prefill_bf16(in, s);
+    default: return launch_paged_prefill_f16(in, s);
+  }
+}
+
+}  // namespace b2pa

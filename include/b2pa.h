@@ -62,7 +62,8 @@ extern "C" {
 typedef enum b2pa_dtype {
   B2PA_DTYPE_F32 = 0,
   B2PA_DTYPE_BF16 = 1,
-  B2PA_DTYPE_F16 = 2
+  B2PA_DTYPE_F16 = 2,
+  B2PA_DTYPE_KV4 = 3 /* 4-bit pages (below); only where an entry point says so */
 } b2pa_dtype;
 
 typedef enum b2pa_status {
@@ -340,6 +341,134 @@ B2PA_API int b2pa_rows_embed(const int64_t* token_ids, const int64_t* positions,
 /* out[m] = the first index of the largest of x[m, 0:N] (int64), m < M. */
 B2PA_API int b2pa_rows_argmax(const float* x, int64_t x_row_stride, int M, int N, int64_t* out,
                               int32_t* status, void* stream);
+
+/*
+ * ---- A cache held in 4 bits ------------------------------------------------
+ *
+ * No counterpart in the reference, whose pools have the model's type.  Each
+ * row of D channels is stored in groups of 16: a scale s and 16 codes c in
+ * -7..7, standing for c * s.  s is max|x| / 7 rounded to nearest even as an
+ * unsigned 8-bit float (5 exponent, 3 mantissa bits: the byte shifted left by
+ * 7 is the fp16 number), at most 9216, and c = round-to-nearest-even(x / s).
+ * So magnitudes up to 64,512 are kept, larger ones saturate, and a group whose
+ * magnitudes all lie below about 2.7e-5 reads back as zeros; a group that
+ * holds a NaN or an infinity reads back as NaN.  c * s is exact in bf16, fp16
+ * and fp32.
+ *
+ * Pools are uint8 [num_blocks, H, block_size, D * 9 / 16], contiguous, base
+ * 16-byte aligned: 4.5 bits a value.  One head's page holds the codes
+ * [block_size, D / 2] (c + 8; the even channel in the low nibble), then the
+ * scales: [block_size, D / 16] in the K pool, [D / 16, block_size] in the V
+ * pool.  head_dim 64, 128 or 256; block_size 8, 16 or 32; dtype is that of
+ * the rows outside the cache (q, new rows, outputs).
+ *
+ * b2pa_kv4_append: as b2pa_kv_append, quantising.  k_new / v_new may have any
+ * element strides; unit-stride rows on 16-byte boundaries are read fastest.
+ * seq_lens_out (may be NULL) receives start_pos[b] + min(lengths[b], T) as
+ * int64, the lengths after the append.
+ */
+B2PA_API int b2pa_kv4_append(const void* k_new, const int64_t new_k_strides[4],
+                   const void* v_new, const int64_t new_v_strides[4],
+                   void* k_pool, void* v_pool, int64_t num_blocks,
+                   const int32_t* page_table, int64_t pt_stride, int max_pages,
+                   const int32_t* start_pos, const int32_t* lengths, int64_t* seq_lens_out,
+                   int B, int H, int T, int D, int block_size, int dtype,
+                   int32_t* status, void* stream);
+
+/*
+ * Reads rows back as the values they stand for: for each b and t <
+ * lengths[b], k_out[b, h, t, :] and v_out[b, h, t, :] are the rows at position
+ * start_pos[b] + t; rows t >= lengths[b] are zeros, and so are rows whose
+ * block id is out of range (B2PA_ERR_BAD_BLOCK_ID in *status).  k_strides /
+ * v_strides: element strides of [B,H,T,D], unit D stride.
+ */
+B2PA_API int b2pa_kv4_read(const void* k_pool, const void* v_pool, int64_t num_blocks,
+                   const int32_t* page_table, int64_t pt_stride, int max_pages,
+                   const int32_t* start_pos, const int32_t* lengths,
+                   void* k_out, const int64_t k_strides[4], void* v_out, const int64_t v_strides[4],
+                   int B, int H, int T, int D, int block_size, int dtype,
+                   int32_t* status, void* stream);
+
+/*
+ * Single-query paged attention over a 4-bit cache: b2pa_paged_decode with
+ * 4-bit pools.  q / out rows 16-byte aligned.  Workspace as reported by the
+ * size function with the device current that will run the call.
+ */
+B2PA_API size_t b2pa_paged_decode_kv4_workspace_size(int B, int H, int D, int max_pages, int block_size);
+B2PA_API int b2pa_paged_decode_kv4(const void* q, const int64_t q_strides[4],
+                      const void* k_pool, const void* v_pool, int64_t num_blocks,
+                      const int32_t* page_table, int64_t pt_stride, int max_pages,
+                      const int32_t* seq_lens, const int32_t* cur_lens,
+                      void* out, const int64_t out_strides[4],
+                      int B, int H, int D, int block_size, float scale, int dtype,
+                      void* workspace, size_t workspace_bytes,
+                      int32_t* status, void* stream);
+
+/*
+ * Chunked-prefill paged attention over a 4-bit cache (any T >= 1):
+ * b2pa_paged_prefill with 4-bit pools.  The workspace holds the pages of the
+ * call in the type of q: 2 * B * max_pages * H * block_size * D elements, and
+ * what b2pa_paged_prefill needs.
+ */
+B2PA_API size_t b2pa_paged_prefill_kv4_workspace_size(int B, int H, int T, int D, int max_pages,
+                                             int block_size, int dtype);
+B2PA_API int b2pa_paged_prefill_kv4(const void* q, const int64_t q_strides[4],
+                       const void* k_pool, const void* v_pool, int64_t num_blocks,
+                       const int32_t* page_table, int64_t pt_stride, int max_pages,
+                       const int32_t* seq_lens, const int32_t* cur_lens,
+                       void* out, const int64_t out_strides[4],
+                       int B, int H, int T, int D, int block_size, float scale,
+                       int dtype, void* workspace, size_t workspace_bytes,
+                       int32_t* status, void* stream);
+
+/*
+ * ---- Eviction by accumulated attention weight -------------------------------
+ *
+ * weights: fp32 [num_blocks, H, block_size], contiguous: one running sum per
+ * head and cached key, at the key's place in the pools.
+ *
+ * b2pa_key_weights adds the attention weight that a call's queries give to
+ * every key: for each head and each position j < seq_lens[b],
+ *   weights_out[slot of j] = weights_in[slot of j] + sum over t of
+ *       softmax_j(q[b, h, t, :] . K^T * scale)
+ * over the counted queries: t < cur_lens[b], and of these the last `window`
+ * when window > 0.  Query t sees keys 0 .. min(seq_lens[b],
+ * seq_lens[b] - cur_lens[b] + t + 1) - 1, as in the attention.  weights_out
+ * may be weights_in; slots that hold no key are left as they are.  pool_dtype:
+ * dtype, or B2PA_DTYPE_KV4 for a 4-bit K pool.  A key whose block id is out of
+ * range is not seen.
+ */
+B2PA_API size_t b2pa_key_weights_workspace_size(int B, int H, int T, int D, int max_pages,
+                                       int block_size, int dtype, int pool_dtype);
+B2PA_API int b2pa_key_weights(const void* q, const int64_t q_strides[4],
+                     const void* k_pool, int pool_dtype, int64_t num_blocks,
+                     const int32_t* page_table, int64_t pt_stride, int max_pages,
+                     const int32_t* seq_lens, const int32_t* cur_lens, int window,
+                     const float* weights_in, float* weights_out,
+                     int B, int H, int T, int D, int block_size, float scale, int dtype,
+                     void* workspace, size_t workspace_bytes,
+                     int32_t* status, void* stream);
+
+/*
+ * Cuts each sequence of n = seq_lens[b] cached tokens to k = min(keep, n),
+ * each head for itself: the last min(recent, k) stay, and of the others those
+ * with the largest weight (ties: the lower position first; a NaN counts as the
+ * largest).  kept (int32 [B, H, keep]) receives their positions in ascending
+ * order, -1 behind the k-th.  The kept rows of K and V and their weights move
+ * to positions 0 .. k-1 in that order: within the sequence's own pages, or,
+ * with an out_table ([B, >= ceil(keep / block_size)], row stride out_stride),
+ * to the pages listed there, which must not occur in page_table.  The slots
+ * behind the k-th row in its page are zeroed.  The pages behind it are left as
+ * they are (the caller's allocator releases them), and so is a sequence of at
+ * most `keep` tokens in place.  pool_dtype: the pools' type, or
+ * B2PA_DTYPE_KV4.  No page may appear twice.
+ */
+B2PA_API int b2pa_evict(void* k_pool, void* v_pool, int pool_dtype, float* weights,
+               int64_t num_blocks, const int32_t* page_table, int64_t pt_stride, int max_pages,
+               const int32_t* out_table, int64_t out_stride,
+               const int32_t* seq_lens, int keep, int recent, int32_t* kept,
+               int B, int H, int D, int block_size,
+               int32_t* status, void* stream);
 
 #ifdef __cplusplus
 }  /* extern "C" */

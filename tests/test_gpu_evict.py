@@ -1,0 +1,365 @@
+"""Key weights and eviction on the GPU against plain 64-bit implementations,
+and the cache objects over a run of steps: prompt, decode steps, eviction,
+more steps, on plain and 4-bit pools."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import b2pa
+from oracle import model as om
+from tests import _compress_oracle as co
+from tests._helpers import random_tables
+from tests.test_gpu_kv4 import DTYPES, _i32, _np, _rows, _table
+
+pytestmark = pytest.mark.gpu
+
+
+def _weights_case(dev, *, lens, cur, T, H, D, bs, dtype, kv4, window, seed, in_place=False):
+    rng = np.random.default_rng(seed)
+    B = len(lens)
+    NB = sum(-(-n // bs) for n in lens) + 3
+    tables = random_tables(rng, lens, NB, bs)
+    k = _rows(rng, (NB, H, bs, D))
+    if kv4:
+        pool, k = torch.from_numpy(co.pack_pages(k, False)).to(dev), co.stored(k)
+    else:
+        pool = torch.from_numpy(k).to(dtype).to(dev)
+        k = _np(pool)
+    q = torch.from_numpy(_rows(rng, (B, T, H, D))).to(dtype).to(dev).transpose(1, 2)
+    w = torch.from_numpy(rng.random((NB, H, bs)) / 50).float().to(dev)
+    out = w.clone() if in_place else torch.full_like(w, 7.0)
+    want = _np(out)
+    bound = np.zeros_like(want)
+    for b in range(B):
+        n, m = lens[b], min(cur[b], T)
+        if n == 0:
+            continue
+        p, size = co.softmax_rows(_np(q)[b], co.rows_of(k, tables[b], n), cur[b], D ** -0.5)
+        first = max(0, m - window) if window else 0
+        add = p[:, first: max(m, first)].sum(1)
+        for j in range(n):
+            at = tables[b][j // bs], slice(None), j % bs
+            want[at] = _np(w)[at] + add[:, j]
+            # each weight's relative error, one rounding per addend, and the stored sum's own
+            bound[at] = add[:, j] * (co.weight_error(D, size, n) + (T + 2) * 2.0 ** -23) + 2.0 ** -24 * want[at] \
+                + 2.0 ** -30
+    got = b2pa.accumulate_key_weights(q, pool, out if in_place else w, _table(tables, dev), _i32(lens, dev),
+                                      _i32(cur, dev), window=window or None, out=None if in_place else out)
+    assert got is out
+    err = np.abs(_np(got) - want)
+    assert (err <= bound).all(), f"worst {err.max()}, {np.max(err / np.maximum(bound, 1e-30)):.2f} of its bound"
+    assert b2pa.read_status(dev) == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kv4", [False, True])
+@pytest.mark.parametrize("D,bs,H", [(64, 16, 3), (128, 8, 2), (128, 32, 1), (256, 16, 2)])
+def test_key_weights(cuda_device, dtype, kv4, D, bs, H):
+    _weights_case(cuda_device, lens=[1, 16, 17, 130, 333], cur=[1] * 5, T=1, H=H, D=D, bs=bs, dtype=dtype, kv4=kv4,
+                  window=0, seed=1, in_place=True)
+    _weights_case(cuda_device, lens=[66, 67 + 40, 3 + 200, 70], cur=[66, 67, 3, 70], T=70, H=H, D=D, bs=bs,
+                  dtype=dtype, kv4=kv4, window=0, seed=2)
+    _weights_case(cuda_device, lens=[66, 67 + 40, 3 + 200, 70], cur=[66, 67, 3, 70], T=70, H=H, D=D, bs=bs,
+                  dtype=dtype, kv4=kv4, window=17, seed=3, in_place=True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [16, 32])
+def test_key_weights_small_heads(cuda_device, dtype, D):
+    for T in (1, 21):
+        _weights_case(cuda_device, lens=[T, T + 31, T + 100], cur=[T, T, max(1, T - 3)], T=T, H=3, D=D, bs=16,
+                      dtype=dtype, kv4=False, window=0, seed=D)
+
+
+@pytest.mark.parametrize("T", [1, 4])
+def test_key_weights_nothing_counts(cuda_device, T):
+    """Empty sequences, no counted query, and queries that see nothing."""
+    _weights_case(cuda_device, lens=[0, 9, 5, 30, 40], cur=[0, 0, 20, 1, 2], T=T, H=2, D=64, bs=16,
+                  dtype=torch.float32, kv4=False, window=0, seed=5)
+    _weights_case(cuda_device, lens=[0, 9, 5, 30, 40], cur=[0, 0, 20, 1, 2], T=T, H=2, D=64, bs=16,
+                  dtype=torch.bfloat16, kv4=True, window=1, seed=5)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,n,T", [(1, 4000, 1), (1, 3333, 300), (24, 500, 1), (2, 1500, 130)])
+def test_key_weights_long(cuda_device, dtype, B, n, T):
+    lens = [n - 7 * b for b in range(B)]
+    _weights_case(cuda_device, lens=lens, cur=[T] * B, T=T, H=4, D=64, bs=16, dtype=dtype, kv4=False, window=0, seed=n)
+    _weights_case(cuda_device, lens=lens, cur=[T] * B, T=T, H=4, D=64, bs=16, dtype=dtype, kv4=True, window=0, seed=n)
+
+
+def _evict_case(dev, *, lens, keep, recent, H, D, bs, dtype, kv4, seed, fresh, weights=None):
+    rng = np.random.default_rng(seed)
+    B = len(lens)
+    pages = [-(-n // bs) for n in lens]
+    new_pages = [-(-min(n, keep) // bs) for n in lens]
+    NB = sum(pages) + sum(new_pages) + 2
+    perm = [int(x) for x in rng.permutation(NB)]
+    tables = [[perm.pop() for _ in range(p)] for p in pages]
+    outs = [[perm.pop() for _ in range(p)] for p in new_pages] if fresh else tables
+    if kv4:
+        k, v = (rng.integers(0, 256, (NB, H, bs, D * 9 // 16)).astype(np.uint8) for _ in range(2))
+        kp, vp = (torch.from_numpy(x).to(dev) for x in (k, v))
+    else:
+        kp, vp = (torch.randn(NB, H, bs, D, generator=torch.Generator().manual_seed(seed + i)).to(dtype).to(dev)
+                  for i in range(2))
+        k, v = (x.cpu().clone().view(torch.uint8).numpy() for x in (kp, vp))
+    w = rng.random((NB, H, bs)).astype(np.float32) if weights is None else weights(rng, (NB, H, bs))
+    wt = torch.from_numpy(w.copy()).to(dev)
+    width = -(-keep // bs)
+    got = b2pa.evict_by_weight(kp, vp, wt, _table(tables, dev), _i32(lens, dev), keep, recent,
+                               _table(outs, dev, width) if fresh else None).cpu().numpy()
+    # row views of the pools: per page and head, slot-major segments
+    def segments(pool, values):
+        if not kv4:
+            return [pool.reshape(NB, H, bs, -1)]
+        flat = pool.reshape(NB, H, -1)
+        s = flat[..., bs * D // 2:]
+        s = s.reshape(NB, H, D // 16, bs).transpose(0, 1, 3, 2) if values else s.reshape(NB, H, bs, D // 16)
+        return [flat[..., : bs * D // 2].reshape(NB, H, bs, D // 2), s]
+
+    want = [k.copy(), v.copy(), w.copy()]
+    src = segments(k, False) + segments(v, True) + [w[..., None]]
+    dst = segments(want[0], False) + segments(want[1], True) + [want[2][..., None]]
+    kept = np.full((B, H, keep), -1)
+    for b, n in enumerate(lens):
+        m = min(n, keep)
+        for h in range(H):
+            flat = w[np.array(tables[b], dtype=int), h].reshape(-1)[:n] if n else np.zeros(0)
+            sel = co.evict(flat, keep, recent)
+            kept[b, h, : len(sel)] = sel
+            if not fresh and n <= keep:
+                continue
+            rows = [[s[tables[b][j // bs], h, j % bs].copy() for j in sel] for s in src]
+            for r in range(-(-m // bs) * bs):
+                for d, row in zip(dst, rows):
+                    d[outs[b][r // bs], h, r % bs] = row[r] if r < m else 0
+    assert np.array_equal(got, kept)
+    for a, x in ((kp, want[0]), (vp, want[1])):
+        assert np.array_equal(a.cpu().contiguous().view(torch.uint8).numpy().reshape(x.shape), x)
+    assert np.array_equal(wt.cpu().numpy(), want[2], equal_nan=True)
+    assert b2pa.read_status(dev) == 0
+
+
+@pytest.mark.parametrize("fresh", [False, True], ids=["in_place", "out_table"])
+@pytest.mark.parametrize("dtype,kv4,D,bs,H", [
+    (torch.float32, False, 64, 16, 3), (torch.float32, False, 16, 8, 2), (torch.bfloat16, False, 128, 16, 2),
+    (torch.float16, False, 16, 32, 1), (torch.float16, False, 256, 8, 1), (torch.bfloat16, False, 32, 16, 4),
+    (None, True, 64, 16, 3), (None, True, 128, 8, 2), (None, True, 256, 32, 1)])
+def test_evict(cuda_device, fresh, dtype, kv4, D, bs, H):
+    for keep, recent in ((1, 0), (1, 1), (7, 3), (16, 16), (33, 100), (40, 0), (64, 13)):
+        _evict_case(cuda_device, lens=[0, 1, 16, 33, 40, 41, 150, 300], keep=keep, recent=recent, H=H, D=D, bs=bs,
+                    dtype=dtype, kv4=kv4, seed=keep, fresh=fresh)
+
+
+def _ties(rng, shape):
+    return np.floor(rng.random(shape) * 3).astype(np.float32)
+
+
+def _special(rng, shape):
+    w = rng.standard_normal(shape).astype(np.float32) * np.float32(1e-3)
+    pick = rng.random(shape)
+    for lo, x in ((0.0, np.nan), (0.05, np.inf), (0.1, -np.inf), (0.15, 0.0), (0.2, -0.0), (0.25, 1e-42), (0.3, 3e38)):
+        w[(pick >= lo) & (pick < lo + 0.05)] = x
+    return w
+
+
+@pytest.mark.parametrize("weights", [_ties, _special, lambda rng, shape: np.zeros(shape, np.float32)],
+                         ids=["ties", "special", "zeros"])
+def test_evict_ties_and_special_weights(cuda_device, weights):
+    for keep, recent in ((5, 2), (64, 0), (100, 10), (257, 7)):
+        _evict_case(cuda_device, lens=[300, 64, 1100], keep=keep, recent=recent, H=2, D=64, bs=16,
+                    dtype=torch.bfloat16, kv4=False, seed=keep, fresh=False, weights=weights)
+
+
+@pytest.mark.parametrize("n,keep", [(9000, 1500), (60000, 30000), (60001, 17)])
+def test_evict_long(cuda_device, n, keep):
+    """Chunks that overlap their destinations, and sequences past what shared memory holds."""
+    _evict_case(cuda_device, lens=[n, 100], keep=keep, recent=5, H=1, D=64, bs=32, dtype=torch.float16, kv4=False,
+                seed=n, fresh=False)
+
+
+def test_evict_bad_pages(cuda_device):
+    dev = cuda_device
+    kp = torch.randn(4, 1, 16, 64, device=dev)
+    vp, w = torch.randn_like(kp), torch.rand(4, 1, 16, device=dev)
+    before = kp.clone()
+    bad = b2pa._lib.STATUS_CODES["B2PA_ERR_BAD_BLOCK_ID"]
+    for table, n in (([[0, 9, 2]], 48), ([[0, -1, 2]], 48), ([[0, 1]], 40)):
+        b2pa.clear_status(dev)
+        b2pa.evict_by_weight(kp, vp, w, _i32(table, dev), _i32([n], dev), 20, 20)
+        assert b2pa.read_status(dev) == bad
+    assert torch.equal(kp[3], before[3])
+    b2pa.clear_status(dev)
+
+
+def test_evict_refusals(cuda_device):
+    dev = cuda_device
+    kp, w = torch.zeros(4, 2, 16, 64, device=dev), torch.zeros(4, 2, 16, device=dev)
+    t, n = _i32([[0, 1]], dev), _i32([20], dev)
+    for bad in (dict(keep=0), dict(keep=4, recent=-1), dict(keep=17, out_table=_i32([[3]], dev))):
+        with pytest.raises(ValueError):
+            b2pa.evict_by_weight(kp, kp.clone(), w, t, n, **bad)
+    with pytest.raises(ValueError):
+        b2pa.evict_by_weight(kp, kp.clone(), w.double(), t, n, 4)
+    with pytest.raises(ValueError):
+        b2pa.evict_by_weight(kp, kp[:, :1].contiguous(), w, t, n, 4)
+    with pytest.raises(TypeError):
+        b2pa.accumulate_key_weights(torch.zeros(1, 2, 1, 64, device=dev, dtype=torch.bfloat16), kp, w, t, n, n)
+    with pytest.raises(ValueError):
+        b2pa.accumulate_key_weights(torch.zeros(1, 2, 1, 64, device=dev), kp, w, t, n, n, window=0)
+
+
+@pytest.mark.parametrize("kv4", [False, True], ids=["plain", "kv4"])
+@pytest.mark.parametrize("fused", [False, True])
+def test_run_of_steps(cuda_device, kv4, fused):
+    """Ragged prompts, decode steps, an eviction, more steps (the block tables regrow), against dense 64-bit
+    bookkeeping: outputs, key weights, kept positions, lengths and freed blocks."""
+    dev, H, D, bs = cuda_device, 3, 64, 16
+    rng = np.random.default_rng(8)
+    pool = (b2pa.Kv4BlockPool if kv4 else b2pa.LayerBlockPool)(bs, 3, 1.5)
+    pool.track_key_weights()
+    states = [b2pa.PagedKVCacheState(pool) for _ in range(3)]
+    K = [np.zeros((0, H, D)) for _ in range(3)]
+    V = [np.zeros((0, H, D)) for _ in range(3)]
+    W = [np.zeros((H, 0)) for _ in range(3)]
+    err = [0.0] * 3
+
+    def step(which, lengths, T):
+        cache = b2pa.BatchedPagedKVCache([states[i] for i in which], pool)
+        x = [torch.from_numpy(rng.standard_normal((len(which), T, H, D))).float().to(dev).transpose(1, 2)
+             for _ in range(3)]
+        got_lens = cache.append_batch(x[1], x[2], lengths)
+        out = b2pa.paged_attention("b200_paged", x[0], cache, lengths)
+        for i, b in enumerate(which):
+            m = lengths[i]
+            new = [_np(t)[i, :, :m].transpose(1, 0, 2) for t in x[1:]]
+            if kv4:
+                new = [co.stored(t) for t in new]
+            K[b], V[b] = np.concatenate([K[b], new[0]]), np.concatenate([V[b], new[1]])
+            n = len(K[b])
+            assert int(got_lens[i]) == n == states[b].seq_len
+            p, size = co.softmax_rows(_np(x[0])[i], K[b], m, D ** -0.5)
+            ref = np.einsum("htn,nhd->htd", p, V[b])
+            bound = co.output_bound(ref, 2.0 ** -24, D, size, n, np.abs(V[b]).max())
+            assert (np.abs(_np(out)[i, :, :m] - ref[:, :m]) <= bound[:, :m]).all()
+            W[b] = np.concatenate([W[b], np.zeros((H, n - W[b].shape[1]))], 1) + p[:, :m].sum(1)
+            err[b] += m * co.weight_error(D, size, n) + 2.0 ** -20
+            kw = _np(pool.key_weights)
+            mine = co.rows_of(kw[..., None], states[b].block_ids, n)[..., 0].T
+            assert (np.abs(mine - W[b]) <= err[b] * np.maximum(W[b], 2.0 ** -10)).all()
+
+    prev = b2pa.set_fused_append(fused)
+    try:
+        step([0, 1, 2], [40, 17, 33], 40)
+        for _ in range(5):
+            step([0, 1, 2], [1, 1, 1], 1)
+        cache = b2pa.BatchedPagedKVCache([states[0], states[2]], pool)
+        free, held = len(pool.free_block_ids), [len(s.block_ids) for s in states]
+        mine = {b: co.rows_of(_np(pool.key_weights)[..., None], states[b].block_ids, len(K[b]))[..., 0].T
+                for b in (0, 2)}
+        kept = cache.evict(20, recent=6).cpu().numpy()
+        for i, b in enumerate((0, 2)):
+            sel = np.stack([co.evict(mine[b][h], 20, 6) for h in range(H)])
+            assert np.array_equal(kept[i], sel)
+            K[b], V[b] = (np.stack([x[sel[h], h] for h in range(H)], 1) for x in (K[b], V[b]))
+            W[b] = np.stack([W[b][h, sel[h]] for h in range(H)])
+            assert states[b].seq_len == 20 and len(states[b].block_ids) == 2
+        assert len(pool.free_block_ids) - free == held[0] + held[2] - 4
+        for t in (pool.k_blocks, pool.v_blocks, pool.key_weights):  # freed pages are zero again
+            assert not t[pool.free_block_ids].any()
+        for _ in range(14):
+            step([2, 0], [1, 1], 1)
+        step([0, 1, 2], [3, 20, 20], 20)
+        assert torch.equal(cache.evict(10 ** 6)[:, 0, 0].cpu(), torch.zeros(2, dtype=torch.int32))  # nothing leaves
+    finally:
+        b2pa.set_fused_append(prev)
+    with pytest.raises(ValueError, match="twice"):
+        b2pa.BatchedPagedKVCache([states[0], states[0]], pool).evict(4)
+    assert b2pa.read_status(dev) == 0
+
+
+def _model(dev, kv4):
+    def tracking_pool(*args):
+        pool = (b2pa.Kv4BlockPool if kv4 else b2pa.LayerBlockPool)(*args)
+        pool.track_key_weights()
+        return pool
+
+    back = om.b2pa_backend()
+    back.pool_cls = tracking_pool
+    om.set_seed(11)
+    return om.TinyLM(300, 128, 2, 3, 256, 512, back, kv_block_size=16, kv_pool_initial_blocks=64,
+                     kv_pool_growth_factor=2.0).to(dev).eval()
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("kv4", [False, True], ids=["plain", "kv4"])
+def test_decoder_graph_with_eviction(cuda_device, kv4):
+    """FusedDecoder under DecodeGraph with tracking pools gives, bit for bit, the logits, pools and key weights of the
+    same steps run eagerly in a DecodeStep, through an eviction of every layer between replays."""
+    dev = cuda_device
+    lengths = [40, 25, 33]
+    runs = []
+    for mode in ("eager", "graph"):
+        model = _model(dev, kv4)
+        prompt = torch.randint(0, 300, (3, 40), generator=torch.Generator().manual_seed(3)).to(dev)
+        cur = torch.tensor(lengths, device=dev)
+        logits, caches = model(prompt, position_offset=0, current_lengths=cur)
+        layer_states = [list(c.states) for c in caches]
+        assert all(st[0].pool.key_weights.any() for st in layer_states)
+        nxt = torch.argmax(logits[torch.arange(3, device=dev), cur - 1, :], dim=-1)
+        batches = [b2pa.BatchedPagedKVCache(list(st), st[0].pool) for st in layer_states]
+        dec = b2pa.FusedDecoder(model, max_batch=4)
+        ids, pos = nxt.clone(), cur.clone()
+        graph = b2pa.DecodeGraph(lambda: dec.step(ids, pos, batches)) if mode == "graph" else None
+        meta, seen = None, []
+        for s in range(24):
+            if s == 12:
+                for c in batches:
+                    c.evict(24, recent=8)
+            if graph:
+                lg, _ = graph(layer_states)
+            else:
+                step = b2pa.DecodeStep(layer_states, meta)
+                with step:
+                    lg, _ = dec.step(ids, pos, batches)
+                meta = step.meta
+            seen.append(lg.clone())
+            ids.copy_(torch.randint(0, 300, (3,), generator=torch.Generator().manual_seed(s)).to(dev))
+            pos.add_(1)
+        assert all(s.seq_len == 36 for st in layer_states for s in st)
+        runs.append((seen, [(st[0].pool.k_blocks, st[0].pool.v_blocks, st[0].pool.key_weights) for st in layer_states],
+                     [[s.block_ids for s in st] for st in layer_states]))
+        if graph:
+            assert graph.replays >= 20
+    for a, b in zip(runs[0][0], runs[1][0]):
+        assert torch.equal(a, b)
+    assert runs[0][2] == runs[1][2]
+    for x, y in zip(runs[0][1], runs[1][1]):
+        assert all(torch.equal(a, b) for a, b in zip(x, y))
+    assert b2pa.read_status(dev) == 0
+
+
+@torch.no_grad()
+def test_executor_bounds_every_cache(cuda_device):
+    """FusedDecodeExecutor with evict_keep: requests run to their end on bounded caches."""
+    from oracle import serving as osv
+
+    dev = cuda_device
+    model = _model(dev, True)
+    ex = osv.ModelExecutors(model, dev)
+    reqs = osv.generate_requests(4, 1000.0, 300, [osv.WorkloadProfile("x", 60, 100, 40, 40, 1.0)], seed=2)
+    decode = b2pa.FusedDecodeExecutor(model, dev, max_batch=4, evict_keep=48, evict_recent=16, evict_slack=8)
+    longest = []
+
+    def step(requests, *args, **kw):
+        out = decode(requests, *args, **kw)
+        longest.append(max(s.seq_len for r in requests for s in r.kv_caches))
+        return out
+
+    done, _ = osv.ContinuousScheduler(4, 128, 512).run(reqs, ex.prefill, step, ex.release)
+    assert len(done) == 4 and all(len(r.generated_token_ids) == 40 for r in done)
+    assert longest and max(longest) < 48 + 8
+    assert b2pa.read_status(dev) == 0

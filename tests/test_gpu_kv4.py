@@ -1,0 +1,388 @@
+"""The 4-bit KV cache on the GPU against plain 64-bit implementations: stored
+values and page bytes exactly, attention within a bound on the rounding errors
+(tests/_compress_oracle.py)."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import b2pa
+from tests import _compress_oracle as co
+from tests._helpers import random_tables
+
+pytestmark = pytest.mark.gpu
+
+HALF_STEP = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+DTYPES = list(HALF_STEP)
+
+
+def _np(t):
+    return t.detach().double().cpu().numpy()
+
+
+def _i32(x, dev):
+    return torch.tensor(np.asarray(x), dtype=torch.int32, device=dev)
+
+
+def _table(tables, dev, width=None):
+    width = width or max(1, max(len(t) for t in tables))
+    a = np.full((len(tables), width), -1, np.int32)
+    for b, t in enumerate(tables):
+        a[b, : len(t)] = t
+    return _i32(a, dev)
+
+
+def _rows(rng, shape):
+    """Rows whose groups span many magnitudes, some of them zero."""
+    x = rng.standard_normal(shape)
+    x *= np.exp2(rng.integers(-6, 5, shape[:-1] + (1,)))
+    x[..., ::37] *= 8
+    x[rng.random(shape[:-1]) < 0.05] = 0
+    return x
+
+
+def _pools(rng, NB, H, bs, D):
+    """Packed K and V pools (numpy), with the values they stand for."""
+    k, v = _rows(rng, (NB, H, bs, D)), _rows(rng, (NB, H, bs, D)) * 0.25
+    return co.pack_pages(k, False), co.pack_pages(v, True), co.stored(k), co.stored(v)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,bs,H", [(64, 8, 1), (64, 16, 8), (128, 16, 3), (128, 32, 5), (256, 16, 2), (256, 8, 1)])
+def test_append_and_read(cuda_device, dtype, D, bs, H):
+    rng = np.random.default_rng(D + bs)
+    T, starts, lens = 23, [0, 5, bs - 1, 40, 7], [23, 1, 17, 0, 30]        # 30: clamped to T
+    B = len(starts)
+    ends = [s + min(n, T) for s, n in zip(starts, lens)]
+    NB = sum(-(-e // bs) for e in ends) + 3
+    tables = random_tables(rng, ends, NB, bs)
+    k = torch.from_numpy(_rows(rng, (B, T, H, D))).to(dtype).to(cuda_device).transpose(1, 2)
+    v = torch.from_numpy(_rows(rng, (B, T, H, D))).to(dtype).to(cuda_device).transpose(1, 2)
+    before = rng.integers(0, 256, (2, NB, H, bs, D * 9 // 16)).astype(np.uint8)
+    kp, vp = (torch.from_numpy(x).to(cuda_device) for x in before)
+    want_k, want_v = before[0].copy(), before[1].copy()
+    for pool, new, values in ((want_k, _np(k), False), (want_v, _np(v), True)):
+        c, s = co.quantise(new)
+        for b in range(B):
+            for t in range(min(lens[b], T)):
+                pos = starts[b] + t
+                page = pool[tables[b][pos // bs]].reshape(H, -1)
+                u = (c[b, :, t].astype(np.int16) + 8).astype(np.uint8)
+                r = pos % bs
+                page[:, r * D // 2: (r + 1) * D // 2] = u[:, 0::2] | (u[:, 1::2] << 4)
+                sc = page[:, bs * D // 2:]
+                if values:
+                    sc.reshape(H, D // 16, bs)[:, :, r] = s[b, :, t]
+                else:
+                    sc.reshape(H, bs, D // 16)[:, r] = s[b, :, t]
+    table = _table(tables, cuda_device)
+    out = torch.full((B,), -7, dtype=torch.int64, device=cuda_device)
+    b2pa.kv4_append(k, v, kp, vp, table, _i32(starts, cuda_device), _i32(lens, cuda_device), out)
+    assert np.array_equal(kp.cpu().numpy(), want_k) and np.array_equal(vp.cpu().numpy(), want_v)
+    assert out.tolist() == ends
+    n = [min(x, T) for x in lens]
+    rk, rv = b2pa.kv4_read(kp, vp, table, _i32(starts, cuda_device), _i32(n, cuda_device), T, dtype)
+    live = (np.arange(T) < np.array(n)[:, None])[:, None, :, None]
+    assert np.array_equal(_np(rk), np.where(live, co.stored(_np(k)), 0))
+    assert np.array_equal(_np(rv), np.where(live, co.stored(_np(v)), 0))
+    assert b2pa.read_status(cuda_device) == 0
+
+
+def test_append_borders(cuda_device):
+    """Every border of the two roundings, its fp32 neighbours, saturation, subnormal scales, NaN and infinity."""
+    tops = []
+    grid = co.GRID
+    for i in range(1, len(grid)):
+        t = np.float32((grid[i] + grid[i - 1]) / 2 * 7)
+        tops += [np.nextafter(t, np.float32(0)), t, np.nextafter(t, np.float32(1e9))]
+    rows = np.zeros((len(tops), 64), np.float32)
+    for i, t in enumerate(tops):
+        s = grid[co.scale_bytes(np.array([float(t)]))[0]]
+        rows[i, 0] = t
+        for m in range(7):
+            x = np.float32((m + 0.5) * s)
+            rows[i, 1 + 2 * m: 3 + 2 * m] = [np.nextafter(x, np.float32(0)), x]
+            rows[i, 17 + 2 * m: 19 + 2 * m] = [-x, -np.nextafter(x, np.float32(1e9))]
+        rows[i, 16] = -t
+    extra = np.zeros((6, 64), np.float32)
+    extra[0, :4] = [1e30, -1e5, 64512, 3]
+    extra[1, 3], extra[1, 20] = np.nan, -np.inf
+    extra[2, :3] = [1e-7, -2e-6, 1e-40]
+    extra[3, 0] = np.float32(3.4e38)
+    extra[4, :2] = [2.0 ** -16, -2.0 ** -17]
+    rows = np.concatenate([rows, extra])
+    n = len(rows)
+    x = torch.from_numpy(rows).to(cuda_device).view(1, 1, n, 64)
+    pages = -(-n // 16)
+    kp = torch.zeros(pages, 1, 16, 36, dtype=torch.uint8, device=cuda_device)
+    vp = torch.zeros_like(kp)
+    table = _i32(np.arange(pages)[None], cuda_device)
+    zero, cnt = _i32([0], cuda_device), _i32([n], cuda_device)
+    b2pa.kv4_append(x, -x, kp, vp, table, zero, cnt)
+    k, v = b2pa.kv4_read(kp, vp, table, zero, cnt, n, torch.float32)
+    np.testing.assert_array_equal(_np(k)[0, 0], co.stored(rows))
+    np.testing.assert_array_equal(_np(v)[0, 0], co.stored(-rows))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_append_takes_any_strides(cuda_device, dtype):
+    """Channel-strided, misaligned and broadcast sources."""
+    gen = torch.Generator().manual_seed(2)
+    base = torch.randn(2, 5, 130, 6, generator=gen).to(dtype).to(cuda_device)
+    k = base[:, :, 1:129, :4].permute(0, 3, 1, 2)                 # [2, 4, 5, 128]: channel stride 6
+    v = torch.randn(2, 5, 129, generator=gen).to(dtype).to(cuda_device)[:, None, :, 1:].expand(2, 4, 5, 128)
+    kp = torch.zeros(2, 4, 8, 72, dtype=torch.uint8, device=cuda_device)
+    vp = torch.zeros_like(kp)
+    table = _i32([[1], [0]], cuda_device)
+    s, n = _i32([3, 0], cuda_device), _i32([5, 4], cuda_device)
+    b2pa.kv4_append(k, v, kp, vp, table, s, n)
+    rk, rv = b2pa.kv4_read(kp, vp, table, s, n, 5, dtype)
+    live = (np.arange(5) < np.array([5, 4])[:, None])[:, None, :, None]
+    assert np.array_equal(_np(rk), np.where(live, co.stored(_np(k)), 0))
+    assert np.array_equal(_np(rv), np.where(live, co.stored(_np(v)), 0))
+
+
+def _attend_case(dev, *, lens, cur, H, D, bs, dtype, T, seed, q_scale=1.0, width=None, tables=None, q=None):
+    rng = np.random.default_rng(seed)
+    B = len(lens)
+    NB = sum(-(-L // bs) for L in lens) + 5
+    kp, vp, k, v = _pools(rng, NB, H, bs, D)
+    tables = tables or random_tables(rng, lens, NB, bs)
+    if q is None:
+        q = torch.from_numpy(_rows(rng, (B, T, H, D)) * q_scale).to(dtype).to(dev).transpose(1, 2)
+    fn = b2pa.paged_attention_decode_kv4 if T == 1 else b2pa.paged_attention_prefill_kv4
+    out = fn(q, torch.from_numpy(kp).to(dev), torch.from_numpy(vp).to(dev), _table(tables, dev, width),
+             _i32(lens, dev), _i32(cur, dev))
+    refs, bounds = [], []
+    for b in range(B):
+        K, V = co.rows_of(k, tables[b], lens[b]), co.rows_of(v, tables[b], lens[b])
+        hidden = [j for j in range(lens[b]) if tables[b][j // bs] < 0]
+        p, size = co.softmax_rows(_np(q)[b], K, cur[b], D ** -0.5, hidden)
+        ref = np.einsum("htn,nhd->htd", p, V)
+        refs.append(ref)
+        bounds.append(co.output_bound(ref, HALF_STEP[dtype], D, size, lens[b], np.abs(V).max(initial=0.0)))
+    return out, np.stack(refs), np.stack(bounds), dict(kp=kp, vp=vp, k=k, v=v, tables=tables, q=q)
+
+
+def _check(out, ref, bound):
+    err = np.abs(_np(out) - ref)
+    assert (err <= bound).all(), f"worst error {err.max()} at {np.unravel_index(err.argmax(), err.shape)}, " \
+                                 f"{(err / bound).max():.2f} of its bound"
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,bs,H", [(64, 8, 3), (64, 16, 8), (64, 32, 1), (128, 8, 2), (128, 16, 5), (128, 32, 4),
+                                    (256, 8, 1), (256, 16, 3), (256, 32, 2)])
+def test_decode(cuda_device, dtype, D, bs, H):
+    lens = [1, 2, 7, 8, 9, 15, 16, 17, 31, 33, 100, 300]
+    out, ref, bound, _ = _attend_case(cuda_device, lens=lens, cur=[1] * len(lens), H=H, D=D, bs=bs, dtype=dtype, T=1,
+                                      seed=D + bs + H)
+    _check(out, ref, bound)
+    assert b2pa.read_status(cuda_device) == 0
+
+
+@pytest.mark.parametrize("T", [1, 3])
+def test_nothing_visible(cuda_device, T):
+    """Empty sequences and current lengths past the sequence leave zero rows; 0 and 2 shift what is seen."""
+    lens, cur = [0, 1, 15, 16, 33, 5, 9, 0], [1, 1, 0, 2, 3, 20, 9, 0]
+    out, ref, bound, _ = _attend_case(cuda_device, lens=lens, cur=cur, H=2, D=64, bs=16, dtype=torch.float32, T=T,
+                                      seed=3)
+    _check(out, ref, bound)
+    assert not out[0].any() and not out[5].any() and not out[7].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,L", [(1, 5000), (2, 2777), (40, 700)])
+def test_decode_long(cuda_device, dtype, B, L):
+    lens = [L - 13 * b for b in range(B)]
+    out, ref, bound, _ = _attend_case(cuda_device, lens=lens, cur=[1] * B, H=4, D=128, bs=16, dtype=dtype, T=1, seed=L)
+    _check(out, ref, bound)
+
+
+def test_decode_offsets_past_32_bits(cuda_device):
+    """Pages at byte offsets past 2^32 of the pool."""
+    H, D, bs = 8, 128, 32
+    page = H * bs * 72
+    NB = (1 << 32) // page + 40
+    kp = torch.empty(NB, H, bs, 72, dtype=torch.uint8, device=cuda_device)
+    vp = torch.empty_like(kp)
+    rng = np.random.default_rng(5)
+    lens = [70, 1000]
+    tables = [[NB - 1 - i for i in range(3)], [NB - 4 - i for i in range(32)]]
+    ids = tables[0] + tables[1]
+    k, v = _rows(rng, (len(ids), H, bs, D)), _rows(rng, (len(ids), H, bs, D))
+    kp[ids], vp[ids] = (torch.from_numpy(co.pack_pages(x, y)).to(cuda_device) for x, y in ((k, False), (v, True)))
+    q = torch.from_numpy(_rows(rng, (2, H, 1, D))).to(torch.float16).to(cuda_device)
+    out = b2pa.paged_attention_decode_kv4(q, kp, vp, _table(tables, cuda_device), _i32(lens, cuda_device),
+                                          _i32([1, 1], cuda_device))
+    at = 0
+    for b, n in enumerate(lens):
+        mine = list(range(at, at + len(tables[b])))
+        at += len(mine)
+        K, V = co.rows_of(co.stored(k), mine, n), co.rows_of(co.stored(v), mine, n)
+        p, size = co.softmax_rows(_np(q)[b], K, 1, D ** -0.5)
+        ref = np.einsum("htn,nhd->htd", p, V)
+        _check(out[b], ref, co.output_bound(ref, 2.0 ** -11, D, size, n, np.abs(V).max()))
+
+
+def test_far_logits(cuda_device):
+    """Logits in the hundreds: the running maximum carries the sums."""
+    out, ref, bound, _ = _attend_case(cuda_device, lens=[333, 40], cur=[1, 1], H=2, D=128, bs=16, dtype=torch.float32,
+                                      T=1, seed=9, q_scale=30.0)
+    _check(out, ref, bound)
+
+
+def test_scales_far_apart(cuda_device):
+    """Value scales over their whole range within one sequence, small first and large first."""
+    rng = np.random.default_rng(4)
+    D, bs, n = 64, 16, 160
+    for order in (1, -1):
+        v = rng.standard_normal((10, 1, bs, D)) * np.exp2(np.linspace(-14, 13, 10))[::order, None, None, None]
+        k = rng.standard_normal((10, 1, bs, D))
+        kp, vp = co.pack_pages(k, False), co.pack_pages(v, True)
+        q = torch.from_numpy(rng.standard_normal((1, 1, 1, D))).float().to(cuda_device)
+        table = _i32(np.arange(10)[None], cuda_device)
+        for m in (n, 16, 32, 1):
+            out = b2pa.paged_attention_decode_kv4(q, torch.from_numpy(kp).to(cuda_device),
+                                                  torch.from_numpy(vp).to(cuda_device), table,
+                                                  _i32([m], cuda_device), _i32([1], cuda_device))
+            K, V = co.rows_of(co.stored(k), range(10), m), co.rows_of(co.stored(v), range(10), m)
+            p, size = co.softmax_rows(_np(q)[0], K, 1, D ** -0.5)
+            ref = np.einsum("htn,nhd->htd", p, V)
+            _check(out[0], ref, co.output_bound(ref, 2.0 ** -24, D, size, m, np.abs(V).max()))
+
+
+def test_nan_reaches_only_its_own(cuda_device):
+    """A NaN group of V makes its channels NaN; one of K the head's output; both only where the key is seen.  Stale
+    NaN rows behind the sequence and of other heads are not read."""
+    rng = np.random.default_rng(6)
+    D, bs, H = 128, 16, 3
+    k, v = rng.standard_normal((4, H, bs, D)), rng.standard_normal((4, H, bs, D))
+    v[1, 0, 3, 40] = np.nan          # sequence 0, position 19, head 0, group 2
+    k[2, 1, 0, 7] = np.inf           # sequence 1, position 0, head 1
+    k[1, :, 9] = np.nan              # sequence 0, position 25: behind its length
+    v[1, :, 9] = np.nan
+    kp, vp = (torch.from_numpy(co.pack_pages(x, y)).to(cuda_device) for x, y in ((k, False), (v, True)))
+    q = torch.from_numpy(rng.standard_normal((2, H, 1, D))).float().to(cuda_device)
+    table = _i32([[0, 1], [2, 3]], cuda_device)
+    for T in (1, 2):
+        fn = b2pa.paged_attention_decode_kv4 if T == 1 else b2pa.paged_attention_prefill_kv4
+        out = fn(q.expand(2, H, T, D).contiguous(), kp, vp, table, _i32([25, 18], cuda_device),
+                 _i32([T, T], cuda_device))
+        bad = torch.isnan(out)
+        assert bad[0, 0, :, 32:48].all() and not bad[0, 0, :, :32].any() and not bad[0, 0, :, 48:].any()
+        assert not bad[0, 1:].any()
+        assert bad[1, 1].all() and not bad[1, 0].any() and not bad[1, 2].any()
+
+
+def test_bad_pages(cuda_device):
+    """Unset pages are not seen; ids past the pool are not read and are reported."""
+    NB = 5 + 4
+    for bad, code in ((-1, 0), (NB + 3, b2pa._lib.STATUS_CODES["B2PA_ERR_BAD_BLOCK_ID"])):
+        b2pa.clear_status(cuda_device)
+        lens = [64]
+        rng = np.random.default_rng(1)
+        kp, vp, k, v = _pools(rng, NB, 2, 16, 64)
+        q = torch.from_numpy(_rows(rng, (1, 2, 1, 64))).float().to(cuda_device)
+        args = (torch.from_numpy(kp).to(cuda_device), torch.from_numpy(vp).to(cuda_device),
+                _table([[3, bad, 1, 0]], cuda_device), _i32(lens, cuda_device), _i32([1], cuda_device))
+        K, V = co.rows_of(k, [3, 0, 1, 0], 64), co.rows_of(v, [3, 0, 1, 0], 64)
+        p, size = co.softmax_rows(_np(q)[0], K, 1, 0.125, hidden=range(16, 32))
+        ref = np.einsum("htn,nhd->htd", p, V)
+        bound = co.output_bound(ref, 2.0 ** -24, 64, size, 64, np.abs(V).max())
+        _check(b2pa.paged_attention_decode_kv4(q, *args)[0], ref, bound)
+        assert b2pa.read_status(cuda_device) == code
+        b2pa.clear_status(cuda_device)
+        _check(b2pa.paged_attention_prefill_kv4(q, *args)[0], ref, bound)
+        assert b2pa.read_status(cuda_device) == code
+    b2pa.clear_status(cuda_device)
+    # a length past the table: the table's rows are seen, and it is reported
+    out = b2pa.paged_attention_decode_kv4(q, args[0], args[1], _table([[3, 2]], cuda_device), _i32([40], cuda_device),
+                                          _i32([1], cuda_device))
+    K, V = co.rows_of(k, [3, 2], 32), co.rows_of(v, [3, 2], 32)
+    p, size = co.softmax_rows(_np(q)[0], K, 0, 0.125)
+    ref = np.einsum("htn,nhd->htd", p, V)
+    _check(out[0], ref, co.output_bound(ref, 2.0 ** -24, 64, size, 32, np.abs(V).max()))
+    assert b2pa.read_status(cuda_device) == b2pa._lib.STATUS_CODES["B2PA_ERR_BAD_BLOCK_ID"]
+    b2pa.clear_status(cuda_device)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,bs,H", [(64, 16, 4), (64, 8, 1), (128, 16, 2), (128, 32, 3), (256, 16, 1)])
+def test_prefill(cuda_device, dtype, D, bs, H):
+    """Chunks of 70 on prefixes, a padded row, a chunk without prefix."""
+    cur = [70, 64, 1, 70]
+    lens = [70, 64 + 33, 1 + 300, 70 + 129]
+    out, ref, bound, _ = _attend_case(cuda_device, lens=lens, cur=cur, H=H, D=D, bs=bs, dtype=dtype, T=70, seed=D + bs)
+    # the plain pools' 16-bit kernels round the softmax weights to the operand type: one half step more of max|v|
+    _check(out, ref, bound + (0 if dtype == torch.float32 else HALF_STEP[dtype] * np.abs(ref).max()))
+    assert b2pa.read_status(cuda_device) == 0
+
+
+def test_streams_layouts_and_capture(cuda_device):
+    """Strided q, a wide table, a non-current stream, and two graphs replayed after the inputs changed."""
+    args = dict(lens=[50, 333], cur=[1, 1], H=4, D=128, bs=16, dtype=torch.bfloat16, T=1)
+    out, ref, bound, st = _attend_case(cuda_device, seed=1, width=40, **args)
+    _check(out, ref, bound)
+    dev = cuda_device
+    kp, vp = (torch.from_numpy(st[x]).to(dev) for x in ("kp", "vp"))
+    table, lens, one = _table(st["tables"], dev), _i32(args["lens"], dev), _i32([1, 1], dev)
+    side = torch.cuda.Stream(dev)
+    side.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(side):
+        other = b2pa.paged_attention_decode_kv4(st["q"], kp, vp, table, lens, one)
+    torch.cuda.current_stream(dev).wait_stream(side)
+    assert torch.equal(other, out)
+    q1, q2 = st["q"].clone(), st["q"].clone()
+    graphs, outs = [], []
+    for q in (q1, q2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(b2pa.paged_attention_decode_kv4(q, kp, vp, table, lens, one))
+        graphs.append(g)
+    q2.mul_(-1.5)
+    wanted = [b2pa.paged_attention_decode_kv4(q, kp, vp, table, lens, one) for q in (q1, q2)]
+    s1, s2 = torch.cuda.Stream(dev), torch.cuda.Stream(dev)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for s, g in ((s1, graphs[0]), (s2, graphs[1])):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], wanted[0]) and torch.equal(outs[1], wanted[1])
+    # a misaligned q is copied, not refused
+    odd = torch.zeros(st["q"].numel() + 1, dtype=torch.bfloat16, device=dev)[1:].view(st["q"].shape)
+    odd.copy_(st["q"])
+    assert torch.equal(b2pa.paged_attention_decode_kv4(odd, kp, vp, table, lens, one), out)
+
+
+def test_refusals(cuda_device):
+    dev = cuda_device
+    kp = torch.zeros(4, 2, 16, 36, dtype=torch.uint8, device=dev)
+    q = torch.zeros(1, 2, 1, 64, device=dev)
+    t, one = _i32([[0, 1]], dev), _i32([1], dev)
+    ok = (q, kp, kp.clone(), t, one, one)
+    b2pa.paged_attention_decode_kv4(*ok)
+    with pytest.raises(TypeError):
+        b2pa.paged_attention_decode_kv4(q, q, q, t, one, one)
+    with pytest.raises(TypeError):
+        b2pa.paged_attention_decode_kv4(q.double(), *ok[1:])
+    with pytest.raises(ValueError):
+        b2pa.paged_attention_decode_kv4(torch.zeros(1, 3, 1, 64, device=dev), *ok[1:])
+    with pytest.raises(ValueError):
+        b2pa.paged_attention_decode_kv4(torch.zeros(1, 2, 1, 128, device=dev), *ok[1:])
+    with pytest.raises(ValueError):
+        b2pa.paged_attention_decode_kv4(torch.zeros(1, 2, 3, 64, device=dev), *ok[1:])
+    with pytest.raises(ValueError):
+        b2pa.paged_attention_decode_kv4(q, kp, kp, t, _i32([1, 1], dev), one)
+    with pytest.raises(ValueError):
+        b2pa.paged_attention_decode_kv4(q, kp, kp, _i32([[0], [1]], dev), one, one)
+    with pytest.raises(TypeError):
+        b2pa.kv4_read(kp.transpose(0, 1), kp, t, one, one, 4, torch.float32)
+    with pytest.raises(TypeError):
+        b2pa.kv4_read(kp, kp, t, one, one, 4, torch.float64)
+    with pytest.raises(RuntimeError, match="block_size"):
+        bad = torch.zeros(4, 2, 12, 36, dtype=torch.uint8, device=dev)
+        b2pa.paged_attention_decode_kv4(q, bad, bad, t, one, one)
+    assert b2pa.read_status(dev) == 0
