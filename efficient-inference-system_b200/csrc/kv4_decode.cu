@@ -6,101 +6,628 @@
 // with K and V the values the pages stand for, in fp32, stored in the type of
 // q; zeros when no key is visible.
 //
-// One CTA per (head, sequence); each warp takes every fourth key with its own
-// online softmax (running maximum, sum and output), joined in shared memory.
+// A cached value is half a byte, so at HBM speed an SM has to take in over 40
+// values a cycle: unpacking, not multiplying, is what could bound this
+// kernel.  It is built to spend few instructions per packed word of 8:
+//
+//   * codes go to the tensor core (mma.sync m16n8k16) as they are.  A masked
+//     nibble in the low bits of a half is the fp16 number c * 2^-24 (a
+//     subnormal; 16 c * 2^-24 for the upper nibble, whose factor the other
+//     operand carries), so a word of 8 codes becomes 4 operand registers with
+//     one shift and four ANDs.  Stored codes are c + 8: the 8 is taken out
+//     through the accumulator (K: it starts at -8 sum(q); V: one more product
+//     against a constant operand sums the weights).
+//   * scales stay out of the unpacking.  The 8 columns of the product that a
+//     single query leaves idle are the groups: column n holds the query's
+//     channels of group n and zeros (K), or the weights times group n's scale
+//     (V).  So S[key] = sum_n s[key, n] C[key, n], one multiply per 16
+//     values, and out[channel] is C[channel, its own group].
+//   * both products keep fp32's accuracy: q and the weights enter as two fp16
+//     halves (hi + lo, 22 bits; a 16-bit q needs one), scaled by powers of two
+//     into fp16's range -- q by its own maximum, the weights by the largest V
+//     scale so far, which is tracked like the softmax maximum.
+//   * a lane fetches exactly the bytes that it consumes (its fragment of the
+//     tile) with asynchronous copies into its own slots of a 4-deep ring, so
+//     the ring needs no block-wide barrier; only a tile's 16 K scales rows and
+//     its visibility mask are read across the warp.
+//
+// One warp works on tiles of 16 keys; the 8 warps of a CTA take turns over a
+// sequence's tiles, and a cluster of 1 to 8 CTAs splits a long sequence.  The
+// partial softmaxes meet in shared memory, across the cluster through
+// distributed shared memory: one launch, no scratch.
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 #include "kernels.h"
 #include "kv4.cuh"
 
+namespace cg = cooperative_groups;
+
 namespace b2pa {
 
-template <typename T, int D>
-__global__ void __launch_bounds__(128) kv4_decode_kernel(AttnArgs a, float qscale) {
-  constexpr int E = D / 32;  // channels per lane
-  __shared__ float sm_m[4], sm_l[4], sm_acc[4][D];
+namespace {
+
+constexpr int kStages = 4;
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Asynchronous copy of N bytes (4, 8 or 16) to shared memory; zeros when !ok.
+template <int N>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool ok) {
+  const int n = ok ? N : 0;
+  if constexpr (N == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(n) : "memory");
+}
+
+__device__ __forceinline__ float warp_redux_max(float x) {
+  float y;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+
+// x as hi + lo fp16 halves, for a pair.
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  hi = half2_bits(h);
+  lo = half2_bits(__floats2half2_rn(x - f.x, y - f.y));
+}
+
+template <int D>
+struct Tile {
+  static constexpr int NG = D / 16;          // groups per row
+  static constexpr int SETS = D == 256 ? 2 : 1;  // column sets of 8 groups
+  static constexpr int KW = D / 32;          // K words per lane and row (rows g and g + 8)
+  static constexpr int VW = D / 64;          // V words per lane and key (keys 4t .. 4t+3)
+  static constexpr int KB = KW * 4 < 16 ? KW * 4 : 16;  // bytes per K copy
+  static constexpr int KC = KW * 4 / KB;     // K copies per row
+  static constexpr int VB = VW * 4;          // bytes per V copy
+  static constexpr int OFF_V = 2 * KC * KB * 32;
+  static constexpr int OFF_KS = OFF_V + 4 * VB * 32;
+  static constexpr int OFF_VS = OFF_KS + 16 * NG;
+  static constexpr int OFF_MASK = OFF_VS + 128 * SETS;
+  static constexpr int BYTES = OFF_MASK + 16;
+  static constexpr int WARPS = D == 256 ? 4 : 8;
+  // first channel of K word w of lane t; its 8 channels lie in one group
+  __device__ static constexpr int k_channel(int w, int t) {
+    return D == 64 ? 16 * t + 8 * w : (w >> 2) * 128 + 32 * t + 8 * (w & 3);
+  }
+};
+
+template <int D>
+struct Smem {
+  float acc[Tile<D>::WARPS][D];
+  float m[Tile<D>::WARPS], l[Tile<D>::WARPS];
+  float cta_acc[D];
+  float cta_m, cta_l;
+};
+
+struct DecodeKv4Params {
+  const void* q;
+  int64_t sq_b, sq_h;
+  const uint8_t* k_pool;
+  const uint8_t* v_pool;
+  int64_t num_blocks;
+  const int32_t* page_table;
+  int64_t pt_stride;
+  int max_pages;
+  const int32_t* seq_lens;
+  const int32_t* cur_lens;
+  void* out;
+  int64_t so_b, so_h;
+  int H;
+  float qscale;  // scale * log2(e)
+  int32_t* status;
+};
+
+}  // namespace
+
+template <typename T, int D, int BS>
+__global__ void __launch_bounds__(Tile<D>::WARPS * 32, 2) kv4_decode_kernel(DecodeKv4Params p) {
+  using C = Tile<D>;
+  constexpr bool QLO = std::is_same<T, float>::value && D != 64;  // D = 64 keeps q's low halves in columns 4..7
+  constexpr int PAGE = kv4_page_bytes(BS, D), CODES = BS * (D / 2);
+  extern __shared__ __align__(16) uint8_t ring_all[];
+  __shared__ Smem<D> sm;
+  const int ns = gridDim.x, rank = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  uint8_t* ring = ring_all + warp * (kStages * C::BYTES);
+  const uint32_t ring_at = smem_u32(ring);
+
   pdl_wait();
   pdl_launch_dependents();
-  const int h = blockIdx.x, b = blockIdx.y;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int BS = a.block_size;
-  int64_t L = a.seq_lens[b];
-  const int64_t cap = (int64_t)a.max_pages * BS;
-  if (L > cap) {
-    if (threadIdx.x == 0) set_status(a.status, B2PA_ERR_BAD_BLOCK_ID);
-    L = cap;
-  }
-  int64_t vis = (int64_t)a.seq_lens[b] - a.cur_lens[b] + 1;
-  vis = vis < L ? vis : L;
-  const T* q = static_cast<const T*>(a.q) + (int64_t)b * a.sq[0] + (int64_t)h * a.sq[1] + lane * E;
-  float x[E], acc[E];
+  const int64_t len = p.seq_lens[b], cap = (int64_t)p.max_pages * BS;
+  int64_t vis = len - p.cur_lens[b] + 1;
+  vis = vis < len ? vis : len;
+  vis = vis < cap ? vis : cap;
+  vis = vis > 0 ? vis : 0;
+  if (len > cap && rank == 0 && h == 0 && tid == 0) set_status(p.status, B2PA_ERR_BAD_BLOCK_ID);
+  const int tiles = (int)((vis + 15) / 16);
+  const int per = (tiles + ns - 1) / ns;  // tiles of this CTA: [first, end)
+  const int first = rank * per < tiles ? rank * per : tiles;
+  const int end = first + per < tiles ? first + per : tiles;
+  const int mine = end > first + warp ? (end - first - warp + C::WARPS - 1) / C::WARPS : 0;
+
+  const int32_t* table = p.page_table + (int64_t)b * p.pt_stride;
+  // block ids of this warp's next 32 tiles, one per lane (two for 8-row pages)
+  int id0 = -1, id1 = -1;
+  auto load_ids = [&](int i0) {
+    const int64_t pos = (int64_t)(first + warp + C::WARPS * (i0 + lane)) * 16;
+    id0 = id1 = -1;
+    if (i0 + lane < mine) {
+      id0 = table[pos / BS];
+      if (BS == 8 && pos + 8 < vis) id1 = table[pos / BS + 1];
+      if (id0 >= p.num_blocks || id1 >= p.num_blocks) set_status(p.status, B2PA_ERR_BAD_BLOCK_ID);
+      if (id0 >= p.num_blocks) id0 = -1;
+      if (id1 >= p.num_blocks) id1 = -1;
+    }
+  };
+  // Starts the copies of this warp's i-th tile.
+  auto fetch = [&](int i) {
+    if (i < mine) {
+      if ((i & 31) == 0) load_ids(i);
+      const int b0 = __shfl_sync(kFullMask, id0, i & 31);
+      const int b1 = BS == 8 ? __shfl_sync(kFullMask, id1, i & 31) : b0;
+      const int64_t pos = (int64_t)(first + warp + C::WARPS * i) * 16;
+      const int row0 = (int)(pos % BS);
+      const uint32_t at = ring_at + (i % kStages) * C::BYTES;
+      const bool ok0 = b0 >= 0, ok1 = b1 >= 0;
+      const int64_t page0 = ((int64_t)(ok0 ? b0 : 0) * p.H + h) * PAGE, page1 = ((int64_t)(ok1 ? b1 : 0) * p.H + h) * PAGE;
+      const uint8_t* k0 = p.k_pool + page0;
+      const uint8_t* k1 = p.k_pool + page1;
+      const int r1 = BS == 8 ? g : row0 + g + 8;  // row of key g + 8 in its page
 #pragma unroll
-  for (int i = 0; i < E; ++i) {
-    x[i] = to_f32(q[i]) * qscale;
-    acc[i] = 0.f;
+      for (int c = 0; c < C::KC; ++c) {
+        const int off = (c * 4 + t) * C::KB;
+        copy_async<C::KB>(at + ((2 * c) * 32 + lane) * C::KB, k0 + (row0 + g) * (D / 2) + off, ok0);
+        copy_async<C::KB>(at + ((2 * c + 1) * 32 + lane) * C::KB, k1 + r1 * (D / 2) + off, ok1);
+      }
+      const bool vok = t < 2 ? ok0 : ok1;
+      const uint8_t* v = p.v_pool + (t < 2 ? page0 : page1);
+      const int vr = BS == 8 ? 4 * (t & 1) : row0 + 4 * t;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        copy_async<C::VB>(at + C::OFF_V + (k * 32 + lane) * C::VB, v + (vr + k) * (D / 2) + g * C::VB, vok);
+      // K scales of the tile's 16 rows, linear: 4-byte pieces
+#pragma unroll
+      for (int s = 0; s < 16 * C::NG / 4; s += 32) {
+        const int piece = s + lane;
+        if (piece < 16 * C::NG / 4) {
+          const int key = piece * 4 / C::NG;
+          const bool up = BS == 8 && key >= 8;
+          copy_async<4>(at + C::OFF_KS + piece * 4,
+                        (up ? k1 : k0) + CODES + (BS == 8 ? (key & 7) : row0 + key) * C::NG + piece * 4 % C::NG,
+                        up ? ok1 : ok0);
+        }
+      }
+      // V scales of keys 4t .. 4t+3 for this lane's column's group(s)
+#pragma unroll
+      for (int s = 0; s < C::SETS; ++s) {
+        const int group = C::SETS == 2 ? 2 * g + s : (D == 64 ? (g & 3) : g);
+        copy_async<4>(at + C::OFF_VS + (s * 32 + lane) * 4, v + CODES + group * BS + vr, vok);
+      }
+      if (lane == 0) {
+        const int64_t left = vis - pos;
+        uint32_t mask = left >= 16 ? 0xffffu : (1u << left) - 1u;
+        if (!ok0) mask &= BS == 8 ? 0xff00u : 0u;
+        if (BS == 8 && !ok1) mask &= 0x00ffu;
+        *reinterpret_cast<uint32_t*>(ring + (i % kStages) * C::BYTES + C::OFF_MASK) = mask;
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) fetch(i);
+
+  // q into the K product's column operand: q scaled by 2^e into fp16's range
+  // (its largest magnitude near 2^13), exact for 16-bit q, hi + lo for fp32.
+  uint32_t qh[C::KW][4], ql[QLO ? C::KW : 1][4];
+  float init[C::SETS][2];  // -8 sum(q) of columns 2t, 2t+1, in the product's units
+  float unit, down_q;      // logit (log2) = product * unit * 2^-e (two factors: neither overflows)
+  {
+    const T* q = static_cast<const T*>(p.q) + (int64_t)b * p.sq_b + (int64_t)h * p.sq_h;
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) top = fmaxf(top, fabsf(to_f32(q[lane + 32 * i])));
+    top = warp_redux_max(top);
+    // 2^e by exponent arithmetic; 0, tiny, infinite and NaN maxima keep a finite factor
+    int e = 140 - (int)(__float_as_uint(top) >> 23);  // top's exponent field + e = 13 + 127
+    e = e > 100 ? 100 : e;
+    const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+    unit = p.qscale * 0x1p24f;
+    down_q = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+    for (int w = 0; w < C::KW; ++w) {
+      const int ch = C::k_channel(w, t), group = ch / 16;
+      const bool hi_col = D == 64 ? g == group : g == (group & 7);
+      const bool lo_col = D == 64 && g == group + 4;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {  // operand register r: channels ch + r and ch + r + 4
+        const float f = (r & 1) ? up * 0.0625f : up;
+        uint32_t hi = 0, lo = 0;
+        if (hi_col || lo_col) split2(to_f32(q[ch + r]) * f, to_f32(q[ch + r + 4]) * f, hi, lo);
+        qh[w][r] = hi_col ? hi : (lo_col ? lo : 0u);
+        if constexpr (QLO) ql[w][r] = hi_col ? lo : 0u;
+      }
+    }
+    // 8 sum(q) of a column: every lane sums its operand registers (undoing the
+    // 1/16), lanes of one column (same g) add up, then columns 2t and 2t+1.
+#pragma unroll
+    for (int s = 0; s < C::SETS; ++s) {
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < C::KW; ++w) {
+        if (C::SETS == 2 && (w >> 2) != s) continue;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&qh[w][r]));
+          float y = x.x + x.y;
+          if constexpr (QLO) {
+            const float2 z = __half22float2(*reinterpret_cast<const __half2*>(&ql[w][r]));
+            y += z.x + z.y;
+          }
+          sum += (r & 1) ? y * 16.f : y;
+        }
+      }
+      sum += __shfl_xor_sync(kFullMask, sum, 1);
+      sum += __shfl_xor_sync(kFullMask, sum, 2);
+      sum *= -8.f * 0x1p-24f;
+      init[s][0] = __shfl_sync(kFullMask, sum, 8 * t);
+      init[s][1] = __shfl_sync(kFullMask, sum, 8 * t + 4);
+    }
   }
+
+  float acc[C::VW][4][4];              // [word][nibble][fragment]: channels 8 * word + nibble (+ 4)
+  float eights[C::SETS][4];            // 8 * sum of the weight operand, per column
+#pragma unroll
+  for (int u = 0; u < C::VW; ++u)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[u][j][k] = 0.f;
+#pragma unroll
+  for (int s = 0; s < C::SETS; ++s)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) eights[s][k] = 0.f;
   float m = -INFINITY, l = 0.f;
-  const int page_bytes = kv4_page_bytes(BS, D);
-  for (int64_t j = warp; j < vis; j += 4) {
-    const int32_t blk = a.page_table[(int64_t)b * a.pt_stride + j / BS];
-    if (blk < 0 || blk >= a.num_blocks) {
-      if (lane == 0 && blk >= a.num_blocks) set_status(a.status, B2PA_ERR_BAD_BLOCK_ID);
-      continue;
-    }
-    const int row = (int)(j % BS);
-    const uint8_t* kp = static_cast<const uint8_t*>(a.k_pool) + ((int64_t)blk * a.H + h) * page_bytes;
-    const uint8_t* vp = static_cast<const uint8_t*>(a.v_pool) + ((int64_t)blk * a.H + h) * page_bytes;
-    const int codes = BS * (D / 2), g = lane * E / 16;
-    const float ks = kv4_scale(kp[codes + row * (D / 16) + g]);
-    const float vs = kv4_scale(vp[codes + g * BS + row]);
-    float dot = 0.f, v[E];
+  uint32_t top_e = 0;  // largest V scale exponent so far; weights are scaled by 2^(29 - top_e)
+
+  auto rescale = [&](float f) {
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const int c = lane * E + i, sh = 4 * (c & 1);
-      dot += x[i] * (float)((int)(kp[row * (D / 2) + c / 2] >> sh & 15) - 8) * ks;
-      v[i] = (float)((int)(vp[row * (D / 2) + c / 2] >> sh & 15) - 8) * vs;
-    }
-    dot = warp_sum(dot);
-    const float mn = fmaxf(m, dot);
-    // a logit of -inf (an infinite query) leaves nothing to subtract
-    const float ref = mn == -INFINITY ? 0.f : mn;
-    const float corr = fast_exp2(m - ref), p = fast_exp2(dot - ref);
-    m = mn;
-    l = l * corr + p;
+    for (int u = 0; u < C::VW; ++u)
 #pragma unroll
-    for (int i = 0; i < E; ++i) acc[i] = acc[i] * corr + p * v[i];
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[u][j][k] *= f;
+#pragma unroll
+    for (int s = 0; s < C::SETS; ++s)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) eights[s][k] *= f;
+  };
+
+  for (int i = 0; i < mine; ++i) {
+    fetch(i + kStages - 1);
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+    __syncwarp();
+    const uint8_t* st = ring + (i % kStages) * C::BYTES;
+    const uint32_t mask = *reinterpret_cast<const uint32_t*>(st + C::OFF_MASK);
+
+    // ---- S = K . q per group column
+    float s[C::SETS][4];
+#pragma unroll
+    for (int x = 0; x < C::SETS; ++x) {
+      s[x][0] = s[x][2] = init[x][0];
+      s[x][1] = s[x][3] = init[x][1];
+    }
+    uint32_t ka[C::KW], kb[C::KW];  // rows g and g + 8
+#pragma unroll
+    for (int c = 0; c < C::KC; ++c) {
+      if constexpr (C::KB == 16) {
+        *reinterpret_cast<uint4*>(&ka[4 * c]) = *reinterpret_cast<const uint4*>(st + ((2 * c) * 32 + lane) * 16);
+        *reinterpret_cast<uint4*>(&kb[4 * c]) = *reinterpret_cast<const uint4*>(st + ((2 * c + 1) * 32 + lane) * 16);
+      } else {
+        *reinterpret_cast<uint2*>(&ka[0]) = *reinterpret_cast<const uint2*>(st + lane * 8);
+        *reinterpret_cast<uint2*>(&kb[0]) = *reinterpret_cast<const uint2*>(st + (32 + lane) * 8);
+      }
+    }
+#pragma unroll
+    for (int w = 0; w < C::KW; ++w) {
+      constexpr uint32_t LO = 0x000f000fu, HI = 0x00f000f0u;
+      float(&c)[4] = s[C::SETS == 2 ? w >> 2 : 0];
+      const uint32_t x = ka[w], y = kb[w], x8 = x >> 8, y8 = y >> 8;
+      mma_f16(c, x & LO, y & LO, x & HI, y & HI, qh[w][0], qh[w][1]);
+      if constexpr (QLO) mma_f16(c, x & LO, y & LO, x & HI, y & HI, ql[w][0], ql[w][1]);
+      mma_f16(c, x8 & LO, y8 & LO, x8 & HI, y8 & HI, qh[w][2], qh[w][3]);
+      if constexpr (QLO) mma_f16(c, x8 & LO, y8 & LO, x8 & HI, y8 & HI, ql[w][2], ql[w][3]);
+    }
+    // ---- scales: this lane's columns are groups 2t, 2t+1 (of each set)
+    float z0 = 0.f, z1 = 0.f;  // logits of keys g, g + 8
+#pragma unroll
+    for (int x = 0; x < C::SETS; ++x) {
+      const int col = D == 64 ? 2 * (t & 1) : 8 * x + 2 * t;
+      const uint32_t w0 = *reinterpret_cast<const uint16_t*>(st + C::OFF_KS + g * C::NG + col);
+      const uint32_t w1 = *reinterpret_cast<const uint16_t*>(st + C::OFF_KS + (g + 8) * C::NG + col);
+      const float2 s0 = __half22float2(__halves2half2(__ushort_as_half((unsigned short)((w0 & 255u) << 7)),
+                                                      __ushort_as_half((unsigned short)((w0 >> 8) << 7))));
+      const float2 s1 = __half22float2(__halves2half2(__ushort_as_half((unsigned short)((w1 & 255u) << 7)),
+                                                      __ushort_as_half((unsigned short)((w1 >> 8) << 7))));
+      z0 = fmaf(s[x][0], s0.x, fmaf(s[x][1], s0.y, z0));
+      z1 = fmaf(s[x][2], s1.x, fmaf(s[x][3], s1.y, z1));
+    }
+    z0 += __shfl_xor_sync(kFullMask, z0, 1);
+    z1 += __shfl_xor_sync(kFullMask, z1, 1);
+    z0 += __shfl_xor_sync(kFullMask, z0, 2);
+    z1 += __shfl_xor_sync(kFullMask, z1, 2);
+    z0 = z0 * unit * down_q;
+    z1 = z1 * unit * down_q;
+    uint32_t vs[C::SETS];
+#pragma unroll
+    for (int x = 0; x < C::SETS; ++x) vs[x] = *reinterpret_cast<const uint32_t*>(st + C::OFF_VS + (x * 32 + lane) * 4);
+    if (mask != 0xffffu) {
+      if (mask == 0) {
+        __syncwarp();
+        continue;
+      }
+      if (!(mask >> g & 1u)) z0 = -INFINITY;
+      if (!(mask >> (g + 8) & 1u)) z1 = -INFINITY;
+      // an unseen key's scale may be anything, NaN included: zero
+      const uint32_t four = mask >> (4 * t) & 15u;
+      const uint32_t keep = (four & 1u) * 0xffu | (four >> 1 & 1u) * 0xff00u | (four >> 2 & 1u) * 0xff0000u |
+                            (four >> 3 & 1u) * 0xff000000u;
+#pragma unroll
+      for (int x = 0; x < C::SETS; ++x) vs[x] &= keep;
+    }
+    // ---- running maximum, weights
+    const float tile_top = warp_redux_max(fmaxf(z0, z1));
+    if (tile_top > m) {
+      const float f = fast_exp2(m - tile_top);  // 0 for the first tile
+      m = tile_top;
+      l *= f;
+      rescale(f);
+    }
+    const float ref = m == -INFINITY ? 0.f : m;
+    const float p0 = fast_exp2(z0 - ref), p1 = fast_exp2(z1 - ref);
+    l += p0 + p1;
+    // ---- largest V scale, as its exponent field
+    uint32_t big = 0;
+#pragma unroll
+    for (int x = 0; x < C::SETS; ++x) big = __vmaxu2(big, __vmaxu2(vs[x] & 0x00ff00ffu, vs[x] >> 8 & 0x00ff00ffu));
+    big = big > (big >> 16 | big << 16) ? big >> 16 : big & 0xffffu;  // larger half
+    big = __reduce_max_sync(kFullMask, big);
+    if (big > kKv4MaxScale) {  // a NaN group: its column is lost, the others keep their range
+      big = 0;
+#pragma unroll
+      for (int x = 0; x < C::SETS; ++x)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t c = vs[x] >> (8 * k) & 255u;
+          big = c <= kKv4MaxScale && c > big ? c : big;
+        }
+      big = __reduce_max_sync(kFullMask, big);
+    }
+    if ((big >> 3) > top_e) {
+      rescale(__uint_as_float((127u - ((big >> 3) - top_e)) << 23));
+      top_e = big >> 3;
+    }
+    const float up = __uint_as_float((127u + 29u - top_e) << 23);
+    // ---- weights of keys 4t .. 4t+3 (lane 4 * (key & 7) holds key and key + 8)
+    const float both = t < 2 ? p0 : p1;
+    float pk[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) pk[k] = __shfl_sync(kFullMask, both, 4 * ((4 * t + k) & 7) + (t < 2 ? 0 : 2)) * up;
+    uint32_t bh[C::SETS][2], bl[C::SETS][2];
+#pragma unroll
+    for (int x = 0; x < C::SETS; ++x) {
+      float w[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[k] = pk[k] * kv4_scale(vs[x] >> (8 * k) & 255u);
+      split2(w[0], w[1], bh[x][0], bl[x][0]);
+      split2(w[2], w[3], bh[x][1], bl[x][1]);
+      if (D == 64 && g >= 4) {  // columns 4..7: the low halves of groups 0..3
+        bh[x][0] = bl[x][0];
+        bh[x][1] = bl[x][1];
+      }
+      constexpr uint32_t EIGHT = 0x00080008u;
+      mma_f16(eights[x], EIGHT, EIGHT, EIGHT, EIGHT, bh[x][0], bh[x][1]);
+      if constexpr (D != 64) mma_f16(eights[x], EIGHT, EIGHT, EIGHT, EIGHT, bl[x][0], bl[x][1]);
+    }
+    // ---- out += V^T . weights
+    uint32_t v[4][C::VW];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint8_t* at = st + C::OFF_V + (k * 32 + lane) * C::VB;
+      if constexpr (C::VW == 1) v[k][0] = *reinterpret_cast<const uint32_t*>(at);
+      if constexpr (C::VW == 2) *reinterpret_cast<uint2*>(&v[k][0]) = *reinterpret_cast<const uint2*>(at);
+      if constexpr (C::VW == 4) *reinterpret_cast<uint4*>(&v[k][0]) = *reinterpret_cast<const uint4*>(at);
+    }
+#pragma unroll
+    for (int u = 0; u < C::VW; ++u) {
+      constexpr uint32_t LO = 0x000f000fu, HI = 0x00f000f0u;
+      const int x = C::SETS == 2 ? u >> 1 : 0;
+      uint32_t c01 = __byte_perm(v[0][u], v[1][u], 0x5410), d01 = __byte_perm(v[0][u], v[1][u], 0x7632);
+      uint32_t c23 = __byte_perm(v[2][u], v[3][u], 0x5410), d23 = __byte_perm(v[2][u], v[3][u], 0x7632);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t mk = (j & 1) ? HI : LO;
+        mma_f16(acc[u][j], c01 & mk, d01 & mk, c23 & mk, d23 & mk, bh[x][0], bh[x][1]);
+        if constexpr (D != 64) mma_f16(acc[u][j], c01 & mk, d01 & mk, c23 & mk, d23 & mk, bl[x][0], bl[x][1]);
+        if (j == 1) c01 >>= 8, d01 >>= 8, c23 >>= 8, d23 >>= 8;
+      }
+    }
+    __syncwarp();  // every lane is done with the stage before it is refilled
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+
+  // ---- this warp's sums: channel c sits in the column of its group
+  l += __shfl_xor_sync(kFullMask, l, 4);
+  l += __shfl_xor_sync(kFullMask, l, 8);
+  l += __shfl_xor_sync(kFullMask, l, 16);
   if (lane == 0) {
-    sm_m[warp] = m;
-    sm_l[warp] = l;
+    sm.m[warp] = m;
+    sm.l[warp] = l;
   }
+  {
+    const float down = __uint_as_float((127u + top_e - 29u + 24u) << 23);
+    const int col = D == 64 ? g >> 1 : g;  // this lane's rows' group, as a column
 #pragma unroll
-  for (int i = 0; i < E; ++i) sm_acc[warp][lane * E + i] = acc[i];
+    for (int u = 0; u < C::VW; ++u)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int x = C::SETS == 2 ? u >> 1 : 0;
+        float lo = (col & 1) ? acc[u][j][1] : acc[u][j][0], hi = (col & 1) ? acc[u][j][3] : acc[u][j][2];
+        const float e = (col & 1) ? eights[x][1] : eights[x][0];
+        if (j & 1) lo *= 0.0625f, hi *= 0.0625f;
+        lo = (lo - e) * down;
+        hi = (hi - e) * down;
+        if (D == 64) {  // the low halves' columns are two lanes further
+          lo += __shfl_xor_sync(kFullMask, lo, 2);
+          hi += __shfl_xor_sync(kFullMask, hi, 2);
+        }
+        if (t == (col >> 1)) {
+          const int ch = g * (D / 8) + 8 * u + j;
+          sm.acc[warp][ch] = lo;
+          sm.acc[warp][ch + 4] = hi;
+        }
+      }
+  }
   __syncthreads();
+  // ---- the CTA's, then the cluster's
   float M = -INFINITY;
-  for (int w = 0; w < 4; ++w) M = fmaxf(M, sm_m[w]);
-  if (M == -INFINITY) M = 0.f;
+#pragma unroll
+  for (int w = 0; w < C::WARPS; ++w) M = fmaxf(M, sm.m[w]);
+  float ref = M == -INFINITY ? 0.f : M;
   float total = 0.f;
-  for (int w = 0; w < 4; ++w) total += sm_l[w] * fast_exp2(sm_m[w] - M);
-  T* out = static_cast<T*>(a.out) + (int64_t)b * a.so[0] + (int64_t)h * a.so[1];
-  for (int d = threadIdx.x; d < D; d += blockDim.x) {
-    float o = 0.f;
-    for (int w = 0; w < 4; ++w) o += sm_acc[w][d] * fast_exp2(sm_m[w] - M);
-    out[d] = from_f32<T>(total != 0.f ? o / total : 0.f);
+#pragma unroll
+  for (int w = 0; w < C::WARPS; ++w) total += sm.l[w] * fast_exp2(sm.m[w] - ref);
+  constexpr int PER = (D + C::WARPS * 32 - 1) / (C::WARPS * 32);
+  float o[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int d = tid + i * C::WARPS * 32;
+    o[i] = 0.f;
+    if (d < D) {
+#pragma unroll
+      for (int w = 0; w < C::WARPS; ++w)
+        if (sm.m[w] != -INFINITY || sm.l[w] != 0.f) o[i] += sm.acc[w][d] * fast_exp2(sm.m[w] - ref);
+    }
+  }
+  if (ns > 1) {
+    cg::cluster_group cluster = cg::this_cluster();
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int d = tid + i * C::WARPS * 32;
+      if (d < D) sm.cta_acc[d] = o[i];
+    }
+    if (tid == 0) {
+      sm.cta_m = M;
+      sm.cta_l = total;
+    }
+    cluster.sync();
+    if (rank == 0) {
+      const int used = per > 0 ? (tiles + per - 1) / per : 0;
+      M = -INFINITY;
+      for (int r = 0; r < used; ++r) M = fmaxf(M, *cluster.map_shared_rank(&sm.cta_m, r));
+      ref = M == -INFINITY ? 0.f : M;
+      total = 0.f;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) o[i] = 0.f;
+      for (int r = 0; r < used; ++r) {
+        const float f = fast_exp2(*cluster.map_shared_rank(&sm.cta_m, r) - ref);
+        total += *cluster.map_shared_rank(&sm.cta_l, r) * f;
+        const float* a = cluster.map_shared_rank(&sm.cta_acc[0], r);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const int d = tid + i * C::WARPS * 32;
+          if (d < D) o[i] += a[d] * f;
+        }
+      }
+    }
+    cluster.sync();  // no CTA leaves while its sums are being read
+    if (rank != 0) return;
+  }
+  T* out = static_cast<T*>(p.out) + (int64_t)b * p.so_b + (int64_t)h * p.so_h;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int d = tid + i * C::WARPS * 32;
+    if (d < D) out[d] = from_f32<T>(total != 0.f ? o[i] / total : 0.f);
+  }
+}
+
+template <typename T, int D, int BS>
+static int decode_launch(const AttnArgs& a, cudaStream_t s) {
+  using C = Tile<D>;
+  DecodeKv4Params p;
+  p.q = a.q;
+  p.sq_b = a.sq[0];
+  p.sq_h = a.sq[1];
+  p.k_pool = static_cast<const uint8_t*>(a.k_pool);
+  p.v_pool = static_cast<const uint8_t*>(a.v_pool);
+  p.num_blocks = a.num_blocks;
+  p.page_table = a.page_table;
+  p.pt_stride = a.pt_stride;
+  p.max_pages = a.max_pages;
+  p.seq_lens = a.seq_lens;
+  p.cur_lens = a.cur_lens;
+  p.out = a.out;
+  p.so_b = a.so[0];
+  p.so_h = a.so[1];
+  p.H = a.H;
+  p.qscale = a.scale * kLog2e;
+  p.status = a.status;
+  // CTAs per sequence and head: enough to fill the device twice over, while a
+  // warp of each keeps at least two tiles of the longest sequence.
+  const int64_t pairs = (int64_t)a.B * a.H;
+  const int64_t longest = ((int64_t)a.max_pages * BS + 15) / 16;
+  int ns = 1;
+  while (ns < 8 && pairs * ns < 4 * device_sm_count() && longest >= 2 * C::WARPS * ns * 2) ns *= 2;
+  constexpr int smem = C::WARPS * kStages * C::BYTES;
+  auto kern = kv4_decode_kernel<T, D, BS>;
+  const int rc = set_max_dynamic_smem_cached(reinterpret_cast<const void*>(kern), smem);
+  if (rc != B2PA_OK) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ns, (unsigned)a.H, (unsigned)a.B);
+  cfg.blockDim = dim3(C::WARPS * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)ns;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
+  if (e != cudaSuccess) return set_error(B2PA_ERR_CUDA, "paged_decode_kv4 launch: %s", cudaGetErrorString(e));
+  return B2PA_OK;
+}
+
+template <typename T, int D>
+static int decode_blocks(const AttnArgs& a, cudaStream_t s) {
+  switch (a.block_size) {
+    case 8: return decode_launch<T, D, 8>(a, s);
+    case 16: return decode_launch<T, D, 16>(a, s);
+    default: return decode_launch<T, D, 32>(a, s);
   }
 }
 
 template <typename T>
 static int decode_as(const AttnArgs& a, cudaStream_t s) {
-  const dim3 grid((unsigned)a.H, (unsigned)a.B);
-  const float qscale = a.scale * kLog2e;
-  cudaError_t e;
   switch (a.D) {
-    case 64: e = launch_pdl(kv4_decode_kernel<T, 64>, grid, dim3(128), 0, s, a, qscale); break;
-    case 128: e = launch_pdl(kv4_decode_kernel<T, 128>, grid, dim3(128), 0, s, a, qscale); break;
-    default: e = launch_pdl(kv4_decode_kernel<T, 256>, grid, dim3(128), 0, s, a, qscale); break;
+    case 64: return decode_blocks<T, 64>(a, s);
+    case 128: return decode_blocks<T, 128>(a, s);
+    default: return decode_blocks<T, 256>(a, s);
   }
-  if (e != cudaSuccess) return set_error(B2PA_ERR_CUDA, "paged_decode_kv4 launch: %s", cudaGetErrorString(e));
-  return B2PA_OK;
 }
 
 size_t kv4_decode_workspace(int, int, int, int, int) { return 0; }
