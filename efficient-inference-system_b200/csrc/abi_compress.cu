@@ -293,6 +293,7 @@ int b2pa_key_weights(const void* q, const int64_t q_strides[4], const void* k_po
   a.block_size = block_size;
   a.dtype = dtype;
   a.pool_dtype = pool_dtype;
+  a.bs_log2 = block_size_log2(block_size);
   a.scale = scale;
   a.workspace = workspace;
   a.status = status;
@@ -341,6 +342,7 @@ int b2pa_evict(void* k_pool, void* v_pool, int pool_dtype, float* weights, int64
   a.D = D;
   a.block_size = block_size;
   a.dtype = pool_dtype;
+  a.bs_log2 = block_size_log2(block_size);
   a.elem = dtype_size(pool_dtype);
   a.status = status;
   return launch_evict(a, static_cast<cudaStream_t>(stream));

@@ -71,9 +71,9 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(EvictArgs 
 
   const int32_t* row = a.page_table + (int64_t)b * a.pt_stride;
   auto key_of = [&](int j) -> uint32_t {
-    const int32_t blk = row[j / a.block_size];
+    const int32_t blk = row[j >> a.bs_log2];
     if (blk < 0 || blk >= a.num_blocks) return 0;  // reported by the move
-    return weight_key(a.weights[((int64_t)blk * a.H + h) * a.block_size + j % a.block_size]);
+    return weight_key(a.weights[((int64_t)blk * a.H + h) * a.block_size + (j & (a.block_size - 1))]);
   };
   if (cached) {
     for (int j = tid; j < cand; j += kSelectThreads) keys[j] = key_of(j);
@@ -164,7 +164,7 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, const Slice& sl, i
     return reinterpret_cast<W*>(sl.pool + ((int64_t)blk * a.H + h) * sl.page_bytes + sl.offset + slot * sl.row_stride +
                                 c * sl.word_stride);
   };
-  const int bs = a.block_size;
+  const int bs = a.block_size, sh = a.bs_log2;
   const int64_t total = (int64_t)s.k * sl.words;
   for (int64_t base = 0; base < total; base += kMoveThreads * kMoveVecs) {
     W v[kMoveVecs];
@@ -176,10 +176,10 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, const Slice& sl, i
       if (e < total) {
         const int r = (int)(e / sl.words), c = (int)(e - (int64_t)r * sl.words);
         const int j = kept[r];
-        const int32_t blk = src_row[j / bs];
+        const int32_t blk = src_row[j >> sh];
         ok[u] = blk >= 0 && blk < a.num_blocks;
         if (ok[u])
-          v[u] = *at(blk, j % bs, c);
+          v[u] = *at(blk, j & (bs - 1), c);
         else
           set_status(a.status, B2PA_ERR_BAD_BLOCK_ID);
       }
@@ -190,9 +190,9 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, const Slice& sl, i
       const int64_t e = base + u * kMoveThreads + threadIdx.x;
       if (ok[u]) {
         const int r = (int)(e / sl.words), c = (int)(e - (int64_t)r * sl.words);
-        const int32_t blk = dst_row[r / bs];
+        const int32_t blk = dst_row[r >> sh];
         if (blk >= 0 && blk < a.num_blocks)
-          *at(blk, r % bs, c) = v[u];
+          *at(blk, r & (bs - 1), c) = v[u];
         else
           set_status(a.status, B2PA_ERR_BAD_BLOCK_ID);
       }
@@ -202,8 +202,8 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, const Slice& sl, i
   const int behind = (s.k + bs - 1) / bs * bs - s.k;
   for (int e = threadIdx.x; e < behind * sl.words; e += kMoveThreads) {
     const int r = s.k + e / sl.words, c = e % sl.words;
-    const int32_t blk = dst_row[r / bs];
-    if (blk >= 0 && blk < a.num_blocks) *at(blk, r % bs, c) = W{};
+    const int32_t blk = dst_row[r >> sh];
+    if (blk >= 0 && blk < a.num_blocks) *at(blk, r & (bs - 1), c) = W{};
   }
 }
 

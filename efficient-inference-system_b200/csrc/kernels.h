@@ -190,9 +190,9 @@ struct KeyWeightArgs {
   float* w_out;
   int window;  // 0: every query counts
   int B, H, T, D, block_size, dtype, pool_dtype;
+  int bs_log2;  // block_size is a power of two
   float scale;
   void* workspace;
-  float* lse;
   int32_t* status;
 };
 
@@ -210,7 +210,8 @@ struct EvictArgs {
   int keep, recent;
   int32_t* kept;
   int B, H, D, block_size, dtype;
-  int elem;  // bytes per element of a plain pool
+  int bs_log2;  // block_size is a power of two
+  int elem;     // bytes per element of a plain pool
   int32_t* status;
 };
 
@@ -238,5 +239,6 @@ inline int dtype_size(int dtype) {
 
 inline bool head_dim_supported(int D) { return D == 16 || D == 32 || D == 64 || D == 128 || D == 256; }
 inline bool block_size_supported(int bs) { return bs == 8 || bs == 16 || bs == 32; }
+inline int block_size_log2(int bs) { return bs == 8 ? 3 : bs == 16 ? 4 : 5; }
 
 }  // namespace b2pa

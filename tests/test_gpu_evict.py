@@ -73,6 +73,33 @@ def test_key_weights_small_heads(cuda_device, dtype, D):
                       dtype=dtype, kv4=False, window=0, seed=D)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kv4", [False, True])
+@pytest.mark.parametrize("T", [1, 40])
+def test_key_weights_precision(cuda_device, dtype, kv4, T):
+    """Even rows (unit normal): the bound on a weight is a few 2^-12, so a product with one rounded half would show."""
+    rng = np.random.default_rng(12)
+    H, D, bs, n = 2, 64, 16, 200
+    NB = -(-n // bs)
+    k = rng.standard_normal((NB, H, bs, D))
+    if kv4:
+        pool, k = torch.from_numpy(co.pack_pages(k, False)).to(cuda_device), co.stored(k)
+    else:
+        pool = torch.from_numpy(k).to(dtype).to(cuda_device)
+        k = _np(pool)
+    q = torch.from_numpy(rng.standard_normal((1, H, T, D))).to(dtype).to(cuda_device)
+    w = torch.zeros(NB, H, bs, device=cuda_device)
+    dev = cuda_device
+    b2pa.accumulate_key_weights(q, pool, w, _i32(np.arange(NB)[None], dev), _i32([n], dev), _i32([T], dev))
+    p, size = co.softmax_rows(_np(q)[0], co.rows_of(k, range(NB), n), T, D ** -0.5)
+    assert size < 20
+    got = co.rows_of(_np(w)[..., None], range(NB), n)[..., 0].T
+    want = p.sum(1)
+    assert (np.abs(got - want) <= want * (co.weight_error(D, size, n) + (T + 2) * 2.0 ** -23) + 2.0 ** -30).all()
+    # as a whole the roundings are independent: a tenth of their bound
+    assert np.linalg.norm(got - want) <= 0.1 * co.weight_error(D, size, n) * np.linalg.norm(want)
+
+
 @pytest.mark.parametrize("T", [1, 4])
 def test_key_weights_nothing_counts(cuda_device, T):
     """Empty sequences, no counted query, and queries that see nothing."""
