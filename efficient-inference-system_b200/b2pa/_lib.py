@@ -61,9 +61,8 @@ SIGNATURES: dict[str, tuple] = {
                              _I, _I, _I, _I, _I, _I, _VP, _VP]),
     "b2pa_kv4_read": (_I, [_VP, _VP, _I64, _VP, _I64, _I, _VP, _VP, _VP, _I64P, _VP, _I64P,
                            _I, _I, _I, _I, _I, _I, _VP, _VP]),
-    "b2pa_paged_decode_kv4_workspace_size": (ctypes.c_size_t, [_I, _I, _I, _I, _I]),
     "b2pa_paged_decode_kv4": (_I, [_VP, _I64P, _VP, _VP, _I64, _VP, _I64, _I, _VP, _VP, _VP, _I64P,
-                                   _I, _I, _I, _I, ctypes.c_float, _I, _VP, ctypes.c_size_t, _VP, _VP]),
+                                   _I, _I, _I, _I, ctypes.c_float, _I, _VP, _VP]),
     "b2pa_paged_prefill_kv4_workspace_size": (ctypes.c_size_t, [_I, _I, _I, _I, _I, _I, _I]),
     "b2pa_paged_prefill_kv4": (_I, [_VP, _I64P, _VP, _VP, _I64, _VP, _I64, _I, _VP, _VP, _VP, _I64P,
                                     _I, _I, _I, _I, _I, ctypes.c_float, _I, _VP, ctypes.c_size_t, _VP, _VP]),
@@ -166,18 +165,6 @@ def workspace(device: torch.device, nbytes: int) -> torch.Tensor:
         buf = torch.empty(size, dtype=torch.uint8, device=torch.device("cuda", idx))
         _workspaces[key] = buf
     return buf
-
-
-def call_workspace(device: torch.device, nbytes: int) -> torch.Tensor | None:
-    """Scratch for one call on the current stream: the cached buffer, or --
-    while the stream is being captured -- a buffer from the graph's own
-    memory, so that captured graphs neither share scratch nor lose it when
-    the cached buffer is replaced by a larger one."""
-    if not nbytes:
-        return None
-    if torch.cuda.is_current_stream_capturing():
-        return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    return workspace(device, nbytes)
 
 
 def read_status(device: torch.device) -> int:

@@ -20,7 +20,8 @@ import math
 import torch
 
 from . import _lib
-from .kv4 import aligned_rows, check_heads, int32_rows, need_cuda, on_device, pool_shape, table_args
+from .kv4 import (aligned_rows, check_heads, int32_rows, need_cuda, on_device, pool_shape, status_at, stream_at,
+                  strides_of, table_args, workspace_of)
 
 PLAIN_HEAD_DIMS = (16, 32, 64, 128, 256)
 
@@ -29,22 +30,21 @@ def _pool_args(what: str, k_pool, v_pool, head_dim: int | None):
     """(blocks, H, block_size, D, type code) of a plain or 4-bit pool."""
     if k_pool.dim() != 4:
         raise ValueError(f"b2pa.{what}: k_pool must be a 4-d pool, not {tuple(k_pool.shape)}")
-    pools = {"k_pool": k_pool} if v_pool is None else {"k_pool": k_pool, "v_pool": v_pool}
-    if k_pool.dtype == torch.uint8:
+    if k_pool.dtype is torch.uint8:
         D = k_pool.shape[3] * 16 // 9 if head_dim is None else head_dim
-        return (*pool_shape(what, D, **pools), D, _lib.DTYPE_KV4)
+        return (*pool_shape(what, D, k_pool, v_pool), D, _lib.DTYPE_KV4)
     code = _lib.dtype_code(k_pool.dtype)
     D = k_pool.shape[3]
-    for name, t in pools.items():
-        if t.dtype != k_pool.dtype or t.shape != k_pool.shape or not t.is_contiguous():
-            raise ValueError(f"b2pa.{what}: {name} must be contiguous [blocks, H, block_size, D] of one type and shape")
+    for t in (k_pool,) if v_pool is None else (k_pool, v_pool):
+        if t.dtype is not k_pool.dtype or t.shape != k_pool.shape or not t.is_contiguous():
+            raise ValueError(f"b2pa.{what}: pools must be contiguous [blocks, H, block_size, D] of one type and shape")
     if D not in PLAIN_HEAD_DIMS or (head_dim is not None and head_dim != D):
         raise ValueError(f"b2pa.{what}: head_dim {head_dim or D} does not fit k_pool of shape {tuple(k_pool.shape)}")
     return k_pool.shape[0], k_pool.shape[1], k_pool.shape[2], D, code
 
 
 def _check_weights(what: str, name: str, w: torch.Tensor, shape: tuple) -> None:
-    if w.dtype != torch.float32 or tuple(w.shape) != shape or not w.is_contiguous():
+    if w.dtype is not torch.float32 or w.shape != shape or not w.is_contiguous():
         raise ValueError(f"b2pa.{what}: {name} must be a contiguous float32 tensor of shape {shape}")
 
 
@@ -83,19 +83,20 @@ def launch_key_weights(q, k_pool, pool_code: int, key_weights, out, table, pt_st
                        window: int | None, ws: torch.Tensor | None = None) -> None:
     """b2pa_key_weights on checked arguments."""
     B, H, T, D = q.shape
-    dev = q.device
+    dev = q.get_device()
     code = _lib.dtype_code(q.dtype)
-    lib = _lib.load()
+    bs = k_pool.shape[2]
     with on_device(dev):
-        nbytes = lib.b2pa_key_weights_workspace_size(B, H, T, D, pages, k_pool.shape[2], code, pool_code)
         if ws is None:
-            ws = _lib.call_workspace(dev, nbytes)
-        rc = lib.b2pa_key_weights(
-            q.data_ptr(), _lib.strides4(q), k_pool.data_ptr(), pool_code, k_pool.shape[0], table.data_ptr(), pt_stride,
+            at, nbytes, ws = workspace_of(dev, "b2pa_key_weights_workspace_size", B, H, T, D, pages, bs, code, pool_code)
+        else:
+            at, nbytes = ws.data_ptr(), ws.numel()
+        rc = _lib.load().b2pa_key_weights(
+            q.data_ptr(), strides_of(q), k_pool.data_ptr(), pool_code, k_pool.shape[0], table.data_ptr(), pt_stride,
             pages, seq_lens.data_ptr(), cur.data_ptr(), window or 0, key_weights.data_ptr(), out.data_ptr(), B, H, T, D,
-            k_pool.shape[2], 1.0 / math.sqrt(D), code, ws.data_ptr() if ws is not None else None,
-            ws.numel() if ws is not None else 0, _lib.status_buffer(dev).data_ptr(), _lib.stream_handle(dev))
-    _lib.check(rc, "b2pa_key_weights")
+            bs, 1.0 / math.sqrt(D), code, at, nbytes, status_at(dev), stream_at(dev))
+    if rc:
+        _lib.check(rc, "b2pa_key_weights")
 
 
 def evict_by_weight(k_pool: torch.Tensor, v_pool: torch.Tensor, key_weights: torch.Tensor, page_table: torch.Tensor,
@@ -108,7 +109,7 @@ def evict_by_weight(k_pool: torch.Tensor, v_pool: torch.Tensor, key_weights: tor
     zeroed; pages behind it are left to the caller.  Returns the kept positions, int32 [B, H, keep], -1 behind k."""
     what = "evict_by_weight"
     dev = need_cuda(what, k_pool=k_pool, v_pool=v_pool, key_weights=key_weights, page_table=page_table,
-                    seq_lens=seq_lens, **({} if out_table is None else {"out_table": out_table}))
+                    seq_lens=seq_lens, out_table=page_table if out_table is None else out_table)
     blocks, H, bs, D, pool_code = _pool_args(what, k_pool, v_pool, None)
     _check_weights(what, "key_weights", key_weights, (blocks, H, bs))
     if keep < 1 or recent < 0:
@@ -121,14 +122,14 @@ def evict_by_weight(k_pool: torch.Tensor, v_pool: torch.Tensor, key_weights: tor
         out_table, out_stride, out_pages = table_args(what, "out_table", out_table, B)
         if out_pages * bs < keep:
             raise ValueError(f"b2pa.{what}: out_table has {out_pages} pages a row, {-(-keep // bs)} needed")
-    kept = torch.empty(B, H, keep, dtype=torch.int32, device=dev)
+    kept = torch.empty(B, H, keep, dtype=torch.int32, device=k_pool.device)
     with on_device(dev):
         rc = _lib.load().b2pa_evict(
             k_pool.data_ptr(), v_pool.data_ptr(), pool_code, key_weights.data_ptr(), blocks, table.data_ptr(),
             pt_stride, pages, out_table.data_ptr() if out_table is not None else None, out_stride,
-            seq_lens.data_ptr(), keep, recent, kept.data_ptr(), B, H, D, bs, _lib.status_buffer(dev).data_ptr(),
-            _lib.stream_handle(dev))
-    _lib.check(rc, "b2pa_evict")
+            seq_lens.data_ptr(), keep, recent, kept.data_ptr(), B, H, D, bs, status_at(dev), stream_at(dev))
+    if rc:
+        _lib.check(rc, "b2pa_evict")
     return kept
 
 
@@ -181,7 +182,7 @@ def evict_batch(cache, keep: int, recent: int = 0) -> torch.Tensor:
     if getattr(pool, "_b2pa_pending", None) is not None:
         flush_pending(pool)
     dev = pool.k_blocks.device
-    with on_device(dev):
+    with on_device(dev.index):
         note_released_rows(cache, dev)
         table, seq_lens, pages = block_table_and_lengths(cache, dev, transient=True)
         kept = evict_by_weight(pool.k_blocks, pool.v_blocks, pool.key_weights, table[:, :pages], seq_lens, keep, recent)

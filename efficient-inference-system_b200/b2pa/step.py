@@ -135,10 +135,7 @@ class SharedStepMetadata:
         code = _lib.dtype_code(dtype)
 
         def need_of(b: int) -> int:
-            if kv4:
-                n = lib.b2pa_paged_decode_kv4_workspace_size(b, H, D, self.width, block_size)
-            else:
-                n = lib.b2pa_paged_decode_workspace_size(b, H, D, self.width, block_size, code)
+            n = 0 if kv4 else lib.b2pa_paged_decode_workspace_size(b, H, D, self.width, block_size, code)
             if weights:
                 n = max(n, lib.b2pa_key_weights_workspace_size(b, H, 1, D, self.width, block_size, code,
                                                                _lib.DTYPE_KV4 if kv4 else code))
@@ -293,7 +290,7 @@ class DecodeStep:
         table = m.table.view(m.capacity, m.width)[: self.B]
         starts, ones, lens = (t[: self.B] for t in (m.start_pos, m.ones, m.seq_lens))
         kv4_append(pend.k_new, pend.v_new, pool.k_blocks, pool.v_blocks, table, starts, ones, m.seq_out[: self.B])
-        return _attend("paged_attention_decode_kv4", q, pool.k_blocks, pool.v_blocks, table, lens, ones, ws=m.workspace)
+        return _attend("paged_attention_decode_kv4", q, pool.k_blocks, pool.v_blocks, table, lens, ones)
 
     def _attend_plain(self, q: torch.Tensor, pool, pend: _StepPending) -> torch.Tensor:
         kb, vb = pool.k_blocks, pool.v_blocks

@@ -196,23 +196,16 @@ int b2pa_kv4_read(const void* k_pool, const void* v_pool, int64_t num_blocks, co
   return launch_kv4_read(a, static_cast<cudaStream_t>(stream));
 }
 
-size_t b2pa_paged_decode_kv4_workspace_size(int B, int H, int D, int max_pages, int block_size) {
-  if (B <= 0 || H <= 0 || D <= 0 || max_pages < 0 || block_size <= 0) return 0;
-  return kv4_decode_workspace(B, H, D, max_pages, block_size);
-}
-
 int b2pa_paged_decode_kv4(const void* q, const int64_t q_strides[4], const void* k_pool, const void* v_pool,
                           int64_t num_blocks, const int32_t* page_table, int64_t pt_stride, int max_pages,
                           const int32_t* seq_lens, const int32_t* cur_lens, void* out, const int64_t out_strides[4],
-                          int B, int H, int D, int block_size, float scale, int dtype, void* workspace,
-                          size_t workspace_bytes, int32_t* status, void* stream) {
+                          int B, int H, int D, int block_size, float scale, int dtype, int32_t* status,
+                          void* stream) {
   const char* fn = "paged_decode_kv4";
   AttnArgs a{};
   B2PA_TRY(attention_args(fn, a, q, q_strides, k_pool, v_pool, num_blocks, page_table, pt_stride, max_pages, seq_lens,
-                          cur_lens, out, out_strides, B, H, 1, D, block_size, scale, dtype, workspace, workspace_bytes,
-                          status));
+                          cur_lens, out, out_strides, B, H, 1, D, block_size, scale, dtype, nullptr, 0, status));
   if (B == 0) return B2PA_OK;
-  B2PA_TRY(check_workspace(fn, workspace, workspace_bytes, kv4_decode_workspace(B, H, D, max_pages, block_size)));
   return launch_kv4_decode(a, static_cast<cudaStream_t>(stream));
 }
 

@@ -218,7 +218,6 @@ struct EvictArgs {
 int launch_kv4_append(const AppendArgs& a, int64_t* seq_lens_out, cudaStream_t s);
 int launch_kv4_read(const Kv4ReadArgs& a, cudaStream_t s);
 
-size_t kv4_decode_workspace(int B, int H, int D, int max_pages, int block_size);
 int launch_kv4_decode(const AttnArgs& a, cudaStream_t s);
 
 struct Kv4PrefillPlan {

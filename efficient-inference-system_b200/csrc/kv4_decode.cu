@@ -630,8 +630,6 @@ static int decode_as(const AttnArgs& a, cudaStream_t s) {
   }
 }
 
-size_t kv4_decode_workspace(int, int, int, int, int) { return 0; }
-
 int launch_kv4_decode(const AttnArgs& a, cudaStream_t s) {
   switch (a.dtype) {
     case B2PA_DTYPE_F32: return decode_as<float>(a, s);

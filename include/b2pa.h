@@ -391,17 +391,14 @@ B2PA_API int b2pa_kv4_read(const void* k_pool, const void* v_pool, int64_t num_b
 
 /*
  * Single-query paged attention over a 4-bit cache: b2pa_paged_decode with
- * 4-bit pools.  q / out rows 16-byte aligned.  Workspace as reported by the
- * size function with the device current that will run the call.
+ * 4-bit pools.  q / out rows 16-byte aligned.  Needs no workspace.
  */
-B2PA_API size_t b2pa_paged_decode_kv4_workspace_size(int B, int H, int D, int max_pages, int block_size);
 B2PA_API int b2pa_paged_decode_kv4(const void* q, const int64_t q_strides[4],
                       const void* k_pool, const void* v_pool, int64_t num_blocks,
                       const int32_t* page_table, int64_t pt_stride, int max_pages,
                       const int32_t* seq_lens, const int32_t* cur_lens,
                       void* out, const int64_t out_strides[4],
                       int B, int H, int D, int block_size, float scale, int dtype,
-                      void* workspace, size_t workspace_bytes,
                       int32_t* status, void* stream);
 
 /*

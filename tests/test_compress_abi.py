@@ -49,7 +49,7 @@ def _decode(lib, **kw):
     a = {**BASE, **kw}
     return lib.b2pa_paged_decode_kv4(a["q"], _i64(a["qs"]), a["kp"], a["vp"], a["nb"], a["pt"], a["pts"], a["mp"],
                                      a["sl"], a["cl"], a["out"], _i64(a["os"]), a["B"], a["H"], a["D"], a["bs"], 0.125,
-                                     a["dt"], a["ws"], a["wsb"], None, None)
+                                     a["dt"], None, None)
 
 
 def _prefill(lib, **kw):
