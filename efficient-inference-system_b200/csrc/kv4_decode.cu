@@ -51,20 +51,20 @@ constexpr int kStages = 4;
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Asynchronous copy of N bytes (4, 8 or 16) to shared memory; zeros when !ok.
-template <int N>
-__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool ok) {
-  const int n = ok ? N : 0;
+// Asynchronous copy of N bytes (4, 8 or 16) to shared memory, both addresses
+// with a constant offset.
+template <int N, int DST, int SRC>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
   if constexpr (N == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+    asm volatile("cp.async.cg.shared.global [%0+%2], [%1+%3], 16;" ::"r"(dst), "l"(src), "n"(DST), "n"(SRC) : "memory");
   else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(n) : "memory");
+    asm volatile("cp.async.ca.shared.global [%0+%2], [%1+%3], %4;" ::"r"(dst), "l"(src), "n"(DST), "n"(SRC), "n"(N)
+                 : "memory");
 }
 
 __device__ __forceinline__ float warp_redux_max(float x) {
@@ -136,6 +136,10 @@ template <typename T, int D, int BS>
 __global__ void __launch_bounds__(Tile<D>::WARPS * 32, 2) kv4_decode_kernel(DecodeKv4Params p) {
   using C = Tile<D>;
   constexpr bool QLO = std::is_same<T, float>::value && D != 64;  // D = 64 keeps q's low halves in columns 4..7
+  // The weights' low halves, likewise.  16-bit outputs do without: a weight
+  // rounded to 11 bits is off by 2^-12, half a step of fp16 and a sixteenth of
+  // bf16's, and the roundings of different keys are independent.
+  constexpr bool PLO = QLO;
   constexpr int PAGE = kv4_page_bytes(BS, D), CODES = BS * (D / 2);
   extern __shared__ __align__(16) uint8_t ring_all[];
   __shared__ Smem<D> sm;
@@ -159,69 +163,83 @@ __global__ void __launch_bounds__(Tile<D>::WARPS * 32, 2) kv4_decode_kernel(Deco
   const int mine = end > first + warp ? (end - first - warp + C::WARPS - 1) / C::WARPS : 0;
 
   const int32_t* table = p.page_table + (int64_t)b * p.pt_stride;
+  const int nvis = (int)vis;
+  const int tile0 = first + warp;  // this warp's tiles: tile0 + i * WARPS
   // block ids of this warp's next 32 tiles, one per lane (two for 8-row pages)
   int id0 = -1, id1 = -1;
   auto load_ids = [&](int i0) {
-    const int64_t pos = (int64_t)(first + warp + C::WARPS * (i0 + lane)) * 16;
+    const int pos = (tile0 + C::WARPS * (i0 + lane)) * 16;
     id0 = id1 = -1;
     if (i0 + lane < mine) {
       id0 = table[pos / BS];
-      if (BS == 8 && pos + 8 < vis) id1 = table[pos / BS + 1];
+      if (BS == 8 && pos + 8 < nvis) id1 = table[pos / BS + 1];
       if (id0 >= p.num_blocks || id1 >= p.num_blocks) set_status(p.status, B2PA_ERR_BAD_BLOCK_ID);
       if (id0 >= p.num_blocks) id0 = -1;
       if (id1 >= p.num_blocks) id1 = -1;
     }
   };
-  // Starts the copies of this warp's i-th tile.
+  // Where this lane's pieces lie in block 0 (a warp's tiles start at the same
+  // row of their pages: WARPS is even) and in stage 0; every other address is
+  // one multiply-add away.
+  const int row0 = BS == 32 ? 16 * (tile0 & 1) : 0;
+  const int64_t block_bytes = (int64_t)p.H * PAGE;
+  const int vrow = BS == 8 ? 4 * (t & 1) : row0 + 4 * t;
+  const int kpiece = 4 * lane % (16 * C::NG);  // K scales: 16 rows, linear
+  const int krow = kpiece / C::NG;
+  const uint8_t* const k_at = p.k_pool + (int64_t)h * PAGE + (row0 + g) * (D / 2) + t * C::KB;
+  const uint8_t* const v_at = p.v_pool + (int64_t)h * PAGE + vrow * (D / 2) + g * C::VB;
+  const uint8_t* const ks_at =
+      p.k_pool + (int64_t)h * PAGE + CODES + (BS == 8 ? krow & 7 : row0 + krow) * C::NG + kpiece % C::NG;
+  const uint8_t* const vs_at =
+      p.v_pool + (int64_t)h * PAGE + CODES + (C::SETS == 2 ? 2 * g : D == 64 ? (g & 3) : g) * BS + vrow;
+  const uint32_t k_to = ring_at + lane * C::KB, v_to = ring_at + C::OFF_V + lane * C::VB,
+                 s_to = ring_at + C::OFF_KS + lane * 4;
+  // Starts the copies of this warp's i-th tile.  A page that is not there is
+  // not copied: the mask hides whatever its stage holds.
   auto fetch = [&](int i) {
     if (i < mine) {
       if ((i & 31) == 0) load_ids(i);
       const int b0 = __shfl_sync(kFullMask, id0, i & 31);
       const int b1 = BS == 8 ? __shfl_sync(kFullMask, id1, i & 31) : b0;
-      const int64_t pos = (int64_t)(first + warp + C::WARPS * i) * 16;
-      const int row0 = (int)(pos % BS);
-      const uint32_t at = ring_at + (i % kStages) * C::BYTES;
-      const bool ok0 = b0 >= 0, ok1 = b1 >= 0;
-      const int64_t page0 = ((int64_t)(ok0 ? b0 : 0) * p.H + h) * PAGE, page1 = ((int64_t)(ok1 ? b1 : 0) * p.H + h) * PAGE;
-      const uint8_t* k0 = p.k_pool + page0;
-      const uint8_t* k1 = p.k_pool + page1;
-      const int r1 = BS == 8 ? g : row0 + g + 8;  // row of key g + 8 in its page
-#pragma unroll
-      for (int c = 0; c < C::KC; ++c) {
-        const int off = (c * 4 + t) * C::KB;
-        copy_async<C::KB>(at + ((2 * c) * 32 + lane) * C::KB, k0 + (row0 + g) * (D / 2) + off, ok0);
-        copy_async<C::KB>(at + ((2 * c + 1) * 32 + lane) * C::KB, k1 + r1 * (D / 2) + off, ok1);
-      }
-      const bool vok = t < 2 ? ok0 : ok1;
-      const uint8_t* v = p.v_pool + (t < 2 ? page0 : page1);
-      const int vr = BS == 8 ? 4 * (t & 1) : row0 + 4 * t;
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        copy_async<C::VB>(at + C::OFF_V + (k * 32 + lane) * C::VB, v + (vr + k) * (D / 2) + g * C::VB, vok);
-      // K scales of the tile's 16 rows, linear: 4-byte pieces
-#pragma unroll
-      for (int s = 0; s < 16 * C::NG / 4; s += 32) {
-        const int piece = s + lane;
-        if (piece < 16 * C::NG / 4) {
-          const int key = piece * 4 / C::NG;
-          const bool up = BS == 8 && key >= 8;
-          copy_async<4>(at + C::OFF_KS + piece * 4,
-                        (up ? k1 : k0) + CODES + (BS == 8 ? (key & 7) : row0 + key) * C::NG + piece * 4 % C::NG,
-                        up ? ok1 : ok0);
+      const uint32_t st = (i % kStages) * C::BYTES;
+      const int bv = BS == 8 && t >= 2 ? b1 : b0;
+      const int bk = BS == 8 && krow >= 8 ? b1 : b0;  // (D = 256: pieces 32.. are of the second page)
+      if (b0 >= 0) {
+        const uint8_t* k = k_at + b0 * block_bytes;
+        copy_async<C::KB, 0, 0>(k_to + st, k);
+        if constexpr (C::KC == 2) copy_async<C::KB, 64 * C::KB, 4 * C::KB>(k_to + st, k);
+        if constexpr (BS != 8) {
+          copy_async<C::KB, 32 * C::KB, 8 * (D / 2)>(k_to + st, k);
+          if constexpr (C::KC == 2) copy_async<C::KB, 96 * C::KB, 8 * (D / 2) + 4 * C::KB>(k_to + st, k);
         }
       }
-      // V scales of keys 4t .. 4t+3 for this lane's column's group(s)
-#pragma unroll
-      for (int s = 0; s < C::SETS; ++s) {
-        const int group = C::SETS == 2 ? 2 * g + s : (D == 64 ? (g & 3) : g);
-        copy_async<4>(at + C::OFF_VS + (s * 32 + lane) * 4, v + CODES + group * BS + vr, vok);
+      if (BS == 8 && b1 >= 0) {
+        const uint8_t* k = k_at + b1 * block_bytes;
+        copy_async<C::KB, 32 * C::KB, 0>(k_to + st, k);
+        if constexpr (C::KC == 2) copy_async<C::KB, 96 * C::KB, 4 * C::KB>(k_to + st, k);
+      }
+      if (bv >= 0) {
+        const uint8_t* v = v_at + bv * block_bytes;
+        copy_async<C::VB, 0, 0>(v_to + st, v);
+        copy_async<C::VB, 32 * C::VB, D / 2>(v_to + st, v);
+        copy_async<C::VB, 64 * C::VB, 2 * (D / 2)>(v_to + st, v);
+        copy_async<C::VB, 96 * C::VB, 3 * (D / 2)>(v_to + st, v);
+        const uint8_t* vs = vs_at + bv * block_bytes;
+        copy_async<4, C::OFF_VS - C::OFF_KS, 0>(s_to + st, vs);
+        if constexpr (C::SETS == 2) copy_async<4, C::OFF_VS - C::OFF_KS + 128, BS>(s_to + st, vs);
+      }
+      if constexpr (D == 256) {  // two pieces per lane, 8 rows apart
+        if (b0 >= 0) copy_async<4, 0, 0>(s_to + st, ks_at + b0 * block_bytes);
+        if (b1 >= 0) copy_async<4, 128, BS == 8 ? 0 : 8 * C::NG>(s_to + st, ks_at + b1 * block_bytes);
+      } else if (bk >= 0 && (D == 128 || lane < 16)) {
+        copy_async<4, 0, 0>(s_to + st, ks_at + bk * block_bytes);
       }
       if (lane == 0) {
-        const int64_t left = vis - pos;
+        const int left = nvis - (tile0 + C::WARPS * i) * 16;
         uint32_t mask = left >= 16 ? 0xffffu : (1u << left) - 1u;
-        if (!ok0) mask &= BS == 8 ? 0xff00u : 0u;
-        if (BS == 8 && !ok1) mask &= 0x00ffu;
-        *reinterpret_cast<uint32_t*>(ring + (i % kStages) * C::BYTES + C::OFF_MASK) = mask;
+        if (b0 < 0) mask &= BS == 8 ? 0xff00u : 0u;
+        if (BS == 8 && b1 < 0) mask &= 0x00ffu;
+        *reinterpret_cast<uint32_t*>(ring + st + C::OFF_MASK) = mask;
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -398,26 +416,26 @@ __global__ void __launch_bounds__(Tile<D>::WARPS * 32, 2) kv4_decode_kernel(Deco
     const float ref = m == -INFINITY ? 0.f : m;
     const float p0 = fast_exp2(z0 - ref), p1 = fast_exp2(z1 - ref);
     l += p0 + p1;
-    // ---- largest V scale, as its exponent field
-    uint32_t big = 0;
+    // ---- a V scale above the largest exponent so far?
+    uint32_t big = 0;  // larger of two bytes, in halves
 #pragma unroll
     for (int x = 0; x < C::SETS; ++x) big = __vmaxu2(big, __vmaxu2(vs[x] & 0x00ff00ffu, vs[x] >> 8 & 0x00ff00ffu));
-    big = big > (big >> 16 | big << 16) ? big >> 16 : big & 0xffffu;  // larger half
-    big = __reduce_max_sync(kFullMask, big);
-    if (big > kKv4MaxScale) {  // a NaN group: its column is lost, the others keep their range
-      big = 0;
+    // a byte of at least 8 (top_e + 1) carries into bit 8
+    if (__any_sync(kFullMask, (big + (0x100u - 8u * (top_e + 1u)) * 0x10001u) & 0x01000100u)) {
+      uint32_t top = 0;
 #pragma unroll
       for (int x = 0; x < C::SETS; ++x)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const uint32_t c = vs[x] >> (8 * k) & 255u;
-          big = c <= kKv4MaxScale && c > big ? c : big;
+          // not a NaN group's: its column is lost, the others keep their range
+          top = c <= kKv4MaxScale && c > top ? c : top;
         }
-      big = __reduce_max_sync(kFullMask, big);
-    }
-    if ((big >> 3) > top_e) {
-      rescale(__uint_as_float((127u - ((big >> 3) - top_e)) << 23));
-      top_e = big >> 3;
+      top = __reduce_max_sync(kFullMask, top) >> 3;
+      if (top > top_e) {
+        rescale(__uint_as_float((127u - (top - top_e)) << 23));
+        top_e = top;
+      }
     }
     const float up = __uint_as_float((127u + 29u - top_e) << 23);
     // ---- weights of keys 4t .. 4t+3 (lane 4 * (key & 7) holds key and key + 8)
@@ -439,7 +457,7 @@ __global__ void __launch_bounds__(Tile<D>::WARPS * 32, 2) kv4_decode_kernel(Deco
       }
       constexpr uint32_t EIGHT = 0x00080008u;
       mma_f16(eights[x], EIGHT, EIGHT, EIGHT, EIGHT, bh[x][0], bh[x][1]);
-      if constexpr (D != 64) mma_f16(eights[x], EIGHT, EIGHT, EIGHT, EIGHT, bl[x][0], bl[x][1]);
+      if constexpr (PLO) mma_f16(eights[x], EIGHT, EIGHT, EIGHT, EIGHT, bl[x][0], bl[x][1]);
     }
     // ---- out += V^T . weights
     uint32_t v[4][C::VW];
@@ -460,7 +478,7 @@ __global__ void __launch_bounds__(Tile<D>::WARPS * 32, 2) kv4_decode_kernel(Deco
       for (int j = 0; j < 4; ++j) {
         const uint32_t mk = (j & 1) ? HI : LO;
         mma_f16(acc[u][j], c01 & mk, d01 & mk, c23 & mk, d23 & mk, bh[x][0], bh[x][1]);
-        if constexpr (D != 64) mma_f16(acc[u][j], c01 & mk, d01 & mk, c23 & mk, d23 & mk, bl[x][0], bl[x][1]);
+        if constexpr (PLO) mma_f16(acc[u][j], c01 & mk, d01 & mk, c23 & mk, d23 & mk, bl[x][0], bl[x][1]);
         if (j == 1) c01 >>= 8, d01 >>= 8, c23 >>= 8, d23 >>= 8;
       }
     }
