@@ -47,7 +47,7 @@ namespace b2pa {
 
 namespace {
 
-constexpr int kStages = 4;
+constexpr int kStages = 2;
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
@@ -83,7 +83,7 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
   lo = half2_bits(__floats2half2_rn(x - f.x, y - f.y));
 }
 
-template <int D>
+template <int D, int W = 8>
 struct Tile {
   static constexpr int NG = D / 16;          // groups per row
   static constexpr int SETS = D == 256 ? 2 : 1;  // column sets of 8 groups
@@ -95,21 +95,26 @@ struct Tile {
   static constexpr int OFF_V = 2 * KC * KB * 32;
   static constexpr int OFF_KS = OFF_V + 4 * VB * 32;
   static constexpr int OFF_VS = OFF_KS + 16 * NG;
-  static constexpr int OFF_MASK = OFF_VS + 128 * SETS;
-  static constexpr int BYTES = OFF_MASK + 16;
-  static constexpr int WARPS = D == 256 ? 4 : 8;
+  static constexpr int OFF_MASK = OFF_VS + 128 * SETS;  // after the last tile
+  static constexpr int TILE = OFF_MASK;      // bytes of one tile
+  static constexpr int TP = D == 256 ? 1 : 2;  // tiles per step: independent work to hide the products' latency
+  static constexpr int BYTES = TP * TILE + 16;
+  static constexpr int WARPS = W;
   // first channel of K word w of lane t; its 8 channels lie in one group
   __device__ static constexpr int k_channel(int w, int t) {
     return D == 64 ? 16 * t + 8 * w : (w >> 2) * 128 + 32 * t + 8 * (w & 3);
   }
 };
 
-template <int D>
+constexpr int kMaxCluster = 8;
+
+template <int D, int W>
 struct Smem {
-  float acc[Tile<D>::WARPS][D];
-  float m[Tile<D>::WARPS], l[Tile<D>::WARPS];
-  float cta_acc[D];
-  float cta_m, cta_l;
+  float acc[W][D];
+  float m[W], l[W];
+  // rank 0: every CTA's sums
+  float cta_acc[kMaxCluster][D];
+  float cta_m[kMaxCluster], cta_l[kMaxCluster];
 };
 
 struct DecodeKv4Params {
@@ -132,9 +137,9 @@ struct DecodeKv4Params {
 
 }  // namespace
 
-template <typename T, int D, int BS>
-__global__ void __launch_bounds__(Tile<D>::WARPS * 32, 2) kv4_decode_kernel(DecodeKv4Params p) {
-  using C = Tile<D>;
+template <typename T, int D, int BS, int W>
+__global__ void __launch_bounds__(W * 32, D == 256 ? 8 / W : 16 / W) kv4_decode_kernel(DecodeKv4Params p) {
+  using C = Tile<D, W>;
   constexpr bool QLO = std::is_same<T, float>::value && D != 64;  // D = 64 keeps q's low halves in columns 4..7
   // The weights' low halves, likewise.  16-bit outputs do without: a weight
   // rounded to 11 bits is off by 2^-12, half a step of fp16 and a sixteenth of
@@ -142,46 +147,57 @@ __global__ void __launch_bounds__(Tile<D>::WARPS * 32, 2) kv4_decode_kernel(Deco
   constexpr bool PLO = QLO;
   constexpr int PAGE = kv4_page_bytes(BS, D), CODES = BS * (D / 2);
   extern __shared__ __align__(16) uint8_t ring_all[];
-  __shared__ Smem<D> sm;
+  __shared__ Smem<D, W> sm;
   const int ns = gridDim.x, rank = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   uint8_t* ring = ring_all + warp * (kStages * C::BYTES);
   const uint32_t ring_at = smem_u32(ring);
 
+  // The cluster's other CTAs have to be running before their shared memory is
+  // written (at the end): arrive here, wait there.
+  if (ns > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   pdl_wait();
   pdl_launch_dependents();
-  const int64_t len = p.seq_lens[b], cap = (int64_t)p.max_pages * BS;
-  int64_t vis = len - p.cur_lens[b] + 1;
+  // Three loads that do not wait for one another: the lengths, q, and the
+  // first block ids.  Steps go round the cluster's warps, so a warp's first
+  // step does not depend on the length.
+  const int64_t len = p.seq_lens[b], cur = p.cur_lens[b], cap = (int64_t)p.max_pages * BS;
+  uint4 qraw[C::KW][sizeof(T) / 2];  // the channels of this lane's column, 8 per word
+  const T* const q = static_cast<const T*>(p.q) + (int64_t)b * p.sq_b + (int64_t)h * p.sq_h;
+  auto column_of = [&](int w) {  // 1: this lane's column is word w's group, 2: it takes its low halves
+    const int group = C::k_channel(w, t) / 16;
+    return (D == 64 ? g == group : g == (group & 7)) ? 1 : D == 64 && g == group + 4 ? 2 : 0;
+  };
+#pragma unroll
+  for (int w = 0; w < C::KW; ++w)
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+      qraw[w][i] = make_uint4(0, 0, 0, 0);
+      if (column_of(w)) qraw[w][i] = ld_global_nc<uint4>(q + C::k_channel(w, t) + i * (16 / (int)sizeof(T)));
+    }
+  constexpr int KEYS = 16 * C::TP;  // per step
+  const int step0 = rank * C::WARPS + warp, turn = ns * C::WARPS;  // this warp's steps: step0 + i * turn
+  const int32_t* table = p.page_table + (int64_t)b * p.pt_stride;
+  // block ids of this warp's next steps, one per lane: a step has PAGES pages
+  constexpr int PAGES = BS >= KEYS ? 1 : KEYS / BS, AHEAD = 32 / PAGES;
+  auto load_ids = [&](int i0) -> int {
+    const int64_t page = (step0 + (int64_t)turn * (i0 + lane / PAGES)) * KEYS / BS + lane % PAGES;
+    return page < p.max_pages ? table[page] : -1;
+  };
+  int ids = load_ids(0);
+
+  int64_t vis = len - cur + 1;
   vis = vis < len ? vis : len;
   vis = vis < cap ? vis : cap;
   vis = vis > 0 ? vis : 0;
   if (len > cap && rank == 0 && h == 0 && tid == 0) set_status(p.status, B2PA_ERR_BAD_BLOCK_ID);
-  const int tiles = (int)((vis + 15) / 16);
-  const int per = (tiles + ns - 1) / ns;  // tiles of this CTA: [first, end)
-  const int first = rank * per < tiles ? rank * per : tiles;
-  const int end = first + per < tiles ? first + per : tiles;
-  const int mine = end > first + warp ? (end - first - warp + C::WARPS - 1) / C::WARPS : 0;
-
-  const int32_t* table = p.page_table + (int64_t)b * p.pt_stride;
   const int nvis = (int)vis;
-  const int tile0 = first + warp;  // this warp's tiles: tile0 + i * WARPS
-  // block ids of this warp's next 32 tiles, one per lane (two for 8-row pages)
-  int id0 = -1, id1 = -1;
-  auto load_ids = [&](int i0) {
-    const int pos = (tile0 + C::WARPS * (i0 + lane)) * 16;
-    id0 = id1 = -1;
-    if (i0 + lane < mine) {
-      id0 = table[pos / BS];
-      if (BS == 8 && pos + 8 < nvis) id1 = table[pos / BS + 1];
-      if (id0 >= p.num_blocks || id1 >= p.num_blocks) set_status(p.status, B2PA_ERR_BAD_BLOCK_ID);
-      if (id0 >= p.num_blocks) id0 = -1;
-      if (id1 >= p.num_blocks) id1 = -1;
-    }
-  };
-  // Where this lane's pieces lie in block 0 (a warp's tiles start at the same
+  const int steps = (nvis + KEYS - 1) / KEYS;
+  const int mine = steps > step0 ? (steps - step0 + turn - 1) / turn : 0;
+  // Where this lane's pieces lie in block 0 (a warp's steps start at the same
   // row of their pages: WARPS is even) and in stage 0; every other address is
   // one multiply-add away.
-  const int row0 = BS == 32 ? 16 * (tile0 & 1) : 0;
+  const int row0 = BS == 32 && C::TP == 1 ? 16 * (step0 & 1) : 0;
   const int64_t block_bytes = (int64_t)p.H * PAGE;
   const int vrow = BS == 8 ? 4 * (t & 1) : row0 + 4 * t;
   const int kpiece = 4 * lane % (16 * C::NG);  // K scales: 16 rows, linear
@@ -194,53 +210,65 @@ __global__ void __launch_bounds__(Tile<D>::WARPS * 32, 2) kv4_decode_kernel(Deco
       p.v_pool + (int64_t)h * PAGE + CODES + (C::SETS == 2 ? 2 * g : D == 64 ? (g & 3) : g) * BS + vrow;
   const uint32_t k_to = ring_at + lane * C::KB, v_to = ring_at + C::OFF_V + lane * C::VB,
                  s_to = ring_at + C::OFF_KS + lane * 4;
-  // Starts the copies of this warp's i-th tile.  A page that is not there is
+  // Starts the copies of this warp's i-th step.  A page that is not there is
   // not copied: the mask hides whatever its stage holds.
   auto fetch = [&](int i) {
     if (i < mine) {
-      if ((i & 31) == 0) load_ids(i);
-      const int b0 = __shfl_sync(kFullMask, id0, i & 31);
-      const int b1 = BS == 8 ? __shfl_sync(kFullMask, id1, i & 31) : b0;
+      if (i % AHEAD == 0 && i > 0) ids = load_ids(i);
       const uint32_t st = (i % kStages) * C::BYTES;
-      const int bv = BS == 8 && t >= 2 ? b1 : b0;
-      const int bk = BS == 8 && krow >= 8 ? b1 : b0;  // (D = 256: pieces 32.. are of the second page)
-      if (b0 >= 0) {
-        const uint8_t* k = k_at + b0 * block_bytes;
-        copy_async<C::KB, 0, 0>(k_to + st, k);
-        if constexpr (C::KC == 2) copy_async<C::KB, 64 * C::KB, 4 * C::KB>(k_to + st, k);
-        if constexpr (BS != 8) {
-          copy_async<C::KB, 32 * C::KB, 8 * (D / 2)>(k_to + st, k);
-          if constexpr (C::KC == 2) copy_async<C::KB, 96 * C::KB, 8 * (D / 2) + 4 * C::KB>(k_to + st, k);
+      const int left = nvis - (step0 + turn * i) * KEYS;
+      uint32_t mask = left >= 32 ? 0xffffffffu : (1u << left) - 1u;
+#pragma unroll
+      for (int x = 0; x < C::TP; ++x) {
+        constexpr int ROWS = BS == 32 ? 16 : 0;  // rows from one tile to the next within a page
+        // ids past the pool are reported where keys would be seen in them
+        int b0 = __shfl_sync(kFullMask, ids, i % AHEAD * PAGES + (BS == 32 ? 0 : x * (16 / BS)));
+        int b1 = BS == 8 ? __shfl_sync(kFullMask, ids, i % AHEAD * PAGES + 2 * x + 1) : b0;
+        if (left <= 16 * x) b0 = -1;
+        if (left <= 16 * x + (BS == 8 ? 8 : 0)) b1 = -1;
+        if (b0 >= p.num_blocks || b1 >= p.num_blocks) {
+          set_status(p.status, B2PA_ERR_BAD_BLOCK_ID);
+          if (b0 >= p.num_blocks) b0 = -1;
+          if (b1 >= p.num_blocks) b1 = -1;
+        }
+        if (b0 < 0) mask &= ~((BS == 8 ? 0xffu : 0xffffu) << (16 * x));
+        if (BS == 8 && b1 < 0) mask &= ~(0xff00u << (16 * x));
+        const int bv = BS == 8 && t >= 2 ? b1 : b0;
+        const int bk = BS == 8 && krow >= 8 ? b1 : b0;  // (D = 256: pieces 32.. are of the second page)
+        const uint32_t kd = k_to + st + x * C::TILE, vd = v_to + st + x * C::TILE, sd = s_to + st + x * C::TILE;
+        if (b0 >= 0) {
+          const uint8_t* k = k_at + b0 * block_bytes + x * ROWS * (D / 2);
+          copy_async<C::KB, 0, 0>(kd, k);
+          if constexpr (C::KC == 2) copy_async<C::KB, 64 * C::KB, 4 * C::KB>(kd, k);
+          if constexpr (BS != 8) {
+            copy_async<C::KB, 32 * C::KB, 8 * (D / 2)>(kd, k);
+            if constexpr (C::KC == 2) copy_async<C::KB, 96 * C::KB, 8 * (D / 2) + 4 * C::KB>(kd, k);
+          }
+        }
+        if (BS == 8 && b1 >= 0) {
+          const uint8_t* k = k_at + b1 * block_bytes;
+          copy_async<C::KB, 32 * C::KB, 0>(kd, k);
+          if constexpr (C::KC == 2) copy_async<C::KB, 96 * C::KB, 4 * C::KB>(kd, k);
+        }
+        if (bv >= 0) {
+          const uint8_t* v = v_at + bv * block_bytes + x * ROWS * (D / 2);
+          copy_async<C::VB, 0, 0>(vd, v);
+          copy_async<C::VB, 32 * C::VB, D / 2>(vd, v);
+          copy_async<C::VB, 64 * C::VB, 2 * (D / 2)>(vd, v);
+          copy_async<C::VB, 96 * C::VB, 3 * (D / 2)>(vd, v);
+          const uint8_t* vs = vs_at + bv * block_bytes + x * ROWS;
+          copy_async<4, C::OFF_VS - C::OFF_KS, 0>(sd, vs);
+          if constexpr (C::SETS == 2) copy_async<4, C::OFF_VS - C::OFF_KS + 128, BS>(sd, vs);
+        }
+        if constexpr (D == 256) {  // two pieces per lane, 8 rows apart
+          if (b0 >= 0) copy_async<4, 0, 0>(sd, ks_at + b0 * block_bytes);
+          if (b1 >= 0) copy_async<4, 128, BS == 8 ? 0 : 8 * C::NG>(sd, ks_at + b1 * block_bytes);
+        } else if (bk >= 0 && (D == 128 || lane < 16)) {
+          copy_async<4, 0, 0>(sd, ks_at + bk * block_bytes + x * ROWS * C::NG);
         }
       }
-      if (BS == 8 && b1 >= 0) {
-        const uint8_t* k = k_at + b1 * block_bytes;
-        copy_async<C::KB, 32 * C::KB, 0>(k_to + st, k);
-        if constexpr (C::KC == 2) copy_async<C::KB, 96 * C::KB, 4 * C::KB>(k_to + st, k);
-      }
-      if (bv >= 0) {
-        const uint8_t* v = v_at + bv * block_bytes;
-        copy_async<C::VB, 0, 0>(v_to + st, v);
-        copy_async<C::VB, 32 * C::VB, D / 2>(v_to + st, v);
-        copy_async<C::VB, 64 * C::VB, 2 * (D / 2)>(v_to + st, v);
-        copy_async<C::VB, 96 * C::VB, 3 * (D / 2)>(v_to + st, v);
-        const uint8_t* vs = vs_at + bv * block_bytes;
-        copy_async<4, C::OFF_VS - C::OFF_KS, 0>(s_to + st, vs);
-        if constexpr (C::SETS == 2) copy_async<4, C::OFF_VS - C::OFF_KS + 128, BS>(s_to + st, vs);
-      }
-      if constexpr (D == 256) {  // two pieces per lane, 8 rows apart
-        if (b0 >= 0) copy_async<4, 0, 0>(s_to + st, ks_at + b0 * block_bytes);
-        if (b1 >= 0) copy_async<4, 128, BS == 8 ? 0 : 8 * C::NG>(s_to + st, ks_at + b1 * block_bytes);
-      } else if (bk >= 0 && (D == 128 || lane < 16)) {
-        copy_async<4, 0, 0>(s_to + st, ks_at + bk * block_bytes);
-      }
-      if (lane == 0) {
-        const int left = nvis - (tile0 + C::WARPS * i) * 16;
-        uint32_t mask = left >= 16 ? 0xffffu : (1u << left) - 1u;
-        if (b0 < 0) mask &= BS == 8 ? 0xff00u : 0u;
-        if (BS == 8 && b1 < 0) mask &= 0x00ffu;
-        *reinterpret_cast<uint32_t*>(ring + st + C::OFF_MASK) = mask;
-      }
+      if (C::TP == 1) mask &= 0xffffu;
+      if (lane == 0) *reinterpret_cast<uint32_t*>(ring + st + C::TP * C::TILE) = mask;
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -253,10 +281,19 @@ __global__ void __launch_bounds__(Tile<D>::WARPS * 32, 2) kv4_decode_kernel(Deco
   float init[C::SETS][2];  // -8 sum(q) of columns 2t, 2t+1, in the product's units
   float unit, down_q;      // logit (log2) = product * unit * 2^-e (two factors: neither overflows)
   {
-    const T* q = static_cast<const T*>(p.q) + (int64_t)b * p.sq_b + (int64_t)h * p.sq_h;
-    float top = 0.f;
+    float x[C::KW][8], top = 0.f;
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) top = fmaxf(top, fabsf(to_f32(q[lane + 32 * i])));
+    for (int w = 0; w < C::KW; ++w) {
+      constexpr int N = 16 / (int)sizeof(T);
+#pragma unroll
+      for (int i = 0; i < 8 / N; ++i) {
+        Vec<T, N> v;
+        v.w = qraw[w][i];
+        v.to_float(&x[w][i * N]);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[w][i]));
+    }
     top = warp_redux_max(top);
     // 2^e by exponent arithmetic; 0, tiny, infinite and NaN maxima keep a finite factor
     int e = 140 - (int)(__float_as_uint(top) >> 23);  // top's exponent field + e = 13 + 127
@@ -266,16 +303,14 @@ __global__ void __launch_bounds__(Tile<D>::WARPS * 32, 2) kv4_decode_kernel(Deco
     down_q = __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
     for (int w = 0; w < C::KW; ++w) {
-      const int ch = C::k_channel(w, t), group = ch / 16;
-      const bool hi_col = D == 64 ? g == group : g == (group & 7);
-      const bool lo_col = D == 64 && g == group + 4;
+      const int col = column_of(w);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {  // operand register r: channels ch + r and ch + r + 4
+      for (int r = 0; r < 4; ++r) {  // operand register r: channels r and r + 4 of the word
         const float f = (r & 1) ? up * 0.0625f : up;
-        uint32_t hi = 0, lo = 0;
-        if (hi_col || lo_col) split2(to_f32(q[ch + r]) * f, to_f32(q[ch + r + 4]) * f, hi, lo);
-        qh[w][r] = hi_col ? hi : (lo_col ? lo : 0u);
-        if constexpr (QLO) ql[w][r] = hi_col ? lo : 0u;
+        uint32_t hi, lo;
+        split2(x[w][r] * f, x[w][r + 4] * f, hi, lo);
+        qh[w][r] = col == 1 ? hi : col == 2 ? lo : 0u;
+        if constexpr (QLO) ql[w][r] = col == 1 ? lo : 0u;
       }
     }
     // 8 sum(q) of a column: every lane sums its operand registers (undoing the
@@ -337,149 +372,180 @@ __global__ void __launch_bounds__(Tile<D>::WARPS * 32, 2) kv4_decode_kernel(Deco
     fetch(i + kStages - 1);
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
     __syncwarp();
-    const uint8_t* st = ring + (i % kStages) * C::BYTES;
-    const uint32_t mask = *reinterpret_cast<const uint32_t*>(st + C::OFF_MASK);
-
-    // ---- S = K . q per group column
-    float s[C::SETS][4];
-#pragma unroll
-    for (int x = 0; x < C::SETS; ++x) {
-      s[x][0] = s[x][2] = init[x][0];
-      s[x][1] = s[x][3] = init[x][1];
+    const uint8_t* stage = ring + (i % kStages) * C::BYTES;
+    const uint32_t mask = *reinterpret_cast<const uint32_t*>(stage + C::TP * C::TILE);
+    if (mask == 0) {
+      __syncwarp();
+      continue;
     }
-    uint32_t ka[C::KW], kb[C::KW];  // rows g and g + 8
+    float z0[C::TP], z1[C::TP];  // logits of keys g, g + 8 of each tile
+    uint32_t vs[C::TP][C::SETS];
 #pragma unroll
-    for (int c = 0; c < C::KC; ++c) {
-      if constexpr (C::KB == 16) {
-        *reinterpret_cast<uint4*>(&ka[4 * c]) = *reinterpret_cast<const uint4*>(st + ((2 * c) * 32 + lane) * 16);
-        *reinterpret_cast<uint4*>(&kb[4 * c]) = *reinterpret_cast<const uint4*>(st + ((2 * c + 1) * 32 + lane) * 16);
+    for (int y = 0; y < C::TP; ++y) {
+      const uint8_t* st = stage + y * C::TILE;
+      // ---- S = K . q per group column, in two chains
+      constexpr int CHAINS = 2;
+      float s[CHAINS][4];
+      if constexpr (C::SETS == 2) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          s[x][0] = s[x][2] = init[x][0];
+          s[x][1] = s[x][3] = init[x][1];
+        }
       } else {
-        *reinterpret_cast<uint2*>(&ka[0]) = *reinterpret_cast<const uint2*>(st + lane * 8);
-        *reinterpret_cast<uint2*>(&kb[0]) = *reinterpret_cast<const uint2*>(st + (32 + lane) * 8);
+        s[0][0] = s[0][2] = init[0][0];
+        s[0][1] = s[0][3] = init[0][1];
+        s[1][0] = s[1][1] = s[1][2] = s[1][3] = 0.f;
+      }
+      uint32_t ka[C::KW], kb[C::KW];  // rows g and g + 8
+#pragma unroll
+      for (int c = 0; c < C::KC; ++c) {
+        if constexpr (C::KB == 16) {
+          *reinterpret_cast<uint4*>(&ka[4 * c]) = *reinterpret_cast<const uint4*>(st + ((2 * c) * 32 + lane) * 16);
+          *reinterpret_cast<uint4*>(&kb[4 * c]) = *reinterpret_cast<const uint4*>(st + ((2 * c + 1) * 32 + lane) * 16);
+        } else {
+          *reinterpret_cast<uint2*>(&ka[0]) = *reinterpret_cast<const uint2*>(st + lane * 8);
+          *reinterpret_cast<uint2*>(&kb[0]) = *reinterpret_cast<const uint2*>(st + (32 + lane) * 8);
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < C::KW; ++w) {
+        constexpr uint32_t LO = 0x000f000fu, HI = 0x00f000f0u;
+        float(&c)[4] = s[C::SETS == 2 ? w >> 2 : w & 1];
+        const uint32_t u = ka[w], v = kb[w], u8 = u >> 8, v8 = v >> 8;
+        mma_f16(c, u & LO, v & LO, u & HI, v & HI, qh[w][0], qh[w][1]);
+        if constexpr (QLO) mma_f16(c, u & LO, v & LO, u & HI, v & HI, ql[w][0], ql[w][1]);
+        mma_f16(c, u8 & LO, v8 & LO, u8 & HI, v8 & HI, qh[w][2], qh[w][3]);
+        if constexpr (QLO) mma_f16(c, u8 & LO, v8 & LO, u8 & HI, v8 & HI, ql[w][2], ql[w][3]);
+      }
+      if constexpr (C::SETS == 1) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s[0][k] += s[1][k];
+      }
+      // ---- scales: this lane's columns are groups 2t, 2t+1 (of each set)
+      z0[y] = z1[y] = 0.f;
+#pragma unroll
+      for (int x = 0; x < C::SETS; ++x) {
+        const int col = D == 64 ? 2 * (t & 1) : 8 * x + 2 * t;
+        const uint32_t w0 = *reinterpret_cast<const uint16_t*>(st + C::OFF_KS + g * C::NG + col);
+        const uint32_t w1 = *reinterpret_cast<const uint16_t*>(st + C::OFF_KS + (g + 8) * C::NG + col);
+        const uint32_t h0 = __byte_perm(w0, 0, 0x4140) << 7, h1 = __byte_perm(w1, 0, 0x4140) << 7;
+        const float2 s0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
+        const float2 s1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+        z0[y] = fmaf(s[x][0], s0.x, fmaf(s[x][1], s0.y, z0[y]));
+        z1[y] = fmaf(s[x][2], s1.x, fmaf(s[x][3], s1.y, z1[y]));
+        vs[y][x] = *reinterpret_cast<const uint32_t*>(st + C::OFF_VS + (x * 32 + lane) * 4);
       }
     }
 #pragma unroll
-    for (int w = 0; w < C::KW; ++w) {
-      constexpr uint32_t LO = 0x000f000fu, HI = 0x00f000f0u;
-      float(&c)[4] = s[C::SETS == 2 ? w >> 2 : 0];
-      const uint32_t x = ka[w], y = kb[w], x8 = x >> 8, y8 = y >> 8;
-      mma_f16(c, x & LO, y & LO, x & HI, y & HI, qh[w][0], qh[w][1]);
-      if constexpr (QLO) mma_f16(c, x & LO, y & LO, x & HI, y & HI, ql[w][0], ql[w][1]);
-      mma_f16(c, x8 & LO, y8 & LO, x8 & HI, y8 & HI, qh[w][2], qh[w][3]);
-      if constexpr (QLO) mma_f16(c, x8 & LO, y8 & LO, x8 & HI, y8 & HI, ql[w][2], ql[w][3]);
+    for (int y = 0; y < C::TP; ++y) {
+      z0[y] += __shfl_xor_sync(kFullMask, z0[y], 1);
+      z1[y] += __shfl_xor_sync(kFullMask, z1[y], 1);
+      z0[y] += __shfl_xor_sync(kFullMask, z0[y], 2);
+      z1[y] += __shfl_xor_sync(kFullMask, z1[y], 2);
+      z0[y] = z0[y] * unit * down_q;
+      z1[y] = z1[y] * unit * down_q;
     }
-    // ---- scales: this lane's columns are groups 2t, 2t+1 (of each set)
-    float z0 = 0.f, z1 = 0.f;  // logits of keys g, g + 8
+    if (mask != (C::TP == 1 ? 0xffffu : 0xffffffffu)) {
 #pragma unroll
-    for (int x = 0; x < C::SETS; ++x) {
-      const int col = D == 64 ? 2 * (t & 1) : 8 * x + 2 * t;
-      const uint32_t w0 = *reinterpret_cast<const uint16_t*>(st + C::OFF_KS + g * C::NG + col);
-      const uint32_t w1 = *reinterpret_cast<const uint16_t*>(st + C::OFF_KS + (g + 8) * C::NG + col);
-      const float2 s0 = __half22float2(__halves2half2(__ushort_as_half((unsigned short)((w0 & 255u) << 7)),
-                                                      __ushort_as_half((unsigned short)((w0 >> 8) << 7))));
-      const float2 s1 = __half22float2(__halves2half2(__ushort_as_half((unsigned short)((w1 & 255u) << 7)),
-                                                      __ushort_as_half((unsigned short)((w1 >> 8) << 7))));
-      z0 = fmaf(s[x][0], s0.x, fmaf(s[x][1], s0.y, z0));
-      z1 = fmaf(s[x][2], s1.x, fmaf(s[x][3], s1.y, z1));
-    }
-    z0 += __shfl_xor_sync(kFullMask, z0, 1);
-    z1 += __shfl_xor_sync(kFullMask, z1, 1);
-    z0 += __shfl_xor_sync(kFullMask, z0, 2);
-    z1 += __shfl_xor_sync(kFullMask, z1, 2);
-    z0 = z0 * unit * down_q;
-    z1 = z1 * unit * down_q;
-    uint32_t vs[C::SETS];
+      for (int y = 0; y < C::TP; ++y) {
+        const uint32_t mk = mask >> (16 * y);
+        if (!(mk >> g & 1u)) z0[y] = -INFINITY;
+        if (!(mk >> (g + 8) & 1u)) z1[y] = -INFINITY;
+        // an unseen key's scale may be anything, NaN included: zero
+        const uint32_t four = mk >> (4 * t) & 15u;
+        const uint32_t keep = (four & 1u) * 0xffu | (four >> 1 & 1u) * 0xff00u | (four >> 2 & 1u) * 0xff0000u |
+                              (four >> 3 & 1u) * 0xff000000u;
 #pragma unroll
-    for (int x = 0; x < C::SETS; ++x) vs[x] = *reinterpret_cast<const uint32_t*>(st + C::OFF_VS + (x * 32 + lane) * 4);
-    if (mask != 0xffffu) {
-      if (mask == 0) {
-        __syncwarp();
-        continue;
+        for (int x = 0; x < C::SETS; ++x) vs[y][x] &= keep;
       }
-      if (!(mask >> g & 1u)) z0 = -INFINITY;
-      if (!(mask >> (g + 8) & 1u)) z1 = -INFINITY;
-      // an unseen key's scale may be anything, NaN included: zero
-      const uint32_t four = mask >> (4 * t) & 15u;
-      const uint32_t keep = (four & 1u) * 0xffu | (four >> 1 & 1u) * 0xff00u | (four >> 2 & 1u) * 0xff0000u |
-                            (four >> 3 & 1u) * 0xff000000u;
-#pragma unroll
-      for (int x = 0; x < C::SETS; ++x) vs[x] &= keep;
     }
     // ---- running maximum, weights
-    const float tile_top = warp_redux_max(fmaxf(z0, z1));
-    if (tile_top > m) {
-      const float f = fast_exp2(m - tile_top);  // 0 for the first tile
-      m = tile_top;
+    float top = fmaxf(z0[0], z1[0]);
+    if constexpr (C::TP == 2) top = fmaxf(top, fmaxf(z0[1], z1[1]));
+    top = warp_redux_max(top);
+    if (top > m) {
+      const float f = fast_exp2(m - top);  // 0 for the first step
+      m = top;
       l *= f;
       rescale(f);
     }
     const float ref = m == -INFINITY ? 0.f : m;
-    const float p0 = fast_exp2(z0 - ref), p1 = fast_exp2(z1 - ref);
-    l += p0 + p1;
     // ---- a V scale above the largest exponent so far?
     uint32_t big = 0;  // larger of two bytes, in halves
 #pragma unroll
-    for (int x = 0; x < C::SETS; ++x) big = __vmaxu2(big, __vmaxu2(vs[x] & 0x00ff00ffu, vs[x] >> 8 & 0x00ff00ffu));
-    // a byte of at least 8 (top_e + 1) carries into bit 8
-    if (__any_sync(kFullMask, (big + (0x100u - 8u * (top_e + 1u)) * 0x10001u) & 0x01000100u)) {
-      uint32_t top = 0;
+    for (int y = 0; y < C::TP; ++y)
 #pragma unroll
       for (int x = 0; x < C::SETS; ++x)
+        big = __vmaxu2(big, __vmaxu2(vs[y][x] & 0x00ff00ffu, vs[y][x] >> 8 & 0x00ff00ffu));
+    // a byte of at least 8 (top_e + 1) carries into bit 8
+    if (__any_sync(kFullMask, (big + (0x100u - 8u * (top_e + 1u)) * 0x10001u) & 0x01000100u)) {
+      uint32_t most = 0;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t c = vs[x] >> (8 * k) & 255u;
-          // not a NaN group's: its column is lost, the others keep their range
-          top = c <= kKv4MaxScale && c > top ? c : top;
-        }
-      top = __reduce_max_sync(kFullMask, top) >> 3;
-      if (top > top_e) {
-        rescale(__uint_as_float((127u - (top - top_e)) << 23));
-        top_e = top;
+      for (int y = 0; y < C::TP; ++y)
+#pragma unroll
+        for (int x = 0; x < C::SETS; ++x)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t c = vs[y][x] >> (8 * k) & 255u;
+            // not a NaN group's: its column is lost, the others keep their range
+            most = c <= kKv4MaxScale && c > most ? c : most;
+          }
+      most = __reduce_max_sync(kFullMask, most) >> 3;
+      if (most > top_e) {
+        rescale(__uint_as_float((127u - (most - top_e)) << 23));
+        top_e = most;
       }
     }
     const float up = __uint_as_float((127u + 29u - top_e) << 23);
-    // ---- weights of keys 4t .. 4t+3 (lane 4 * (key & 7) holds key and key + 8)
-    const float both = t < 2 ? p0 : p1;
-    float pk[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) pk[k] = __shfl_sync(kFullMask, both, 4 * ((4 * t + k) & 7) + (t < 2 ? 0 : 2)) * up;
-    uint32_t bh[C::SETS][2], bl[C::SETS][2];
+    for (int y = 0; y < C::TP; ++y) {
+      const uint8_t* st = stage + y * C::TILE;
+      const float p0 = fast_exp2(z0[y] - ref), p1 = fast_exp2(z1[y] - ref);
+      l += p0 + p1;
+      // ---- weights of keys 4t .. 4t+3 (lane 4 * (key & 7) holds key and key + 8)
+      const float both = (t < 2 ? p0 : p1) * up;
+      float pk[4];
 #pragma unroll
-    for (int x = 0; x < C::SETS; ++x) {
-      float w[4];
+      for (int k = 0; k < 4; ++k) pk[k] = __shfl_sync(kFullMask, both, 4 * ((4 * t + k) & 7) + (t < 2 ? 0 : 2));
+      uint32_t bh[C::SETS][2], bl[C::SETS][2];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) w[k] = pk[k] * kv4_scale(vs[x] >> (8 * k) & 255u);
-      split2(w[0], w[1], bh[x][0], bl[x][0]);
-      split2(w[2], w[3], bh[x][1], bl[x][1]);
-      if (D == 64 && g >= 4) {  // columns 4..7: the low halves of groups 0..3
-        bh[x][0] = bl[x][0];
-        bh[x][1] = bl[x][1];
+      for (int x = 0; x < C::SETS; ++x) {
+        const uint32_t h01 = __byte_perm(vs[y][x], 0, 0x4140) << 7, h23 = __byte_perm(vs[y][x], 0, 0x4342) << 7;
+        const float2 s01 = __half22float2(*reinterpret_cast<const __half2*>(&h01));
+        const float2 s23 = __half22float2(*reinterpret_cast<const __half2*>(&h23));
+        split2(pk[0] * s01.x, pk[1] * s01.y, bh[x][0], bl[x][0]);
+        split2(pk[2] * s23.x, pk[3] * s23.y, bh[x][1], bl[x][1]);
+        if (D == 64 && g >= 4) {  // columns 4..7: the low halves of groups 0..3
+          bh[x][0] = bl[x][0];
+          bh[x][1] = bl[x][1];
+        }
+        constexpr uint32_t EIGHT = 0x00080008u;
+        mma_f16(eights[x], EIGHT, EIGHT, EIGHT, EIGHT, bh[x][0], bh[x][1]);
+        if constexpr (PLO) mma_f16(eights[x], EIGHT, EIGHT, EIGHT, EIGHT, bl[x][0], bl[x][1]);
       }
-      constexpr uint32_t EIGHT = 0x00080008u;
-      mma_f16(eights[x], EIGHT, EIGHT, EIGHT, EIGHT, bh[x][0], bh[x][1]);
-      if constexpr (PLO) mma_f16(eights[x], EIGHT, EIGHT, EIGHT, EIGHT, bl[x][0], bl[x][1]);
-    }
-    // ---- out += V^T . weights
-    uint32_t v[4][C::VW];
+      // ---- out += V^T . weights
+      uint32_t v[4][C::VW];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint8_t* at = st + C::OFF_V + (k * 32 + lane) * C::VB;
-      if constexpr (C::VW == 1) v[k][0] = *reinterpret_cast<const uint32_t*>(at);
-      if constexpr (C::VW == 2) *reinterpret_cast<uint2*>(&v[k][0]) = *reinterpret_cast<const uint2*>(at);
-      if constexpr (C::VW == 4) *reinterpret_cast<uint4*>(&v[k][0]) = *reinterpret_cast<const uint4*>(at);
-    }
+      for (int k = 0; k < 4; ++k) {
+        const uint8_t* at = st + C::OFF_V + (k * 32 + lane) * C::VB;
+        if constexpr (C::VW == 1) v[k][0] = *reinterpret_cast<const uint32_t*>(at);
+        if constexpr (C::VW == 2) *reinterpret_cast<uint2*>(&v[k][0]) = *reinterpret_cast<const uint2*>(at);
+        if constexpr (C::VW == 4) *reinterpret_cast<uint4*>(&v[k][0]) = *reinterpret_cast<const uint4*>(at);
+      }
 #pragma unroll
-    for (int u = 0; u < C::VW; ++u) {
-      constexpr uint32_t LO = 0x000f000fu, HI = 0x00f000f0u;
-      const int x = C::SETS == 2 ? u >> 1 : 0;
-      uint32_t c01 = __byte_perm(v[0][u], v[1][u], 0x5410), d01 = __byte_perm(v[0][u], v[1][u], 0x7632);
-      uint32_t c23 = __byte_perm(v[2][u], v[3][u], 0x5410), d23 = __byte_perm(v[2][u], v[3][u], 0x7632);
+      for (int u = 0; u < C::VW; ++u) {
+        constexpr uint32_t LO = 0x000f000fu, HI = 0x00f000f0u;
+        const int x = C::SETS == 2 ? u >> 1 : 0;
+        uint32_t c01 = __byte_perm(v[0][u], v[1][u], 0x5410), d01 = __byte_perm(v[0][u], v[1][u], 0x7632);
+        uint32_t c23 = __byte_perm(v[2][u], v[3][u], 0x5410), d23 = __byte_perm(v[2][u], v[3][u], 0x7632);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t mk = (j & 1) ? HI : LO;
-        mma_f16(acc[u][j], c01 & mk, d01 & mk, c23 & mk, d23 & mk, bh[x][0], bh[x][1]);
-        if constexpr (PLO) mma_f16(acc[u][j], c01 & mk, d01 & mk, c23 & mk, d23 & mk, bl[x][0], bl[x][1]);
-        if (j == 1) c01 >>= 8, d01 >>= 8, c23 >>= 8, d23 >>= 8;
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t mk = (j & 1) ? HI : LO;
+          mma_f16(acc[u][j], c01 & mk, d01 & mk, c23 & mk, d23 & mk, bh[x][0], bh[x][1]);
+          if constexpr (PLO) mma_f16(acc[u][j], c01 & mk, d01 & mk, c23 & mk, d23 & mk, bl[x][0], bl[x][1]);
+          if (j == 1) c01 >>= 8, d01 >>= 8, c23 >>= 8, d23 >>= 8;
+        }
       }
     }
     __syncwarp();  // every lane is done with the stage before it is refilled
@@ -540,38 +606,37 @@ __global__ void __launch_bounds__(Tile<D>::WARPS * 32, 2) kv4_decode_kernel(Deco
     }
   }
   if (ns > 1) {
+    // every CTA writes its sums into rank 0's shared memory and leaves
     cg::cluster_group cluster = cg::this_cluster();
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    Smem<D, W>* dst = cluster.map_shared_rank(&sm, 0);
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int d = tid + i * C::WARPS * 32;
-      if (d < D) sm.cta_acc[d] = o[i];
+      if (d < D) dst->cta_acc[rank][d] = o[i];
     }
     if (tid == 0) {
-      sm.cta_m = M;
-      sm.cta_l = total;
+      dst->cta_m[rank] = M;
+      dst->cta_l[rank] = total;
     }
-    cluster.sync();
-    if (rank == 0) {
-      const int used = per > 0 ? (tiles + per - 1) / per : 0;
-      M = -INFINITY;
-      for (int r = 0; r < used; ++r) M = fmaxf(M, *cluster.map_shared_rank(&sm.cta_m, r));
-      ref = M == -INFINITY ? 0.f : M;
-      total = 0.f;
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    if (rank != 0) return;
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    M = -INFINITY;
+    for (int r = 0; r < ns; ++r) M = fmaxf(M, sm.cta_m[r]);
+    ref = M == -INFINITY ? 0.f : M;
+    total = 0.f;
 #pragma unroll
-      for (int i = 0; i < PER; ++i) o[i] = 0.f;
-      for (int r = 0; r < used; ++r) {
-        const float f = fast_exp2(*cluster.map_shared_rank(&sm.cta_m, r) - ref);
-        total += *cluster.map_shared_rank(&sm.cta_l, r) * f;
-        const float* a = cluster.map_shared_rank(&sm.cta_acc[0], r);
+    for (int i = 0; i < PER; ++i) o[i] = 0.f;
+    for (int r = 0; r < ns; ++r) {
+      const float f = fast_exp2(sm.cta_m[r] - ref);
+      total += sm.cta_l[r] * f;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          const int d = tid + i * C::WARPS * 32;
-          if (d < D) o[i] += a[d] * f;
-        }
+      for (int i = 0; i < PER; ++i) {
+        const int d = tid + i * C::WARPS * 32;
+        if (d < D) o[i] += sm.cta_acc[r][d] * f;
       }
     }
-    cluster.sync();  // no CTA leaves while its sums are being read
-    if (rank != 0) return;
   }
   T* out = static_cast<T*>(p.out) + (int64_t)b * p.so_b + (int64_t)h * p.so_h;
 #pragma unroll
@@ -581,9 +646,9 @@ __global__ void __launch_bounds__(Tile<D>::WARPS * 32, 2) kv4_decode_kernel(Deco
   }
 }
 
-template <typename T, int D, int BS>
-static int decode_launch(const AttnArgs& a, cudaStream_t s) {
-  using C = Tile<D>;
+template <typename T, int D, int BS, int W>
+static int decode_launch(const AttnArgs& a, int ns, cudaStream_t s) {
+  using C = Tile<D, W>;
   DecodeKv4Params p;
   p.q = a.q;
   p.sq_b = a.sq[0];
@@ -602,14 +667,8 @@ static int decode_launch(const AttnArgs& a, cudaStream_t s) {
   p.H = a.H;
   p.qscale = a.scale * kLog2e;
   p.status = a.status;
-  // CTAs per sequence and head: enough to fill the device twice over, while a
-  // warp of each keeps at least two tiles of the longest sequence.
-  const int64_t pairs = (int64_t)a.B * a.H;
-  const int64_t longest = ((int64_t)a.max_pages * BS + 15) / 16;
-  int ns = 1;
-  while (ns < 8 && pairs * ns < 4 * device_sm_count() && longest >= 2 * C::WARPS * ns * 2) ns *= 2;
   constexpr int smem = C::WARPS * kStages * C::BYTES;
-  auto kern = kv4_decode_kernel<T, D, BS>;
+  auto kern = kv4_decode_kernel<T, D, BS, W>;
   const int rc = set_max_dynamic_smem_cached(reinterpret_cast<const void*>(kern), smem);
   if (rc != B2PA_OK) return rc;
   cudaLaunchConfig_t cfg = {};
@@ -632,10 +691,22 @@ static int decode_launch(const AttnArgs& a, cudaStream_t s) {
 
 template <typename T, int D>
 static int decode_blocks(const AttnArgs& a, cudaStream_t s) {
+  // CTAs per sequence and head: one wave of the two CTAs an SM holds, while
+  // every warp keeps a step of the longest sequence.  A CTA costs about 4 us
+  // beside its keys (loads that depend on one another, the merge), so more
+  // waves of smaller shares are slower: 64 sequences of 128-1,024 tokens and 8
+  // heads of 64 take 15.4 us with 1 CTA each, 23.6 with 2; one sequence of
+  // 8,001 tokens and 32 heads of 128 takes 44 us with 1, 25 with 2, 18 with 4,
+  // 15 with 8.
+  constexpr int W = D == 256 ? 4 : 8;
+  const int64_t pairs = (int64_t)a.B * a.H;
+  const int64_t steps = ((int64_t)a.max_pages * a.block_size + 31) / 32;
+  int ns = 1;
+  while (ns < kMaxCluster && pairs * ns < 2 * device_sm_count() && steps > W * ns) ns *= 2;
   switch (a.block_size) {
-    case 8: return decode_launch<T, D, 8>(a, s);
-    case 16: return decode_launch<T, D, 16>(a, s);
-    default: return decode_launch<T, D, 32>(a, s);
+    case 8: return decode_launch<T, D, 8, W>(a, ns, s);
+    case 16: return decode_launch<T, D, 16, W>(a, ns, s);
+    default: return decode_launch<T, D, 32, W>(a, ns, s);
   }
 }
 
