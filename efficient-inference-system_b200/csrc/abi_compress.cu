@@ -312,6 +312,8 @@ int b2pa_evict(void* k_pool, void* v_pool, int pool_dtype, float* weights, int64
   if (B == 0 || keep == 0) return B2PA_OK;
   if (!k_pool || !v_pool || !weights || !seq_lens || !kept)
     return set_error(B2PA_ERR_INVALID_ARGUMENT, "%s: null pointer argument", fn);
+  if (!aligned_to(weights, 16))
+    return set_error(B2PA_ERR_UNSUPPORTED, "%s: weights must be 16-byte aligned", fn);
   B2PA_TRY(check_table(fn, page_table, pt_stride, max_pages));
   if (out_table && out_stride * (int64_t)block_size < keep)
     return set_error(B2PA_ERR_INVALID_ARGUMENT, "%s: out_table rows of %lld pages do not hold %d rows", fn,

@@ -421,8 +421,8 @@ B2PA_API int b2pa_paged_prefill_kv4(const void* q, const int64_t q_strides[4],
 /*
  * ---- Eviction by accumulated attention weight -------------------------------
  *
- * weights: fp32 [num_blocks, H, block_size], contiguous: one running sum per
- * head and cached key, at the key's place in the pools.
+ * weights: fp32 [num_blocks, H, block_size], contiguous, 16-byte aligned: one
+ * running sum per head and cached key, at the key's place in the pools.
  *
  * b2pa_key_weights adds the attention weight that a call's queries give to
  * every key: for each head and each position j < seq_lens[b],

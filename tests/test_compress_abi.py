@@ -117,6 +117,7 @@ def test_evict_refusals(lib):
     assert _evict(lib, keep=-1) == -1 and _evict(lib, recent=-1) == -1
     assert _evict(lib, pd=5) == -2 and _evict(lib, D=48) == -2
     assert _evict(lib, w=0) == -1 and _evict(lib, kept=0) == -1 and _evict(lib, sl=0) == -1
+    assert _evict(lib, w=65544) == -2                # weights not 16-byte aligned
     assert _evict(lib, ot=64, ots=1, keep=17) == -1  # one page of 16 slots a row
     assert _evict(lib, keep=0) == 0 and _evict(lib, B=0) == 0
 
