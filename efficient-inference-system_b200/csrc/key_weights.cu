@@ -530,94 +530,155 @@ __global__ void __launch_bounds__(kTileThreads) key_weights_tile_kernel(KeyWeigh
 // ------------------------------------------------------------------ one query
 constexpr int kStepThreads = 256;
 
+// How a warp takes its rows.  16-bit rows are tensor-core operands as they
+// lie: a lane loads its fragment (16 bytes of row g and of row g + 8 per 64
+// bytes of row), and the one query stands in all 8 columns, so every lane gets
+// its rows' logits without a conversion or a shuffle.  fp32 rows are summed by
+// the lanes that share a row.
+template <typename T, int D>
+struct StepRows {
+  static constexpr int RB = D * (int)sizeof(T);
+  static constexpr bool MMA = sizeof(T) == 2;
+  // MMA: 64-byte blocks per row, 16-row tiles per turn (8 loads in flight)
+  static constexpr int NB = RB < 64 ? 1 : RB / 64, TILES = NB < 4 ? 4 / NB : 1;
+  // else: lanes per row, 16-byte pieces per lane, rows per load, rows per lane
+  static constexpr int LPR = RB / 16 < 32 ? RB / 16 : 32, CPL = RB / 16 / LPR, RP = 32 / LPR, R = 8 / CPL;
+  static constexpr int RW = MMA ? 16 * TILES : RP * R;  // rows per warp and turn
+};
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kStepThreads) key_weights_step_kernel(KeyWeightArgs a, float qscale, float* far,
                                                                         int64_t far_stride) {
-  constexpr int RB = D * (int)sizeof(T);
-  constexpr int LPR = RB / 16 < 32 ? RB / 16 : 32;  // lanes per row, 16 bytes each
-  constexpr int CPL = RB / 16 / LPR;                // 16-byte pieces per lane and row
-  constexpr int RP = 32 / LPR;                      // rows per load
-  constexpr int R = 8 / CPL;                        // rows per lane and turn: 8 loads in flight
-  constexpr int RW = RP * R;                        // rows per warp and turn
-  constexpr int E = 16 / (int)sizeof(T);
+  using S = StepRows<T, D>;
+  using O = Op<T, false>;
+  constexpr int RB = S::RB, RW = S::RW, E = 16 / (int)sizeof(T);
   extern __shared__ float near[];
   __shared__ float red[2][kStepThreads / 32];
   __shared__ float cta_m, cta_l;
   pdl_wait();
   pdl_launch_dependents();
   const int ns = gridDim.x, rank = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = lane % LPR;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Span s = span_of(a, b);
   if (rank == 0 && h == 0 && tid == 0 && (int64_t)a.seq_lens[b] > s.L) set_status(a.status, B2PA_ERR_BAD_BLOCK_ID);
-  const int64_t L = s.L > 0 ? s.L : 0;
-  int64_t vis = s.past + 1 < L ? s.past + 1 : L;
-  if (s.count == 0 || vis < 0) vis = 0;
-  const int64_t turns = (L + RW - 1) / RW, per = (turns + ns - 1) / ns * RW;  // keys per CTA
-  const int64_t lo = rank * per < L ? rank * per : L, hi = lo + per < L ? lo + per : L;
+  const uint32_t blocks = a.num_blocks < INT32_MAX ? (uint32_t)a.num_blocks : (uint32_t)INT32_MAX;
+  const int L = s.L > 0 ? (int)s.L : 0;  // positions fit 31 bits
+  int vis = s.past + 1 < L ? (int)(s.past + 1) : L;
+  if (s.count == 0 || vis < 0 || blocks == 0) vis = 0;
+  const int turns = (L + RW - 1) / RW, per = (turns + ns - 1) / ns * RW;  // keys per CTA
+  const int64_t lo64 = (int64_t)rank * per;
+  const int lo = lo64 < L ? (int)lo64 : L, hi = lo + (int64_t)per < L ? lo + per : L;
   const int bs = a.block_size, sh = a.bs_log2;
   const int32_t* table = a.page_table + (int64_t)b * a.pt_stride;
   // logits of this CTA's keys
   float* z = far ? far + ((int64_t)b * a.H + h) * far_stride + lo : near;
+  const int seen = vis < hi ? vis : hi;  // keys [lo, seen) have a logit
+  const char* const pages = static_cast<const char*>(a.k_pool) + (int64_t)h * bs * RB;
+  const uint64_t block_bytes = (uint64_t)a.H * bs * RB;
+  const T* const q = static_cast<const T*>(a.q) + (int64_t)b * a.sq[0] + (int64_t)h * a.sq[1];
 
-  float q[CPL][E];
-  {
-    const T* src = static_cast<const T*>(a.q) + (int64_t)b * a.sq[0] + (int64_t)h * a.sq[1];
-#pragma unroll
-    for (int c = 0; c < CPL; ++c) {
-      Vec<T, E> v;
-      v.w = ld_global_nc<uint4>(src + (c * LPR + sub) * E);
-      v.to_float(q[c]);
-#pragma unroll
-      for (int i = 0; i < E; ++i) q[c][i] *= qscale;
-    }
-  }
   float top = -INFINITY;
   constexpr int kWarps = kStepThreads / 32;
   auto ids_of = [&](int64_t j0) {  // lane l: the l-th page from key j0's
     const int64_t pg = (j0 >> sh) + lane;
-    return j0 < hi && pg << sh < vis ? table[pg] : -1;
+    return j0 < seen && pg << sh < seen ? table[pg] : -1;
   };
   int64_t j0 = lo + warp * RW;
   int ids = ids_of(j0);
-  for (; j0 < hi; j0 += kWarps * RW) {
-    const int next = ids_of(j0 + kWarps * RW);
-    uint4 raw[R][CPL];
-    bool ok[R];
+  bool past_pool = false;
+  // Row j of the turn at j0: where it is (block 0 for one that is not seen).
+  auto locate = [&](int64_t j, bool& ok) -> const char* {
+    const uint32_t blk = (uint32_t)__shfl_sync(kFullMask, ids, (int)((j >> sh) - (j0 >> sh)));
+    ok = j < seen && blk < blocks;
+    past_pool |= j < seen && (int)blk >= (int)blocks;
+    return pages + (ok ? blk : 0u) * block_bytes + (int)(j & (bs - 1)) * RB;
+  };
+  if constexpr (S::MMA) {
+    const int g = lane >> 2, t = lane & 3;
+    uint4 qf[S::NB];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int64_t j = j0 + r * RP + lane / LPR;
-      const int blk = __shfl_sync(kFullMask, ids, (int)((j >> sh) - (j0 >> sh)));
-      ok[r] = j < vis && blk >= 0 && blk < a.num_blocks;
-      if (j < vis && blk >= a.num_blocks) set_status(a.status, B2PA_ERR_BAD_BLOCK_ID);
-      if (ok[r]) {
-        const char* src = static_cast<const char*>(a.k_pool) + (((int64_t)blk * a.H + h) * bs + (j & (bs - 1))) * RB;
-#pragma unroll
-        for (int c = 0; c < CPL; ++c) raw[r][c] = ld_global_nc<uint4>(src + (c * LPR + sub) * 16);
-      }
+    for (int c = 0; c < S::NB; ++c) {
+      qf[c] = make_uint4(0, 0, 0, 0);
+      if (c * 32 + 8 * t < D) qf[c] = ld_global_nc<uint4>(q + c * 32 + 8 * t);
     }
+    for (; j0 < seen; j0 += kWarps * RW) {
+      const int next = ids_of(j0 + kWarps * RW);
+      uint4 raw[S::TILES][2][S::NB];
+      bool ok[S::TILES][2];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      float dot = 0.f;
-      if (ok[r]) {
+      for (int x = 0; x < S::TILES; ++x)
 #pragma unroll
-        for (int c = 0; c < CPL; ++c) {
+        for (int i = 0; i < 2; ++i) {
+          const char* src = locate(j0 + x * 16 + g + 8 * i, ok[x][i]);
+#pragma unroll
+          for (int c = 0; c < S::NB; ++c) {
+            raw[x][i][c] = make_uint4(0, 0, 0, 0);
+            if (RB >= 64 || 16 * t < RB) raw[x][i][c] = ld_global_nc<uint4>(src + c * 64 + 16 * t);
+          }
+        }
+#pragma unroll
+      for (int x = 0; x < S::TILES; ++x) {
+        float c0[4] = {}, c1[4] = {};
+#pragma unroll
+        for (int c = 0; c < S::NB; ++c) {
+          const uint4 &u = raw[x][0][c], &v = raw[x][1][c], &y = qf[c];
+          mma16<O>(c0, u.x, v.x, u.y, v.y, y.x, y.y);
+          mma16<O>(c1, u.z, v.z, u.w, v.w, y.z, y.w);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float dot = ok[x][i] ? (c0[2 * i] + c1[2 * i]) * qscale : -INFINITY;
+          top = fmaxf(top, dot);
+          const int64_t j = j0 + x * 16 + g + 8 * i;
+          if (t == 0 && j < seen) z[j - lo] = dot;
+        }
+      }
+      ids = next;
+    }
+  } else {
+    const int sub = lane % S::LPR;
+    float qf[S::CPL][E];
+#pragma unroll
+    for (int c = 0; c < S::CPL; ++c) {
+      Vec<T, E> v;
+      v.w = ld_global_nc<uint4>(q + (c * S::LPR + sub) * E);
+      v.to_float(qf[c]);
+#pragma unroll
+      for (int i = 0; i < E; ++i) qf[c][i] *= qscale;
+    }
+    for (; j0 < seen; j0 += kWarps * RW) {
+      const int next = ids_of(j0 + kWarps * RW);
+      uint4 raw[S::R][S::CPL];
+      bool ok[S::R];
+#pragma unroll
+      for (int r = 0; r < S::R; ++r) {
+        const char* src = locate(j0 + r * S::RP + lane / S::LPR, ok[r]);
+#pragma unroll
+        for (int c = 0; c < S::CPL; ++c) raw[r][c] = ld_global_nc<uint4>(src + (c * S::LPR + sub) * 16);
+      }
+#pragma unroll
+      for (int r = 0; r < S::R; ++r) {
+        float dot = 0.f;
+#pragma unroll
+        for (int c = 0; c < S::CPL; ++c) {
           Vec<T, E> v;
           v.w = raw[r][c];
           float k[E];
           v.to_float(k);
 #pragma unroll
-          for (int i = 0; i < E; ++i) dot = fmaf(q[c][i], k[i], dot);
+          for (int i = 0; i < E; ++i) dot = fmaf(qf[c][i], k[i], dot);
         }
-      }
 #pragma unroll
-      for (int o = LPR / 2; o >= 1; o >>= 1) dot += __shfl_xor_sync(kFullMask, dot, o);
-      if (!ok[r]) dot = -INFINITY;
-      top = fmaxf(top, dot);
-      const int64_t j = j0 + r * RP + lane / LPR;
-      if (sub == r % LPR && j < hi) z[j - lo] = dot;
+        for (int o = S::LPR / 2; o >= 1; o >>= 1) dot += __shfl_xor_sync(kFullMask, dot, o);
+        if (!ok[r]) dot = -INFINITY;
+        top = fmaxf(top, dot);
+        const int64_t j = j0 + r * S::RP + lane / S::LPR;
+        if (sub == r % S::LPR && j < seen) z[j - lo] = dot;
+      }
+      ids = next;
     }
-    ids = next;
   }
+  if (past_pool) set_status(a.status, B2PA_ERR_BAD_BLOCK_ID);
   // this CTA's maximum and sum
   top = warp_max(top);
   if (lane == 0) red[0][warp] = top;
@@ -626,8 +687,8 @@ __global__ void __launch_bounds__(kStepThreads) key_weights_step_kernel(KeyWeigh
   for (int w = 0; w < kWarps; ++w) top = fmaxf(top, red[0][w]);
   float ref = top == -INFINITY ? 0.f : top;
   float sum = 0.f;
-  const int mine = (int)(hi - lo);
-  for (int i = tid; i < mine; i += kStepThreads) sum += fast_exp2(z[i] - ref);
+  const int mine = hi - lo, logits = seen > lo ? seen - lo : 0;
+  for (int i = tid; i < logits; i += kStepThreads) sum += fast_exp2(z[i] - ref);
   sum = warp_sum(sum);
   if (lane == 0) red[1][warp] = sum;
   __syncthreads();
@@ -651,12 +712,14 @@ __global__ void __launch_bounds__(kStepThreads) key_weights_step_kernel(KeyWeigh
     cluster.sync();
   }
   const float lse = sum != 0.f ? ref + log2f(sum) : INFINITY;
+  float* const w_out = a.w_out + (int64_t)h * bs;
+  const float* const w_in = a.w_in + (int64_t)h * bs;
   for (int i = tid; i < mine; i += kStepThreads) {
-    const int64_t j = lo + i;
-    const int32_t blk = table[j >> sh];
-    if (blk >= 0 && blk < a.num_blocks) {
-      const int64_t at = ((int64_t)blk * a.H + h) * bs + (j & (bs - 1));
-      a.w_out[at] = a.w_in[at] + (j < vis ? fast_exp2(z[i] - lse) : 0.f);
+    const int j = lo + i;
+    const uint32_t blk = (uint32_t)__ldg(table + (j >> sh));
+    if (blk < blocks) {
+      const uint64_t at = (uint64_t)blk * (uint32_t)(a.H * bs) + (j & (bs - 1));
+      w_out[at] = w_in[at] + (i < logits ? fast_exp2(z[i] - lse) : 0.f);
     }
   }
 }
