@@ -6,16 +6,20 @@
 // pos + 1) - 1, and counting when cur_len - window <= t < cur_len (all of
 // them without a window).
 //
-// Several queries (key_weights_tile_kernel): two launches of one matrix
-// product Q.K^T, on the tensor cores.  The first has queries as rows and
-// keeps each row's running maximum and sum (keys may be split between CTAs);
-// the second has keys as rows and adds exp(logit - lse) along its columns, so
-// every key's sum stays in one thread and needs no atomics: results do not
-// depend on the order of anything.  The product is computed twice because the
-// alternative, keeping T x L logits, costs more bytes than the product costs
-// time.  Operands: 16-bit types as they are; fp32 in two tf32 halves (three
-// products, 22 bits); 4-bit keys as fp16 (exact), with q scaled by a power of
-// two into fp16's range, in two halves if it is fp32.
+// Several queries (key_weights_tile_kernel): two launches over one matrix
+// product K.Q^T on the tensor cores (mma.sync), keys as rows, 64 queries as
+// columns.  A key row is used by one warp only, so its fragments go from
+// global memory to registers and only queries lie in shared memory.  The first
+// launch keeps, per lane and column, a running maximum and sum over the rows
+// that the lane sees, joined at the end (keys may be split between CTAs); the
+// second adds exp(logit - lse) along the columns, so every key's sum stays in
+// one thread and needs no atomics: results do not depend on the order of
+// anything.  The product is computed twice because the alternative, keeping
+// T x L logits, costs more bytes than the product costs time.  What bounds it
+// is instruction issue: four instructions per logit (scale and shift, compare,
+// exponential, add) beside the products'.  Operands: 16-bit types as they are;
+// 4-bit keys unpacked (exactly) to the type of q; fp32 as two fp16 halves each
+// (22 bits, three products), rows scaled by powers of two into fp16's range.
 //
 // One query (key_weights_step_kernel, plain pools): bound by reading K once.
 // A cluster of CTAs shares a sequence, each keeps its logits in shared
@@ -55,294 +59,260 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool ok) {
 }
 
 // ------------------------------------------------------------ several queries
-template <typename T, bool KV4>
+template <typename T>
 struct Op {
-  static constexpr bool TF32 = std::is_same<T, float>::value && !KV4;
-  static constexpr int PARTS = std::is_same<T, float>::value && KV4 ? 2 : 1;  // halves of q held in shared memory
-  static constexpr int BYTES = TF32 ? 4 : 2;
-  static constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value && !KV4;
-  static constexpr bool SCALED = KV4 && !std::is_same<T, __half>::value;  // q scaled per row into fp16's range
-};
-
-// Rows of the product's two operands in shared memory.  A warp reads 16-byte
-// pieces of 8 rows (4 lanes along a row): with a row pitch of 64 modulo 128
-// bytes no two lanes of a quarter warp meet in a bank.
-template <typename T, bool KV4, int D, int PASS>
-struct Shape {
-  using O = Op<T, KV4>;
-  static constexpr int RB = D * O::BYTES < 64 ? 64 : D * O::BYTES;  // bytes per row, whole 64-byte blocks
-  static constexpr int PITCH = RB % 128 == 0 ? RB + 64 : RB;
-  static constexpr int MT = RB <= 256 && PASS == 2 ? 2 : 1;  // 16-row tiles per warp
-  static constexpr int ROWS = 64 * MT;
-  static constexpr int COLS = RB <= 512 ? 64 : 32;
-  static constexpr int NT = COLS / 8;
-  static constexpr int ROW_PARTS = PASS == 1 ? O::PARTS : 1;
-  static constexpr int COL_PARTS = PASS == 1 ? 1 : O::PARTS;
-  static constexpr int ROW_BYTES = ROWS * PITCH, COL_BYTES = COLS * PITCH;
-  static constexpr int SMEM = ROW_PARTS * ROW_BYTES + 2 * COL_PARTS * COL_BYTES;
+  static constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+  static constexpr bool F32 = std::is_same<T, float>::value;  // q as two fp16 halves, scaled per row
 };
 
 template <typename O>
 __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                       uint32_t b1) {
   if constexpr (O::BF16)
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ void mma_tf32(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+__device__ __forceinline__ uint32_t bits_of(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+__device__ __forceinline__ uint32_t bits_of(__nv_bfloat162 h) { return *reinterpret_cast<uint32_t*>(&h); }
+
+// Eight fp32 values, scaled, as fp16 halves hi + lo.
+__device__ __forceinline__ void split8(const float* x, float f, uint4& hi, uint4& lo) {
+  uint32_t* h = &hi.x;
+  uint32_t* l = &lo.x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float u = x[2 * i] * f, v = x[2 * i + 1] * f;
+    const __half2 p = __floats2half2_rn(u, v);
+    const float2 w = __half22float2(p);
+    h[i] = bits_of(p);
+    l[i] = bits_of(__floats2half2_rn(u - w.x, v - w.y));
+  }
 }
 
-// x = hi + lo with hi of 11 significant bits (tf32); lo keeps the next 11.
-__device__ __forceinline__ void split_tf32(const uint32_t x, uint32_t& hi, uint32_t& lo) {
-  hi = x & 0xffffe000u;
-  lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(hi));
-}
-// In place: x becomes hi.
-__device__ __forceinline__ void split_tf32(uint4& x, uint4& lo) {
-  split_tf32(x.x, x.x, lo.x);
-  split_tf32(x.y, x.y, lo.y);
-  split_tf32(x.z, x.z, lo.z);
-  split_tf32(x.w, x.w, lo.w);
+// A power of two that brings magnitudes up to `top` near 2^10, and its
+// inverse; 0, tiny, infinite and NaN maxima keep a finite factor.
+__device__ __forceinline__ float range_factor(float top, float& back) {
+  int e = 137 - (int)(__float_as_uint(top) >> 23);
+  e = e > 100 ? 100 : e;
+  back = __uint_as_float((uint32_t)(127 - e) << 23);
+  return __uint_as_float((uint32_t)(127 + e) << 23);
 }
 
-// One 4-bit word as 8 fp16 values in the order 0 4 1 5 2 6 3 7 (each masked
-// pair of nibbles gives one register: 1024 + c, then 16 (64 + c) for the
-// upper nibbles).
-__device__ __forceinline__ uint4 word_to_half(uint32_t w, __half2 s) {
+// One 4-bit word (8 channels of scale code sc) as 4 operand registers, exact.
+__device__ __forceinline__ uint4 unpack_word(uint32_t w, uint32_t sc, __half) {
+  // a masked nibble pair in the mantissa: 1024 + c, and 16 (64 + c) above
+  const __half2 s = __half2half2(__ushort_as_half((unsigned short)(sc << 7)));
   const __half2 k1032 = __half2half2(__ushort_as_half(0x6408)), k72 = __half2half2(__ushort_as_half(0xd480)),
                 k16th = __half2half2(__ushort_as_half(0x2c00));
   auto lo = [&](uint32_t x) {
     const uint32_t y = (x & 0x000f000fu) | 0x64006400u;
-    return __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&y), k1032), s);
+    return bits_of(__hmul2(__hsub2(*reinterpret_cast<const __half2*>(&y), k1032), s));
   };
   auto hi = [&](uint32_t x) {
     const uint32_t y = (x & 0x00f000f0u) | 0x64006400u;
-    return __hmul2(__hfma2(*reinterpret_cast<const __half2*>(&y), k16th, k72), s);
+    return bits_of(__hmul2(__hfma2(*reinterpret_cast<const __half2*>(&y), k16th, k72), s));
   };
-  uint4 r;
-  __half2 h[4] = {lo(w), hi(w), lo(w >> 8), hi(w >> 8)};
-  r.x = *reinterpret_cast<uint32_t*>(&h[0]);
-  r.y = *reinterpret_cast<uint32_t*>(&h[1]);
-  r.z = *reinterpret_cast<uint32_t*>(&h[2]);
-  r.w = *reinterpret_cast<uint32_t*>(&h[3]);
-  return r;
+  const uint32_t c04 = lo(w), c15 = hi(w), c26 = lo(w >> 8), c37 = hi(w >> 8);
+  return make_uint4(__byte_perm(c04, c15, 0x5410), __byte_perm(c26, c37, 0x5410), __byte_perm(c04, c15, 0x7632),
+                    __byte_perm(c26, c37, 0x7632));
+}
+__device__ __forceinline__ uint4 unpack_word(uint32_t w, uint32_t sc, __nv_bfloat16) {
+  const __nv_bfloat162 s = __float2bfloat162_rn(kv4_scale(sc));  // 4 significant bits
+  const __nv_bfloat162 k136 = __float2bfloat162_rn(136.f);
+  auto pick = [&](uint32_t x) {
+    const uint32_t y = (x & 0x000f000fu) | 0x43004300u;  // 128 + c
+    return bits_of(__hmul2(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&y), k136), s));
+  };
+  const uint32_t c04 = pick(w), c15 = pick(w >> 4), c26 = pick(w >> 8), c37 = pick(w >> 12);
+  return make_uint4(__byte_perm(c04, c15, 0x5410), __byte_perm(c26, c37, 0x5410), __byte_perm(c04, c15, 0x7632),
+                    __byte_perm(c26, c37, 0x7632));
 }
 
 constexpr int kTileThreads = 128;
+constexpr int kCols = 64;  // queries per tile
 
-// Loads key rows (plain: asynchronously; 4-bit: through registers, so that
-// the loads of the next tile are in flight during the product of this one).
-template <typename T, bool KV4, int D, int N, int RB, int PITCH>
-struct KeyLoader {
-  static constexpr int UNITS = KV4 ? N * (D / 32) : N * (RB / 16);
-  static constexpr int PER = (UNITS + kTileThreads - 1) / kTileThreads;
-  uint4 raw[KV4 ? PER : 1];
-  uint32_t scales[KV4 ? PER : 1];
-
-  __device__ __forceinline__ static int32_t block_of(const KeyWeightArgs& a, const int32_t* table, int64_t j, int64_t L) {
-    if (j >= L) return -1;
-    const int32_t blk = table[j >> a.bs_log2];
-    return blk < a.num_blocks ? blk : -1;
+template <typename T, bool KV4, int D>
+struct Shape {
+  using O = Op<T>;
+  static constexpr int NB = D < 32 ? 1 : D / 32;          // blocks of 32 channels: two products of 16
+  static constexpr int KPARTS = O::F32 && !KV4 ? 2 : 1;   // halves of a key / of a query
+  static constexpr int QPARTS = O::F32 ? 2 : 1;
+  static constexpr int MT = NB * KPARTS <= 4 ? 2 : 1;     // 16-row tiles per warp: up to 64 registers of keys
+  static constexpr int WROWS = 16 * MT, ROWS = 4 * WROWS;  // keys per warp and CTA
+  static constexpr int PITCH = NB * 64 % 128 == 0 ? NB * 64 + 64 : NB * 64;  // a quarter warp's two rows in other banks
+  static constexpr int Q_BYTES = QPARTS * kCols * PITCH;
+  // where 8 consecutive channels (number c8) of a query row go: 4-bit keys
+  // are loaded 16 bytes (4 words) a lane, so word w of lane t is block w's
+  __device__ static constexpr int place(int c8) {
+    return !KV4 ? 16 * c8 : D == 64 ? (c8 & 1) * 64 + (c8 >> 1) * 16
+                                    : ((c8 >> 4) * 4 + (c8 & 3)) * 64 + ((c8 >> 2) & 3) * 16;
   }
+};
 
-  __device__ __forceinline__ void fetch(const KeyWeightArgs& a, const int32_t* table, int h, int64_t j0, int64_t L,
-                                        uint32_t dst) {
-    const int bs = a.block_size;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int u = threadIdx.x + i * kTileThreads;
-      if (UNITS % kTileThreads != 0 && u >= UNITS) break;
-      if constexpr (KV4) {
-        const int r = u / (D / 32), c = u % (D / 32);
-        const int64_t j = j0 + r;
-        const int32_t blk = block_of(a, table, j, L);
-        raw[i] = make_uint4(0, 0, 0, 0);
-        scales[i] = 0;
-        if (blk >= 0) {
-          const uint8_t* page = static_cast<const uint8_t*>(a.k_pool) + ((int64_t)blk * a.H + h) * kv4_page_bytes(bs, D);
-          const int row = (int)(j & (bs - 1));
-          raw[i] = *reinterpret_cast<const uint4*>(page + row * (D / 2) + 16 * c);
-          scales[i] = *reinterpret_cast<const uint16_t*>(page + bs * (D / 2) + row * (D / 16) + 2 * c);
-        }
-      } else {
-        const int r = u / (RB / 16), c = u % (RB / 16);
-        const int64_t j = j0 + r;
-        const int32_t blk = block_of(a, table, j, L);
-        const bool ok = blk >= 0 && 16 * c < D * (int)sizeof(T);
-        const char* src = static_cast<const char*>(a.k_pool);
-        if (ok) src += ((((int64_t)blk * a.H + h) * bs + (j & (bs - 1))) * D) * (int64_t)sizeof(T) + 16 * c;
-        copy16(dst + r * PITCH + 16 * c, src, ok);
+// Counted queries i0 .. i0 + 63 into shared memory (zeros past the count):
+// copies of the rows, or for fp32 their scaled halves with unit[r], the factor
+// that undoes the scaling.
+template <typename T, bool KV4, int D>
+__device__ __forceinline__ void load_queries(const KeyWeightArgs& a, const Span& s, int h, int b, int i0, uint8_t* dst,
+                                             float* unit) {
+  using S = Shape<T, KV4, D>;
+  constexpr int C8 = S::NB * 4;  // 8-channel pieces per row (whole blocks)
+  const T* q = static_cast<const T*>(a.q) + (int64_t)b * a.sq[0] + (int64_t)h * a.sq[1];
+  if constexpr (!S::O::F32) {
+    for (int u = threadIdx.x; u < kCols * C8; u += kTileThreads) {
+      const int r = u / C8, c = u % C8;
+      const bool ok = i0 + r < s.count && 8 * c < D;
+      copy16(smem_u32(dst) + r * S::PITCH + S::place(c), ok ? q + (int64_t)(s.first + i0 + r) * a.sq[2] + 8 * c : q, ok);
+    }
+  } else {
+    constexpr int LPR = C8 < 32 ? C8 : 32;  // lanes per row
+    const int lane = threadIdx.x & 31, c = lane % LPR;
+    for (int r = (threadIdx.x >> 5) * (32 / LPR) + lane / LPR; r < kCols; r += kTileThreads / LPR) {
+      float x[8] = {}, top = 0.f;
+      if (i0 + r < s.count && 8 * c < D) {
+        const float4* row = reinterpret_cast<const float4*>(q + (int64_t)(s.first + i0 + r) * a.sq[2] + 8 * c);
+        *reinterpret_cast<float4*>(x) = __ldg(row);
+        *reinterpret_cast<float4*>(x + 4) = __ldg(row + 1);
       }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
+#pragma unroll
+      for (int o = LPR / 2; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, o));
+      float back;
+      const float f = range_factor(top, back);
+      uint4 hi, lo;
+      split8(x, f, hi, lo);
+      *reinterpret_cast<uint4*>(dst + r * S::PITCH + S::place(c)) = hi;
+      *reinterpret_cast<uint4*>(dst + kCols * S::PITCH + r * S::PITCH + S::place(c)) = lo;
+      if (c == 0) unit[r] = back;
     }
   }
-  __device__ __forceinline__ void store(uint8_t* dst) {
-    if constexpr (KV4) {
+}
+
+// A warp's key rows as operand fragments: rows g and g + 8 of each 16-row tile.
+template <typename T, bool KV4, int D>
+struct Keys {
+  using S = Shape<T, KV4, D>;
+  uint4 x[S::MT][2][S::NB];
+  uint4 lo[S::KPARTS == 2 ? S::MT : 1][2][S::KPARTS == 2 ? S::NB : 1];
+  float back[S::MT][2];  // undoes the scaling of fp32 rows
+  bool ok[S::MT][2];     // the row is a key (its page exists)
+
+  // Rows j0 + 16 m + g (+ 8), those below `end`.
+  __device__ __forceinline__ void load(const KeyWeightArgs& a, const int32_t* table, int h, int64_t j0, int64_t end,
+                                       uint32_t blocks, bool& past_pool) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int bs = a.block_size;
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const int u = threadIdx.x + i * kTileThreads;
-        if (UNITS % kTileThreads != 0 && u >= UNITS) break;
-        const int r = u / (D / 32), c = u % (D / 32);
-        const uint32_t* w = &raw[i].x;
-        const __half2 s0 = __half2half2(__ushort_as_half((unsigned short)((scales[i] & 255u) << 7)));
-        const __half2 s1 = __half2half2(__ushort_as_half((unsigned short)((scales[i] >> 8) << 7)));
+    for (int m = 0; m < S::MT; ++m)
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          *reinterpret_cast<uint4*>(dst + r * PITCH + 64 * c + 16 * k) = word_to_half(w[k], k < 2 ? s0 : s1);
+      for (int i = 0; i < 2; ++i) {
+        const int64_t j = j0 + 16 * m + 8 * i + g;
+        uint32_t blk = j < end ? (uint32_t)__ldg(table + (j >> a.bs_log2)) : 0xffffffffu;
+        ok[m][i] = blk < blocks;
+        past_pool |= (int)blk >= (int)blocks;
+        blk = ok[m][i] ? blk : 0u;
+        const int row = (int)(j & (bs - 1));
+        uint4(&f)[S::NB] = x[m][i];
+        if constexpr (KV4) {
+          const uint8_t* page = static_cast<const uint8_t*>(a.k_pool) +
+                                (uint64_t)(blk * (uint64_t)a.H + h) * (uint32_t)kv4_page_bytes(bs, D);
+          const uint8_t* scales = page + bs * (D / 2) + row * (D / 16);
+          using E = typename std::conditional<S::O::BF16, __nv_bfloat16, __half>::type;
+          if constexpr (D == 64) {
+            const uint2 w = __ldg(reinterpret_cast<const uint2*>(page + row * 32 + 8 * t));
+            const uint32_t sc = __ldg(scales + t);
+            f[0] = unpack_word(w.x, sc, E{});
+            f[1] = unpack_word(w.y, sc, E{});
+          } else {
+#pragma unroll
+            for (int c = 0; c < D / 128; ++c) {
+              const uint4 w = __ldg(reinterpret_cast<const uint4*>(page + row * (D / 2) + 64 * c + 16 * t));
+              const uint32_t sc = __ldg(reinterpret_cast<const uint16_t*>(scales + 8 * c + 2 * t));
+              f[4 * c + 0] = unpack_word(w.x, sc & 255u, E{});
+              f[4 * c + 1] = unpack_word(w.y, sc & 255u, E{});
+              f[4 * c + 2] = unpack_word(w.z, sc >> 8, E{});
+              f[4 * c + 3] = unpack_word(w.w, sc >> 8, E{});
+            }
+          }
+        } else {
+          const T* src = static_cast<const T*>(a.k_pool) + ((blk * (uint64_t)a.H + h) * bs + row) * D + 8 * t;
+          if constexpr (!S::O::F32) {
+#pragma unroll
+            for (int c = 0; c < S::NB; ++c) {
+              f[c] = make_uint4(0, 0, 0, 0);
+              if (D >= 32 || 8 * t < D) f[c] = __ldg(reinterpret_cast<const uint4*>(src + 32 * c));
+            }
+          } else {
+            float v[S::NB][8], top = 0.f;
+#pragma unroll
+            for (int c = 0; c < S::NB; ++c)
+#pragma unroll
+              for (int k = 0; k < 8; k += 4) {
+                float4 y = make_float4(0, 0, 0, 0);
+                if (D >= 32 || 8 * t < D) y = __ldg(reinterpret_cast<const float4*>(src + 32 * c + k));
+                *reinterpret_cast<float4*>(&v[c][k]) = y;
+                top = fmaxf(top, fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
+              }
+            top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 2));
+            const float up = range_factor(top, back[m][i]);
+#pragma unroll
+            for (int c = 0; c < S::NB; ++c) split8(v[c], up, f[c], lo[m][i][c]);
+          }
+        }
+      }
+  }
+
+  // acc = rows . columns 8n .. 8n+7
+  __device__ __forceinline__ void product(const uint8_t* q, int n, float (&acc)[S::MT][4]) const {
+    using O = typename S::O;
+    const int lane = threadIdx.x & 31;
+    const uint8_t* at = q + (n * 8 + (lane >> 2)) * S::PITCH + 16 * (lane & 3);
+#pragma unroll
+    for (int m = 0; m < S::MT; ++m)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[m][k] = 0.f;
+#pragma unroll
+    for (int c = 0; c < S::NB; ++c) {
+      const uint4 y = *reinterpret_cast<const uint4*>(at + 64 * c);
+      uint4 yl;
+      if constexpr (S::QPARTS == 2) yl = *reinterpret_cast<const uint4*>(at + kCols * S::PITCH + 64 * c);
+#pragma unroll
+      for (int m = 0; m < S::MT; ++m) {
+        const uint4 &u = x[m][0][c], &v = x[m][1][c];
+        if constexpr (S::KPARTS == 2) {
+          const uint4 &ul = lo[m][0][c], &vl = lo[m][1][c];
+          mma16<O>(acc[m], ul.x, vl.x, ul.y, vl.y, y.x, y.y);
+          mma16<O>(acc[m], ul.z, vl.z, ul.w, vl.w, y.z, y.w);
+        }
+        if constexpr (S::QPARTS == 2) {
+          mma16<O>(acc[m], u.x, v.x, u.y, v.y, yl.x, yl.y);
+          mma16<O>(acc[m], u.z, v.z, u.w, v.w, yl.z, yl.w);
+        }
+        mma16<O>(acc[m], u.x, v.x, u.y, v.y, y.x, y.y);
+        mma16<O>(acc[m], u.z, v.z, u.w, v.w, y.z, y.w);
       }
     }
   }
 };
 
-// Loads counted queries i0 .. i0 + N - 1; zeros past the count.  4-bit pools:
-// converted to fp16 (one warp per row), unit[r] = the factor that turns the
-// product back into a logit.
-template <typename T, bool KV4, int D, int N, int RB, int PITCH>
-__device__ __forceinline__ void load_queries(const KeyWeightArgs& a, const Span& s, int h, int b, int i0, uint8_t* dst,
-                                             float* unit, float qscale) {
-  using O = Op<T, KV4>;
-  const T* q = static_cast<const T*>(a.q) + (int64_t)b * a.sq[0] + (int64_t)h * a.sq[1];
-  if constexpr (!KV4) {
-    constexpr int CH = RB / 16;
-    for (int u = threadIdx.x; u < N * CH; u += kTileThreads) {
-      const int r = u / CH, c = u % CH;
-      const bool ok = i0 + r < s.count && 16 * c < D * (int)sizeof(T);
-      const char* src = reinterpret_cast<const char*>(q);
-      if (ok) src += (int64_t)(s.first + i0 + r) * a.sq[2] * (int)sizeof(T) + 16 * c;
-      copy16(smem_u32(dst) + r * PITCH + 16 * c, src, ok);
-    }
-  } else {
-    constexpr int LPR = D / 8;  // lanes per row, 8 channels each
-    const int lane = threadIdx.x & 31, sub = lane % LPR;
-    for (int r = (threadIdx.x >> 5) * (32 / LPR) + lane / LPR; r < N; r += kTileThreads / LPR) {
-      float x[8] = {};
-      const bool ok = i0 + r < s.count;
-      if (ok) {
-        const T* row = q + (int64_t)(s.first + i0 + r) * a.sq[2] + 8 * sub;
-        constexpr int V = 16 / (int)sizeof(T);
-#pragma unroll
-        for (int i = 0; i < 8; i += V) {
-          Vec<T, V> v;
-          v.w = ld_global_nc<uint4>(row + i);
-          v.to_float(x + i);
-        }
-      }
-      float f = 1.f, back = 1.f;
-      if constexpr (O::SCALED) {
-        float top = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
-#pragma unroll
-        for (int o = LPR / 2; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, o));
-        int e = 137 - (int)(__float_as_uint(top) >> 23);  // largest magnitude near 2^10
-        e = e > 100 ? 100 : e;
-        f = __uint_as_float((uint32_t)(127 + e) << 23);
-        back = __uint_as_float((uint32_t)(127 - e) << 23);
-      }
-      uint32_t hi[4], lo[4];
-      constexpr int order[8] = {0, 4, 1, 5, 2, 6, 3, 7};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float u = x[order[2 * i]] * f, v = x[order[2 * i + 1]] * f;
-        const __half2 hh = __floats2half2_rn(u, v);
-        hi[i] = *reinterpret_cast<const uint32_t*>(&hh);
-        if constexpr (O::PARTS == 2) {
-          const float2 w = __half22float2(hh);
-          const __half2 ll = __floats2half2_rn(u - w.x, v - w.y);
-          lo[i] = *reinterpret_cast<const uint32_t*>(&ll);
-        }
-      }
-      *reinterpret_cast<uint4*>(dst + r * PITCH + 16 * sub) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      if constexpr (O::PARTS == 2)
-        *reinterpret_cast<uint4*>(dst + N * PITCH + r * PITCH + 16 * sub) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-      if (sub == 0) unit[r] = back;
-    }
-  }
-}
-
-// acc = rows . cols^T for this warp's MT * 16 rows and all NT * 8 columns.
-template <typename S>
-__device__ __forceinline__ void product(const uint8_t* rows, const uint8_t* cols, float (&acc)[S::MT][S::NT][4]) {
-  using O = typename S::O;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-#pragma unroll
-  for (int m = 0; m < S::MT; ++m)
-#pragma unroll
-    for (int n = 0; n < S::NT; ++n)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) acc[m][n][k] = 0.f;
-  const uint8_t* ra = rows + (warp * S::MT * 16 + g) * S::PITCH + 16 * t;
-  const uint8_t* cb = cols + g * S::PITCH + 16 * t;
-#pragma unroll 2
-  for (int kb = 0; kb < S::RB; kb += 64) {
-    uint4 x[S::MT][2], xl[S::MT][2];
-#pragma unroll
-    for (int m = 0; m < S::MT; ++m)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        x[m][i] = *reinterpret_cast<const uint4*>(ra + (m * 16 + 8 * i) * S::PITCH + kb);
-        if constexpr (O::TF32) split_tf32(x[m][i], xl[m][i]);
-        if constexpr (S::ROW_PARTS == 2)
-          xl[m][i] = *reinterpret_cast<const uint4*>(ra + S::ROW_BYTES + (m * 16 + 8 * i) * S::PITCH + kb);
-      }
-#pragma unroll
-    for (int n = 0; n < S::NT; ++n) {
-      uint4 y = *reinterpret_cast<const uint4*>(cb + n * 8 * S::PITCH + kb), yl;
-      if constexpr (O::TF32) split_tf32(y, yl);
-      if constexpr (S::COL_PARTS == 2) yl = *reinterpret_cast<const uint4*>(cb + S::COL_BYTES + n * 8 * S::PITCH + kb);
-#pragma unroll
-      for (int m = 0; m < S::MT; ++m) {
-        float(&c)[4] = acc[m][n];
-        const uint4 &u = x[m][0], &v = x[m][1], &ul = xl[m][0], &vl = xl[m][1];
-        if constexpr (O::TF32) {
-          mma_tf32(c, ul.x, vl.x, ul.y, vl.y, y.x, y.y);
-          mma_tf32(c, u.x, v.x, u.y, v.y, yl.x, yl.y);
-          mma_tf32(c, u.x, v.x, u.y, v.y, y.x, y.y);
-          mma_tf32(c, ul.z, vl.z, ul.w, vl.w, y.z, y.w);
-          mma_tf32(c, u.z, v.z, u.w, v.w, yl.z, yl.w);
-          mma_tf32(c, u.z, v.z, u.w, v.w, y.z, y.w);
-        } else {
-          if constexpr (S::ROW_PARTS == 2) {
-            mma16<O>(c, ul.x, vl.x, ul.y, vl.y, y.x, y.y);
-            mma16<O>(c, ul.z, vl.z, ul.w, vl.w, y.z, y.w);
-          }
-          if constexpr (S::COL_PARTS == 2) {
-            mma16<O>(c, u.x, v.x, u.y, v.y, yl.x, yl.y);
-            mma16<O>(c, u.z, v.z, u.w, v.w, yl.z, yl.w);
-          }
-          mma16<O>(c, u.x, v.x, u.y, v.y, y.x, y.y);
-          mma16<O>(c, u.z, v.z, u.w, v.w, y.z, y.w);
-        }
-      }
-    }
-  }
-}
-
-// PASS 1: rows are queries, (maximum, sum) of each over one of nsplit ranges
-// of keys goes to part[query][split].  PASS 2: rows are keys, columns queries.
+// PASS 1: grid (query tile x key range, head, sequence); (maximum, sum) of
+// each query over one of nsplit ranges of keys goes to part[query][split].
+// PASS 2: grid (key tiles, taken in turn; head; sequence).
 template <typename T, bool KV4, int D, int PASS>
 __global__ void __launch_bounds__(kTileThreads) key_weights_tile_kernel(KeyWeightArgs a, float qscale, int nsplit,
                                                                         float2* part) {
-  using S = Shape<T, KV4, D, PASS>;
-  using O = Op<T, KV4>;
-  extern __shared__ __align__(16) uint8_t tile_smem[];
-  __shared__ float row_unit[S::ROWS], col_unit[2][S::COLS], col_lse[2][S::COLS];
-  __shared__ uint8_t col_ok[2][S::COLS];
-  uint8_t* rows = tile_smem;
-  uint8_t* cols[2] = {tile_smem + S::ROW_PARTS * S::ROW_BYTES,
-                      tile_smem + S::ROW_PARTS * S::ROW_BYTES + S::COL_PARTS * S::COL_BYTES};
+  using S = Shape<T, KV4, D>;
+  using O = typename S::O;
+  extern __shared__ __align__(16) uint8_t queries[];  // PASS 2: two tiles
+  __shared__ float col_unit[2][kCols], col_lse[2][kCols];
   pdl_wait();
   pdl_launch_dependents();
   const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
@@ -350,114 +320,109 @@ __global__ void __launch_bounds__(kTileThreads) key_weights_tile_kernel(KeyWeigh
   const Span s = span_of(a, b);
   const int32_t* table = a.page_table + (int64_t)b * a.pt_stride;
   const int64_t head = (int64_t)b * a.H + h;
-  float acc[S::MT][S::NT][4];
+  const uint32_t blocks = a.num_blocks < INT32_MAX ? (uint32_t)a.num_blocks : (uint32_t)INT32_MAX;
+  if (blocks == 0) return;
+  bool past_pool = false;
+  Keys<T, KV4, D> keys;
+  float acc[S::MT][4];
+  constexpr int NT = kCols / 8;
 
   if constexpr (PASS == 1) {
     const int tile = blockIdx.x / nsplit, split = blockIdx.x % nsplit;
-    const int i0 = tile * S::ROWS;
+    const int i0 = tile * kCols;
     if (blockIdx.x == 0 && h == 0 && tid == 0 && (int64_t)a.seq_lens[b] > s.L)
       set_status(a.status, B2PA_ERR_BAD_BLOCK_ID);
     if (i0 >= s.count) return;
-    const int last = i0 + S::ROWS < s.count ? i0 + S::ROWS : s.count;
-    int64_t kend = s.past + s.first + last;
-    kend = kend < s.L ? kend : s.L;
-    const int64_t tiles = kend > 0 ? (kend + S::COLS - 1) / S::COLS : 0, per = (tiles + nsplit - 1) / nsplit;
-    const int64_t c0 = split * per < tiles ? split * per : tiles, c1 = c0 + per < tiles ? c0 + per : tiles;
-    load_queries<T, KV4, D, S::ROWS, S::RB, S::PITCH>(a, s, h, b, i0, rows, row_unit, qscale);
-    KeyLoader<T, KV4, D, S::COLS, S::RB, S::PITCH> keys;
-    auto mark = [&](int64_t c, int buf) {
-      for (int r = tid; r < S::COLS; r += kTileThreads) {
-        const int64_t j = c * S::COLS + r;
-        int ok = 0;
-        if (j < kend) {
-          const int32_t blk = table[j >> a.bs_log2];
-          ok = blk >= 0 && blk < a.num_blocks;
-          if (blk >= a.num_blocks) set_status(a.status, B2PA_ERR_BAD_BLOCK_ID);
-        }
-        col_ok[buf][r] = (uint8_t)ok;
-      }
-    };
-    float m[S::MT][2], l[S::MT][2], unit[S::MT][2];
-#pragma unroll
-    for (int x = 0; x < S::MT; ++x) m[x][0] = m[x][1] = -INFINITY, l[x][0] = l[x][1] = 0.f;
-    if (c0 < c1) {
-      keys.fetch(a, table, h, c0 * S::COLS, kend, smem_u32(cols[0]));
-      keys.store(cols[0]);
-      mark(c0, 0);
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    for (int64_t c = c0; c < c1; ++c) {
-      const int buf = (int)(c - c0) & 1;
-      if (c + 1 < c1) keys.fetch(a, table, h, (c + 1) * S::COLS, kend, smem_u32(cols[buf ^ 1]));
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      asm volatile("cp.async.wait_group 1;" ::: "memory");
-      __syncthreads();
-      if (c == c0) {
-#pragma unroll
-        for (int x = 0; x < S::MT; ++x)
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            unit[x][i] = O::SCALED ? qscale * row_unit[warp * S::MT * 16 + x * 16 + g + 8 * i] : qscale;
-      }
-      product<S>(rows, cols[buf], acc);
-#pragma unroll
-      for (int x = 0; x < S::MT; ++x)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int r = i0 + warp * S::MT * 16 + x * 16 + g + 8 * i;
-          const int64_t seen = s.past + s.first + r + 1 - c * S::COLS;  // columns below it are visible
-          float top = -INFINITY;
-#pragma unroll
-          for (int n = 0; n < S::NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int col = n * 8 + 2 * t + e;
-              float& z = acc[x][n][2 * i + e];
-              z = col < seen && col_ok[buf][col] ? z * unit[x][i] : -INFINITY;
-              top = fmaxf(top, z);
-            }
-          top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 1));
-          top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 2));
-          const float mn = fmaxf(m[x][i], top), ref = mn == -INFINITY ? 0.f : mn;
-          float sum = 0.f;
-#pragma unroll
-          for (int n = 0; n < S::NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) sum += fast_exp2(acc[x][n][2 * i + e] - ref);
-          l[x][i] = l[x][i] * fast_exp2(m[x][i] - ref) + sum;
-          m[x][i] = mn;
-        }
-      __syncthreads();
-      if (c + 1 < c1) {
-        keys.store(cols[buf ^ 1]);
-        mark(c + 1, buf ^ 1);
-      }
-    }
+    load_queries<T, KV4, D>(a, s, h, b, i0, queries, col_unit[0]);
     asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+    const int last = i0 + kCols < s.count ? i0 + kCols : s.count;
+    int64_t kend = s.past + s.first + last;  // keys that the last of the queries sees
+    kend = kend < s.L ? kend : s.L;
+    const int64_t tiles = kend > 0 ? (kend + S::WROWS - 1) / S::WROWS : 0;
+    const int64_t whole = s.past + s.first + i0 + 1;  // keys below it are seen by every query
+    // per column (8n + 2t + e): reference and sum of exp2(logit - reference)
+    float m[NT][2], l[NT][2];
 #pragma unroll
-    for (int x = 0; x < S::MT; ++x)
+    for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.f;
+    for (int64_t c = split * 4 + warp; c < tiles; c += nsplit * 4) {
+      const int64_t j0 = c * S::WROWS;
+      keys.load(a, table, h, j0, kend, blocks, past_pool);
+      bool plain = j0 + S::WROWS <= whole;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        l[x][i] += __shfl_xor_sync(kFullMask, l[x][i], 1);
-        l[x][i] += __shfl_xor_sync(kFullMask, l[x][i], 2);
-        const int r = i0 + warp * S::MT * 16 + x * 16 + g + 8 * i;
-        if (t == 0 && r < s.count) part[(head * a.T + r) * nsplit + split] = make_float2(m[x][i], l[x][i]);
+      for (int x = 0; x < S::MT; ++x) plain = plain && keys.ok[x][0] && keys.ok[x][1];
+      plain = __all_sync(kFullMask, plain);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        keys.product(queries, n, acc);
+        float z[S::MT][2][2];  // [tile][column][row]
+        float top = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int col = n * 8 + 2 * t + e;
+          const float unit = O::F32 ? qscale * col_unit[0][col] : qscale;
+#pragma unroll
+          for (int x = 0; x < S::MT; ++x)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              float u = unit;
+              if constexpr (S::KPARTS == 2) u *= keys.back[x][i];
+              z[x][e][i] = fmaf(acc[x][2 * i + e], u, m[n][e] == -INFINITY ? 0.f : -m[n][e]);
+              if (!plain && !(keys.ok[x][i] && j0 + 16 * x + 8 * i + g < whole + col)) z[x][e][i] = -INFINITY;
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < S::MT; ++x) top = fmaxf(top, fmaxf(fmaxf(z[x][0][0], z[x][0][1]), fmaxf(z[x][1][0], z[x][1][1])));
+        // The reference need not be the maximum: it moves when a logit passes
+        // it by 2^8, and at first.
+        const bool fresh = m[n][0] == -INFINITY || m[n][1] == -INFINITY;
+        if (__any_sync(kFullMask, top > (fresh ? -INFINITY : 8.f))) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float up = fmaxf(z[0][e][0], z[0][e][1]);
+            if constexpr (S::MT == 2) up = fmaxf(up, fmaxf(z[1][e][0], z[1][e][1]));
+            const bool first = m[n][e] == -INFINITY;
+            if (up == -INFINITY || (!first && !(up > 0.f))) continue;
+            l[n][e] = first ? 0.f : l[n][e] * fast_exp2(-up);
+            m[n][e] = first ? up : m[n][e] + up;
+#pragma unroll
+            for (int x = 0; x < S::MT; ++x) z[x][e][0] -= up, z[x][e][1] -= up;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int x = 0; x < S::MT; ++x) l[n][e] += fast_exp2(z[x][e][0]) + fast_exp2(z[x][e][1]);
       }
-  } else {
-    const int64_t j0 = (int64_t)blockIdx.x * S::ROWS;
-    if (j0 >= s.L) return;
-    // the first counted query that sees key j0 or a later one
-    int64_t from = j0 - s.past - s.first;
-    from = from > 0 ? from : 0;
-    const int c0 = from < s.count ? (int)(from / S::COLS) : 0;
-    const int c1 = from < s.count ? (s.count + S::COLS - 1) / S::COLS : 0;
-    float sum[S::MT][2];
+    }
+    if (past_pool) set_status(a.status, B2PA_ERR_BAD_BLOCK_ID);
+    // join: the 8 lanes of a column, then the warps
+    __shared__ float2 joined[4][kCols];
 #pragma unroll
-    for (int x = 0; x < S::MT; ++x) sum[x][0] = sum[x][1] = 0.f;
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float M = m[n][e];
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) M = fmaxf(M, __shfl_xor_sync(kFullMask, M, o));
+        float sum = l[n][e] * fast_exp2(m[n][e] - (M == -INFINITY ? 0.f : M));
+        if (m[n][e] == -INFINITY) sum = l[n][e];  // nothing seen (0), or NaN
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
+        if (g == 0) joined[warp][n * 8 + 2 * t + e] = make_float2(M, sum);
+      }
+    __syncthreads();
+    if (tid < kCols && i0 + tid < s.count) {
+      float M = -INFINITY, sum = 0.f;
+      for (int w = 0; w < 4; ++w) M = fmaxf(M, joined[w][tid].x);
+      for (int w = 0; w < 4; ++w) sum += joined[w][tid].y * fast_exp2(joined[w][tid].x - (M == -INFINITY ? 0.f : M));
+      part[(head * a.T + i0 + tid) * nsplit + split] = make_float2(M, sum);
+    }
+  } else {
     // columns' log-sum-exps, +inf where a query does not count or sees nothing
     auto load_lse = [&](int c, int buf) {
-      for (int r = tid; r < S::COLS; r += kTileThreads) {
-        const int i = c * S::COLS + r;
+      for (int r = tid; r < kCols; r += kTileThreads) {
+        const int i = c * kCols + r;
         float lse = INFINITY;
         if (i < s.count) {
           const float2* p = part + (head * a.T + i) * nsplit;
@@ -470,60 +435,80 @@ __global__ void __launch_bounds__(kTileThreads) key_weights_tile_kernel(KeyWeigh
         col_lse[buf][r] = lse;
       }
     };
-    KeyLoader<T, KV4, D, S::ROWS, S::RB, S::PITCH> keys;
-    if (c0 < c1) {
-      keys.fetch(a, table, h, j0, s.L, smem_u32(rows));
-      load_queries<T, KV4, D, S::COLS, S::RB, S::PITCH>(a, s, h, b, c0 * S::COLS, cols[0], col_unit[0], qscale);
-      load_lse(c0, 0);
-      keys.store(rows);
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    for (int c = c0; c < c1; ++c) {
-      const int buf = (c - c0) & 1;
-      if (c + 1 < c1) {
-        load_queries<T, KV4, D, S::COLS, S::RB, S::PITCH>(a, s, h, b, (c + 1) * S::COLS, cols[buf ^ 1],
-                                                          col_unit[buf ^ 1], qscale);
-        load_lse(c + 1, buf ^ 1);
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      asm volatile("cp.async.wait_group 1;" ::: "memory");
-      __syncthreads();
-      product<S>(rows, cols[buf], acc);
-      // key j is seen by columns at or above j - past - first - c * COLS
-      const int64_t base = j0 - s.past - s.first - (int64_t)c * S::COLS;
-      const bool whole = base + S::ROWS - 1 <= 0;
+    const int chunks = (s.count + kCols - 1) / kCols;
+    int held = -1;  // the only query tile, once loaded
+    for (int64_t j0 = (int64_t)blockIdx.x * S::ROWS; j0 < s.L; j0 += (int64_t)gridDim.x * S::ROWS) {
+      const int64_t w0 = j0 + warp * S::WROWS;
+      keys.load(a, table, h, w0, s.L, blocks, past_pool);
+      float sum[S::MT][2];
 #pragma unroll
-      for (int n = 0; n < S::NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int col = n * 8 + 2 * t + e;
-          const float lse = col_lse[buf][col], unit = O::SCALED ? qscale * col_unit[buf][col] : qscale;
+      for (int x = 0; x < S::MT; ++x) sum[x][0] = sum[x][1] = 0.f;
+      // the first counted query that sees key j0 or a later one
+      int64_t from = j0 - s.past - s.first;
+      from = from > 0 ? from : 0;
+      const int c0 = from < s.count ? (int)(from / kCols) : chunks;
+      auto fetch = [&](int c) {
+        if (c < chunks && !(chunks == 1 && held == 0)) {
+          load_queries<T, KV4, D>(a, s, h, b, c * kCols, queries + (c & 1) * S::Q_BYTES, col_unit[c & 1]);
+          load_lse(c, c & 1);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
+      fetch(c0);
+      for (int c = c0; c < chunks; ++c) {
+        const int buf = c & 1;
+        fetch(c + 1);
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        __syncthreads();
+        // key j is seen by columns at or above j - past - first - 64 c
+        const int64_t base = w0 - s.past - s.first - (int64_t)c * kCols;
+        const int left = s.count - c * kCols;  // columns that are queries
+        const bool plain = base + S::WROWS - 1 <= 0 && left >= kCols;
+#pragma unroll 2
+        for (int n = 0; n < NT; ++n) {
+          keys.product(queries + buf * S::Q_BYTES, n, acc);
+          const int col = n * 8 + 2 * t;
+          const float2 lse = *reinterpret_cast<const float2*>(&col_lse[buf][col]);
+          float2 unit = make_float2(qscale, qscale);
+          if constexpr (O::F32) {
+            const float2 back = *reinterpret_cast<const float2*>(&col_unit[buf][col]);
+            unit.x *= back.x;
+            unit.y *= back.y;
+          }
 #pragma unroll
           for (int x = 0; x < S::MT; ++x)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              const int r = warp * S::MT * 16 + x * 16 + g + 8 * i;
-              const float p = fast_exp2(fmaf(acc[x][n][2 * i + e], unit, -lse));
-              if (whole || base + r <= col) sum[x][i] += p;
+              float u0 = unit.x, u1 = unit.y;
+              if constexpr (S::KPARTS == 2) u0 *= keys.back[x][i], u1 *= keys.back[x][i];
+              float p0 = fast_exp2(fmaf(acc[x][2 * i], u0, -lse.x)), p1 = fast_exp2(fmaf(acc[x][2 * i + 1], u1, -lse.y));
+              if (!plain) {
+                const int64_t r = base + 16 * x + 8 * i + g;
+                if (r > col || col >= left) p0 = 0.f;
+                if (r > col + 1 || col + 1 >= left) p1 = 0.f;
+              }
+              sum[x][i] += p0 + p1;
             }
         }
-      __syncthreads();
-    }
+        __syncthreads();
+      }
+      if (chunks == 1 && c0 == 0) held = 0;
 #pragma unroll
-    for (int x = 0; x < S::MT; ++x)
+      for (int x = 0; x < S::MT; ++x)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        sum[x][i] += __shfl_xor_sync(kFullMask, sum[x][i], 1);
-        sum[x][i] += __shfl_xor_sync(kFullMask, sum[x][i], 2);
-        const int64_t j = j0 + warp * S::MT * 16 + x * 16 + g + 8 * i;
-        if (t == 0 && j < s.L) {
-          const int32_t blk = table[j >> a.bs_log2];
-          if (blk >= 0 && blk < a.num_blocks) {
-            const int64_t at = ((int64_t)blk * a.H + h) * a.block_size + (j & (a.block_size - 1));
+        for (int i = 0; i < 2; ++i) {
+          sum[x][i] += __shfl_xor_sync(kFullMask, sum[x][i], 1);
+          sum[x][i] += __shfl_xor_sync(kFullMask, sum[x][i], 2);
+          const int64_t j = w0 + 16 * x + 8 * i + g;
+          if (t == 0 && keys.ok[x][i]) {
+            const uint32_t blk = (uint32_t)__ldg(table + (j >> a.bs_log2));
+            const uint64_t at = (blk * (uint64_t)a.H + h) * a.block_size + (j & (a.block_size - 1));
             a.w_out[at] = a.w_in[at] + sum[x][i];
           }
         }
-      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (past_pool) set_status(a.status, B2PA_ERR_BAD_BLOCK_ID);
   }
 }
 
@@ -550,7 +535,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kStepThreads) key_weights_step_kernel(KeyWeightArgs a, float qscale, float* far,
                                                                         int64_t far_stride) {
   using S = StepRows<T, D>;
-  using O = Op<T, false>;
+  using O = Op<T>;
   constexpr int RB = S::RB, RW = S::RW, E = 16 / (int)sizeof(T);
   extern __shared__ float near[];
   __shared__ float red[2][kStepThreads / 32];
@@ -725,11 +710,12 @@ __global__ void __launch_bounds__(kStepThreads) key_weights_step_kernel(KeyWeigh
 }
 
 // ------------------------------------------------------------------- launches
-// Key ranges of the first pass: enough CTAs for two waves of four per SM.
-int split_of(int B, int H, int count, int64_t keys, int rows, int cols) {
-  const int64_t tiles = (int64_t)B * H * ((count + rows - 1) / rows);
+// Key ranges of the first pass: enough CTAs for two waves of four per SM,
+// with four tiles of 32 keys a warp.
+int split_of(int B, int H, int count, int64_t keys) {
+  const int64_t tiles = (int64_t)B * H * ((count + kCols - 1) / kCols);
   int ns = 1;
-  while (ns < 16 && tiles * ns < 4 * device_sm_count() && keys >= (int64_t)cols * 4 * ns * 2) ns *= 2;
+  while (ns < 16 && tiles * ns < 4 * device_sm_count() && keys >= 4 * 32 * 4 * ns) ns *= 2;
   return ns;
 }
 
@@ -737,23 +723,30 @@ int counted_most(int T, int window) { return window > 0 && window < T ? window :
 
 template <typename T, bool KV4, int D>
 int tile_launch(const KeyWeightArgs& a, cudaStream_t st) {
-  using S1 = Shape<T, KV4, D, 1>;
-  using S2 = Shape<T, KV4, D, 2>;
+  using S = Shape<T, KV4, D>;
   const float qscale = a.scale * kLog2e;
   const int64_t keys = (int64_t)a.max_pages * a.block_size;
+  if (keys == 0) return B2PA_OK;
   const int count = counted_most(a.T, a.window);
-  const int ns = split_of(a.B, a.H, count, keys, S1::ROWS, S1::COLS);
+  const int ns = split_of(a.B, a.H, count, keys);
   float2* part = static_cast<float2*>(a.workspace);
   auto k1 = key_weights_tile_kernel<T, KV4, D, 1>;
   auto k2 = key_weights_tile_kernel<T, KV4, D, 2>;
-  int rc = set_max_dynamic_smem_cached(reinterpret_cast<const void*>(k1), S1::SMEM);
-  if (rc == B2PA_OK) rc = set_max_dynamic_smem_cached(reinterpret_cast<const void*>(k2), S2::SMEM);
-  if (rc != B2PA_OK || keys == 0) return rc;
-  cudaError_t e = launch_pdl(k1, dim3((unsigned)((count + S1::ROWS - 1) / S1::ROWS * ns), (unsigned)a.H, (unsigned)a.B),
-                             dim3(kTileThreads), S1::SMEM, st, a, qscale, ns, part);
+  int rc = set_max_dynamic_smem_cached(reinterpret_cast<const void*>(k1), S::Q_BYTES);
+  if (rc == B2PA_OK) rc = set_max_dynamic_smem_cached(reinterpret_cast<const void*>(k2), 2 * S::Q_BYTES);
+  if (rc != B2PA_OK) return rc;
+  cudaError_t e = launch_pdl(k1, dim3((unsigned)((count + kCols - 1) / kCols * ns), (unsigned)a.H, (unsigned)a.B),
+                             dim3(kTileThreads), S::Q_BYTES, st, a, qscale, ns, part);
+  // One tile of queries stays in shared memory while a CTA takes several key
+  // tiles; more than one passes by for every key tile.
+  int64_t tiles = (keys + S::ROWS - 1) / S::ROWS;
+  if (count <= kCols) {
+    const int64_t most = (int64_t)8 * device_sm_count() / ((int64_t)a.B * a.H) + 1;
+    tiles = tiles < most ? tiles : most;
+  }
   if (e == cudaSuccess)
-    e = launch_pdl(k2, dim3((unsigned)((keys + S2::ROWS - 1) / S2::ROWS), (unsigned)a.H, (unsigned)a.B),
-                   dim3(kTileThreads), S2::SMEM, st, a, qscale, ns, part);
+    e = launch_pdl(k2, dim3((unsigned)tiles, (unsigned)a.H, (unsigned)a.B), dim3(kTileThreads), 2 * S::Q_BYTES, st, a,
+                   qscale, ns, part);
   if (e != cudaSuccess) return set_error(B2PA_ERR_CUDA, "key_weights launch: %s", cudaGetErrorString(e));
   return B2PA_OK;
 }
