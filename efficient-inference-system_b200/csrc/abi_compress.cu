@@ -153,6 +153,7 @@ int b2pa_kv4_append(const void* k_new, const int64_t new_k_strides[4], const voi
   a.D = D;
   a.block_size = block_size;
   a.dtype = dtype;
+  a.bs_log2 = block_size_log2(block_size);
   a.status = status;
   return launch_kv4_append(a, seq_lens_out, static_cast<cudaStream_t>(stream));
 }
@@ -192,6 +193,7 @@ int b2pa_kv4_read(const void* k_pool, const void* v_pool, int64_t num_blocks, co
   a.D = D;
   a.block_size = block_size;
   a.dtype = dtype;
+  a.bs_log2 = block_size_log2(block_size);
   a.status = status;
   return launch_kv4_read(a, static_cast<cudaStream_t>(stream));
 }

@@ -59,6 +59,7 @@ struct AppendArgs {
   const int32_t* start_pos;
   const int32_t* lengths;
   int B, H, T, D, block_size, dtype;
+  int bs_log2;  // 4-bit pools only
   int32_t* status;
 };
 
@@ -173,6 +174,7 @@ struct Kv4ReadArgs {
   void* v_out;
   int64_t sk[4], sv[4];  // element strides of [B,H,T,D], unit D stride
   int B, H, T, D, block_size, dtype;
+  int bs_log2;
   int32_t* status;
 };
 

@@ -59,10 +59,12 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool ok) {
 }
 
 // ------------------------------------------------------------ several queries
-template <typename T>
+template <typename T, bool KV4>
 struct Op {
-  static constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
-  static constexpr bool F32 = std::is_same<T, float>::value;  // q as two fp16 halves, scaled per row
+  static constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value && !KV4;  // operand type (else fp16)
+  static constexpr bool F32 = std::is_same<T, float>::value;                   // in two fp16 halves
+  static constexpr bool SCALED = F32 || (KV4 && std::is_same<T, __nv_bfloat16>::value);  // q rows, into fp16's range
+  static constexpr bool PREP = F32 || KV4;  // q rows are converted or reordered: once, by the first pass
 };
 
 template <typename O>
@@ -79,7 +81,6 @@ __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, u
 }
 
 __device__ __forceinline__ uint32_t bits_of(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-__device__ __forceinline__ uint32_t bits_of(__nv_bfloat162 h) { return *reinterpret_cast<uint32_t*>(&h); }
 
 // Eight fp32 values, scaled, as fp16 halves hi + lo.
 __device__ __forceinline__ void split8(const float* x, float f, uint4& hi, uint4& lo) {
@@ -104,10 +105,10 @@ __device__ __forceinline__ float range_factor(float top, float& back) {
   return __uint_as_float((uint32_t)(127 + e) << 23);
 }
 
-// One 4-bit word (8 channels of scale code sc) as 4 operand registers, exact.
-__device__ __forceinline__ uint4 unpack_word(uint32_t w, uint32_t sc, __half) {
-  // a masked nibble pair in the mantissa: 1024 + c, and 16 (64 + c) above
-  const __half2 s = __half2half2(__ushort_as_half((unsigned short)(sc << 7)));
+// One 4-bit word (8 channels of scale s) as 4 operand registers, exact, in
+// the order 0 4 1 5 2 6 3 7: a masked nibble pair in the mantissa is 1024 + c,
+// or 16 (64 + c) for the upper nibbles.
+__device__ __forceinline__ uint4 unpack_word(uint32_t w, __half2 s) {
   const __half2 k1032 = __half2half2(__ushort_as_half(0x6408)), k72 = __half2half2(__ushort_as_half(0xd480)),
                 k16th = __half2half2(__ushort_as_half(0x2c00));
   auto lo = [&](uint32_t x) {
@@ -118,20 +119,12 @@ __device__ __forceinline__ uint4 unpack_word(uint32_t w, uint32_t sc, __half) {
     const uint32_t y = (x & 0x00f000f0u) | 0x64006400u;
     return bits_of(__hmul2(__hfma2(*reinterpret_cast<const __half2*>(&y), k16th, k72), s));
   };
-  const uint32_t c04 = lo(w), c15 = hi(w), c26 = lo(w >> 8), c37 = hi(w >> 8);
-  return make_uint4(__byte_perm(c04, c15, 0x5410), __byte_perm(c26, c37, 0x5410), __byte_perm(c04, c15, 0x7632),
-                    __byte_perm(c26, c37, 0x7632));
+  return make_uint4(lo(w), hi(w), lo(w >> 8), hi(w >> 8));
 }
-__device__ __forceinline__ uint4 unpack_word(uint32_t w, uint32_t sc, __nv_bfloat16) {
-  const __nv_bfloat162 s = __float2bfloat162_rn(kv4_scale(sc));  // 4 significant bits
-  const __nv_bfloat162 k136 = __float2bfloat162_rn(136.f);
-  auto pick = [&](uint32_t x) {
-    const uint32_t y = (x & 0x000f000fu) | 0x43004300u;  // 128 + c
-    return bits_of(__hmul2(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&y), k136), s));
-  };
-  const uint32_t c04 = pick(w), c15 = pick(w >> 4), c26 = pick(w >> 8), c37 = pick(w >> 12);
-  return make_uint4(__byte_perm(c04, c15, 0x5410), __byte_perm(c26, c37, 0x5410), __byte_perm(c04, c15, 0x7632),
-                    __byte_perm(c26, c37, 0x7632));
+// Two scale codes, in the low bytes, as pairs.
+__device__ __forceinline__ __half2 scale_pair(uint32_t codes, uint32_t select) {
+  const uint32_t x = __byte_perm(codes, 0, select) << 7;
+  return *reinterpret_cast<const __half2*>(&x);
 }
 
 constexpr int kTileThreads = 128;
@@ -139,14 +132,19 @@ constexpr int kCols = 64;  // queries per tile
 
 template <typename T, bool KV4, int D>
 struct Shape {
-  using O = Op<T>;
+  using O = Op<T, KV4>;
   static constexpr int NB = D < 32 ? 1 : D / 32;          // blocks of 32 channels: two products of 16
   static constexpr int KPARTS = O::F32 && !KV4 ? 2 : 1;   // halves of a key / of a query
   static constexpr int QPARTS = O::F32 ? 2 : 1;
-  static constexpr int MT = NB * KPARTS <= 4 ? 2 : 1;     // 16-row tiles per warp: up to 64 registers of keys
+  // 16-row tiles per warp: two share every load of the queries, while their
+  // fragments fit 64 registers; one leaves room for more warps, which pays
+  // for fp32 (three products a load).  256-query fp32 chunks: 57 us with two,
+  // 51 with one; 4-bit keys, 64 queries: 112 and 144.
+  static constexpr int MT = KPARTS == 1 && NB <= 4 ? 2 : 1;
   static constexpr int WROWS = 16 * MT, ROWS = 4 * WROWS;  // keys per warp and CTA
   static constexpr int PITCH = NB * 64 % 128 == 0 ? NB * 64 + 64 : NB * 64;  // a quarter warp's two rows in other banks
-  static constexpr int Q_BYTES = QPARTS * kCols * PITCH;
+  static constexpr int Q_BYTES = QPARTS * kCols * PITCH;  // a tile of queries
+  static constexpr int Q_SAVED = O::PREP ? Q_BYTES + kCols * 4 : 0;  // ... with its factors, in the workspace
   // where 8 consecutive channels (number c8) of a query row go: 4-bit keys
   // are loaded 16 bytes (4 words) a lane, so word w of lane t is block w's
   __device__ static constexpr int place(int c8) {
@@ -156,15 +154,16 @@ struct Shape {
 };
 
 // Counted queries i0 .. i0 + 63 into shared memory (zeros past the count):
-// copies of the rows, or for fp32 their scaled halves with unit[r], the factor
-// that undoes the scaling.
+// copies of the rows, or what the first pass converts them to, with unit[r]
+// the factor that undoes a row's scaling.
 template <typename T, bool KV4, int D>
 __device__ __forceinline__ void load_queries(const KeyWeightArgs& a, const Span& s, int h, int b, int i0, uint8_t* dst,
                                              float* unit) {
   using S = Shape<T, KV4, D>;
+  using O = typename S::O;
   constexpr int C8 = S::NB * 4;  // 8-channel pieces per row (whole blocks)
   const T* q = static_cast<const T*>(a.q) + (int64_t)b * a.sq[0] + (int64_t)h * a.sq[1];
-  if constexpr (!S::O::F32) {
+  if constexpr (!O::PREP) {
     for (int u = threadIdx.x; u < kCols * C8; u += kTileThreads) {
       const int r = u / C8, c = u % C8;
       const bool ok = i0 + r < s.count && 8 * c < D;
@@ -172,27 +171,54 @@ __device__ __forceinline__ void load_queries(const KeyWeightArgs& a, const Span&
     }
   } else {
     constexpr int LPR = C8 < 32 ? C8 : 32;  // lanes per row
+    constexpr int V = 16 / (int)sizeof(T);
     const int lane = threadIdx.x & 31, c = lane % LPR;
+#pragma unroll 4
     for (int r = (threadIdx.x >> 5) * (32 / LPR) + lane / LPR; r < kCols; r += kTileThreads / LPR) {
-      float x[8] = {}, top = 0.f;
+      float x[8] = {};
       if (i0 + r < s.count && 8 * c < D) {
-        const float4* row = reinterpret_cast<const float4*>(q + (int64_t)(s.first + i0 + r) * a.sq[2] + 8 * c);
-        *reinterpret_cast<float4*>(x) = __ldg(row);
-        *reinterpret_cast<float4*>(x + 4) = __ldg(row + 1);
+        const T* row = q + (int64_t)(s.first + i0 + r) * a.sq[2] + 8 * c;
+#pragma unroll
+        for (int i = 0; i < 8; i += V) {
+          Vec<T, V> v;
+          v.w = ld_global_nc<uint4>(row + i);
+          v.to_float(x + i);
+        }
       }
+      float f = 1.f, back = 1.f;
+      if constexpr (O::SCALED) {
+        float top = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
 #pragma unroll
-      for (int o = LPR / 2; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, o));
-      float back;
-      const float f = range_factor(top, back);
+        for (int o = LPR / 2; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, o));
+        f = range_factor(top, back);
+      }
+      if constexpr (KV4) {  // in the order of unpacked keys
+        const float y[8] = {x[0], x[4], x[1], x[5], x[2], x[6], x[3], x[7]};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = y[i];
+      }
       uint4 hi, lo;
       split8(x, f, hi, lo);
       *reinterpret_cast<uint4*>(dst + r * S::PITCH + S::place(c)) = hi;
-      *reinterpret_cast<uint4*>(dst + kCols * S::PITCH + r * S::PITCH + S::place(c)) = lo;
+      if constexpr (S::QPARTS == 2) *reinterpret_cast<uint4*>(dst + kCols * S::PITCH + r * S::PITCH + S::place(c)) = lo;
       if (c == 0) unit[r] = back;
     }
   }
+}
+
+// A converted tile to and from the workspace.
+template <typename S>
+__device__ __forceinline__ void save_queries(uint8_t* to, const uint8_t* tile, const float* unit) {
+  for (int i = threadIdx.x * 16; i < S::Q_BYTES; i += kTileThreads * 16)
+    *reinterpret_cast<uint4*>(to + i) = *reinterpret_cast<const uint4*>(tile + i);
+  if (threadIdx.x < kCols) reinterpret_cast<float*>(to + S::Q_BYTES)[threadIdx.x] = unit[threadIdx.x];
+}
+template <typename S>
+__device__ __forceinline__ void fetch_saved(uint8_t* tile, float* unit, const uint8_t* from) {
+  for (int i = threadIdx.x * 16; i < S::Q_BYTES; i += kTileThreads * 16) copy16(smem_u32(tile) + i, from + i, true);
+  if (threadIdx.x < kCols / 4) copy16(smem_u32(unit) + 16 * threadIdx.x, from + S::Q_BYTES + 16 * threadIdx.x, true);
 }
 
 // A warp's key rows as operand fragments: rows g and g + 8 of each 16-row tile.
@@ -204,6 +230,14 @@ struct Keys {
   float back[S::MT][2];  // undoes the scaling of fp32 rows
   bool ok[S::MT][2];     // the row is a key (its page exists)
 
+  __device__ __forceinline__ static uint32_t block_of(const KeyWeightArgs& a, const int32_t* table, int64_t j,
+                                                      int64_t end, uint32_t blocks, bool& ok, bool& past_pool) {
+    const uint32_t blk = j < end ? (uint32_t)__ldg(table + (j >> a.bs_log2)) : 0xffffffffu;
+    ok = blk < blocks;
+    past_pool |= (int)blk >= (int)blocks;
+    return ok ? blk : 0u;
+  }
+
   // Rows j0 + 16 m + g (+ 8), those below `end`.
   __device__ __forceinline__ void load(const KeyWeightArgs& a, const int32_t* table, int h, int64_t j0, int64_t end,
                                        uint32_t blocks, bool& past_pool) {
@@ -213,32 +247,29 @@ struct Keys {
     for (int m = 0; m < S::MT; ++m)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int64_t j = j0 + 16 * m + 8 * i + g;
-        uint32_t blk = j < end ? (uint32_t)__ldg(table + (j >> a.bs_log2)) : 0xffffffffu;
-        ok[m][i] = blk < blocks;
-        past_pool |= (int)blk >= (int)blocks;
-        blk = ok[m][i] ? blk : 0u;
-        const int row = (int)(j & (bs - 1));
         uint4(&f)[S::NB] = x[m][i];
+        const int64_t j = j0 + 16 * m + 8 * i + g;
+        const uint32_t blk = block_of(a, table, j, end, blocks, ok[m][i], past_pool);
+        const int row = (int)(j & (bs - 1));
         if constexpr (KV4) {
           const uint8_t* page = static_cast<const uint8_t*>(a.k_pool) +
                                 (uint64_t)(blk * (uint64_t)a.H + h) * (uint32_t)kv4_page_bytes(bs, D);
           const uint8_t* scales = page + bs * (D / 2) + row * (D / 16);
-          using E = typename std::conditional<S::O::BF16, __nv_bfloat16, __half>::type;
           if constexpr (D == 64) {
             const uint2 w = __ldg(reinterpret_cast<const uint2*>(page + row * 32 + 8 * t));
-            const uint32_t sc = __ldg(scales + t);
-            f[0] = unpack_word(w.x, sc, E{});
-            f[1] = unpack_word(w.y, sc, E{});
+            const __half2 sc = scale_pair(__ldg(scales + t), 0x4040);
+            f[0] = unpack_word(w.x, sc);
+            f[1] = unpack_word(w.y, sc);
           } else {
 #pragma unroll
             for (int c = 0; c < D / 128; ++c) {
               const uint4 w = __ldg(reinterpret_cast<const uint4*>(page + row * (D / 2) + 64 * c + 16 * t));
               const uint32_t sc = __ldg(reinterpret_cast<const uint16_t*>(scales + 8 * c + 2 * t));
-              f[4 * c + 0] = unpack_word(w.x, sc & 255u, E{});
-              f[4 * c + 1] = unpack_word(w.y, sc & 255u, E{});
-              f[4 * c + 2] = unpack_word(w.z, sc >> 8, E{});
-              f[4 * c + 3] = unpack_word(w.w, sc >> 8, E{});
+              const __half2 s0 = scale_pair(sc, 0x4040), s1 = scale_pair(sc, 0x4141);
+              f[4 * c + 0] = unpack_word(w.x, s0);
+              f[4 * c + 1] = unpack_word(w.y, s0);
+              f[4 * c + 2] = unpack_word(w.z, s1);
+              f[4 * c + 3] = unpack_word(w.w, s1);
             }
           }
         } else {
@@ -307,12 +338,12 @@ struct Keys {
 // each query over one of nsplit ranges of keys goes to part[query][split].
 // PASS 2: grid (key tiles, taken in turn; head; sequence).
 template <typename T, bool KV4, int D, int PASS>
-__global__ void __launch_bounds__(kTileThreads) key_weights_tile_kernel(KeyWeightArgs a, float qscale, int nsplit,
-                                                                        float2* part) {
+__global__ void __launch_bounds__(kTileThreads, Shape<T, KV4, D>::KPARTS == 2 && D <= 128 ? 4 : 0) key_weights_tile_kernel(KeyWeightArgs a, float qscale, int nsplit,
+                                                                        float2* part, uint8_t* saved, int chunks_most) {
   using S = Shape<T, KV4, D>;
   using O = typename S::O;
   extern __shared__ __align__(16) uint8_t queries[];  // PASS 2: two tiles
-  __shared__ float col_unit[2][kCols], col_lse[2][kCols];
+  __shared__ __align__(16) float col_unit[2][kCols], col_lse[2][kCols];
   pdl_wait();
   pdl_launch_dependents();
   const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
@@ -336,63 +367,91 @@ __global__ void __launch_bounds__(kTileThreads) key_weights_tile_kernel(KeyWeigh
     load_queries<T, KV4, D>(a, s, h, b, i0, queries, col_unit[0]);
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
+    if (O::PREP && split == 0) save_queries<S>(saved + (head * chunks_most + tile) * S::Q_SAVED, queries, col_unit[0]);
     const int last = i0 + kCols < s.count ? i0 + kCols : s.count;
     int64_t kend = s.past + s.first + last;  // keys that the last of the queries sees
     kend = kend < s.L ? kend : s.L;
-    const int64_t tiles = kend > 0 ? (kend + S::WROWS - 1) / S::WROWS : 0;
     const int64_t whole = s.past + s.first + i0 + 1;  // keys below it are seen by every query
-    // per column (8n + 2t + e): reference and sum of exp2(logit - reference)
+    // Per column (8n + 2t + e): reference and sum of exp2(logit - reference)
+    // over the rows of this lane.  The reference need not be the maximum: it
+    // moves when a logit passes it by 2^8.
     float m[NT][2], l[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.f;
-    for (int64_t c = split * 4 + warp; c < tiles; c += nsplit * 4) {
-      const int64_t j0 = c * S::WROWS;
+    bool set = false;  // every column of this warp has a reference
+    const int64_t turn = (int64_t)nsplit * 4 * S::WROWS;
+    const int64_t start = ((int64_t)split * 4 + warp) * S::WROWS;
+    for (int64_t j0 = start; j0 < kend; j0 += turn) {
       keys.load(a, table, h, j0, kend, blocks, past_pool);
       bool plain = j0 + S::WROWS <= whole;
 #pragma unroll
       for (int x = 0; x < S::MT; ++x) plain = plain && keys.ok[x][0] && keys.ok[x][1];
       plain = __all_sync(kFullMask, plain);
+      auto unit_of = [&](int col, int x, int i) {
+        float u = O::SCALED ? qscale * col_unit[0][col] : qscale;
+        if constexpr (S::KPARTS == 2) u *= keys.back[x][i];
+        return u;
+      };
+      auto highest = [&](const float (&z)[S::MT][2]) {
+        float up = fmaxf(z[0][0], z[0][1]);
+        if constexpr (S::MT == 2) up = fmaxf(up, fmaxf(z[1][0], z[1][1]));
+        return up;
+      };
+      if (plain && set) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        keys.product(queries, n, acc);
-        float z[S::MT][2][2];  // [tile][column][row]
-        float top = -INFINITY;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int col = n * 8 + 2 * t + e;
-          const float unit = O::F32 ? qscale * col_unit[0][col] : qscale;
-#pragma unroll
-          for (int x = 0; x < S::MT; ++x)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              float u = unit;
-              if constexpr (S::KPARTS == 2) u *= keys.back[x][i];
-              z[x][e][i] = fmaf(acc[x][2 * i + e], u, m[n][e] == -INFINITY ? 0.f : -m[n][e]);
-              if (!plain && !(keys.ok[x][i] && j0 + 16 * x + 8 * i + g < whole + col)) z[x][e][i] = -INFINITY;
-            }
-        }
-#pragma unroll
-        for (int x = 0; x < S::MT; ++x) top = fmaxf(top, fmaxf(fmaxf(z[x][0][0], z[x][0][1]), fmaxf(z[x][1][0], z[x][1][1])));
-        // The reference need not be the maximum: it moves when a logit passes
-        // it by 2^8, and at first.
-        const bool fresh = m[n][0] == -INFINITY || m[n][1] == -INFINITY;
-        if (__any_sync(kFullMask, top > (fresh ? -INFINITY : 8.f))) {
+        for (int n = 0; n < NT; ++n) {
+          keys.product(queries, n, acc);
+          float z[2][S::MT][2], top[2];  // logit - reference
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float up = fmaxf(z[0][e][0], z[0][e][1]);
-            if constexpr (S::MT == 2) up = fmaxf(up, fmaxf(z[1][e][0], z[1][e][1]));
-            const bool first = m[n][e] == -INFINITY;
-            if (up == -INFINITY || (!first && !(up > 0.f))) continue;
-            l[n][e] = first ? 0.f : l[n][e] * fast_exp2(-up);
-            m[n][e] = first ? up : m[n][e] + up;
 #pragma unroll
-            for (int x = 0; x < S::MT; ++x) z[x][e][0] -= up, z[x][e][1] -= up;
+            for (int x = 0; x < S::MT; ++x)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) z[e][x][i] = fmaf(acc[x][2 * i + e], unit_of(n * 8 + 2 * t + e, x, i), -m[n][e]);
+            top[e] = highest(z[e]);
+          }
+          if (__any_sync(kFullMask, fmaxf(top[0], top[1]) > 8.f)) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if (top[e] > 8.f) {
+                l[n][e] *= fast_exp2(-top[e]);
+                m[n][e] += top[e];
+#pragma unroll
+                for (int x = 0; x < S::MT; ++x) z[e][x][0] -= top[e], z[e][x][1] -= top[e];
+              }
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int x = 0; x < S::MT; ++x) l[n][e] += fast_exp2(z[e][x][0]) + fast_exp2(z[e][x][1]);
+        }
+      } else {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          keys.product(queries, n, acc);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int col = n * 8 + 2 * t + e;
+            float z[S::MT][2];  // logit
+#pragma unroll
+            for (int x = 0; x < S::MT; ++x)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                z[x][i] = acc[x][2 * i + e] * unit_of(col, x, i);
+                if (!(keys.ok[x][i] && j0 + 16 * x + 8 * i + g < whole + col)) z[x][i] = -INFINITY;
+              }
+            const float up = fmaxf(m[n][e], highest(z)), ref = up == -INFINITY ? 0.f : up;
+            l[n][e] = m[n][e] == -INFINITY ? l[n][e] : l[n][e] * fast_exp2(m[n][e] - ref);
+            m[n][e] = up;
+#pragma unroll
+            for (int x = 0; x < S::MT; ++x) l[n][e] += fast_exp2(z[x][0] - ref) + fast_exp2(z[x][1] - ref);
           }
         }
+        // (a column whose logits are all -inf or NaN keeps the careful path)
+        bool all_set = true;
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-          for (int x = 0; x < S::MT; ++x) l[n][e] += fast_exp2(z[x][e][0]) + fast_exp2(z[x][e][1]);
+        for (int n = 0; n < NT; ++n) all_set = all_set && m[n][0] > -INFINITY && m[n][1] > -INFINITY;
+        set = __all_sync(kFullMask, all_set);
       }
     }
     if (past_pool) set_status(a.status, B2PA_ERR_BAD_BLOCK_ID);
@@ -437,8 +496,9 @@ __global__ void __launch_bounds__(kTileThreads) key_weights_tile_kernel(KeyWeigh
     };
     const int chunks = (s.count + kCols - 1) / kCols;
     int held = -1;  // the only query tile, once loaded
-    for (int64_t j0 = (int64_t)blockIdx.x * S::ROWS; j0 < s.L; j0 += (int64_t)gridDim.x * S::ROWS) {
-      const int64_t w0 = j0 + warp * S::WROWS;
+    const int64_t turn = (int64_t)gridDim.x * S::ROWS, mine = warp * S::WROWS;
+    for (int64_t j0 = (int64_t)blockIdx.x * S::ROWS; j0 < s.L; j0 += turn) {
+      const int64_t w0 = j0 + mine;
       keys.load(a, table, h, w0, s.L, blocks, past_pool);
       float sum[S::MT][2];
 #pragma unroll
@@ -449,7 +509,11 @@ __global__ void __launch_bounds__(kTileThreads) key_weights_tile_kernel(KeyWeigh
       const int c0 = from < s.count ? (int)(from / kCols) : chunks;
       auto fetch = [&](int c) {
         if (c < chunks && !(chunks == 1 && held == 0)) {
-          load_queries<T, KV4, D>(a, s, h, b, c * kCols, queries + (c & 1) * S::Q_BYTES, col_unit[c & 1]);
+          uint8_t* to = queries + (c & 1) * S::Q_BYTES;
+          if constexpr (O::PREP)
+            fetch_saved<S>(to, col_unit[c & 1], saved + (head * chunks_most + c) * S::Q_SAVED);
+          else
+            load_queries<T, KV4, D>(a, s, h, b, c * kCols, to, col_unit[c & 1]);
           load_lse(c, c & 1);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -464,32 +528,38 @@ __global__ void __launch_bounds__(kTileThreads) key_weights_tile_kernel(KeyWeigh
         const int64_t base = w0 - s.past - s.first - (int64_t)c * kCols;
         const int left = s.count - c * kCols;  // columns that are queries
         const bool plain = base + S::WROWS - 1 <= 0 && left >= kCols;
+        auto add = [&](auto masked) {
 #pragma unroll 2
-        for (int n = 0; n < NT; ++n) {
-          keys.product(queries + buf * S::Q_BYTES, n, acc);
-          const int col = n * 8 + 2 * t;
-          const float2 lse = *reinterpret_cast<const float2*>(&col_lse[buf][col]);
-          float2 unit = make_float2(qscale, qscale);
-          if constexpr (O::F32) {
-            const float2 back = *reinterpret_cast<const float2*>(&col_unit[buf][col]);
-            unit.x *= back.x;
-            unit.y *= back.y;
-          }
-#pragma unroll
-          for (int x = 0; x < S::MT; ++x)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              float u0 = unit.x, u1 = unit.y;
-              if constexpr (S::KPARTS == 2) u0 *= keys.back[x][i], u1 *= keys.back[x][i];
-              float p0 = fast_exp2(fmaf(acc[x][2 * i], u0, -lse.x)), p1 = fast_exp2(fmaf(acc[x][2 * i + 1], u1, -lse.y));
-              if (!plain) {
-                const int64_t r = base + 16 * x + 8 * i + g;
-                if (r > col || col >= left) p0 = 0.f;
-                if (r > col + 1 || col + 1 >= left) p1 = 0.f;
-              }
-              sum[x][i] += p0 + p1;
+          for (int n = 0; n < NT; ++n) {
+            keys.product(queries + buf * S::Q_BYTES, n, acc);
+            const int col = n * 8 + 2 * t;
+            const float2 lse = *reinterpret_cast<const float2*>(&col_lse[buf][col]);
+            float2 unit = make_float2(qscale, qscale);
+            if constexpr (O::SCALED) {
+              const float2 back = *reinterpret_cast<const float2*>(&col_unit[buf][col]);
+              unit.x *= back.x;
+              unit.y *= back.y;
             }
-        }
+#pragma unroll
+            for (int x = 0; x < S::MT; ++x)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                float u0 = unit.x, u1 = unit.y;
+                if constexpr (S::KPARTS == 2) u0 *= keys.back[x][i], u1 *= keys.back[x][i];
+                float p0 = fast_exp2(fmaf(acc[x][2 * i], u0, -lse.x)), p1 = fast_exp2(fmaf(acc[x][2 * i + 1], u1, -lse.y));
+                if constexpr (decltype(masked)::value) {
+                  const int64_t r = base + 16 * x + 8 * i + g;
+                  if (r > col || col >= left) p0 = 0.f;
+                  if (r > col + 1 || col + 1 >= left) p1 = 0.f;
+                }
+                sum[x][i] += p0 + p1;
+              }
+          }
+        };
+        if (plain)
+          add(std::false_type{});
+        else
+          add(std::true_type{});
         __syncthreads();
       }
       if (chunks == 1 && c0 == 0) held = 0;
@@ -535,7 +605,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kStepThreads) key_weights_step_kernel(KeyWeightArgs a, float qscale, float* far,
                                                                         int64_t far_stride) {
   using S = StepRows<T, D>;
-  using O = Op<T>;
+  using O = Op<T, false>;
   constexpr int RB = S::RB, RW = S::RW, E = 16 / (int)sizeof(T);
   extern __shared__ float near[];
   __shared__ float red[2][kStepThreads / 32];
@@ -710,13 +780,18 @@ __global__ void __launch_bounds__(kStepThreads) key_weights_step_kernel(KeyWeigh
 }
 
 // ------------------------------------------------------------------- launches
-// Key ranges of the first pass: enough CTAs for two waves of four per SM,
-// with four tiles of 32 keys a warp.
-int split_of(int B, int H, int count, int64_t keys) {
+size_t up256(size_t x) { return (x + 255) / 256 * 256; }
+
+// Key ranges of the first pass: one wave of per_sm CTAs per SM, with
+// two tiles of 32 keys a warp.  A CTA costs 4 us beside its keys (lengths,
+// then queries, then a table entry, then keys), so more and smaller ones are
+// slower.
+int split_of(int B, int H, int count, int64_t keys, int per_sm) {
   const int64_t tiles = (int64_t)B * H * ((count + kCols - 1) / kCols);
-  int ns = 1;
-  while (ns < 16 && tiles * ns < 4 * device_sm_count() && keys >= 4 * 32 * 4 * ns) ns *= 2;
-  return ns;
+  int64_t ns = per_sm * device_sm_count() / tiles;
+  const int64_t most = keys / (4 * 32 * 2);
+  ns = ns < most ? ns : most;
+  return ns < 1 ? 1 : ns > 16 ? 16 : (int)ns;
 }
 
 int counted_most(int T, int window) { return window > 0 && window < T ? window : T; }
@@ -728,15 +803,17 @@ int tile_launch(const KeyWeightArgs& a, cudaStream_t st) {
   const int64_t keys = (int64_t)a.max_pages * a.block_size;
   if (keys == 0) return B2PA_OK;
   const int count = counted_most(a.T, a.window);
-  const int ns = split_of(a.B, a.H, count, keys);
+  const int ns = split_of(a.B, a.H, count, keys, S::KPARTS == 2 ? 4 : 3);
   float2* part = static_cast<float2*>(a.workspace);
+  const int chunks = (count + kCols - 1) / kCols;
+  uint8_t* saved = static_cast<uint8_t*>(a.workspace) + up256((size_t)a.B * a.H * a.T * 16 * sizeof(float2));
   auto k1 = key_weights_tile_kernel<T, KV4, D, 1>;
   auto k2 = key_weights_tile_kernel<T, KV4, D, 2>;
   int rc = set_max_dynamic_smem_cached(reinterpret_cast<const void*>(k1), S::Q_BYTES);
   if (rc == B2PA_OK) rc = set_max_dynamic_smem_cached(reinterpret_cast<const void*>(k2), 2 * S::Q_BYTES);
   if (rc != B2PA_OK) return rc;
   cudaError_t e = launch_pdl(k1, dim3((unsigned)((count + kCols - 1) / kCols * ns), (unsigned)a.H, (unsigned)a.B),
-                             dim3(kTileThreads), S::Q_BYTES, st, a, qscale, ns, part);
+                             dim3(kTileThreads), S::Q_BYTES, st, a, qscale, ns, part, saved, chunks);
   // One tile of queries stays in shared memory while a CTA takes several key
   // tiles; more than one passes by for every key tile.
   int64_t tiles = (keys + S::ROWS - 1) / S::ROWS;
@@ -746,7 +823,7 @@ int tile_launch(const KeyWeightArgs& a, cudaStream_t st) {
   }
   if (e == cudaSuccess)
     e = launch_pdl(k2, dim3((unsigned)tiles, (unsigned)a.H, (unsigned)a.B), dim3(kTileThreads), 2 * S::Q_BYTES, st, a,
-                   qscale, ns, part);
+                   qscale, ns, part, saved, chunks);
   if (e != cudaSuccess) return set_error(B2PA_ERR_CUDA, "key_weights launch: %s", cudaGetErrorString(e));
   return B2PA_OK;
 }
@@ -814,13 +891,19 @@ int weights_as(const KeyWeightArgs& a, cudaStream_t s) {
 }  // namespace
 
 size_t key_weights_workspace(int B, int H, int T, int D, int max_pages, int block_size, int dtype, int pool_dtype) {
-  (void)D, (void)dtype;
   const int64_t keys = (int64_t)max_pages * block_size;
   if (T == 1 && pool_dtype != B2PA_DTYPE_KV4) {
     const int ns = step_split((int64_t)B * H, keys);
     return (keys + ns - 1) / ns > kNearKeys ? (size_t)B * H * keys * sizeof(float) : 0;
   }
-  return (size_t)B * H * T * 16 * sizeof(float2);
+  // the first pass's partials, then its converted queries: at most two fp16
+  // halves a channel, rows padded by a block, and a factor each
+  size_t saved = 0;
+  if (pool_dtype == B2PA_DTYPE_KV4 || dtype == B2PA_DTYPE_F32) {
+    const size_t blocks = D < 32 ? 1 : D / 32, parts = dtype == B2PA_DTYPE_F32 ? 2 : 1;
+    saved = (size_t)B * H * ((T + kCols - 1) / kCols) * (parts * kCols * (blocks + 1) * 64 + kCols * 4);
+  }
+  return up256((size_t)B * H * T * 16 * sizeof(float2)) + saved;
 }
 
 int launch_key_weights(const KeyWeightArgs& a, cudaStream_t s) {

@@ -60,23 +60,95 @@ __device__ __forceinline__ uint32_t kv4_scale_code(uint32_t max_bits) {
 }
 
 // Eight codes of one group, packed; s is the value of its scale code.
+template <typename T>
 __device__ __forceinline__ uint32_t kv4_pack8(const float* x, float s) {
+  if (!(s > 0.f)) return 0x88888888u;  // a zero scale, or a NaN: zeros
   uint32_t w = 0;
+  if constexpr (std::is_same<T, float>::value) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    int c = 0;
-    if (s > 0.f) {  // false for a zero scale and for a NaN
-      c = __float2int_rn(__fdiv_rn(x[i], s));
+    for (int i = 0; i < 8; ++i) {
+      int c = __float2int_rn(__fdiv_rn(x[i], s));
       c = c < -7 ? -7 : (c > 7 ? 7 : c);
+      w |= (uint32_t)(c + 8) << (4 * i);
     }
-    w |= (uint32_t)(c + 8) << (4 * i);
+  } else {
+    // 16-bit x: |x| times the two neighbours of 1 / s, each rounded to an
+    // integer in the addition to 1.5 * 2^23.  A neighbour is off by less than
+    // 2^-22 and x has at most 11 bits, so the two agree unless x lies on a
+    // border, where they differ by one: the even one is taken.  About 9
+    // instructions a value where the division takes over 16.
+    const float r = __frcp_rn(s), e = fmaf(s, r, -1.f);
+    const float up = e < 0.f ? __uint_as_float(__float_as_uint(r) + 1u) : r;
+    const float down = e > 0.f ? __uint_as_float(__float_as_uint(r) - 1u) : r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t u = __float_as_uint(fmaf(fabsf(x[i]), up, 12582912.f));
+      const uint32_t d = __float_as_uint(fmaf(fabsf(x[i]), down, 12582912.f));
+      uint32_t c = (u ^ ((u ^ d) & u & 1u)) & 15u;
+      c = c < 7u ? c : 7u;
+      w += (x[i] < 0.f ? 8u - c : 8u + c) << (4 * i);
+    }
   }
   return w;
 }
 
+// Eight values of one group, exact.
+// fp32: a nibble in the mantissa of 2^23, one subtraction, one multiplication
+// (packed pairs).
 __device__ __forceinline__ void kv4_unpack8(uint32_t w, float s, float* x) {
+  const float2 m = make_float2(-8388616.f, -8388616.f), z = make_float2(0.f, 0.f), ss = make_float2(s, s);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = (float)((int)((w >> (4 * i)) & 15u) - 8) * s;
+  for (int i = 0; i < 8; i += 2) {
+    float2 v = make_float2(__uint_as_float((w >> (4 * i) & 15u) | 0x4b000000u),
+                           __uint_as_float((w >> (4 * i + 4) & 15u) | 0x4b000000u));
+    v = fma2(add2(v, m), ss, z);
+    x[i] = v.x;
+    x[i + 1] = v.y;
+  }
+}
+// 16-bit types: the same two steps on the pairs that a mask leaves (channels
+// i and i + 4), then the pairs in order.
+__device__ __forceinline__ uint4 kv4_in_order(uint32_t c04, uint32_t c15, uint32_t c26, uint32_t c37) {
+  return make_uint4(__byte_perm(c04, c15, 0x5410), __byte_perm(c26, c37, 0x5410), __byte_perm(c04, c15, 0x7632),
+                    __byte_perm(c26, c37, 0x7632));
+}
+__device__ __forceinline__ uint4 kv4_unpack8(uint32_t w, uint32_t code, __half) {
+  const __half2 s = __half2half2(__ushort_as_half((unsigned short)(code << 7)));
+  const __half2 k1032 = __half2half2(__ushort_as_half(0x6408)), k72 = __half2half2(__ushort_as_half(0xd480)),
+                k16th = __half2half2(__ushort_as_half(0x2c00));
+  auto lo = [&](uint32_t x) {  // 1024 + c
+    const uint32_t y = (x & 0x000f000fu) | 0x64006400u;
+    const __half2 v = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&y), k1032), s);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  };
+  auto hi = [&](uint32_t x) {  // 16 (64 + c)
+    const uint32_t y = (x & 0x00f000f0u) | 0x64006400u;
+    const __half2 v = __hmul2(__hfma2(*reinterpret_cast<const __half2*>(&y), k16th, k72), s);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  };
+  return kv4_in_order(lo(w), hi(w), lo(w >> 8), hi(w >> 8));
+}
+__device__ __forceinline__ uint4 kv4_unpack8(uint32_t w, uint32_t code, __nv_bfloat16) {
+  const __nv_bfloat162 s = __float2bfloat162_rn(kv4_scale(code)), k136 = __float2bfloat162_rn(136.f);
+  auto pick = [&](uint32_t x) {
+    const uint32_t y = (x & 0x000f000fu) | 0x43004300u;  // 128 + c
+    const __nv_bfloat162 v = __hmul2(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&y), k136), s);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  };
+  return kv4_in_order(pick(w), pick(w >> 4), pick(w >> 8), pick(w >> 12));
+}
+
+// Eight values of one group, to 16-byte aligned memory.
+template <typename T>
+__device__ __forceinline__ void kv4_store8(T* dst, uint32_t w, uint32_t code) {
+  if constexpr (std::is_same<T, float>::value) {
+    float x[8];
+    kv4_unpack8(w, kv4_scale(code), x);
+    reinterpret_cast<float4*>(dst)[0] = make_float4(x[0], x[1], x[2], x[3]);
+    reinterpret_cast<float4*>(dst)[1] = make_float4(x[4], x[5], x[6], x[7]);
+  } else {
+    *reinterpret_cast<uint4*>(dst) = kv4_unpack8(w, code, T{});
+  }
 }
 
 }  // namespace b2pa

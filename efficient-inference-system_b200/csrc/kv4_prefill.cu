@@ -31,27 +31,23 @@ __global__ void __launch_bounds__(256) kv4_unpack_kernel(AttnArgs a, T* k_out, T
   if (threadIdx.x == 0) table[slot] = blk >= 0 ? (int32_t)slot : -1;
   if (blk < 0) return;
   const int page_bytes = kv4_page_bytes(BS, D), codes = BS * (D / 2);
-  const int wpr = D / 8, per_head = BS * wpr, total = a.H * per_head;
-  constexpr int N = 16 / (int)sizeof(T);
-  for (int i = threadIdx.x; i < total; i += blockDim.x) {
-    const int h = i / per_head, r = i - h * per_head;
-    const int row = r / wpr, w = r - row * wpr;
-    const uint8_t* kh = static_cast<const uint8_t*>(a.k_pool) + ((int64_t)blk * a.H + h) * page_bytes;
-    const uint8_t* vh = static_cast<const uint8_t*>(a.v_pool) + ((int64_t)blk * a.H + h) * page_bytes;
-    float xk[8] = {}, xv[8] = {};
-    if (first + row < L) {
-      kv4_unpack8(*reinterpret_cast<const uint32_t*>(kh + 4 * r), kv4_scale(kh[codes + row * (D / 16) + w / 2]), xk);
-      kv4_unpack8(*reinterpret_cast<const uint32_t*>(vh + 4 * r), kv4_scale(vh[codes + (w / 2) * BS + row]), xv);
-    }
-    const int64_t o = (slot * a.H * per_head + i) * 8;
-#pragma unroll
-    for (int c = 0; c < 8; c += N) {
-      Vec<T, N> k, v;
-      k.from_float(xk + c);
-      v.from_float(xv + c);
-      *reinterpret_cast<uint4*>(k_out + o + c) = k.w;
-      *reinterpret_cast<uint4*>(v_out + o + c) = v.w;
-    }
+  const int wpr_log2 = 31 - __clz(D / 8), head_log2 = wpr_log2 + (31 - __clz(BS));  // words per row, per head page
+  const uint8_t* kp = static_cast<const uint8_t*>(a.k_pool) + (uint64_t)blk * a.H * page_bytes;
+  const uint8_t* vp = static_cast<const uint8_t*>(a.v_pool) + (uint64_t)blk * a.H * page_bytes;
+  T* ko = k_out + ((slot * a.H) << head_log2) * 8;
+  T* vo = v_out + ((slot * a.H) << head_log2) * 8;
+  const int rows = L - first < BS ? (int)(L - first) : BS;  // the others are zeros
+#pragma unroll 2
+  for (int i = threadIdx.x; i < a.H << head_log2; i += blockDim.x) {
+    const int h = i >> head_log2, r = i & ((1 << head_log2) - 1);  // word r of the head's page
+    const int row = r >> wpr_log2, g = (r & ((1 << wpr_log2) - 1)) >> 1;
+    const uint8_t* kh = kp + h * page_bytes;
+    const uint8_t* vh = vp + h * page_bytes;
+    uint32_t wk = *reinterpret_cast<const uint32_t*>(kh + 4 * r), wv = *reinterpret_cast<const uint32_t*>(vh + 4 * r);
+    uint32_t ck = kh[codes + row * (D / 16) + g], cv = vh[codes + g * BS + row];
+    if (row >= rows) wk = wv = 0x88888888u, ck = cv = 0;
+    kv4_store8(ko + (int64_t)i * 8, wk, ck);
+    kv4_store8(vo + (int64_t)i * 8, wv, cv);
   }
 }
 
