@@ -21,15 +21,16 @@
 // 4-bit keys unpacked (exactly) to the type of q; fp32 as two fp16 halves each
 // (22 bits, three products), rows scaled by powers of two into fp16's range.
 //
-// One query (key_weights_step_kernel, plain pools): bound by reading K once.
+// One query (key_weights_step_kernel): bound by reading K once.
 // A cluster of CTAs shares a sequence, each keeps its logits in shared
 // memory, and after one exchange of (maximum, sum) writes its own weights:
-// one launch.  4-bit pools take the decode kernel's K half (kv4_decode.cu).
+// one launch.  4-bit keys take the product of the decode kernel (kv4_mma.cuh).
 #include <cooperative_groups.h>
 
 #include "common.cuh"
 #include "kernels.h"
 #include "kv4.cuh"
+#include "kv4_mma.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -589,22 +590,24 @@ constexpr int kStepThreads = 256;
 // lie: a lane loads its fragment (16 bytes of row g and of row g + 8 per 64
 // bytes of row), and the one query stands in all 8 columns, so every lane gets
 // its rows' logits without a conversion or a shuffle.  fp32 rows are summed by
-// the lanes that share a row.
-template <typename T, int D>
+// the lanes that share a row.  4-bit rows: packed words and scale codes, as
+// KeyQuery wants them.
+template <typename T, bool KV4, int D>
 struct StepRows {
-  static constexpr int RB = D * (int)sizeof(T);
+  static constexpr int RB = KV4 ? D / 2 : D * (int)sizeof(T);
   static constexpr bool MMA = sizeof(T) == 2;
   // MMA: 64-byte blocks per row, 16-row tiles per turn (8 loads in flight)
   static constexpr int NB = RB < 64 ? 1 : RB / 64, TILES = NB < 4 ? 4 / NB : 1;
   // else: lanes per row, 16-byte pieces per lane, rows per load, rows per lane
   static constexpr int LPR = RB / 16 < 32 ? RB / 16 : 32, CPL = RB / 16 / LPR, RP = 32 / LPR, R = 8 / CPL;
-  static constexpr int RW = MMA ? 16 * TILES : RP * R;  // rows per warp and turn
+  static constexpr int PACKED = D == 256 ? 2 : 4;  // 16-row tiles of 4-bit rows per turn
+  static constexpr int RW = KV4 ? 16 * PACKED : MMA ? 16 * TILES : RP * R;  // rows per warp and turn
 };
 
-template <typename T, int D>
+template <typename T, bool KV4, int D>
 __global__ void __launch_bounds__(kStepThreads) key_weights_step_kernel(KeyWeightArgs a, float qscale, float* far,
                                                                         int64_t far_stride) {
-  using S = StepRows<T, D>;
+  using S = StepRows<T, KV4, D>;
   using O = Op<T, false>;
   constexpr int RB = S::RB, RW = S::RW, E = 16 / (int)sizeof(T);
   extern __shared__ float near[];
@@ -628,8 +631,9 @@ __global__ void __launch_bounds__(kStepThreads) key_weights_step_kernel(KeyWeigh
   // logits of this CTA's keys
   float* z = far ? far + ((int64_t)b * a.H + h) * far_stride + lo : near;
   const int seen = vis < hi ? vis : hi;  // keys [lo, seen) have a logit
-  const char* const pages = static_cast<const char*>(a.k_pool) + (int64_t)h * bs * RB;
-  const uint64_t block_bytes = (uint64_t)a.H * bs * RB;
+  const uint32_t page_bytes = KV4 ? kv4_page_bytes(bs, D) : bs * RB;
+  const char* const pages = static_cast<const char*>(a.k_pool) + (int64_t)h * page_bytes;
+  const uint64_t block_bytes = (uint64_t)a.H * page_bytes;
   const T* const q = static_cast<const T*>(a.q) + (int64_t)b * a.sq[0] + (int64_t)h * a.sq[1];
 
   float top = -INFINITY;
@@ -641,14 +645,61 @@ __global__ void __launch_bounds__(kStepThreads) key_weights_step_kernel(KeyWeigh
   int64_t j0 = lo + warp * RW;
   int ids = ids_of(j0);
   bool past_pool = false;
-  // Row j of the turn at j0: where it is (block 0 for one that is not seen).
-  auto locate = [&](int64_t j, bool& ok) -> const char* {
+  // Row j of the turn at j0: its page (block 0's for one that is not seen).
+  auto page_of = [&](int64_t j, bool& ok) -> const char* {
     const uint32_t blk = (uint32_t)__shfl_sync(kFullMask, ids, (int)((j >> sh) - (j0 >> sh)));
     ok = j < seen && blk < blocks;
     past_pool |= j < seen && (int)blk >= (int)blocks;
-    return pages + (ok ? blk : 0u) * block_bytes + (int)(j & (bs - 1)) * RB;
+    return pages + (ok ? blk : 0u) * block_bytes;
   };
-  if constexpr (S::MMA) {
+  auto locate = [&](int64_t j, bool& ok) -> const char* { return page_of(j, ok) + (int)(j & (bs - 1)) * RB; };
+  if constexpr (KV4) {
+    using W = KeyWords<D>;
+    using Q = KeyQuery<T, D>;
+    const int g = lane >> 2, t = lane & 3;
+    Q query;
+    query.load(q);
+    query.prepare(qscale);
+    for (; j0 < seen; j0 += kWarps * RW) {
+      const int next = ids_of(j0 + kWarps * RW);
+      uint32_t words[S::PACKED][2][W::KW], codes[S::PACKED][2][W::SETS];
+      bool ok[S::PACKED][2];
+#pragma unroll
+      for (int x = 0; x < S::PACKED; ++x)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int64_t j = j0 + x * 16 + g + 8 * i;
+          const char* page = page_of(j, ok[x][i]);
+          const int row = (int)(j & (bs - 1));
+          const char* src = page + row * RB + t * W::KB;
+#pragma unroll
+          for (int c = 0; c < W::KC; ++c) {
+            if constexpr (W::KB == 16)
+              *reinterpret_cast<uint4*>(&words[x][i][4 * c]) = ld_global_nc<uint4>(src + 64 * c);
+            else
+              *reinterpret_cast<uint2*>(&words[x][i][0]) = ld_global_nc<uint2>(src);
+          }
+          const char* sc = page + bs * RB + row * (D / 16);
+#pragma unroll
+          for (int k = 0; k < W::SETS; ++k)
+            codes[x][i][k] = __ldg(reinterpret_cast<const uint16_t*>(sc + Q::scale_at(k)));
+        }
+#pragma unroll
+      for (int x = 0; x < S::PACKED; ++x) {
+        float z2[2];
+        query.logits(words[x][0], words[x][1], codes[x][0], codes[x][1], z2[0], z2[1]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float all = query.finish(z2[i]);
+          const float dot = ok[x][i] ? all : -INFINITY;
+          top = fmaxf(top, dot);
+          const int64_t j = j0 + x * 16 + g + 8 * i;
+          if (t == 0 && j < seen) z[j - lo] = dot;
+        }
+      }
+      ids = next;
+    }
+  } else if constexpr (S::MMA) {
     const int g = lane >> 2, t = lane & 3;
     uint4 qf[S::NB];
 #pragma unroll
@@ -837,7 +888,7 @@ int step_split(int64_t pairs, int64_t keys) {
   return ns;
 }
 
-template <typename T, int D>
+template <typename T, bool KV4, int D>
 int step_launch(const KeyWeightArgs& a, cudaStream_t st) {
   const int64_t keys = (int64_t)a.max_pages * a.block_size;
   if (keys == 0) return B2PA_OK;
@@ -845,7 +896,7 @@ int step_launch(const KeyWeightArgs& a, cudaStream_t st) {
   const int64_t per = (keys + ns - 1) / ns + 128;  // a CTA's keys, rounded up to whole turns
   const bool far = per > kNearKeys + 128;
   const int smem = far ? 0 : (int)(per * 4);
-  auto kern = key_weights_step_kernel<T, D>;
+  auto kern = key_weights_step_kernel<T, KV4, D>;
   const int rc = set_max_dynamic_smem_cached(reinterpret_cast<const void*>(kern), smem);
   if (rc != B2PA_OK) return rc;
   cudaLaunchConfig_t cfg = {};
@@ -871,19 +922,19 @@ template <typename T>
 int weights_as(const KeyWeightArgs& a, cudaStream_t s) {
   if (a.pool_dtype == B2PA_DTYPE_KV4) {
     switch (a.D) {
-      case 64: return tile_launch<T, true, 64>(a, s);
-      case 128: return tile_launch<T, true, 128>(a, s);
-      default: return tile_launch<T, true, 256>(a, s);
+      case 64: return a.T == 1 ? step_launch<T, true, 64>(a, s) : tile_launch<T, true, 64>(a, s);
+      case 128: return a.T == 1 ? step_launch<T, true, 128>(a, s) : tile_launch<T, true, 128>(a, s);
+      default: return a.T == 1 ? step_launch<T, true, 256>(a, s) : tile_launch<T, true, 256>(a, s);
     }
   }
 #define B2PA_WEIGHTS_CASE(DD) \
-  case DD: return a.T == 1 ? step_launch<T, DD>(a, s) : tile_launch<T, false, DD>(a, s);
+  case DD: return a.T == 1 ? step_launch<T, false, DD>(a, s) : tile_launch<T, false, DD>(a, s);
   switch (a.D) {
     B2PA_WEIGHTS_CASE(16)
     B2PA_WEIGHTS_CASE(32)
     B2PA_WEIGHTS_CASE(64)
     B2PA_WEIGHTS_CASE(128)
-    default: return a.T == 1 ? step_launch<T, 256>(a, s) : tile_launch<T, false, 256>(a, s);
+    default: return a.T == 1 ? step_launch<T, false, 256>(a, s) : tile_launch<T, false, 256>(a, s);
   }
 #undef B2PA_WEIGHTS_CASE
 }
@@ -892,7 +943,7 @@ int weights_as(const KeyWeightArgs& a, cudaStream_t s) {
 
 size_t key_weights_workspace(int B, int H, int T, int D, int max_pages, int block_size, int dtype, int pool_dtype) {
   const int64_t keys = (int64_t)max_pages * block_size;
-  if (T == 1 && pool_dtype != B2PA_DTYPE_KV4) {
+  if (T == 1) {
     const int ns = step_split((int64_t)B * H, keys);
     return (keys + ns - 1) / ns > kNearKeys ? (size_t)B * H * keys * sizeof(float) : 0;
   }

@@ -40,6 +40,7 @@
 #include "common.cuh"
 #include "kernels.h"
 #include "kv4.cuh"
+#include "kv4_mma.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -48,13 +49,6 @@ namespace b2pa {
 namespace {
 
 constexpr int kStages = 2;
-
-__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                        uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 
 // Asynchronous copy of N bytes (4, 8 or 16) to shared memory, both addresses
 // with a constant offset.
@@ -67,30 +61,13 @@ __device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
                  : "memory");
 }
 
-__device__ __forceinline__ float warp_redux_max(float x) {
-  float y;
-  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-__device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-
-// x as hi + lo fp16 halves, for a pair.
-__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
-  const __half2 h = __floats2half2_rn(x, y);
-  const float2 f = __half22float2(h);
-  hi = half2_bits(h);
-  lo = half2_bits(__floats2half2_rn(x - f.x, y - f.y));
-}
-
 template <int D, int W = 8>
-struct Tile {
-  static constexpr int NG = D / 16;          // groups per row
-  static constexpr int SETS = D == 256 ? 2 : 1;  // column sets of 8 groups
-  static constexpr int KW = D / 32;          // K words per lane and row (rows g and g + 8)
+struct Tile : KeyWords<D> {
+  using KeyWords<D>::NG;
+  using KeyWords<D>::SETS;
+  using KeyWords<D>::KB;
+  using KeyWords<D>::KC;
   static constexpr int VW = D / 64;          // V words per lane and key (keys 4t .. 4t+3)
-  static constexpr int KB = KW * 4 < 16 ? KW * 4 : 16;  // bytes per K copy
-  static constexpr int KC = KW * 4 / KB;     // K copies per row
   static constexpr int VB = VW * 4;          // bytes per V copy
   static constexpr int OFF_V = 2 * KC * KB * 32;
   static constexpr int OFF_KS = OFF_V + 4 * VB * 32;
@@ -100,10 +77,6 @@ struct Tile {
   static constexpr int TP = D == 256 ? 1 : 2;  // tiles per step: independent work to hide the products' latency
   static constexpr int BYTES = TP * TILE + 16;
   static constexpr int WARPS = W;
-  // first channel of K word w of lane t; its 8 channels lie in one group
-  __device__ static constexpr int k_channel(int w, int t) {
-    return D == 64 ? 16 * t + 8 * w : (w >> 2) * 128 + 32 * t + 8 * (w & 3);
-  }
 };
 
 constexpr int kMaxCluster = 8;
@@ -140,11 +113,12 @@ struct DecodeKv4Params {
 template <typename T, int D, int BS, int W>
 __global__ void __launch_bounds__(W * 32, D == 256 ? 8 / W : 16 / W) kv4_decode_kernel(DecodeKv4Params p) {
   using C = Tile<D, W>;
-  constexpr bool QLO = std::is_same<T, float>::value && D != 64;  // D = 64 keeps q's low halves in columns 4..7
-  // The weights' low halves, likewise.  16-bit outputs do without: a weight
-  // rounded to 11 bits is off by 2^-12, half a step of fp16 and a sixteenth of
-  // bf16's, and the roundings of different keys are independent.
-  constexpr bool PLO = QLO;
+  using Q = KeyQuery<T, D>;
+  // The weights' low halves.  16-bit outputs do without: a weight rounded to
+  // 11 bits is off by 2^-12, half a step of fp16 and a sixteenth of bf16's,
+  // and the roundings of different keys are independent.  (D = 64 has them in
+  // columns 4..7, at no cost.)
+  constexpr bool PLO = std::is_same<T, float>::value && D != 64;
   constexpr int PAGE = kv4_page_bytes(BS, D), CODES = BS * (D / 2);
   extern __shared__ __align__(16) uint8_t ring_all[];
   __shared__ Smem<D, W> sm;
@@ -162,19 +136,8 @@ __global__ void __launch_bounds__(W * 32, D == 256 ? 8 / W : 16 / W) kv4_decode_
   // first block ids.  Steps go round the cluster's warps, so a warp's first
   // step does not depend on the length.
   const int64_t len = p.seq_lens[b], cur = p.cur_lens[b], cap = (int64_t)p.max_pages * BS;
-  uint4 qraw[C::KW][sizeof(T) / 2];  // the channels of this lane's column, 8 per word
-  const T* const q = static_cast<const T*>(p.q) + (int64_t)b * p.sq_b + (int64_t)h * p.sq_h;
-  auto column_of = [&](int w) {  // 1: this lane's column is word w's group, 2: it takes its low halves
-    const int group = C::k_channel(w, t) / 16;
-    return (D == 64 ? g == group : g == (group & 7)) ? 1 : D == 64 && g == group + 4 ? 2 : 0;
-  };
-#pragma unroll
-  for (int w = 0; w < C::KW; ++w)
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
-      qraw[w][i] = make_uint4(0, 0, 0, 0);
-      if (column_of(w)) qraw[w][i] = ld_global_nc<uint4>(q + C::k_channel(w, t) + i * (16 / (int)sizeof(T)));
-    }
+  Q query;
+  query.load(static_cast<const T*>(p.q) + (int64_t)b * p.sq_b + (int64_t)h * p.sq_h);
   constexpr int KEYS = 16 * C::TP;  // per step
   const int step0 = rank * C::WARPS + warp, turn = ns * C::WARPS;  // this warp's steps: step0 + i * turn
   const int32_t* table = p.page_table + (int64_t)b * p.pt_stride;
@@ -275,70 +238,7 @@ __global__ void __launch_bounds__(W * 32, D == 256 ? 8 / W : 16 / W) kv4_decode_
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) fetch(i);
 
-  // q into the K product's column operand: q scaled by 2^e into fp16's range
-  // (its largest magnitude near 2^13), exact for 16-bit q, hi + lo for fp32.
-  uint32_t qh[C::KW][4], ql[QLO ? C::KW : 1][4];
-  float init[C::SETS][2];  // -8 sum(q) of columns 2t, 2t+1, in the product's units
-  float unit, down_q;      // logit (log2) = product * unit * 2^-e (two factors: neither overflows)
-  {
-    float x[C::KW][8], top = 0.f;
-#pragma unroll
-    for (int w = 0; w < C::KW; ++w) {
-      constexpr int N = 16 / (int)sizeof(T);
-#pragma unroll
-      for (int i = 0; i < 8 / N; ++i) {
-        Vec<T, N> v;
-        v.w = qraw[w][i];
-        v.to_float(&x[w][i * N]);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[w][i]));
-    }
-    top = warp_redux_max(top);
-    // 2^e by exponent arithmetic; 0, tiny, infinite and NaN maxima keep a finite factor
-    int e = 140 - (int)(__float_as_uint(top) >> 23);  // top's exponent field + e = 13 + 127
-    e = e > 100 ? 100 : e;
-    const float up = __uint_as_float((uint32_t)(127 + e) << 23);
-    unit = p.qscale * 0x1p24f;
-    down_q = __uint_as_float((uint32_t)(127 - e) << 23);
-#pragma unroll
-    for (int w = 0; w < C::KW; ++w) {
-      const int col = column_of(w);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {  // operand register r: channels r and r + 4 of the word
-        const float f = (r & 1) ? up * 0.0625f : up;
-        uint32_t hi, lo;
-        split2(x[w][r] * f, x[w][r + 4] * f, hi, lo);
-        qh[w][r] = col == 1 ? hi : col == 2 ? lo : 0u;
-        if constexpr (QLO) ql[w][r] = col == 1 ? lo : 0u;
-      }
-    }
-    // 8 sum(q) of a column: every lane sums its operand registers (undoing the
-    // 1/16), lanes of one column (same g) add up, then columns 2t and 2t+1.
-#pragma unroll
-    for (int s = 0; s < C::SETS; ++s) {
-      float sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < C::KW; ++w) {
-        if (C::SETS == 2 && (w >> 2) != s) continue;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&qh[w][r]));
-          float y = x.x + x.y;
-          if constexpr (QLO) {
-            const float2 z = __half22float2(*reinterpret_cast<const __half2*>(&ql[w][r]));
-            y += z.x + z.y;
-          }
-          sum += (r & 1) ? y * 16.f : y;
-        }
-      }
-      sum += __shfl_xor_sync(kFullMask, sum, 1);
-      sum += __shfl_xor_sync(kFullMask, sum, 2);
-      sum *= -8.f * 0x1p-24f;
-      init[s][0] = __shfl_sync(kFullMask, sum, 8 * t);
-      init[s][1] = __shfl_sync(kFullMask, sum, 8 * t + 4);
-    }
-  }
+  query.prepare(p.qscale);
 
   float acc[C::VW][4][4];              // [word][nibble][fragment]: channels 8 * word + nibble (+ 4)
   float eights[C::SETS][4];            // 8 * sum of the weight operand, per column
@@ -383,20 +283,7 @@ __global__ void __launch_bounds__(W * 32, D == 256 ? 8 / W : 16 / W) kv4_decode_
 #pragma unroll
     for (int y = 0; y < C::TP; ++y) {
       const uint8_t* st = stage + y * C::TILE;
-      // ---- S = K . q per group column, in two chains
-      constexpr int CHAINS = 2;
-      float s[CHAINS][4];
-      if constexpr (C::SETS == 2) {
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          s[x][0] = s[x][2] = init[x][0];
-          s[x][1] = s[x][3] = init[x][1];
-        }
-      } else {
-        s[0][0] = s[0][2] = init[0][0];
-        s[0][1] = s[0][3] = init[0][1];
-        s[1][0] = s[1][1] = s[1][2] = s[1][3] = 0.f;
-      }
+      // ---- logits
       uint32_t ka[C::KW], kb[C::KW];  // rows g and g + 8
 #pragma unroll
       for (int c = 0; c < C::KC; ++c) {
@@ -408,43 +295,19 @@ __global__ void __launch_bounds__(W * 32, D == 256 ? 8 / W : 16 / W) kv4_decode_
           *reinterpret_cast<uint2*>(&kb[0]) = *reinterpret_cast<const uint2*>(st + (32 + lane) * 8);
         }
       }
-#pragma unroll
-      for (int w = 0; w < C::KW; ++w) {
-        constexpr uint32_t LO = 0x000f000fu, HI = 0x00f000f0u;
-        float(&c)[4] = s[C::SETS == 2 ? w >> 2 : w & 1];
-        const uint32_t u = ka[w], v = kb[w], u8 = u >> 8, v8 = v >> 8;
-        mma_f16(c, u & LO, v & LO, u & HI, v & HI, qh[w][0], qh[w][1]);
-        if constexpr (QLO) mma_f16(c, u & LO, v & LO, u & HI, v & HI, ql[w][0], ql[w][1]);
-        mma_f16(c, u8 & LO, v8 & LO, u8 & HI, v8 & HI, qh[w][2], qh[w][3]);
-        if constexpr (QLO) mma_f16(c, u8 & LO, v8 & LO, u8 & HI, v8 & HI, ql[w][2], ql[w][3]);
-      }
-      if constexpr (C::SETS == 1) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) s[0][k] += s[1][k];
-      }
-      // ---- scales: this lane's columns are groups 2t, 2t+1 (of each set)
-      z0[y] = z1[y] = 0.f;
+      uint32_t w0[C::SETS], w1[C::SETS];
 #pragma unroll
       for (int x = 0; x < C::SETS; ++x) {
-        const int col = D == 64 ? 2 * (t & 1) : 8 * x + 2 * t;
-        const uint32_t w0 = *reinterpret_cast<const uint16_t*>(st + C::OFF_KS + g * C::NG + col);
-        const uint32_t w1 = *reinterpret_cast<const uint16_t*>(st + C::OFF_KS + (g + 8) * C::NG + col);
-        const uint32_t h0 = __byte_perm(w0, 0, 0x4140) << 7, h1 = __byte_perm(w1, 0, 0x4140) << 7;
-        const float2 s0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
-        const float2 s1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
-        z0[y] = fmaf(s[x][0], s0.x, fmaf(s[x][1], s0.y, z0[y]));
-        z1[y] = fmaf(s[x][2], s1.x, fmaf(s[x][3], s1.y, z1[y]));
+        w0[x] = *reinterpret_cast<const uint16_t*>(st + C::OFF_KS + g * C::NG + Q::scale_at(x));
+        w1[x] = *reinterpret_cast<const uint16_t*>(st + C::OFF_KS + (g + 8) * C::NG + Q::scale_at(x));
         vs[y][x] = *reinterpret_cast<const uint32_t*>(st + C::OFF_VS + (x * 32 + lane) * 4);
       }
+      query.logits(ka, kb, w0, w1, z0[y], z1[y]);
     }
 #pragma unroll
     for (int y = 0; y < C::TP; ++y) {
-      z0[y] += __shfl_xor_sync(kFullMask, z0[y], 1);
-      z1[y] += __shfl_xor_sync(kFullMask, z1[y], 1);
-      z0[y] += __shfl_xor_sync(kFullMask, z0[y], 2);
-      z1[y] += __shfl_xor_sync(kFullMask, z1[y], 2);
-      z0[y] = z0[y] * unit * down_q;
-      z1[y] = z1[y] * unit * down_q;
+      z0[y] = query.finish(z0[y]);
+      z1[y] = query.finish(z1[y]);
     }
     if (mask != (C::TP == 1 ? 0xffffu : 0xffffffffu)) {
 #pragma unroll

@@ -1,0 +1,192 @@
+// kv4_mma.cuh -- one query against packed 4-bit keys on the tensor core
+// (mma.sync m16n8k16), shared by the decode attention and the accumulation of
+// key weights.  How codes become operands is told in kv4_decode.cu.
+#pragma once
+
+#include "common.cuh"
+#include "kv4.cuh"
+
+namespace b2pa {
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ float warp_redux_max(float x) {
+  float y;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+
+// x as hi + lo fp16 halves, for a pair.
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  hi = half2_bits(h);
+  lo = half2_bits(__floats2half2_rn(x - f.x, y - f.y));
+}
+
+// How a lane (g = lane / 4, t = lane % 4) holds the K row of one key.
+template <int D>
+struct KeyWords {
+  static constexpr int NG = D / 16;              // groups per row
+  static constexpr int SETS = D == 256 ? 2 : 1;  // column sets of 8 groups
+  static constexpr int KW = D / 32;              // words per lane and row (rows g and g + 8)
+  static constexpr int KB = KW * 4 < 16 ? KW * 4 : 16;  // bytes per piece: bytes t * KB + c * 4 * KB of the row
+  static constexpr int KC = KW * 4 / KB;         // pieces per row
+  // first channel of word w of lane t; its 8 channels lie in one group
+  __device__ static constexpr int channel(int w, int t) {
+    return D == 64 ? 16 * t + 8 * w : (w >> 2) * 128 + 32 * t + 8 * (w & 3);
+  }
+};
+
+// The query as the product's column operand: column n holds its channels of
+// group n (D = 64: the low halves of group n - 4 from column 4 on; D = 256: a
+// second set for groups 8..15), scaled by 2^e into fp16's range (its largest
+// magnitude near 2^13): exact for 16-bit q, hi + lo for fp32.
+template <typename T, int D>
+struct KeyQuery {
+  using C = KeyWords<D>;
+  static constexpr bool QLO = std::is_same<T, float>::value && D != 64;  // low halves as a second product
+  uint4 raw[C::KW][sizeof(T) / 2];  // the channels of this lane's column, 8 per word
+  uint32_t qh[C::KW][4], ql[QLO ? C::KW : 1][4];
+  float init[C::SETS][2];  // -8 sum(q) of columns 2t, 2t+1, in the product's units
+  float unit, down_q;      // logit (log2) = product * unit * 2^-e (two factors: neither overflows)
+
+  // 1: word w's group is this lane's column, 2: the column takes its low halves
+  __device__ __forceinline__ static int column_of(int w) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int group = C::channel(w, t) / 16;
+    return (D == 64 ? g == group : g == (group & 7)) ? 1 : D == 64 && g == group + 4 ? 2 : 0;
+  }
+  __device__ __forceinline__ void load(const T* q) {
+    const int t = threadIdx.x & 3;
+#pragma unroll
+    for (int w = 0; w < C::KW; ++w)
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+        raw[w][i] = make_uint4(0, 0, 0, 0);
+        if (column_of(w)) raw[w][i] = ld_global_nc<uint4>(q + C::channel(w, t) + i * (16 / (int)sizeof(T)));
+      }
+  }
+  __device__ __forceinline__ void prepare(float qscale) {
+    const int t = threadIdx.x & 3;
+    float x[C::KW][8], top = 0.f;
+#pragma unroll
+    for (int w = 0; w < C::KW; ++w) {
+      constexpr int N = 16 / (int)sizeof(T);
+#pragma unroll
+      for (int i = 0; i < 8 / N; ++i) {
+        Vec<T, N> v;
+        v.w = raw[w][i];
+        v.to_float(&x[w][i * N]);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[w][i]));
+    }
+    top = warp_redux_max(top);
+    // 2^e by exponent arithmetic; 0, tiny, infinite and NaN maxima keep a finite factor
+    int e = 140 - (int)(__float_as_uint(top) >> 23);  // top's exponent field + e = 13 + 127
+    e = e > 100 ? 100 : e;
+    const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+    unit = qscale * 0x1p24f;
+    down_q = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+    for (int w = 0; w < C::KW; ++w) {
+      const int col = column_of(w);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {  // operand register r: channels r and r + 4 of the word
+        const float f = (r & 1) ? up * 0.0625f : up;
+        uint32_t hi, lo;
+        split2(x[w][r] * f, x[w][r + 4] * f, hi, lo);
+        qh[w][r] = col == 1 ? hi : col == 2 ? lo : 0u;
+        if constexpr (QLO) ql[w][r] = col == 1 ? lo : 0u;
+      }
+    }
+    // 8 sum(q) of a column: every lane sums its operand registers (undoing the
+    // 1/16), lanes of one column (same g) add up, then columns 2t and 2t+1.
+#pragma unroll
+    for (int s = 0; s < C::SETS; ++s) {
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < C::KW; ++w) {
+        if (C::SETS == 2 && (w >> 2) != s) continue;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&qh[w][r]));
+          float z = y.x + y.y;
+          if constexpr (QLO) {
+            const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&ql[w][r]));
+            z += v.x + v.y;
+          }
+          sum += (r & 1) ? z * 16.f : z;
+        }
+      }
+      sum += __shfl_xor_sync(kFullMask, sum, 1);
+      sum += __shfl_xor_sync(kFullMask, sum, 2);
+      sum *= -8.f * 0x1p-24f;
+      init[s][0] = __shfl_sync(kFullMask, sum, 8 * t);
+      init[s][1] = __shfl_sync(kFullMask, sum, 8 * t + 4);
+    }
+  }
+
+  // This lane's part of the products of keys g and g + 8 (words ka, kb; w0 and
+  // w1: the scale codes of groups 2t, 2t+1 of each set, in the low bytes).
+  // The four lanes of a key have to be added up and scaled: finish().
+  __device__ __forceinline__ void logits(const uint32_t (&ka)[C::KW], const uint32_t (&kb)[C::KW],
+                                         const uint32_t (&w0)[C::SETS], const uint32_t (&w1)[C::SETS], float& z0,
+                                         float& z1) const {
+    float s[2][4];  // two chains of products
+    if constexpr (C::SETS == 2) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        s[x][0] = s[x][2] = init[x][0];
+        s[x][1] = s[x][3] = init[x][1];
+      }
+    } else {
+      s[0][0] = s[0][2] = init[0][0];
+      s[0][1] = s[0][3] = init[0][1];
+      s[1][0] = s[1][1] = s[1][2] = s[1][3] = 0.f;
+    }
+#pragma unroll
+    for (int w = 0; w < C::KW; ++w) {
+      constexpr uint32_t LO = 0x000f000fu, HI = 0x00f000f0u;
+      float(&c)[4] = s[C::SETS == 2 ? w >> 2 : w & 1];
+      const uint32_t u = ka[w], v = kb[w], u8 = u >> 8, v8 = v >> 8;
+      mma_f16(c, u & LO, v & LO, u & HI, v & HI, qh[w][0], qh[w][1]);
+      if constexpr (QLO) mma_f16(c, u & LO, v & LO, u & HI, v & HI, ql[w][0], ql[w][1]);
+      mma_f16(c, u8 & LO, v8 & LO, u8 & HI, v8 & HI, qh[w][2], qh[w][3]);
+      if constexpr (QLO) mma_f16(c, u8 & LO, v8 & LO, u8 & HI, v8 & HI, ql[w][2], ql[w][3]);
+    }
+    if constexpr (C::SETS == 1) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s[0][k] += s[1][k];
+    }
+    z0 = z1 = 0.f;
+#pragma unroll
+    for (int x = 0; x < C::SETS; ++x) {
+      const uint32_t h0 = __byte_perm(w0[x], 0, 0x4140) << 7, h1 = __byte_perm(w1[x], 0, 0x4140) << 7;
+      const float2 s0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
+      const float2 s1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+      z0 = fmaf(s[x][0], s0.x, fmaf(s[x][1], s0.y, z0));
+      z1 = fmaf(s[x][2], s1.x, fmaf(s[x][3], s1.y, z1));
+    }
+  }
+  __device__ __forceinline__ float finish(float z) const {
+    z += __shfl_xor_sync(kFullMask, z, 1);
+    z += __shfl_xor_sync(kFullMask, z, 2);
+    return z * unit * down_q;
+  }
+  // Where a lane's two scale codes of set x lie in the row's codes.
+  __device__ __forceinline__ static int scale_at(int x) {
+    const int t = threadIdx.x & 3;
+    return D == 64 ? 2 * (t & 1) : 8 * x + 2 * t;
+  }
+};
+
+}  // namespace b2pa
