@@ -227,6 +227,7 @@ struct Kv4PrefillPlan {
 };
 Kv4PrefillPlan make_kv4_prefill_plan(int B, int H, int T, int D, int max_pages, int block_size, int dtype);
 int launch_kv4_prefill(const AttnArgs& a, const Kv4PrefillPlan& plan, cudaStream_t s);
+int launch_kv4_prefill_mma(const AttnArgs& a, cudaStream_t s);
 
 size_t key_weights_workspace(int B, int H, int T, int D, int max_pages, int block_size, int dtype, int pool_dtype);
 int launch_key_weights(const KeyWeightArgs& a, cudaStream_t s);

@@ -81,53 +81,6 @@ __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, u
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ uint32_t bits_of(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-
-// Eight fp32 values, scaled, as fp16 halves hi + lo.
-__device__ __forceinline__ void split8(const float* x, float f, uint4& hi, uint4& lo) {
-  uint32_t* h = &hi.x;
-  uint32_t* l = &lo.x;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float u = x[2 * i] * f, v = x[2 * i + 1] * f;
-    const __half2 p = __floats2half2_rn(u, v);
-    const float2 w = __half22float2(p);
-    h[i] = bits_of(p);
-    l[i] = bits_of(__floats2half2_rn(u - w.x, v - w.y));
-  }
-}
-
-// A power of two that brings magnitudes up to `top` near 2^10, and its
-// inverse; 0, tiny, infinite and NaN maxima keep a finite factor.
-__device__ __forceinline__ float range_factor(float top, float& back) {
-  int e = 137 - (int)(__float_as_uint(top) >> 23);
-  e = e > 100 ? 100 : e;
-  back = __uint_as_float((uint32_t)(127 - e) << 23);
-  return __uint_as_float((uint32_t)(127 + e) << 23);
-}
-
-// One 4-bit word (8 channels of scale s) as 4 operand registers, exact, in
-// the order 0 4 1 5 2 6 3 7: a masked nibble pair in the mantissa is 1024 + c,
-// or 16 (64 + c) for the upper nibbles.
-__device__ __forceinline__ uint4 unpack_word(uint32_t w, __half2 s) {
-  const __half2 k1032 = __half2half2(__ushort_as_half(0x6408)), k72 = __half2half2(__ushort_as_half(0xd480)),
-                k16th = __half2half2(__ushort_as_half(0x2c00));
-  auto lo = [&](uint32_t x) {
-    const uint32_t y = (x & 0x000f000fu) | 0x64006400u;
-    return bits_of(__hmul2(__hsub2(*reinterpret_cast<const __half2*>(&y), k1032), s));
-  };
-  auto hi = [&](uint32_t x) {
-    const uint32_t y = (x & 0x00f000f0u) | 0x64006400u;
-    return bits_of(__hmul2(__hfma2(*reinterpret_cast<const __half2*>(&y), k16th, k72), s));
-  };
-  return make_uint4(lo(w), hi(w), lo(w >> 8), hi(w >> 8));
-}
-// Two scale codes, in the low bytes, as pairs.
-__device__ __forceinline__ __half2 scale_pair(uint32_t codes, uint32_t select) {
-  const uint32_t x = __byte_perm(codes, 0, select) << 7;
-  return *reinterpret_cast<const __half2*>(&x);
-}
-
 constexpr int kTileThreads = 128;
 constexpr int kCols = 64;  // queries per tile
 
@@ -146,12 +99,6 @@ struct Shape {
   static constexpr int PITCH = NB * 64 % 128 == 0 ? NB * 64 + 64 : NB * 64;  // a quarter warp's two rows in other banks
   static constexpr int Q_BYTES = QPARTS * kCols * PITCH;  // a tile of queries
   static constexpr int Q_SAVED = O::PREP ? Q_BYTES + kCols * 4 : 0;  // ... with its factors, in the workspace
-  // where 8 consecutive channels (number c8) of a query row go: 4-bit keys
-  // are loaded 16 bytes (4 words) a lane, so word w of lane t is block w's
-  __device__ static constexpr int place(int c8) {
-    return !KV4 ? 16 * c8 : D == 64 ? (c8 & 1) * 64 + (c8 >> 1) * 16
-                                    : ((c8 >> 4) * 4 + (c8 & 3)) * 64 + ((c8 >> 2) & 3) * 16;
-  }
 };
 
 // Counted queries i0 .. i0 + 63 into shared memory (zeros past the count):
@@ -168,44 +115,11 @@ __device__ __forceinline__ void load_queries(const KeyWeightArgs& a, const Span&
     for (int u = threadIdx.x; u < kCols * C8; u += kTileThreads) {
       const int r = u / C8, c = u % C8;
       const bool ok = i0 + r < s.count && 8 * c < D;
-      copy16(smem_u32(dst) + r * S::PITCH + S::place(c), ok ? q + (int64_t)(s.first + i0 + r) * a.sq[2] + 8 * c : q, ok);
+      copy16(smem_u32(dst) + r * S::PITCH + 16 * c, ok ? q + (int64_t)(s.first + i0 + r) * a.sq[2] + 8 * c : q, ok);
     }
   } else {
-    constexpr int LPR = C8 < 32 ? C8 : 32;  // lanes per row
-    constexpr int V = 16 / (int)sizeof(T);
-    const int lane = threadIdx.x & 31, c = lane % LPR;
-#pragma unroll 4
-    for (int r = (threadIdx.x >> 5) * (32 / LPR) + lane / LPR; r < kCols; r += kTileThreads / LPR) {
-      float x[8] = {};
-      if (i0 + r < s.count && 8 * c < D) {
-        const T* row = q + (int64_t)(s.first + i0 + r) * a.sq[2] + 8 * c;
-#pragma unroll
-        for (int i = 0; i < 8; i += V) {
-          Vec<T, V> v;
-          v.w = ld_global_nc<uint4>(row + i);
-          v.to_float(x + i);
-        }
-      }
-      float f = 1.f, back = 1.f;
-      if constexpr (O::SCALED) {
-        float top = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
-#pragma unroll
-        for (int o = LPR / 2; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, o));
-        f = range_factor(top, back);
-      }
-      if constexpr (KV4) {  // in the order of unpacked keys
-        const float y[8] = {x[0], x[4], x[1], x[5], x[2], x[6], x[3], x[7]};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = y[i];
-      }
-      uint4 hi, lo;
-      split8(x, f, hi, lo);
-      *reinterpret_cast<uint4*>(dst + r * S::PITCH + S::place(c)) = hi;
-      if constexpr (S::QPARTS == 2) *reinterpret_cast<uint4*>(dst + kCols * S::PITCH + r * S::PITCH + S::place(c)) = lo;
-      if (c == 0) unit[r] = back;
-    }
+    convert_queries<T, KV4, D, kCols, S::PITCH, S::QPARTS, kTileThreads>(q + (int64_t)(s.first + i0) * a.sq[2], a.sq[2],
+                                                                        s.count - i0, dst, unit);
   }
 }
 
@@ -255,24 +169,7 @@ struct Keys {
         if constexpr (KV4) {
           const uint8_t* page = static_cast<const uint8_t*>(a.k_pool) +
                                 (uint64_t)(blk * (uint64_t)a.H + h) * (uint32_t)kv4_page_bytes(bs, D);
-          const uint8_t* scales = page + bs * (D / 2) + row * (D / 16);
-          if constexpr (D == 64) {
-            const uint2 w = __ldg(reinterpret_cast<const uint2*>(page + row * 32 + 8 * t));
-            const __half2 sc = scale_pair(__ldg(scales + t), 0x4040);
-            f[0] = unpack_word(w.x, sc);
-            f[1] = unpack_word(w.y, sc);
-          } else {
-#pragma unroll
-            for (int c = 0; c < D / 128; ++c) {
-              const uint4 w = __ldg(reinterpret_cast<const uint4*>(page + row * (D / 2) + 64 * c + 16 * t));
-              const uint32_t sc = __ldg(reinterpret_cast<const uint16_t*>(scales + 8 * c + 2 * t));
-              const __half2 s0 = scale_pair(sc, 0x4040), s1 = scale_pair(sc, 0x4141);
-              f[4 * c + 0] = unpack_word(w.x, s0);
-              f[4 * c + 1] = unpack_word(w.y, s0);
-              f[4 * c + 2] = unpack_word(w.z, s1);
-              f[4 * c + 3] = unpack_word(w.w, s1);
-            }
-          }
+          unpack_key_row<D>(page, row, bs, f);
         } else {
           const T* src = static_cast<const T*>(a.k_pool) + ((blk * (uint64_t)a.H + h) * bs + row) * D + 8 * t;
           if constexpr (!S::O::F32) {
@@ -600,12 +497,12 @@ struct StepRows {
   static constexpr int NB = RB < 64 ? 1 : RB / 64, TILES = NB < 4 ? 4 / NB : 1;
   // else: lanes per row, 16-byte pieces per lane, rows per load, rows per lane
   static constexpr int LPR = RB / 16 < 32 ? RB / 16 : 32, CPL = RB / 16 / LPR, RP = 32 / LPR, R = 8 / CPL;
-  static constexpr int PACKED = D == 256 ? 2 : 4;  // 16-row tiles of 4-bit rows per turn
+  static constexpr int PACKED = D == 256 ? 1 : 2;  // 16-row tiles of 4-bit rows per turn
   static constexpr int RW = KV4 ? 16 * PACKED : MMA ? 16 * TILES : RP * R;  // rows per warp and turn
 };
 
 template <typename T, bool KV4, int D>
-__global__ void __launch_bounds__(kStepThreads) key_weights_step_kernel(KeyWeightArgs a, float qscale, float* far,
+__global__ void __launch_bounds__(kStepThreads, KV4 ? 3 : 0) key_weights_step_kernel(KeyWeightArgs a, float qscale, float* far,
                                                                         int64_t far_stride) {
   using S = StepRows<T, KV4, D>;
   using O = Op<T, false>;

@@ -31,6 +31,52 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
   lo = half2_bits(__floats2half2_rn(x - f.x, y - f.y));
 }
 
+
+// Eight fp32 values, scaled, as fp16 halves hi + lo.
+__device__ __forceinline__ void split8(const float* x, float f, uint4& hi, uint4& lo) {
+  uint32_t* h = &hi.x;
+  uint32_t* l = &lo.x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float u = x[2 * i] * f, v = x[2 * i + 1] * f;
+    const __half2 p = __floats2half2_rn(u, v);
+    const float2 w = __half22float2(p);
+    h[i] = half2_bits(p);
+    l[i] = half2_bits(__floats2half2_rn(u - w.x, v - w.y));
+  }
+}
+
+// A power of two that brings magnitudes up to `top` near 2^10, and its
+// inverse; 0, tiny, infinite and NaN maxima keep a finite factor.
+__device__ __forceinline__ float range_factor(float top, float& back) {
+  int e = 137 - (int)(__float_as_uint(top) >> 23);
+  e = e > 100 ? 100 : e;
+  back = __uint_as_float((uint32_t)(127 - e) << 23);
+  return __uint_as_float((uint32_t)(127 + e) << 23);
+}
+
+// One 4-bit word (8 channels of scale s) as 4 operand registers, exact, in
+// the order 0 4 1 5 2 6 3 7: a masked nibble pair in the mantissa is 1024 + c,
+// or 16 (64 + c) for the upper nibbles.
+__device__ __forceinline__ uint4 unpack_word(uint32_t w, __half2 s) {
+  const __half2 k1032 = __half2half2(__ushort_as_half(0x6408)), k72 = __half2half2(__ushort_as_half(0xd480)),
+                k16th = __half2half2(__ushort_as_half(0x2c00));
+  auto lo = [&](uint32_t x) {
+    const uint32_t y = (x & 0x000f000fu) | 0x64006400u;
+    return half2_bits(__hmul2(__hsub2(*reinterpret_cast<const __half2*>(&y), k1032), s));
+  };
+  auto hi = [&](uint32_t x) {
+    const uint32_t y = (x & 0x00f000f0u) | 0x64006400u;
+    return half2_bits(__hmul2(__hfma2(*reinterpret_cast<const __half2*>(&y), k16th, k72), s));
+  };
+  return make_uint4(lo(w), hi(w), lo(w >> 8), hi(w >> 8));
+}
+// Two scale codes, in the low bytes, as pairs.
+__device__ __forceinline__ __half2 scale_pair(uint32_t codes, uint32_t select) {
+  const uint32_t x = __byte_perm(codes, 0, select) << 7;
+  return *reinterpret_cast<const __half2*>(&x);
+}
+
 // How a lane (g = lane / 4, t = lane % 4) holds the K row of one key.
 template <int D>
 struct KeyWords {
@@ -44,6 +90,85 @@ struct KeyWords {
     return D == 64 ? 16 * t + 8 * w : (w >> 2) * 128 + 32 * t + 8 * (w & 3);
   }
 };
+
+// One key row as operand registers with its scales applied: block w (word w
+// of lane t) of a product over D channels.
+template <int D>
+__device__ __forceinline__ void unpack_key_row(const uint8_t* page, int row, int bs, uint4 (&f)[D / 32]) {
+  const int t = threadIdx.x & 3;
+  const uint8_t* scales = page + bs * (D / 2) + row * (D / 16);
+  if constexpr (D == 64) {
+    const uint2 w = __ldg(reinterpret_cast<const uint2*>(page + row * 32 + 8 * t));
+    const __half2 sc = scale_pair(__ldg(scales + t), 0x4040);
+    f[0] = unpack_word(w.x, sc);
+    f[1] = unpack_word(w.y, sc);
+  } else {
+#pragma unroll
+    for (int c = 0; c < D / 128; ++c) {
+      const uint4 w = __ldg(reinterpret_cast<const uint4*>(page + row * (D / 2) + 64 * c + 16 * t));
+      const uint32_t sc = __ldg(reinterpret_cast<const uint16_t*>(scales + 8 * c + 2 * t));
+      const __half2 s0 = scale_pair(sc, 0x4040), s1 = scale_pair(sc, 0x4141);
+      f[4 * c + 0] = unpack_word(w.x, s0);
+      f[4 * c + 1] = unpack_word(w.y, s0);
+      f[4 * c + 2] = unpack_word(w.z, s1);
+      f[4 * c + 3] = unpack_word(w.w, s1);
+    }
+  }
+}
+
+// Where 8 consecutive channels (number c8) of a query row go, in bytes, so
+// that its blocks match unpack_key_row's.
+template <int D>
+__device__ constexpr int query_place(int c8) {
+  return D == 64 ? (c8 & 1) * 64 + (c8 >> 1) * 16 : ((c8 >> 4) * 4 + (c8 & 3)) * 64 + ((c8 >> 2) & 3) * 16;
+}
+
+// ROWS query rows (zeros from `count` on) into shared memory as fp16 operands:
+// rows of fp32 (PARTS = 2: hi, then lo ROWS * PITCH bytes on) and of bf16 are
+// scaled into fp16's range, unit[r] undoing it; KV4: in query_place's blocks
+// and unpack_word's order, else as they lie.
+template <typename T, bool KV4, int D, int ROWS, int PITCH, int PARTS, int THREADS>
+__device__ __forceinline__ void convert_queries(const T* q, int64_t stride, int count, uint8_t* dst, float* unit) {
+  constexpr bool SCALED = !std::is_same<T, __half>::value;
+  constexpr int C8 = (D < 32 ? 32 : D) / 8;  // 8-channel pieces per row (whole blocks)
+  constexpr int LPR = C8 < 32 ? C8 : 32;     // lanes per row
+  constexpr int V = 16 / (int)sizeof(T);
+  const int lane = threadIdx.x & 31, c = lane % LPR;
+#pragma unroll 4
+  for (int r = (threadIdx.x >> 5) * (32 / LPR) + lane / LPR; r < ROWS; r += THREADS / LPR) {
+    float x[8] = {};
+    if (r < count && 8 * c < D) {
+      const T* row = q + r * stride + 8 * c;
+#pragma unroll
+      for (int i = 0; i < 8; i += V) {
+        Vec<T, V> v;
+        v.w = ld_global_nc<uint4>(row + i);
+        v.to_float(x + i);
+      }
+    }
+    float f = 1.f, back = 1.f;
+    if constexpr (SCALED) {
+      float top = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
+#pragma unroll
+      for (int o = LPR / 2; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, o));
+      f = range_factor(top, back);
+    }
+    int at = 16 * c;
+    if constexpr (KV4) {
+      const float y[8] = {x[0], x[4], x[1], x[5], x[2], x[6], x[3], x[7]};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = y[i];
+      at = query_place<D>(c);
+    }
+    uint4 hi, lo;
+    split8(x, f, hi, lo);
+    *reinterpret_cast<uint4*>(dst + r * PITCH + at) = hi;
+    if constexpr (PARTS == 2) *reinterpret_cast<uint4*>(dst + (ROWS + r) * PITCH + at) = lo;
+    if (c == 0) unit[r] = back;
+  }
+}
 
 // The query as the product's column operand: column n holds its channels of
 // group n (D = 64: the low halves of group n - 4 from column 4 on; D = 256: a

@@ -1,10 +1,11 @@
 // kv4_prefill.cu -- chunked prefill over a 4-bit cache (format: kv4.cuh).
 //
 // A prompt chunk of T queries makes 4 T L D operations of every L keys, so
-// its time is the tensor cores' and not the cache's.  The pages the call
-// reads are first written out in the type of q in the workspace, as a pool of
+// its time is the tensor cores' and not the cache's.  Where a tcgen05 kernel
+// of the plain pools does the rest (fp32 with head_dim 64, 16-bit types with
+// 64 and 128; else kv4_prefill_mma.cu), the pages the call reads are written out in the type of q in the workspace, as a pool of
 // B * max_pages blocks with a table of their own (exact: a stored value has 7
-// significant bits), and the prefill kernels of the plain pools run on it.
+// significant bits), and that kernel runs on it.
 // Rows past a sequence's length are written as zeros.
 #include "common.cuh"
 #include "kernels.h"
@@ -53,8 +54,18 @@ __global__ void __launch_bounds__(256) kv4_unpack_kernel(AttnArgs a, T* k_out, T
 
 static size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
+// Shapes without a tcgen05 kernel of the plain pools behind the unpacking: the
+// others' kernels there run on the CUDA cores.  Unpacking and plain kernel ->
+// straight from the pages (us; 2 sequences, 32 heads, 1,021 queries on 1,024
+// to 7,168 keys): fp32 head_dim 64 403 -> 918, 128 5,524 -> 1,399, 256 29,044
+// -> 2,477; bf16 64 205 -> 753, 128 305 -> 1,107, 256 26,457 -> 1,752.
+static bool takes_mma(int D, int dtype) {
+  return D == 256 || (D == 128 && dtype == B2PA_DTYPE_F32);
+}
+
 Kv4PrefillPlan make_kv4_prefill_plan(int B, int H, int T, int D, int max_pages, int block_size, int dtype) {
-  Kv4PrefillPlan pl;
+  Kv4PrefillPlan pl = {};
+  if (takes_mma(D, dtype)) return pl;
   const size_t pool = up256((size_t)B * max_pages * H * block_size * D * dtype_size(dtype));
   pl.off_k = 0;
   pl.off_v = pool;
@@ -73,6 +84,7 @@ static cudaError_t unpack_as(const AttnArgs& a, char* ws, const Kv4PrefillPlan& 
 }
 
 int launch_kv4_prefill(const AttnArgs& a, const Kv4PrefillPlan& pl, cudaStream_t s) {
+  if (takes_mma(a.D, a.dtype)) return launch_kv4_prefill_mma(a, s);
   char* ws = static_cast<char*>(a.workspace);
   AttnArgs in = a;
   if (a.max_pages > 0) {
