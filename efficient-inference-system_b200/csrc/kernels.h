@@ -231,6 +231,7 @@ int launch_kv4_prefill_mma(const AttnArgs& a, cudaStream_t s);
 
 size_t key_weights_workspace(int B, int H, int T, int D, int max_pages, int block_size, int dtype, int pool_dtype);
 int launch_key_weights(const KeyWeightArgs& a, cudaStream_t s);
+int launch_key_weights_tc(const KeyWeightArgs& a, int count, cudaStream_t s);
 int launch_evict(const EvictArgs& a, cudaStream_t s);
 
 inline bool kv4_head_dim_supported(int D) { return D == 64 || D == 128 || D == 256; }

@@ -6,20 +6,21 @@
 // pos + 1) - 1, and counting when cur_len - window <= t < cur_len (all of
 // them without a window).
 //
-// Several queries (key_weights_tile_kernel): two launches over one matrix
-// product K.Q^T on the tensor cores (mma.sync), keys as rows, 64 queries as
-// columns.  A key row is used by one warp only, so its fragments go from
-// global memory to registers and only queries lie in shared memory.  The first
-// launch keeps, per lane and column, a running maximum and sum over the rows
-// that the lane sees, joined at the end (keys may be split between CTAs); the
-// second adds exp(logit - lse) along the columns, so every key's sum stays in
-// one thread and needs no atomics: results do not depend on the order of
-// anything.  The product is computed twice because the alternative, keeping
-// T x L logits, costs more bytes than the product costs time.  What bounds it
-// is instruction issue: four instructions per logit (scale and shift, compare,
-// exponential, add) beside the products'.  Operands: 16-bit types as they are;
-// 4-bit keys unpacked (exactly) to the type of q; fp32 as two fp16 halves each
-// (22 bits, three products), rows scaled by powers of two into fp16's range.
+// Several queries: two launches over one matrix product K.Q^T on the tensor
+// cores.  The first finds each query's maximum and sum (keys may be split
+// between CTAs); the second, with keys as rows, adds exp(logit - lse) along the
+// queries, so every key's sum stays in one thread and needs no atomics: results
+// do not depend on the order of anything.  The product is computed twice
+// because the alternative, keeping T x L logits, costs more bytes than the
+// product costs time.  Operands: 16-bit types as they are; 4-bit keys unpacked
+// (exactly) to fp16; fp32 as two fp16 halves each (22 bits, three products),
+// rows scaled by powers of two into fp16's range.
+//   head_dim 64 and 128: key_weights_tc.cu (tcgen05).
+//   head_dim 16, 32 and 256: key_weights_tile_kernel here (mma.sync), whose key
+//   rows go from global memory to registers -- each is used by one warp only --
+//   with 64 queries in shared memory as columns; the first launch keeps, per
+//   lane and column, a maximum and a sum over the rows that the lane sees.
+//   Bound by instruction issue, about four instructions a logit.
 //
 // One query (key_weights_step_kernel): bound by reading K once.
 // A cluster of CTAs shares a sequence, each keeps its logits in shared
@@ -90,10 +91,9 @@ struct Shape {
   static constexpr int NB = D < 32 ? 1 : D / 32;          // blocks of 32 channels: two products of 16
   static constexpr int KPARTS = O::F32 && !KV4 ? 2 : 1;   // halves of a key / of a query
   static constexpr int QPARTS = O::F32 ? 2 : 1;
-  // 16-row tiles per warp: two share every load of the queries, while their
-  // fragments fit 64 registers; one leaves room for more warps, which pays
-  // for fp32 (three products a load).  256-query fp32 chunks: 57 us with two,
-  // 51 with one; 4-bit keys, 64 queries: 112 and 144.
+  // 16-row tiles per warp: two share every load of the queries, one leaves
+  // room for more warps, which pays for fp32 (three products a load; 256
+  // queries, head_dim 64: 57 us with two, 51 with one) and for wide rows
   static constexpr int MT = KPARTS == 1 && NB <= 4 ? 2 : 1;
   static constexpr int WROWS = 16 * MT, ROWS = 4 * WROWS;  // keys per warp and CTA
   static constexpr int PITCH = NB * 64 % 128 == 0 ? NB * 64 + 64 : NB * 64;  // a quarter warp's two rows in other banks
@@ -742,6 +742,8 @@ int split_of(int B, int H, int count, int64_t keys, int per_sm) {
   return ns < 1 ? 1 : ns > 16 ? 16 : (int)ns;
 }
 
+bool takes_tcgen05(int D) { return D == 64 || D == 128; }  // key_weights_tc.cu
+
 int counted_most(int T, int window) { return window > 0 && window < T ? window : T; }
 
 template <typename T, bool KV4, int D>
@@ -819,21 +821,18 @@ template <typename T>
 int weights_as(const KeyWeightArgs& a, cudaStream_t s) {
   if (a.pool_dtype == B2PA_DTYPE_KV4) {
     switch (a.D) {
-      case 64: return a.T == 1 ? step_launch<T, true, 64>(a, s) : tile_launch<T, true, 64>(a, s);
-      case 128: return a.T == 1 ? step_launch<T, true, 128>(a, s) : tile_launch<T, true, 128>(a, s);
+      case 64: return step_launch<T, true, 64>(a, s);
+      case 128: return step_launch<T, true, 128>(a, s);
       default: return a.T == 1 ? step_launch<T, true, 256>(a, s) : tile_launch<T, true, 256>(a, s);
     }
   }
-#define B2PA_WEIGHTS_CASE(DD) \
-  case DD: return a.T == 1 ? step_launch<T, false, DD>(a, s) : tile_launch<T, false, DD>(a, s);
   switch (a.D) {
-    B2PA_WEIGHTS_CASE(16)
-    B2PA_WEIGHTS_CASE(32)
-    B2PA_WEIGHTS_CASE(64)
-    B2PA_WEIGHTS_CASE(128)
+    case 16: return a.T == 1 ? step_launch<T, false, 16>(a, s) : tile_launch<T, false, 16>(a, s);
+    case 32: return a.T == 1 ? step_launch<T, false, 32>(a, s) : tile_launch<T, false, 32>(a, s);
+    case 64: return step_launch<T, false, 64>(a, s);
+    case 128: return step_launch<T, false, 128>(a, s);
     default: return a.T == 1 ? step_launch<T, false, 256>(a, s) : tile_launch<T, false, 256>(a, s);
   }
-#undef B2PA_WEIGHTS_CASE
 }
 
 }  // namespace
@@ -847,7 +846,7 @@ size_t key_weights_workspace(int B, int H, int T, int D, int max_pages, int bloc
   // the first pass's partials, then its converted queries: at most two fp16
   // halves a channel, rows padded by a block, and a factor each
   size_t saved = 0;
-  if (pool_dtype == B2PA_DTYPE_KV4 || dtype == B2PA_DTYPE_F32) {
+  if (!takes_tcgen05(D) && (pool_dtype == B2PA_DTYPE_KV4 || dtype == B2PA_DTYPE_F32)) {
     const size_t blocks = D < 32 ? 1 : D / 32, parts = dtype == B2PA_DTYPE_F32 ? 2 : 1;
     saved = (size_t)B * H * ((T + kCols - 1) / kCols) * (parts * kCols * (blocks + 1) * 64 + kCols * 4);
   }
@@ -855,6 +854,7 @@ size_t key_weights_workspace(int B, int H, int T, int D, int max_pages, int bloc
 }
 
 int launch_key_weights(const KeyWeightArgs& a, cudaStream_t s) {
+  if (a.T > 1 && takes_tcgen05(a.D)) return launch_key_weights_tc(a, counted_most(a.T, a.window), s);
   switch (a.dtype) {
     case B2PA_DTYPE_F32: return weights_as<float>(a, s);
     case B2PA_DTYPE_BF16: return weights_as<__nv_bfloat16>(a, s);
