@@ -16,7 +16,11 @@
 //     operand carries), so a word of 8 codes becomes 4 operand registers with
 //     one shift and four ANDs.  Stored codes are c + 8: the 8 is taken out
 //     through the accumulator (K: it starts at -8 sum(q); V: one more product
-//     against a constant operand sums the weights).
+//     against a constant operand sums the weights).  That leaves the rounding
+//     of sums that are larger than the result, by 8 sum(p s) / |sum(p s c)|,
+//     a hundred times for 1,000 keys of like weight: 1e-5 of the output, far
+//     below a 16-bit one's own rounding; for fp32 one subtraction per register
+//     takes it out first (5.1e-5 -> below 1e-6 of the output).
 //   * scales stay out of the unpacking.  The 8 columns of the product that a
 //     single query leaves idle are the groups: column n holds the query's
 //     channels of group n and zeros (K), or the weights times group n's scale
@@ -114,11 +118,12 @@ template <typename T, int D, int BS, int W>
 __global__ void __launch_bounds__(W * 32, D == 256 ? 8 / W : 16 / W) kv4_decode_kernel(DecodeKv4Params p) {
   using C = Tile<D, W>;
   using Q = KeyQuery<T, D>;
-  // The weights' low halves.  16-bit outputs do without: a weight rounded to
-  // 11 bits is off by 2^-12, half a step of fp16 and a sixteenth of bf16's,
-  // and the roundings of different keys are independent.  (D = 64 has them in
+  // The weights' low halves.  bf16 outputs do without: a weight rounded to 11
+  // bits is off by 2^-12 at most, an eighth of the output's own rounding, and
+  // the roundings of different keys are independent.  (D = 64 has them in
   // columns 4..7, at no cost.)
-  constexpr bool PLO = std::is_same<T, float>::value && D != 64;
+  constexpr bool PLO = !std::is_same<T, __nv_bfloat16>::value && D != 64;
+  constexpr bool SIGNED = Q::SIGNED;
   constexpr int PAGE = kv4_page_bytes(BS, D), CODES = BS * (D / 2);
   extern __shared__ __align__(16) uint8_t ring_all[];
   __shared__ Smem<D, W> sm;
@@ -384,8 +389,8 @@ __global__ void __launch_bounds__(W * 32, D == 256 ? 8 / W : 16 / W) kv4_decode_
           bh[x][1] = bl[x][1];
         }
         constexpr uint32_t EIGHT = 0x00080008u;
-        mma_f16(eights[x], EIGHT, EIGHT, EIGHT, EIGHT, bh[x][0], bh[x][1]);
-        if constexpr (PLO) mma_f16(eights[x], EIGHT, EIGHT, EIGHT, EIGHT, bl[x][0], bl[x][1]);
+        if constexpr (!SIGNED) mma_f16(eights[x], EIGHT, EIGHT, EIGHT, EIGHT, bh[x][0], bh[x][1]);
+        if constexpr (!SIGNED && PLO) mma_f16(eights[x], EIGHT, EIGHT, EIGHT, EIGHT, bl[x][0], bl[x][1]);
       }
       // ---- out += V^T . weights
       uint32_t v[4][C::VW];
@@ -398,17 +403,21 @@ __global__ void __launch_bounds__(W * 32, D == 256 ? 8 / W : 16 / W) kv4_decode_
       }
 #pragma unroll
       for (int u = 0; u < C::VW; ++u) {
-        constexpr uint32_t LO = 0x000f000fu, HI = 0x00f000f0u;
         const int x = C::SETS == 2 ? u >> 1 : 0;
         uint32_t c01 = __byte_perm(v[0][u], v[1][u], 0x5410), d01 = __byte_perm(v[0][u], v[1][u], 0x7632);
         uint32_t c23 = __byte_perm(v[2][u], v[3][u], 0x5410), d23 = __byte_perm(v[2][u], v[3][u], 0x7632);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t mk = (j & 1) ? HI : LO;
-          mma_f16(acc[u][j], c01 & mk, d01 & mk, c23 & mk, d23 & mk, bh[x][0], bh[x][1]);
-          if constexpr (PLO) mma_f16(acc[u][j], c01 & mk, d01 & mk, c23 & mk, d23 & mk, bl[x][0], bl[x][1]);
-          if (j == 1) c01 >>= 8, d01 >>= 8, c23 >>= 8, d23 >>= 8;
-        }
+        auto add = [&](auto j_) {
+          constexpr int j = decltype(j_)::value;
+          const uint32_t a0 = code_pair<SIGNED, j>(c01), a1 = code_pair<SIGNED, j>(d01),
+                         a2 = code_pair<SIGNED, j>(c23), a3 = code_pair<SIGNED, j>(d23);
+          mma_f16(acc[u][j], a0, a1, a2, a3, bh[x][0], bh[x][1]);
+          if constexpr (PLO) mma_f16(acc[u][j], a0, a1, a2, a3, bl[x][0], bl[x][1]);
+        };
+        add(std::integral_constant<int, 0>{});
+        add(std::integral_constant<int, 1>{});
+        c01 >>= 8, d01 >>= 8, c23 >>= 8, d23 >>= 8;
+        add(std::integral_constant<int, 2>{});
+        add(std::integral_constant<int, 3>{});
       }
     }
     __syncwarp();  // every lane is done with the stage before it is refilled
@@ -424,7 +433,7 @@ __global__ void __launch_bounds__(W * 32, D == 256 ? 8 / W : 16 / W) kv4_decode_
     sm.l[warp] = l;
   }
   {
-    const float down = __uint_as_float((127u + top_e - 29u + 24u) << 23);
+    const float down = __uint_as_float((127u + top_e - 29u + (SIGNED ? 0u : 24u)) << 23);
     const int col = D == 64 ? g >> 1 : g;  // this lane's rows' group, as a column
 #pragma unroll
     for (int u = 0; u < C::VW; ++u)

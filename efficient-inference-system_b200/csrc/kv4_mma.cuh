@@ -77,6 +77,25 @@ __device__ __forceinline__ __half2 scale_pair(uint32_t codes, uint32_t select) {
   return *reinterpret_cast<const __half2*>(&x);
 }
 
+// A pair of codes in nibble J & 1 of the low bytes of x as fp16 numbers (16
+// times them for an upper nibble): the nibble alone, a subnormal, (c + 8) *
+// 2^-24, or, SIGNED, c itself, taken exactly from 1024 + (c + 8).
+template <bool SIGNED, int J>
+__device__ __forceinline__ uint32_t code_pair(uint32_t x) {
+  constexpr uint32_t mask = (J & 1) ? 0x00f000f0u : 0x000f000fu;
+  if constexpr (!SIGNED) return x & mask;
+  const uint32_t y = (x & mask) | 0x64006400u, off = (J & 1) ? 0x64806480u : 0x64086408u;  // 1152, 1032
+  return half2_bits(__hsub2(*reinterpret_cast<const __half2*>(&y), *reinterpret_cast<const __half2*>(&off)));
+}
+// Channels r and r + 4 of a word, r = 0 .. 3.
+template <bool SIGNED>
+__device__ __forceinline__ void code_pairs(uint32_t w, uint32_t (&f)[4]) {
+  f[0] = code_pair<SIGNED, 0>(w);
+  f[1] = code_pair<SIGNED, 1>(w);
+  f[2] = code_pair<SIGNED, 0>(w >> 8);
+  f[3] = code_pair<SIGNED, 1>(w >> 8);
+}
+
 // How a lane (g = lane / 4, t = lane % 4) holds the K row of one key.
 template <int D>
 struct KeyWords {
@@ -178,6 +197,11 @@ template <typename T, int D>
 struct KeyQuery {
   using C = KeyWords<D>;
   static constexpr bool QLO = std::is_same<T, float>::value && D != 64;  // low halves as a second product
+  // Codes enter as subnormals c + 8, with the 8 taken out of the sums, or as
+  // numbers c.  The former costs a few 2^-20 of a logit: the sums are larger
+  // than the result, and the product aligns subnormal operands by an exponent
+  // up to 10 too large.
+  static constexpr bool SIGNED = std::is_same<T, float>::value;
   uint4 raw[C::KW][sizeof(T) / 2];  // the channels of this lane's column, 8 per word
   uint32_t qh[C::KW][4], ql[QLO ? C::KW : 1][4];
   float init[C::SETS][2];  // -8 sum(q) of columns 2t, 2t+1, in the product's units
@@ -219,7 +243,7 @@ struct KeyQuery {
     int e = 140 - (int)(__float_as_uint(top) >> 23);  // top's exponent field + e = 13 + 127
     e = e > 100 ? 100 : e;
     const float up = __uint_as_float((uint32_t)(127 + e) << 23);
-    unit = qscale * 0x1p24f;
+    unit = SIGNED ? qscale : qscale * 0x1p24f;
     down_q = __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
     for (int w = 0; w < C::KW; ++w) {
@@ -254,7 +278,7 @@ struct KeyQuery {
       }
       sum += __shfl_xor_sync(kFullMask, sum, 1);
       sum += __shfl_xor_sync(kFullMask, sum, 2);
-      sum *= -8.f * 0x1p-24f;
+      sum *= SIGNED ? 0.f : -8.f * 0x1p-24f;
       init[s][0] = __shfl_sync(kFullMask, sum, 8 * t);
       init[s][1] = __shfl_sync(kFullMask, sum, 8 * t + 4);
     }
@@ -280,13 +304,15 @@ struct KeyQuery {
     }
 #pragma unroll
     for (int w = 0; w < C::KW; ++w) {
-      constexpr uint32_t LO = 0x000f000fu, HI = 0x00f000f0u;
       float(&c)[4] = s[C::SETS == 2 ? w >> 2 : w & 1];
-      const uint32_t u = ka[w], v = kb[w], u8 = u >> 8, v8 = v >> 8;
-      mma_f16(c, u & LO, v & LO, u & HI, v & HI, qh[w][0], qh[w][1]);
-      if constexpr (QLO) mma_f16(c, u & LO, v & LO, u & HI, v & HI, ql[w][0], ql[w][1]);
-      mma_f16(c, u8 & LO, v8 & LO, u8 & HI, v8 & HI, qh[w][2], qh[w][3]);
-      if constexpr (QLO) mma_f16(c, u8 & LO, v8 & LO, u8 & HI, v8 & HI, ql[w][2], ql[w][3]);
+      uint32_t u[4], v[4];
+      code_pairs<SIGNED>(ka[w], u);
+      code_pairs<SIGNED>(kb[w], v);
+#pragma unroll
+      for (int r = 0; r < 4; r += 2) {
+        mma_f16(c, u[r], v[r], u[r + 1], v[r + 1], qh[w][r], qh[w][r + 1]);
+        if constexpr (QLO) mma_f16(c, u[r], v[r], u[r + 1], v[r + 1], ql[w][r], ql[w][r + 1]);
+      }
     }
     if constexpr (C::SETS == 1) {
 #pragma unroll

@@ -200,6 +200,63 @@ def test_decode_long(cuda_device, dtype, B, L):
     _check(out, ref, bound)
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("T", [1, 60])
+def test_fp32_precision(cuda_device, D, T):
+    """Even rows (unit normal, outputs a thirtieth of a value): fp32 outputs are right as a whole to 2^-19.
+
+    With |logit| under 8, two halves of q and fp32 sums leave a logit off by 2^-21 at most in the mean square, the
+    weights by e^ that; n = 1,000 independent roundings of the sums of p v add 2^-24 * 1000^(1/2) * 4 at most
+    relative to |out|.  Sums that carry an offset of the codes (5e-5 before they were kept apart) show."""
+    rng = np.random.default_rng(D)
+    H, bs, n = 2, 16, 1000
+    NB = -(-n // bs)
+    k, v = rng.standard_normal((NB, H, bs, D)), rng.standard_normal((NB, H, bs, D))
+    q = torch.from_numpy(rng.standard_normal((1, H, T, D))).float().to(cuda_device)
+    fn = b2pa.paged_attention_decode_kv4 if T == 1 else b2pa.paged_attention_prefill_kv4
+    out = fn(q, torch.from_numpy(co.pack_pages(k, False)).to(cuda_device),
+             torch.from_numpy(co.pack_pages(v, True)).to(cuda_device), _i32(np.arange(NB)[None], cuda_device),
+             _i32([n], cuda_device), _i32([T], cuda_device))
+    p, _ = co.softmax_rows(_np(q)[0], co.rows_of(co.stored(k), range(NB), n), T, D ** -0.5)
+    ref = np.einsum("htn,nhd->htd", p, co.rows_of(co.stored(v), range(NB), n))
+    assert np.linalg.norm(_np(out)[0] - ref) <= 2.0 ** -19 * np.linalg.norm(ref)
+
+
+@pytest.mark.parametrize("dtype,D", [(torch.float32, 64), (torch.float32, 128), (torch.bfloat16, 256),
+                                     (torch.float16, 128)])
+def test_prefill_long(cuda_device, dtype, D):
+    """Few queries on many keys (keys split between CTAs), and more queries than one CTA takes."""
+    for T, lens in ((5, [6000, 4001]), (201, [201, 900])):
+        cur = [T] * 2
+        out, ref, bound, _ = _attend_case(cuda_device, lens=lens, cur=cur, H=2, D=D, bs=16, dtype=dtype, T=T, seed=T)
+        _check(out, ref, bound + (0 if dtype == torch.float32 else HALF_STEP[dtype] * np.abs(ref).max()))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,bs,H", [(64, 16, 3), (128, 8, 2), (256, 32, 1)])
+def test_append_many_is_append_one_by_one(cuda_device, dtype, D, bs, H):
+    """A long ragged prompt batch (an odd number of slots) leaves the pages that its tokens leave one at a time, and
+    reads back alike."""
+    rng = np.random.default_rng(D)
+    B, T = 9, 151
+    starts, lens = [0, 1, bs - 1, 7, 0, 3, 64, 0, 2], [151, 150, 1, 0, 77, 151, 8, 2, 149]
+    ends = [a + n for a, n in zip(starts, lens)]
+    NB = sum(-(-e // bs) for e in ends) + 2
+    table = _table(random_tables(rng, ends, NB, bs), cuda_device)
+    k, v = (torch.from_numpy(_rows(rng, (B, T, H, D))).to(dtype).to(cuda_device).transpose(1, 2) for _ in range(2))
+    pools = [torch.full((NB, H, bs, D * 9 // 16), 5, dtype=torch.uint8, device=cuda_device) for _ in range(4)]
+    b2pa.kv4_append(k, v, *pools[:2], table, _i32(starts, cuda_device), _i32(lens, cuda_device))
+    for t in range(T):
+        live = [int(t < n) for n in lens]
+        b2pa.kv4_append(k[:, :, t:t + 1], v[:, :, t:t + 1], *pools[2:], table,
+                        _i32([a + t for a in starts], cuda_device), _i32(live, cuda_device))
+    assert torch.equal(pools[0], pools[2]) and torch.equal(pools[1], pools[3])
+    args = table, _i32(starts, cuda_device), _i32(lens, cuda_device), T, dtype
+    live = (np.arange(T) < np.array(lens)[:, None])[:, None, :, None]
+    for got, x in zip(b2pa.kv4_read(*pools[:2], *args), (k, v)):
+        assert np.array_equal(_np(got), np.where(live, co.stored(_np(x)), 0))
+
+
 def test_decode_offsets_past_32_bits(cuda_device):
     """Pages at byte offsets past 2^32 of the pool."""
     H, D, bs = 8, 128, 32
