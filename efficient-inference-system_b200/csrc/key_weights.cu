@@ -527,7 +527,7 @@ __global__ void __launch_bounds__(kStepThreads, KV4 ? 3 : 0) key_weights_step_ke
   const int32_t* table = a.page_table + (int64_t)b * a.pt_stride;
   // logits of this CTA's keys
   float* z = far ? far + ((int64_t)b * a.H + h) * far_stride + lo : near;
-  const int seen = vis < hi ? vis : hi;  // keys [lo, seen) have a logit
+  const uint32_t seen = vis < hi ? vis : hi;  // keys [lo, seen) have a logit
   const uint32_t page_bytes = KV4 ? kv4_page_bytes(bs, D) : bs * RB;
   const char* const pages = static_cast<const char*>(a.k_pool) + (int64_t)h * page_bytes;
   const uint64_t block_bytes = (uint64_t)a.H * page_bytes;
@@ -535,21 +535,21 @@ __global__ void __launch_bounds__(kStepThreads, KV4 ? 3 : 0) key_weights_step_ke
 
   float top = -INFINITY;
   constexpr int kWarps = kStepThreads / 32;
-  auto ids_of = [&](int64_t j0) {  // lane l: the l-th page from key j0's
-    const int64_t pg = (j0 >> sh) + lane;
+  auto ids_of = [&](uint32_t j0) {  // lane l: the l-th page from key j0's
+    const uint32_t pg = (j0 >> sh) + lane;
     return j0 < seen && pg << sh < seen ? table[pg] : -1;
   };
-  int64_t j0 = lo + warp * RW;
+  uint32_t j0 = lo + warp * RW;  // (a turn past the last position fits 32 bits unsigned)
   int ids = ids_of(j0);
   bool past_pool = false;
   // Row j of the turn at j0: its page (block 0's for one that is not seen).
-  auto page_of = [&](int64_t j, bool& ok) -> const char* {
+  auto page_of = [&](uint32_t j, bool& ok) -> const char* {
     const uint32_t blk = (uint32_t)__shfl_sync(kFullMask, ids, (int)((j >> sh) - (j0 >> sh)));
     ok = j < seen && blk < blocks;
     past_pool |= j < seen && (int)blk >= (int)blocks;
     return pages + (ok ? blk : 0u) * block_bytes;
   };
-  auto locate = [&](int64_t j, bool& ok) -> const char* { return page_of(j, ok) + (int)(j & (bs - 1)) * RB; };
+  auto locate = [&](uint32_t j, bool& ok) -> const char* { return page_of(j, ok) + (int)(j & (bs - 1)) * RB; };
   if constexpr (KV4) {
     using W = KeyWords<D>;
     using Q = KeyQuery<T, D>;
@@ -562,11 +562,19 @@ __global__ void __launch_bounds__(kStepThreads, KV4 ? 3 : 0) key_weights_step_ke
       uint32_t words[S::PACKED][2][W::KW], codes[S::PACKED][2][W::SETS];
       bool ok[S::PACKED][2];
 #pragma unroll
-      for (int x = 0; x < S::PACKED; ++x)
+      for (int x = 0; x < S::PACKED; ++x) {
+        const char* above = pages;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int64_t j = j0 + x * 16 + g + 8 * i;
-          const char* page = page_of(j, ok[x][i]);
+          const uint32_t j = j0 + x * 16 + g + 8 * i;
+          const char* page;
+          if (i == 1 && bs >= 16) {  // on the page of the row 8 above
+            page = above;
+            ok[x][1] = ok[x][0] && j < seen;
+          } else {
+            page = page_of(j, ok[x][i]);
+          }
+          above = page;
           const int row = (int)(j & (bs - 1));
           const char* src = page + row * RB + t * W::KB;
 #pragma unroll
@@ -581,6 +589,7 @@ __global__ void __launch_bounds__(kStepThreads, KV4 ? 3 : 0) key_weights_step_ke
           for (int k = 0; k < W::SETS; ++k)
             codes[x][i][k] = __ldg(reinterpret_cast<const uint16_t*>(sc + Q::scale_at(k)));
         }
+      }
 #pragma unroll
       for (int x = 0; x < S::PACKED; ++x) {
         float z2[2];
@@ -590,7 +599,7 @@ __global__ void __launch_bounds__(kStepThreads, KV4 ? 3 : 0) key_weights_step_ke
           const float all = query.finish(z2[i]);
           const float dot = ok[x][i] ? all : -INFINITY;
           top = fmaxf(top, dot);
-          const int64_t j = j0 + x * 16 + g + 8 * i;
+          const uint32_t j = j0 + x * 16 + g + 8 * i;
           if (t == 0 && j < seen) z[j - lo] = dot;
         }
       }
@@ -632,7 +641,7 @@ __global__ void __launch_bounds__(kStepThreads, KV4 ? 3 : 0) key_weights_step_ke
         for (int i = 0; i < 2; ++i) {
           const float dot = ok[x][i] ? (c0[2 * i] + c1[2 * i]) * qscale : -INFINITY;
           top = fmaxf(top, dot);
-          const int64_t j = j0 + x * 16 + g + 8 * i;
+          const uint32_t j = j0 + x * 16 + g + 8 * i;
           if (t == 0 && j < seen) z[j - lo] = dot;
         }
       }
@@ -675,7 +684,7 @@ __global__ void __launch_bounds__(kStepThreads, KV4 ? 3 : 0) key_weights_step_ke
         for (int o = S::LPR / 2; o >= 1; o >>= 1) dot += __shfl_xor_sync(kFullMask, dot, o);
         if (!ok[r]) dot = -INFINITY;
         top = fmaxf(top, dot);
-        const int64_t j = j0 + r * S::RP + lane / S::LPR;
+        const uint32_t j = j0 + r * S::RP + lane / S::LPR;
         if (sub == r % S::LPR && j < seen) z[j - lo] = dot;
       }
       ids = next;
@@ -690,7 +699,7 @@ __global__ void __launch_bounds__(kStepThreads, KV4 ? 3 : 0) key_weights_step_ke
   for (int w = 0; w < kWarps; ++w) top = fmaxf(top, red[0][w]);
   float ref = top == -INFINITY ? 0.f : top;
   float sum = 0.f;
-  const int mine = hi - lo, logits = seen > lo ? seen - lo : 0;
+  const int mine = hi - lo, logits = (int)seen > lo ? (int)seen - lo : 0;
   for (int i = tid; i < logits; i += kStepThreads) sum += fast_exp2(z[i] - ref);
   sum = warp_sum(sum);
   if (lane == 0) red[1][warp] = sum;

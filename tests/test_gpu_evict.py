@@ -117,6 +117,84 @@ def test_key_weights_long(cuda_device, dtype, B, n, T):
     _weights_case(cuda_device, lens=lens, cur=[T] * B, T=T, H=4, D=64, bs=16, dtype=dtype, kv4=True, window=0, seed=n)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kv4", [False, True])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_key_weights_many_queries(cuda_device, dtype, kv4, D):
+    """Several tiles of queries, with a window that begins inside one; one query past a tile, one past half of it."""
+    for T, window in ((300, 0), (300, 150), (129, 0), (65, 0), (200, 64)):
+        _weights_case(cuda_device, lens=[T, T + 211, 150], cur=[T, T - 5, 150 if T > 150 else 30], T=T, H=2, D=D, bs=16,
+                      dtype=dtype, kv4=kv4, window=window, seed=T + window)
+
+
+@pytest.mark.parametrize("kv4", [False, True])
+@pytest.mark.parametrize("T", [1, 3])
+def test_key_weights_wide_table(cuda_device, kv4, T):
+    """A table far wider than its sequences (more keys than logits fit on chip) gives what a narrow one gives."""
+    dev, H, D, bs = cuda_device, 2, 64, 16
+    rng = np.random.default_rng(3)
+    lens = [333, 40]
+    tables = random_tables(rng, lens, 30, bs)
+    k = rng.standard_normal((30, H, bs, D))
+    pool = torch.from_numpy(co.pack_pages(k, False)).to(dev) if kv4 else torch.from_numpy(k).to(torch.float16).to(dev)
+    q = torch.from_numpy(rng.standard_normal((2, H, T, D))).to(torch.float16).to(dev)
+    w = torch.zeros(30, H, bs, device=dev)
+    narrow, wide = (b2pa.accumulate_key_weights(q, pool, w, _table(tables, dev, width), _i32(lens, dev),
+                                                _i32([T, T], dev), out=torch.zeros_like(w)) for width in (None, 20000))
+    # the same products, summed in another order: n roundings of a sum of exponentials and one of its logarithm
+    torch.testing.assert_close(wide, narrow, rtol=(333 + 16) * 2.0 ** -24, atol=0)
+    assert narrow.sum().item() == pytest.approx(2 * H * T, rel=1e-4)
+
+
+def test_two_graphs_and_a_side_stream(cuda_device):
+    """Weights and eviction on another stream, and in two captured graphs that replay at the same time."""
+    dev, H, D, bs, T = cuda_device, 2, 64, 16, 30
+    rng = np.random.default_rng(21)
+    lens, cur = [200, 90], [T, T]
+    table, n, c = _i32([list(range(13)), list(range(13, 26))], dev), _i32(lens, dev), _i32(cur, dev)
+
+    def inputs(seed):
+        gen = torch.Generator().manual_seed(seed)
+        return [torch.randn(*shape, generator=gen).to(dev) for shape in
+                ((2, H, T, D), (26, H, bs, D), (26, H, bs, D))] + [torch.rand(26, H, bs, generator=gen).to(dev)]
+
+    def work(q, k, v, w):
+        b2pa.accumulate_key_weights(q, k, w, table, n, c)
+        return b2pa.evict_by_weight(k, v, w, table, n, 50, 10)
+
+    sets = [inputs(0), inputs(1)]
+    want = []
+    for x in sets:
+        y = [t.clone() for t in x]
+        want.append([work(*y)] + y)
+    side = torch.cuda.Stream(dev)
+    side.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(side):
+        y = [t.clone() for t in sets[0]]
+        got = [work(*y)] + y
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want[0]))
+    live = [[t.clone() for t in x] for x in sets]
+    graphs, outs = [], []
+    for x in live:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(work(*x))
+        graphs.append(g)
+    streams = [torch.cuda.Stream(dev) for _ in graphs]
+    for _ in range(5):
+        for x, y in zip(live, sets):
+            for a, b in zip(x, y):
+                a.copy_(b)
+        torch.cuda.synchronize()
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for x, o, y in zip(live, outs, want):
+            assert all(torch.equal(a, b) for a, b in zip([o] + x, y))
+
+
 def _evict_case(dev, *, lens, keep, recent, H, D, bs, dtype, kv4, seed, fresh, weights=None):
     rng = np.random.default_rng(seed)
     B = len(lens)
