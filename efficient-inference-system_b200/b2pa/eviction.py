@@ -24,6 +24,7 @@ from .kv4 import (aligned_rows, check_heads, int32_rows, need_cuda, on_device, p
                   strides_of, table_args, workspace_of)
 
 PLAIN_HEAD_DIMS = (16, 32, 64, 128, 256)
+_MOST = 2 ** 31 - 1  # positions are 32-bit
 
 
 def _pool_args(what: str, k_pool, v_pool, head_dim: int | None):
@@ -67,8 +68,10 @@ def accumulate_key_weights(q: torch.Tensor, k_pool: torch.Tensor, key_weights: t
     code = _lib.dtype_code(q.dtype)
     if pool_code != _lib.DTYPE_KV4 and pool_code != code:
         raise TypeError(f"pool dtype {k_pool.dtype} differs from q dtype {q.dtype}")
-    if window is not None and window < 1:
-        raise ValueError(f"b2pa.{what}: window {window} < 1")
+    if window is not None:
+        if window < 1:
+            raise ValueError(f"b2pa.{what}: window {window} < 1")
+        window = min(window, T)
     for name, w in (("key_weights", key_weights), ("out", out)):
         _check_weights(what, name, w, (blocks, H, bs))
     table, pt_stride, pages = table_args(what, "page_table", page_table, B)
@@ -114,6 +117,9 @@ def evict_by_weight(k_pool: torch.Tensor, v_pool: torch.Tensor, key_weights: tor
     _check_weights(what, "key_weights", key_weights, (blocks, H, bs))
     if keep < 1 or recent < 0:
         raise ValueError(f"b2pa.{what}: keep must be at least 1 and recent not negative, got {keep} and {recent}")
+    if keep > _MOST:
+        raise ValueError(f"b2pa.{what}: keep {keep} is above {_MOST}")
+    recent = min(recent, keep)
     B = page_table.shape[0]
     table, pt_stride, pages = table_args(what, "page_table", page_table, B)
     seq_lens = int32_rows(what, "seq_lens", seq_lens, B)
@@ -159,7 +165,7 @@ def accumulate_from(kv_cache, q: torch.Tensor, current_lengths) -> None:
     kb = pool.k_blocks
     launch_key_weights(aligned_rows(q), kb, _lib.DTYPE_KV4 if kb.dtype == torch.uint8 else _lib.dtype_code(kb.dtype),
                        pool.key_weights, pool.key_weights, table, table.stride(0), pages, seq_lens, cur,
-                       pool.key_weight_window)
+                       min(pool.key_weight_window or T, T))
 
 
 def evict_batch(cache, keep: int, recent: int = 0) -> torch.Tensor:
@@ -185,7 +191,8 @@ def evict_batch(cache, keep: int, recent: int = 0) -> torch.Tensor:
     with on_device(dev.index):
         note_released_rows(cache, dev)
         table, seq_lens, pages = block_table_and_lengths(cache, dev, transient=True)
-        kept = evict_by_weight(pool.k_blocks, pool.v_blocks, pool.key_weights, table[:, :pages], seq_lens, keep, recent)
+        most = max(1, min(keep, max((s.seq_len for s in states), default=1)))  # no sequence keeps more
+        kept = evict_by_weight(pool.k_blocks, pool.v_blocks, pool.key_weights, table[:, :pages], seq_lens, most, recent)
         left = -(-keep // pool.block_size)
         freed = []
         for s in states:

@@ -225,7 +225,8 @@ class BatchedPagedKVCache:
         largest accumulated attention weight (the pool must track them:
         ``track_key_weights``).  The kept tokens move together in order and
         the freed blocks return to the pool.  Returns the kept positions,
-        int32 [B, H, keep], -1 behind a shorter sequence's last."""
+        int32 [B, H, min(keep, longest sequence)], -1 behind a shorter
+        sequence's last."""
         from .eviction import evict_batch
 
         return evict_batch(self, keep, recent)

@@ -280,7 +280,7 @@ class DecodeStep:
             m, kb = self.meta, pool.k_blocks
             code = _lib.DTYPE_KV4 if kb.dtype == torch.uint8 else _lib.dtype_code(kb.dtype)
             launch_key_weights(aligned_rows(q), kb, code, weights, weights, m.table, m.width, m.width, m.seq_lens,
-                               m.ones, pool.key_weight_window, m.workspace)
+                               m.ones, None, m.workspace)  # one query: any window counts it
         return out
 
     def _attend_kv4(self, q: torch.Tensor, pool, pend: _StepPending) -> torch.Tensor:

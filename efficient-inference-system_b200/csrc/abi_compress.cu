@@ -128,8 +128,8 @@ int b2pa_kv4_append(const void* k_new, const int64_t new_k_strides[4], const voi
   B2PA_TRY(check_sizes(fn, B, H, T, D, block_size, max_pages, num_blocks));
   if (dtype_size(dtype) == 0) return set_error(B2PA_ERR_UNSUPPORTED, "%s: unknown dtype %d", fn, dtype);
   B2PA_TRY(check_kv4(fn, D, k_pool, v_pool));
-  if (B == 0 || T == 0) return B2PA_OK;
-  if (!k_new || !v_new || !k_pool || !v_pool || !new_k_strides || !new_v_strides || !start_pos || !lengths)
+  if (B == 0 || (T == 0 && !seq_lens_out)) return B2PA_OK;
+  if ((T > 0 && (!k_new || !v_new)) || !k_pool || !v_pool || !new_k_strides || !new_v_strides || !start_pos || !lengths)
     return set_error(B2PA_ERR_INVALID_ARGUMENT, "%s: null pointer argument", fn);
   B2PA_TRY(check_table(fn, page_table, pt_stride, max_pages));
   AppendArgs a{};

@@ -208,7 +208,8 @@ static bool many_tokens(int B, int T) { return (int64_t)B * ((T + 1) / 2) >= 4 *
 template <typename T>
 static int append_as(const AppendArgs& a, int64_t* seq_out, cudaStream_t s) {
   const bool vec = rows16(a.k_new, a.sk, sizeof(T)) && rows16(a.v_new, a.sv, sizeof(T));
-  const dim3 one((unsigned)a.T, (unsigned)a.B), two((unsigned)((a.T + 1) / 2), (unsigned)a.B);
+  // (no tokens: the lengths are still written)
+  const dim3 one((unsigned)(a.T > 0 ? a.T : 1), (unsigned)a.B), two((unsigned)((a.T + 1) / 2), (unsigned)a.B);
   cudaError_t e;
   if (!vec)
     e = launch_pdl(kv4_append_kernel<T, false, 1>, one, dim3(128), 0, s, a, seq_out);

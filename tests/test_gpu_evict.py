@@ -304,7 +304,8 @@ def test_evict_refusals(cuda_device):
     dev = cuda_device
     kp, w = torch.zeros(4, 2, 16, 64, device=dev), torch.zeros(4, 2, 16, device=dev)
     t, n = _i32([[0, 1]], dev), _i32([20], dev)
-    for bad in (dict(keep=0), dict(keep=4, recent=-1), dict(keep=17, out_table=_i32([[3]], dev))):
+    for bad in (dict(keep=0), dict(keep=4, recent=-1), dict(keep=17, out_table=_i32([[3]], dev)),
+                dict(keep=2 ** 32 + 4)):
         with pytest.raises(ValueError):
             b2pa.evict_by_weight(kp, kp.clone(), w, t, n, **bad)
     with pytest.raises(ValueError):
@@ -315,6 +316,28 @@ def test_evict_refusals(cuda_device):
         b2pa.accumulate_key_weights(torch.zeros(1, 2, 1, 64, device=dev, dtype=torch.bfloat16), kp, w, t, n, n)
     with pytest.raises(ValueError):
         b2pa.accumulate_key_weights(torch.zeros(1, 2, 1, 64, device=dev), kp, w, t, n, n, window=0)
+
+
+def test_counts_past_32_bits(cuda_device):
+    """``recent`` and ``window`` of any size mean all of them; a batch cut to any number keeps what it has."""
+    dev = cuda_device
+    gen = torch.Generator().manual_seed(0)
+    k, v = (torch.randn(3, 2, 16, 64, generator=gen).to(dev) for _ in range(2))
+    w, q = torch.rand(3, 2, 16, generator=gen).to(dev), torch.randn(1, 2, 5, 64, generator=gen).to(dev)
+    t, n, five = _i32([[2, 0, 1]], dev), _i32([40], dev), _i32([5], dev)
+    assert b2pa.evict_by_weight(k, v, w, t, n, 7, 2 ** 32 + 1).tolist() == [[list(range(33, 40))] * 2]
+    n = _i32([7], dev)
+    for window in (5, 2 ** 31, 2 ** 32 + 1):
+        assert torch.equal(b2pa.accumulate_key_weights(q, k, w, t, n, five, window=window, out=torch.zeros_like(w)),
+                           b2pa.accumulate_key_weights(q, k, w, t, n, five, out=torch.zeros_like(w)))
+    pool = b2pa.LayerBlockPool(16, 3, 1.5)
+    pool.track_key_weights(2 ** 32 + 1)
+    state = b2pa.PagedKVCacheState(pool)
+    cache = b2pa.BatchedPagedKVCache([state], pool)
+    cache.append_batch(q, q, [5])
+    b2pa.paged_attention("b200_paged", q, cache, [5])
+    assert pool.key_weights.sum().item() == pytest.approx(10, rel=1e-5)
+    assert cache.evict(2 ** 40).tolist() == [[list(range(5))] * 2] and state.seq_len == 5
 
 
 @pytest.mark.parametrize("kv4", [False, True], ids=["plain", "kv4"])

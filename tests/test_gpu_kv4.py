@@ -414,6 +414,34 @@ def test_streams_layouts_and_capture(cuda_device):
     assert torch.equal(b2pa.paged_attention_decode_kv4(odd, kp, vp, table, lens, one), out)
 
 
+def test_nothing_to_do(cuda_device):
+    """Empty batches, chunks without tokens and pools without blocks: empty results, and the lengths all the same."""
+    dev = cuda_device
+    kp, vp = (torch.zeros(4, 2, 16, 36, dtype=torch.uint8, device=dev) for _ in range(2))
+    t, five = _i32([[0, 1]], dev), _i32([5], dev)
+    none, no_table = _i32(np.zeros(0), dev), torch.zeros(0, 2, dtype=torch.int32, device=dev)
+    out = torch.full((1,), -7, dtype=torch.int64, device=dev)
+    rows = torch.zeros(1, 2, 0, 64, device=dev)
+    b2pa.kv4_append(rows, rows, kp, vp, t, five, five, out)
+    assert out.tolist() == [5]
+    assert b2pa.kv4_read(kp, vp, t, five, five, 0, torch.float32)[0].shape == (1, 2, 0, 64)
+    assert b2pa.paged_attention_prefill_kv4(rows, kp, vp, t, five, five).shape == (1, 2, 0, 64)
+    for T in (1, 3):
+        rows = torch.zeros(0, 2, T, 64, device=dev)
+        b2pa.kv4_append(rows, rows, kp, vp, no_table, none, none)
+        fn = b2pa.paged_attention_decode_kv4 if T == 1 else b2pa.paged_attention_prefill_kv4
+        assert fn(rows, kp, vp, no_table, none, none).shape == (0, 2, T, 64)
+        w = torch.ones(4, 2, 16, device=dev)
+        assert b2pa.accumulate_key_weights(rows, kp, w, no_table, none, none).eq(1).all()
+        # no pages at all
+        q = torch.ones(1, 2, T, 64, device=dev)
+        assert not fn(q, kp, vp, t[:, :0], _i32([0], dev), _i32([T], dev)).any()
+        assert b2pa.accumulate_key_weights(q, kp, w, t[:, :0], _i32([0], dev), _i32([T], dev)).eq(1).all()
+    assert b2pa.evict_by_weight(kp, vp, w, no_table, none, 4).shape == (0, 2, 4)
+    assert b2pa.evict_by_weight(kp, vp, w, t[:, :0], _i32([0], dev), 4).eq(-1).all()
+    assert not kp.any() and not vp.any() and b2pa.read_status(dev) == 0
+
+
 def test_refusals(cuda_device):
     dev = cuda_device
     kp = torch.zeros(4, 2, 16, 36, dtype=torch.uint8, device=dev)
