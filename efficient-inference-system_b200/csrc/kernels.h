@@ -157,6 +157,10 @@ PrefillPlan make_prefill_plan_f32_tiled(int B, int H, int T, int D, int max_page
 bool prefill_uses_tensor_cores(int D, int block_size, int dtype, int64_t pool_rows);
 
 int launch_paged_prefill_f32(const AttnArgs& a, cudaStream_t s);
+// fp32 q with head_dim 64 on fp16 pages (make_prefill_plan's split_tc; the flag
+// at its off_flag): inputs that are out of range leave `epoch` in the flag, and
+// the caller's next kernel redoes the call.
+int launch_paged_prefill_f32_on_halves(const AttnArgs& a, uint32_t epoch, cudaStream_t s);
 int launch_paged_prefill_bf16(const AttnArgs& a, cudaStream_t s);
 int launch_paged_prefill_f16(const AttnArgs& a, cudaStream_t s);
 
@@ -223,11 +227,13 @@ int launch_kv4_read(const Kv4ReadArgs& a, cudaStream_t s);
 int launch_kv4_decode(const AttnArgs& a, cudaStream_t s);
 
 struct Kv4PrefillPlan {
-  size_t off_k, off_v, off_table, off_inner, inner_bytes, bytes;
+  int unpack;  // 0: straight from the pages, no workspace
+  size_t off_k, off_v, off_table, off_flag, off_inner, inner_bytes, bytes;
 };
 Kv4PrefillPlan make_kv4_prefill_plan(int B, int H, int T, int D, int max_pages, int block_size, int dtype);
 int launch_kv4_prefill(const AttnArgs& a, const Kv4PrefillPlan& plan, cudaStream_t s);
-int launch_kv4_prefill_mma(const AttnArgs& a, cudaStream_t s);
+// flag (may be null: always): runs only where *flag == epoch by then.
+int launch_kv4_prefill_mma(const AttnArgs& a, const uint32_t* flag, uint32_t epoch, cudaStream_t s);
 
 size_t key_weights_workspace(int B, int H, int T, int D, int max_pages, int block_size, int dtype, int pool_dtype);
 int launch_key_weights(const KeyWeightArgs& a, cudaStream_t s);

@@ -2,11 +2,20 @@
 //
 // A prompt chunk of T queries makes 4 T L D operations of every L keys, so
 // its time is the tensor cores' and not the cache's.  Where a tcgen05 kernel
-// of the plain pools does the rest (fp32 with head_dim 64, 16-bit types with
-// 64 and 128; else kv4_prefill_mma.cu), the pages the call reads are written out in the type of q in the workspace, as a pool of
-// B * max_pages blocks with a table of their own (exact: a stored value has 7
-// significant bits), and that kernel runs on it.
-// Rows past a sequence's length are written as zeros.
+// of the plain pools can do the rest (fp32 with head_dim 64, 16-bit types with
+// 64 and 128; else kv4_prefill_mma.cu does it all), the pages the call reads
+// are written out in the workspace, in q's type or, for fp32, in fp16 (exact
+// either way: a stored value has 7 significant bits), as a pool of
+// B * max_pages blocks with a table of their own, and that kernel runs on it;
+// rows past a sequence's length are written as zeros.
+// Two kinds of inputs are not for that kernel: fp32 queries of 2^15 and more,
+// which it splits into fp16 halves as they are, and NaN groups of V at keys
+// that only some of the chunk's queries see (a zero weight times NaN).  They
+// leave the call's number in a flag, and the kernel of kv4_prefill_mma.cu,
+// launched behind it, redoes the call if it finds it there.  The number is part
+// of a captured graph: once a replay has set it, later ones redo the call too.
+#include <atomic>
+
 #include "common.cuh"
 #include "kernels.h"
 #include "kv4.cuh"
@@ -15,7 +24,8 @@ namespace b2pa {
 
 // One CTA per (page, sequence): dequantises every head's K and V page.
 template <typename T>
-__global__ void __launch_bounds__(256) kv4_unpack_kernel(AttnArgs a, T* k_out, T* v_out, int32_t* table) {
+__global__ void __launch_bounds__(256) kv4_unpack_kernel(AttnArgs a, T* k_out, T* v_out, int32_t* table,
+                                                         uint32_t* flag, uint32_t epoch) {
   pdl_wait();
   pdl_launch_dependents();
   const int p = blockIdx.x, b = blockIdx.y;
@@ -38,6 +48,8 @@ __global__ void __launch_bounds__(256) kv4_unpack_kernel(AttnArgs a, T* k_out, T
   T* ko = k_out + ((slot * a.H) << head_log2) * 8;
   T* vo = v_out + ((slot * a.H) << head_log2) * 8;
   const int rows = L - first < BS ? (int)(L - first) : BS;  // the others are zeros
+  const int64_t all_see = L - a.cur_lens[b] + 1 - first;      // rows below it are seen by every query
+  bool nan = false;
 #pragma unroll 2
   for (int i = threadIdx.x; i < a.H << head_log2; i += blockDim.x) {
     const int h = i >> head_log2, r = i & ((1 << head_log2) - 1);  // word r of the head's page
@@ -47,53 +59,64 @@ __global__ void __launch_bounds__(256) kv4_unpack_kernel(AttnArgs a, T* k_out, T
     uint32_t wk = *reinterpret_cast<const uint32_t*>(kh + 4 * r), wv = *reinterpret_cast<const uint32_t*>(vh + 4 * r);
     uint32_t ck = kh[codes + row * (D / 16) + g], cv = vh[codes + g * BS + row];
     if (row >= rows) wk = wv = 0x88888888u, ck = cv = 0;
+    nan |= cv == kKv4NanScale && row >= all_see;
     kv4_store8(ko + (int64_t)i * 8, wk, ck);
     kv4_store8(vo + (int64_t)i * 8, wv, cv);
   }
+  if (nan) *flag = epoch;
 }
 
 static size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
-// Shapes without a tcgen05 kernel of the plain pools behind the unpacking: the
-// others' kernels there run on the CUDA cores.  Unpacking and plain kernel ->
-// straight from the pages (us; 2 sequences, 32 heads, 1,021 queries on 1,024
-// to 7,168 keys): fp32 head_dim 64 403 -> 918, 128 5,524 -> 1,399, 256 29,044
-// -> 2,477; bf16 64 205 -> 753, 128 305 -> 1,107, 256 26,457 -> 1,752.
-static bool takes_mma(int D, int dtype) {
-  return D == 256 || (D == 128 && dtype == B2PA_DTYPE_F32);
+// Whether a tcgen05 kernel of the plain pools takes the shape; their others run
+// on the CUDA cores.  Unpacking and plain kernel -> straight from the pages
+// (us; 2 sequences, 32 heads, 1,021 queries on 1,024 to 7,168 keys): fp32
+// head_dim 64 403 -> 918, 128 5,524 -> 1,399, 256 29,044 -> 2,477; bf16 64
+// 205 -> 753, 128 305 -> 1,107, 256 26,457 -> 1,752.
+static bool takes_unpacked(int B, int H, int D, int max_pages, int block_size, int dtype, const PrefillPlan& inner) {
+  if (dtype == B2PA_DTYPE_F32) return D == 64 && inner.split_tc;
+  return prefill_uses_tensor_cores(D, block_size, dtype, (int64_t)B * max_pages * H * block_size);
 }
 
 Kv4PrefillPlan make_kv4_prefill_plan(int B, int H, int T, int D, int max_pages, int block_size, int dtype) {
   Kv4PrefillPlan pl = {};
-  if (takes_mma(D, dtype)) return pl;
+  const PrefillPlan inner = make_prefill_plan(B, H, T, D, max_pages, block_size, dtype);
+  if (!takes_unpacked(B, H, D, max_pages, block_size, dtype, inner)) return pl;
+  pl.unpack = 1;
+  pl.inner_bytes = inner.bytes;
+  if (dtype == B2PA_DTYPE_F32) {  // in the places of the fp32 pages' split copies
+    pl.off_k = inner.off_split_k;
+    pl.off_v = inner.off_split_v;
+    pl.off_table = inner.off_slots;
+    pl.off_flag = inner.off_flag;
+    pl.bytes = inner.bytes;
+    return pl;
+  }
   const size_t pool = up256((size_t)B * max_pages * H * block_size * D * dtype_size(dtype));
-  pl.off_k = 0;
   pl.off_v = pool;
   pl.off_table = 2 * pool;
-  pl.off_inner = up256(2 * pool + 4 * (size_t)B * max_pages);
-  pl.inner_bytes = make_prefill_plan(B, H, T, D, max_pages, block_size, dtype).bytes;
+  pl.off_flag = up256(2 * pool + 4 * (size_t)B * max_pages);
+  pl.off_inner = pl.off_flag + 256;
   pl.bytes = pl.off_inner + pl.inner_bytes;
   return pl;
 }
 
 template <typename T>
-static cudaError_t unpack_as(const AttnArgs& a, char* ws, const Kv4PrefillPlan& pl, cudaStream_t s) {
+static cudaError_t unpack_as(const AttnArgs& a, char* ws, const Kv4PrefillPlan& pl, uint32_t epoch, cudaStream_t s) {
   return launch_pdl(kv4_unpack_kernel<T>, dim3((unsigned)a.max_pages, (unsigned)a.B), dim3(256), 0, s, a,
                     reinterpret_cast<T*>(ws + pl.off_k), reinterpret_cast<T*>(ws + pl.off_v),
-                    reinterpret_cast<int32_t*>(ws + pl.off_table));
+                    reinterpret_cast<int32_t*>(ws + pl.off_table), reinterpret_cast<uint32_t*>(ws + pl.off_flag), epoch);
 }
 
 int launch_kv4_prefill(const AttnArgs& a, const Kv4PrefillPlan& pl, cudaStream_t s) {
-  if (takes_mma(a.D, a.dtype)) return launch_kv4_prefill_mma(a, s);
+  if (!pl.unpack) return launch_kv4_prefill_mma(a, nullptr, 0, s);
+  static std::atomic<uint32_t> calls{0};
+  const uint32_t epoch = calls.fetch_add(1, std::memory_order_relaxed) * 2654435761u + 0x9e3779b9u;
   char* ws = static_cast<char*>(a.workspace);
   AttnArgs in = a;
   if (a.max_pages > 0) {
-    cudaError_t e;
-    switch (a.dtype) {
-      case B2PA_DTYPE_F32: e = unpack_as<float>(a, ws, pl, s); break;
-      case B2PA_DTYPE_BF16: e = unpack_as<__nv_bfloat16>(a, ws, pl, s); break;
-      default: e = unpack_as<__half>(a, ws, pl, s); break;
-    }
+    const cudaError_t e = a.dtype == B2PA_DTYPE_BF16 ? unpack_as<__nv_bfloat16>(a, ws, pl, epoch, s)
+                                                     : unpack_as<__half>(a, ws, pl, epoch, s);
     if (e != cudaSuccess) return set_error(B2PA_ERR_CUDA, "paged_prefill_kv4 launch: %s", cudaGetErrorString(e));
   }
   in.k_pool = ws + pl.off_k;
@@ -103,11 +126,14 @@ int launch_kv4_prefill(const AttnArgs& a, const Kv4PrefillPlan& pl, cudaStream_t
   in.pt_stride = a.max_pages;
   in.workspace = ws + pl.off_inner;
   in.workspace_bytes = pl.inner_bytes;
+  int rc;
   switch (a.dtype) {
-    case B2PA_DTYPE_F32: return launch_paged_prefill_f32(in, s);
-    case B2PA_DTYPE_BF16: return launch_paged_prefill_bf16(in, s);
-    default: return launch_paged_prefill_f16(in, s);
+    case B2PA_DTYPE_F32: rc = launch_paged_prefill_f32_on_halves(in, epoch, s); break;
+    case B2PA_DTYPE_BF16: rc = launch_paged_prefill_bf16(in, s); break;
+    default: rc = launch_paged_prefill_f16(in, s); break;
   }
+  if (rc != B2PA_OK) return rc;
+  return launch_kv4_prefill_mma(a, reinterpret_cast<const uint32_t*>(ws + pl.off_flag), epoch, s);
 }
 
 }  // namespace b2pa

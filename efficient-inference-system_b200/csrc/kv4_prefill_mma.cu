@@ -1,6 +1,7 @@
 // kv4_prefill_mma.cu -- chunked prefill straight from 4-bit pages, for the
 // shapes that have no tcgen05 kernel to run on unpacked pages (head_dim 256,
-// and fp32 with head_dim 128): see kv4_prefill.cu for which call takes which.
+// and fp32 with head_dim 128), and for inputs that those kernels do not take:
+// see kv4_prefill.cu for which call takes which.
 //
 // One CTA takes 64 queries of a (head, sequence); each of its 4 warps 16 of
 // them with all channels.  Tiles of keys are unpacked to fp16 (exact) into
@@ -12,6 +13,9 @@
 // as one half (a rounding of 2^-12, below that of 16-bit outputs) or two.
 // A cluster of up to 8 CTAs shares the keys of few queries and joins the
 // partial results through distributed shared memory.
+// A NaN group of V at a key that only some of the tile's queries see must not
+// meet the others' zero weights: it is put in shared memory as zeros, and the
+// queries that see the first of a group's get their NaN at the end.
 // What bounds it: mma.sync, about 520 TFLOP/s on this device, and the shared
 // memory reads that feed it (half a 16-byte read per product).
 #include <cooperative_groups.h>
@@ -56,18 +60,22 @@ __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[VL]) 
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, 2) kv4_prefill_kernel(AttnArgs a, float qscale) {
+__global__ void __launch_bounds__(kThreads, 2)
+    kv4_prefill_kernel(AttnArgs a, float qscale, const uint32_t* flag, uint32_t epoch) {
   using P = Pf<T, D>;
   constexpr int KT = P::KT, NK = KT / 8, NC = D / 8;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float unit[kRows];
   __shared__ uint8_t key_ok[KT];
   __shared__ float2 row_ml[kRows];
+  __shared__ int any_nan;
+  __shared__ int nan_at[D / 16];  // first key, of those that not every query of the tile sees, with a NaN group
   uint8_t* const qs = smem;
   uint4* const kf = reinterpret_cast<uint4*>(smem + P::Q_BYTES);               // [key / 8][block][lane]
   uint4* const vf = reinterpret_cast<uint4*>(smem + P::Q_BYTES + P::T_BYTES);  // [key / 16][channel pair][lane]
   pdl_wait();
   pdl_launch_dependents();
+  if (flag != nullptr && *reinterpret_cast<const volatile uint32_t*>(flag) != epoch) return;  // nothing to redo
   cg::cluster_group cluster = cg::this_cluster();
   const int ns = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
@@ -88,6 +96,8 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_prefill_kernel(AttnArgs a, fl
       static_cast<const T*>(a.q) + (int64_t)b * a.sq[0] + (int64_t)h * a.sq[1] + (int64_t)i0 * a.sq[2], a.sq[2], a.T - i0,
       qs, unit);
 
+  if (tid < D / 16) nan_at[tid] = INT32_MAX;
+  if (tid == 0) any_nan = 0;
   float o[NC][4];  // rows g, g + 8; channels 2t * NC + n and (2t + 1) * NC + n
 #pragma unroll
   for (int n = 0; n < NC; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
@@ -141,6 +151,16 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_prefill_kernel(AttnArgs a, fl
           sc[k][0] = sc[k][1] = 0;
 #pragma unroll
           for (int u = 0; u < P::VL; ++u) v[k][u] = 0x88888888u;
+        }
+        if (j0 + KT > first_seen && j >= first_seen) {  // (the former is the same for the CTA)
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            if (sc[k][x] == kKv4NanScale) {
+              const int group = D == 256 ? 2 * g + (P::VL == 4 ? x : u0 >> 1) : D == 64 ? g >> 1 : g;
+              atomicMin(&nan_at[group], (int)j);
+              any_nan = 1;
+              sc[k][x] = 0;
+            }
         }
       }
       const __half2 k1032 = __half2half2(__ushort_as_half(0x6408)), k72 = __half2half2(__ushort_as_half(0xd480)),
@@ -263,6 +283,15 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_prefill_kernel(AttnArgs a, fl
     l[r] += __shfl_xor_sync(kFullMask, l[r], 1);
     l[r] += __shfl_xor_sync(kFullMask, l[r], 2);
   }
+  __syncthreads();
+  if (any_nan) {
+#pragma unroll
+    for (int n = 0; n < NC; ++n)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (nan_at[((2 * t + (k & 1)) * NC + n) / 16] < first_seen + warp * 16 + g + 8 * (k >> 1))
+          o[n][k] = __uint_as_float(0x7fffffffu);
+  }
   T* const out = static_cast<T*>(a.out) + (int64_t)b * a.so[0] + (int64_t)h * a.so[1] + (int64_t)i0 * a.so[2];
   constexpr int V = 16 / (int)sizeof(T);
   if (ns == 1) {
@@ -329,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_prefill_kernel(AttnArgs a, fl
 }
 
 template <typename T, int D>
-int prefill_as(const AttnArgs& a, cudaStream_t s) {
+int prefill_as(const AttnArgs& a, const uint32_t* flag, uint32_t epoch, cudaStream_t s) {
   using P = Pf<T, D>;
   const int64_t tiles = (int64_t)a.B * a.H * ((a.T + kRows - 1) / kRows);
   const int64_t keys = (int64_t)a.max_pages * a.block_size;
@@ -351,27 +380,27 @@ int prefill_as(const AttnArgs& a, cudaStream_t s) {
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a, a.scale * kLog2e);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a, a.scale * kLog2e, flag, epoch);
   if (e != cudaSuccess) return set_error(B2PA_ERR_CUDA, "paged_prefill_kv4 launch: %s", cudaGetErrorString(e));
   return B2PA_OK;
 }
 
 template <typename T>
-int prefill_dims(const AttnArgs& a, cudaStream_t s) {
+int prefill_dims(const AttnArgs& a, const uint32_t* flag, uint32_t epoch, cudaStream_t s) {
   switch (a.D) {
-    case 64: return prefill_as<T, 64>(a, s);
-    case 128: return prefill_as<T, 128>(a, s);
-    default: return prefill_as<T, 256>(a, s);
+    case 64: return prefill_as<T, 64>(a, flag, epoch, s);
+    case 128: return prefill_as<T, 128>(a, flag, epoch, s);
+    default: return prefill_as<T, 256>(a, flag, epoch, s);
   }
 }
 
 }  // namespace
 
-int launch_kv4_prefill_mma(const AttnArgs& a, cudaStream_t s) {
+int launch_kv4_prefill_mma(const AttnArgs& a, const uint32_t* flag, uint32_t epoch, cudaStream_t s) {
   switch (a.dtype) {
-    case B2PA_DTYPE_F32: return prefill_dims<float>(a, s);
-    case B2PA_DTYPE_BF16: return prefill_dims<__nv_bfloat16>(a, s);
-    default: return prefill_dims<__half>(a, s);
+    case B2PA_DTYPE_F32: return prefill_dims<float>(a, flag, epoch, s);
+    case B2PA_DTYPE_BF16: return prefill_dims<__nv_bfloat16>(a, flag, epoch, s);
+    default: return prefill_dims<__half>(a, flag, epoch, s);
   }
 }
 

@@ -44,4 +44,12 @@ int launch_paged_prefill_f32(const AttnArgs& a, cudaStream_t s) {
 #undef B2PA_PF32_CASE
   return dispatch_prefill<float>(a, s);
 }
+
+int launch_paged_prefill_f32_on_halves(const AttnArgs& a, uint32_t epoch, cudaStream_t s) {
+  switch (a.block_size) {
+    case 8: return launch_prefill_tc<float, 64, 8, true>(a, s, epoch);
+    case 16: return launch_prefill_tc<float, 64, 16, true>(a, s, epoch);
+    default: return launch_prefill_tc<float, 64, 32, true>(a, s, epoch);
+  }
+}
 }  // namespace b2pa

@@ -121,13 +121,16 @@ __device__ __forceinline__ void prefill_tile_range(const PfTcParams& p, int b, i
 // the general fp32 CUDA-core kernel, launched after this one as a backup that
 // does nothing otherwise.  The K/V pages are split into a workspace copy
 // beforehand (prefill_split_pages_kernel); q and P are split in the kernel.
-template <int D, int BS, bool SPLIT = false>
+// HALVES: fp32 q on K/V pages whose values fp16 holds exactly (they are fp16
+// in memory): their lo tiles, and the products with them, drop out.
+template <int D, int BS, bool SPLIT = false, bool HALVES = false>
 struct PfTcCfg {
   static constexpr int BM = 128;         // query rows per CTA (UMMA M)
   static constexpr int BN = 64;          // keys per tile
   static constexpr int KB = D / 64;      // 128-byte column blocks of a row
   static constexpr int PAGES = BN / BS;  // pages per key tile
   static constexpr int NOP = SPLIT ? 2 : 1;  // bf16 tiles per operand tile (hi, lo)
+  static constexpr int NOP_KV = HALVES ? 1 : NOP;  // ... of K and V
   // Softmax warpgroups.  With two, key tiles alternate between them (tile j
   // -> group j % NG) and each keeps its own running max, denominator and O
   // accumulator; the groups are merged in the epilogue.  Two groups put two
@@ -141,12 +144,12 @@ struct PfTcCfg {
   // Depth of the K ring and of the V ring.  A K stage is refilled once the
   // Q.K^T that read it is done, a V stage once its P.V is done, so each ring
   // loads up to STAGES tiles ahead of its consumer.
-  static constexpr int STAGES = SPLIT ? 3 : (D == 64 ? 6 : 4);
+  static constexpr int STAGES = SPLIT && !HALVES ? 3 : (D == 64 ? 6 : 4);
   static constexpr int Q_TILE = BM * D * 2;   // one bf16 / fp16 tile
   static constexpr int KV_TILE = BN * D * 2;
   static constexpr int P_TILE = BM * BN * 2;
   static constexpr int Q_BYTES = NOP * Q_TILE;  // hi tile, then lo tile
-  static constexpr int KV_BYTES = NOP * KV_TILE;
+  static constexpr int KV_BYTES = NOP_KV * KV_TILE;
   static constexpr int P_BYTES = NOP * P_TILE;
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_K = OFF_Q + Q_BYTES;
@@ -243,12 +246,12 @@ __device__ __forceinline__ void split_f16x8(const float (&f)[8], uint4& hi, uint
   lo = make_uint4(l[0], l[1], l[2], l[3]);
 }
 
-template <typename T, int D, int BS>
-__global__ void __launch_bounds__(PfTcCfg<D, BS, kPfSplit<T>>::THREADS, 1)
+template <typename T, int D, int BS, bool HALVES = false>
+__global__ void __launch_bounds__(PfTcCfg<D, BS, kPfSplit<T>, HALVES>::THREADS, 1)
     paged_prefill_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                             const __grid_constant__ CUtensorMap tm_q, PfTcParams p) {
   constexpr bool SPLIT = kPfSplit<T>;
-  using C = PfTcCfg<D, BS, SPLIT>;
+  using C = PfTcCfg<D, BS, SPLIT, HALVES>;
   constexpr int NG = C::NG, NSLOT = C::NSLOT;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem =
@@ -435,12 +438,12 @@ __global__ void __launch_bounds__(PfTcCfg<D, BS, kPfSplit<T>>::THREADS, 1)
       for (int pg = 0; pg < C::PAGES; ++pg) {
         const int blk = __shfl_sync(kFullMask, blk_lane, (lp + pg) & 31);
         if (blk >= 0) {
-          bytes += (uint32_t)(C::NOP * BS * D * 2);
+          bytes += (uint32_t)(C::NOP_KV * BS * D * 2);
         } else {
           // Pages that are not loaded must not hold stale or uninitialised
           // bytes: their softmax weight is 0, but 0 * NaN is NaN in P.V.
 #pragma unroll
-          for (int op = 0; op < C::NOP; ++op)
+          for (int op = 0; op < C::NOP_KV; ++op)
 #pragma unroll
             for (int kb = 0; kb < C::KB; ++kb) {
               const int off = st * C::KV_BYTES + op * C::KV_TILE + kb * (C::BN * 128) + pg * (BS * 128);
@@ -459,7 +462,7 @@ __global__ void __launch_bounds__(PfTcCfg<D, BS, kPfSplit<T>>::THREADS, 1)
         // split variant: the workspace rows hold hi in columns [0, D) and
         // lo in [D, 2D)
 #pragma unroll
-        for (int op = 0; op < C::NOP; ++op)
+        for (int op = 0; op < C::NOP_KV; ++op)
 #pragma unroll
           for (int kb = 0; kb < C::KB; ++kb) {
             const int off = st * C::KV_BYTES + op * C::KV_TILE + kb * (C::BN * 128) + pg * (BS * 128);
@@ -514,7 +517,8 @@ __global__ void __launch_bounds__(PfTcCfg<D, BS, kPfSplit<T>>::THREADS, 1)
           const uint64_t bd = dKs + (uint64_t)((kb * (C::BN * 128) + kk * 32) >> 4);
           tc::mma_f16_ss(tS, a, bd, idesc_s, k > 0);
           if constexpr (SPLIT) {
-            tc::mma_f16_ss(tS, a, bd + (uint64_t)(C::KV_TILE >> 4), idesc_s, true);  // q_hi . k_lo
+            if constexpr (!HALVES)
+              tc::mma_f16_ss(tS, a, bd + (uint64_t)(C::KV_TILE >> 4), idesc_s, true);  // q_hi . k_lo
             tc::mma_f16_ss(tS, a + (uint64_t)(C::Q_TILE >> 4), bd, idesc_s, true);   // q_lo . k_hi
           }
         }
@@ -538,8 +542,9 @@ __global__ void __launch_bounds__(PfTcCfg<D, BS, kPfSplit<T>>::THREADS, 1)
         for (int k = 0; k < C::BN / 16; ++k) {
           tc::mma_f16_ss(tO, dPs + (uint64_t)(k * 2), dVs + (uint64_t)(k * 128), idesc_o, j >= NG || k > 0);
           if constexpr (SPLIT) {
-            tc::mma_f16_ss(tO, dPs + (uint64_t)(k * 2), dVs + (uint64_t)((C::KV_TILE >> 4) + k * 128), idesc_o,
-                           true);  // p_hi . v_lo
+            if constexpr (!HALVES)
+              tc::mma_f16_ss(tO, dPs + (uint64_t)(k * 2), dVs + (uint64_t)((C::KV_TILE >> 4) + k * 128), idesc_o,
+                             true);  // p_hi . v_lo
             tc::mma_f16_ss(tO, dPs + (uint64_t)((C::P_TILE >> 4) + k * 2), dVs + (uint64_t)(k * 128), idesc_o,
                            true);  // p_lo . v_hi
           }
@@ -976,10 +981,11 @@ bool encode_q_tensor_map(CUtensorMap* map, const void* q, int B, int H, int T, i
                          int dim_of[3]);
 
 // epoch: the fp32 variant's number of this call (marks the range flag).
-template <typename T, int D, int BS>
+// HALVES: a's pools are fp16, the table and the flag in place.
+template <typename T, int D, int BS, bool HALVES = false>
 int launch_prefill_tc(const AttnArgs& a, cudaStream_t stream, uint32_t epoch = 0) {
   constexpr bool SPLIT = kPfSplit<T>;
-  using C = PfTcCfg<D, BS, SPLIT>;
+  using C = PfTcCfg<D, BS, SPLIT, HALVES>;
   const PrefillPlan plan = make_prefill_plan(a.B, a.H, a.T, a.D, a.max_pages, BS, a.dtype);
   if (plan.bytes > 0 && (!a.workspace || a.workspace_bytes < plan.bytes))
     return set_error(B2PA_ERR_WORKSPACE, "paged_prefill: workspace of %zu bytes, %zu needed", a.workspace_bytes,
@@ -989,7 +995,14 @@ int launch_prefill_tc(const AttnArgs& a, cudaStream_t stream, uint32_t epoch = 0
   const int32_t* table = a.page_table;
   int64_t pt_stride = a.pt_stride;
   int64_t num_blocks = a.num_blocks;
-  if constexpr (SPLIT) {
+  if constexpr (HALVES) {
+    if (!plan.split_tc) return set_error(B2PA_ERR_UNSUPPORTED, "paged_prefill: fp32 split plan not applicable");
+    range_flag = reinterpret_cast<uint32_t*>(static_cast<char*>(a.workspace) + plan.off_flag);
+    const int64_t rows = a.num_blocks * a.H * BS;
+    if (!encode_pool_tensor_map(&tmk, a.k_pool, rows, D, BS, B2PA_DTYPE_F16) ||
+        !encode_pool_tensor_map(&tmv, a.v_pool, rows, D, BS, B2PA_DTYPE_F16))
+      return set_error(B2PA_ERR_CUDA, "paged_prefill: cuTensorMapEncodeTiled failed for the fp16 pages");
+  } else if constexpr (SPLIT) {
     if (!plan.split_tc) return set_error(B2PA_ERR_UNSUPPORTED, "paged_prefill: fp32 split plan not applicable");
     char* ws = static_cast<char*>(a.workspace);
     PfSplitArgs sa;
@@ -1072,7 +1085,7 @@ int launch_prefill_tc(const AttnArgs& a, cudaStream_t stream, uint32_t epoch = 0
   const size_t smem = C::SMEM_FIXED + 4 * (size_t)p.max_cta_pages;
   if (smem > (size_t)device_max_smem_optin())
     return set_error(B2PA_ERR_UNSUPPORTED, "paged_prefill: %d pages per CTA exceed shared memory", p.max_cta_pages);
-  auto kern = paged_prefill_tc_kernel<T, D, BS>;
+  auto kern = paged_prefill_tc_kernel<T, D, BS, HALVES>;
   int rc_attr = set_max_dynamic_smem_cached(reinterpret_cast<const void*>(kern), (int)smem);
   if (rc_attr != B2PA_OK) return rc_attr;
   cudaError_t e;

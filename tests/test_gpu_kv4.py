@@ -333,6 +333,67 @@ def test_nan_reaches_only_its_own(cuda_device):
         assert bad[1, 1].all() and not bad[1, 0].any() and not bad[1, 2].any()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,bs", [(64, 16), (128, 16), (128, 8), (256, 32)])
+def test_nan_behind_the_mask(cuda_device, dtype, D, bs):
+    """Within a chunk: NaN groups of V at the last position and of K at the one before reach only the queries that see
+    them; a padded query that is NaN reaches nothing."""
+    rng = np.random.default_rng(16)
+    H, n, T = 2, 150, 70
+    NB = -(-n // bs)
+    clean_k, clean_v = rng.standard_normal((NB, H, bs, D)), rng.standard_normal((NB, H, bs, D))
+    k, v = clean_k.copy(), clean_v.copy()
+    at = lambda j: (j // bs, 0, j % bs)  # noqa: E731
+    v[at(n - 1)][5] = np.nan
+    k[at(n - 2)][20] = np.inf
+    q = torch.from_numpy(rng.standard_normal((1, H, T + 3, D))).to(dtype).to(cuda_device)
+    q[:, :, T:] = float("nan")
+    table, lens, cur = _i32(np.arange(NB)[None], cuda_device), _i32([n], cuda_device), _i32([T], cuda_device)
+    pools = [[torch.from_numpy(co.pack_pages(x, y)).to(cuda_device) for x, y in ((a, False), (b, True))]
+             for a, b in ((clean_k, clean_v), (k, v))]
+    p, size = co.softmax_rows(_np(q)[0, :, :T], co.rows_of(co.stored(clean_k), range(NB), n), T, D ** -0.5)
+    V = co.rows_of(co.stored(clean_v), range(NB), n)
+    ref = np.einsum("htn,nhd->htd", p, V)
+    # (the unpacked pages' 16-bit kernels round the weights to the operand type, as in test_prefill)
+    bound = co.output_bound(ref, HALF_STEP[dtype], D, size, n, np.abs(V).max()) \
+        + (0 if dtype == torch.float32 else HALF_STEP[dtype] * np.abs(ref).max())
+    for kp, vp, lost in ((0, 0, ()), (1, 1, ((T - 2, slice(None)), (T - 1, slice(None)))), (0, 1, ((T - 1, slice(0, 16)),)),
+                         (1, 0, ((T - 2, slice(None)), (T - 1, slice(None))))):
+        out = _np(b2pa.paged_attention_prefill_kv4(q, pools[kp][0], pools[vp][1], table, lens, cur))[0, :, :T]
+        want = np.zeros(ref.shape, bool)
+        for t, ch in lost:
+            want[0, t, ch] = True
+        assert np.array_equal(np.isnan(out), want), (kp, vp)
+        assert (np.abs(out - ref) <= bound)[~want].all(), (kp, vp)
+    w = torch.zeros(NB, H, bs, device=cuda_device)
+    got = b2pa.accumulate_key_weights(q, pools[0][0], w, table, lens, cur, out=torch.zeros_like(w))
+    assert got.sum().item() == pytest.approx(H * T, rel=1e-5)
+    bad = b2pa.accumulate_key_weights(q, pools[1][0], w, table, lens, cur, out=torch.zeros_like(w))
+    assert torch.equal(bad[:, 1], got[:, 1]) and torch.isnan(bad[:, 0].flatten()[:n]).all()
+
+
+def test_far_queries(cuda_device):
+    """fp32 queries past 2^15, and a row of them that is not finite, on keys small enough for usual logits."""
+    rng = np.random.default_rng(26)
+    for D in (64, 128):
+        H, bs, n, T = 2, 16, 90, 33
+        NB = -(-n // bs)
+        k, v = rng.standard_normal((NB, H, bs, D)) * 2.0 ** -14, rng.standard_normal((NB, H, bs, D))
+        q = rng.standard_normal((1, H, T, D)) * 2.0 ** 15
+        qt = torch.from_numpy(q).float().to(cuda_device)
+        qt[0, 1, 4, 7] = float("inf")
+        out = b2pa.paged_attention_prefill_kv4(
+            qt, *(torch.from_numpy(co.pack_pages(x, y)).to(cuda_device) for x, y in ((k, False), (v, True))),
+            _i32(np.arange(NB)[None], cuda_device), _i32([n], cuda_device), _i32([T], cuda_device))
+        p, size = co.softmax_rows(_np(torch.from_numpy(q).float())[0], co.rows_of(co.stored(k), range(NB), n), T, D ** -0.5)
+        V = co.rows_of(co.stored(v), range(NB), n)
+        ref = np.einsum("htn,nhd->htd", p, V)
+        bound = co.output_bound(ref, 2.0 ** -24, D, size, n, np.abs(V).max())
+        ok = np.ones((H, T), bool)
+        ok[1, 4] = False
+        assert (np.abs(_np(out)[0] - ref) <= bound)[ok].all() and np.isnan(_np(out)[0][~ok]).all()
+
+
 def test_bad_pages(cuda_device):
     """Unset pages are not seen; ids past the pool are not read and are reported."""
     NB = 5 + 4
