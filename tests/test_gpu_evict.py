@@ -318,6 +318,43 @@ def test_evict_refusals(cuda_device):
         b2pa.accumulate_key_weights(torch.zeros(1, 2, 1, 64, device=dev), kp, w, t, n, n, window=0)
 
 
+@pytest.mark.parametrize("kv4", [False, True], ids=["plain", "kv4"])
+def test_offsets_past_32_bits(cuda_device, kv4):
+    """Every call on pages at the far end of pools of more than 2^32 bytes (plain: 2^31 elements) gives what it gives
+    on small pools."""
+    dev, H, D, bs = cuda_device, 8, 128, 32
+    cols, dtype = (72, torch.uint8) if kv4 else (D, torch.float16)
+    block = H * bs * cols * (1 if kv4 else 2)
+    NB, n = (1 << 32) // block + 40, 20
+    gen = torch.Generator().manual_seed(1)
+    small = [torch.randint(0, 200, (n, H, bs, cols), generator=gen, dtype=torch.uint8).to(dev) if kv4 else
+             torch.randn(n, H, bs, cols, generator=gen).to(dtype).to(dev) for _ in range(2)]
+    w_small = torch.rand(n, H, bs, generator=gen).to(dev)
+    big = [torch.empty(NB, H, bs, cols, dtype=dtype, device=dev) for _ in range(2)]
+    w_big = torch.empty(NB, H, bs, device=dev)
+    for a, b in zip(big + [w_big], small + [w_small]):
+        a[NB - n:] = b
+    ids = torch.randperm(n, generator=gen).to(torch.int32).to(dev).view(2, n // 2)
+    lens, T = _i32([300, 211], dev), 40
+    q = torch.randn(2, H, T, D, generator=gen).to(torch.float16).to(dev)
+    rows = torch.randn(2, H, T, D, generator=gen).to(torch.float16).to(dev)
+    got = []
+    for (kp, vp), w, table in ((small, w_small, ids), (big, w_big, ids + (NB - n))):
+        res = []
+        if kv4:
+            b2pa.kv4_append(rows, -rows, kp, vp, table, lens - T, _i32([T, 7], dev))
+            res += b2pa.kv4_read(kp, vp, table, lens - T, _i32([T, T], dev), T, torch.float32)
+            res.append(b2pa.paged_attention_prefill_kv4(q, kp, vp, table, lens, _i32([T, T], dev)))
+            res.append(b2pa.paged_attention_decode_kv4(q[:, :, :1], kp, vp, table, lens, _i32([1, 1], dev)))
+        for x in (q, q[:, :, :1]):
+            b2pa.accumulate_key_weights(x, kp, w, table, lens, _i32([x.shape[2]] * 2, dev))
+        res.append(b2pa.evict_by_weight(kp, vp, w, table, lens, 100, 10))
+        got.append(res + [t[-n:] for t in (kp, vp, w)])
+    for a, b in zip(*got):
+        assert torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8))
+    assert b2pa.read_status(dev) == 0
+
+
 def test_counts_past_32_bits(cuda_device):
     """``recent`` and ``window`` of any size mean all of them; a batch cut to any number keeps what it has."""
     dev = cuda_device
