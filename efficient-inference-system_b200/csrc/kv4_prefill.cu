@@ -71,8 +71,8 @@ static size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 // Whether a tcgen05 kernel of the plain pools takes the shape; their others run
 // on the CUDA cores.  Unpacking and plain kernel -> straight from the pages
 // (us; 2 sequences, 32 heads, 1,021 queries on 1,024 to 7,168 keys): fp32
-// head_dim 64 403 -> 918, 128 5,524 -> 1,399, 256 29,044 -> 2,477; bf16 64
-// 205 -> 753, 128 305 -> 1,107, 256 26,457 -> 1,752.
+// head_dim 64 271 -> 918, 128 5,524 -> 1,406, 256 29,044 -> 2,507; bf16 64
+// 205 -> 753, 128 305 -> 1,107, 256 26,457 -> 1,745.
 static bool takes_unpacked(int B, int H, int D, int max_pages, int block_size, int dtype, const PrefillPlan& inner) {
   if (dtype == B2PA_DTYPE_F32) return D == 64 && inner.split_tc;
   return prefill_uses_tensor_cores(D, block_size, dtype, (int64_t)B * max_pages * H * block_size);

@@ -152,16 +152,20 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
           for (int u = 0; u < P::VL; ++u) v[k][u] = 0x88888888u;
         }
-        if (j0 + KT > first_seen && j >= first_seen) {  // (the former is the same for the CTA)
+      }
+      if (j0 + KT > first_seen) {  // (all loads are under way by now)
 #pragma unroll
-          for (int x = 0; x < 2; ++x)
-            if (sc[k][x] == kKv4NanScale) {
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int64_t j = j0 + ks * 16 + (k & 1) + 2 * t + (k >> 1) * 8;
+            if (sc[k][x] == kKv4NanScale && j >= first_seen) {
               const int group = D == 256 ? 2 * g + (P::VL == 4 ? x : u0 >> 1) : D == 64 ? g >> 1 : g;
               atomicMin(&nan_at[group], (int)j);
               any_nan = 1;
               sc[k][x] = 0;
             }
-        }
+          }
       }
       const __half2 k1032 = __half2half2(__ushort_as_half(0x6408)), k72 = __half2half2(__ushort_as_half(0xd480)),
                     k16th = __half2half2(__ushort_as_half(0x2c00));
