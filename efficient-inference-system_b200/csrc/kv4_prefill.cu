@@ -1,13 +1,13 @@
 // kv4_prefill.cu -- chunked prefill over a 4-bit cache (format: kv4.cuh).
 //
 // A prompt chunk of T queries makes 4 T L D operations of every L keys, so
-// its time is the tensor cores' and not the cache's.  Where a tcgen05 kernel
-// of the plain pools can do the rest (fp32 with head_dim 64, 16-bit types with
-// 64 and 128; else kv4_prefill_mma.cu does it all), the pages the call reads
-// are written out in the workspace, in q's type or, for fp32, in fp16 (exact
-// either way: a stored value has 7 significant bits), as a pool of
-// B * max_pages blocks with a table of their own, and that kernel runs on it;
-// rows past a sequence's length are written as zeros.
+// its time is the tensor cores' and not the cache's.  Where the tcgen05 kernel
+// of the plain pools can do the rest (head_dim 64 and 128; else
+// kv4_prefill_mma.cu does it all), the pages that the call reads are written out in the workspace, in q's type or, for fp32, in fp16 (exact
+// either way: a stored value has 7 significant bits, so fp32 q needs two
+// products where fp32 pages need three), as a pool of B * max_pages blocks with
+// a table of their own, and that kernel runs on it; rows past a sequence's
+// length are written as zeros.
 // Two kinds of inputs are not for that kernel: fp32 queries of 2^15 and more,
 // which it splits into fp16 halves as they are, and NaN groups of V at keys
 // that only some of the chunk's queries see (a zero weight times NaN).  They
@@ -68,31 +68,21 @@ __global__ void __launch_bounds__(256) kv4_unpack_kernel(AttnArgs a, T* k_out, T
 
 static size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
-// Whether a tcgen05 kernel of the plain pools takes the shape; their others run
-// on the CUDA cores.  Unpacking and plain kernel -> straight from the pages
-// (us; 2 sequences, 32 heads, 1,021 queries on 1,024 to 7,168 keys): fp32
-// head_dim 64 271 -> 918, 128 5,524 -> 1,406, 256 29,044 -> 2,507; bf16 64
-// 205 -> 753, 128 305 -> 1,107, 256 26,457 -> 1,745.
-static bool takes_unpacked(int B, int H, int D, int max_pages, int block_size, int dtype, const PrefillPlan& inner) {
-  if (dtype == B2PA_DTYPE_F32) return D == 64 && inner.split_tc;
-  return prefill_uses_tensor_cores(D, block_size, dtype, (int64_t)B * max_pages * H * block_size);
+// Whether the tcgen05 kernel takes the shape.  Unpacking and that kernel -> straight
+// from the pages (us; 2 sequences, 32 heads, 1,021 queries on 1,024 to 7,168
+// keys): fp32 head_dim 64 271 -> 918, 128 417 -> 1,406; bf16 64 205 -> 753, 128
+// 305 -> 1,107; head_dim 256 only straight, 2,507 and 1,745.
+static bool takes_unpacked(int B, int H, int D, int max_pages, int block_size, int type) {
+  return max_pages > 0 && prefill_uses_tensor_cores(D, block_size, type, (int64_t)B * max_pages * H * block_size);
 }
 
 Kv4PrefillPlan make_kv4_prefill_plan(int B, int H, int T, int D, int max_pages, int block_size, int dtype) {
   Kv4PrefillPlan pl = {};
-  const PrefillPlan inner = make_prefill_plan(B, H, T, D, max_pages, block_size, dtype);
-  if (!takes_unpacked(B, H, D, max_pages, block_size, dtype, inner)) return pl;
+  const int type = dtype == B2PA_DTYPE_F32 ? (int)B2PA_DTYPE_F16 : dtype;  // of the unpacked pages
+  if (!takes_unpacked(B, H, D, max_pages, block_size, type)) return pl;
   pl.unpack = 1;
-  pl.inner_bytes = inner.bytes;
-  if (dtype == B2PA_DTYPE_F32) {  // in the places of the fp32 pages' split copies
-    pl.off_k = inner.off_split_k;
-    pl.off_v = inner.off_split_v;
-    pl.off_table = inner.off_slots;
-    pl.off_flag = inner.off_flag;
-    pl.bytes = inner.bytes;
-    return pl;
-  }
-  const size_t pool = up256((size_t)B * max_pages * H * block_size * D * dtype_size(dtype));
+  pl.inner_bytes = make_prefill_plan(B, H, T, D, max_pages, block_size, type).bytes;
+  const size_t pool = up256((size_t)B * max_pages * H * block_size * D * 2);
   pl.off_v = pool;
   pl.off_table = 2 * pool;
   pl.off_flag = up256(2 * pool + 4 * (size_t)B * max_pages);
@@ -113,12 +103,11 @@ int launch_kv4_prefill(const AttnArgs& a, const Kv4PrefillPlan& pl, cudaStream_t
   static std::atomic<uint32_t> calls{0};
   const uint32_t epoch = calls.fetch_add(1, std::memory_order_relaxed) * 2654435761u + 0x9e3779b9u;
   char* ws = static_cast<char*>(a.workspace);
+  uint32_t* flag = reinterpret_cast<uint32_t*>(ws + pl.off_flag);
   AttnArgs in = a;
-  if (a.max_pages > 0) {
-    const cudaError_t e = a.dtype == B2PA_DTYPE_BF16 ? unpack_as<__nv_bfloat16>(a, ws, pl, epoch, s)
-                                                     : unpack_as<__half>(a, ws, pl, epoch, s);
-    if (e != cudaSuccess) return set_error(B2PA_ERR_CUDA, "paged_prefill_kv4 launch: %s", cudaGetErrorString(e));
-  }
+  const cudaError_t e = a.dtype == B2PA_DTYPE_BF16 ? unpack_as<__nv_bfloat16>(a, ws, pl, epoch, s)
+                                                   : unpack_as<__half>(a, ws, pl, epoch, s);
+  if (e != cudaSuccess) return set_error(B2PA_ERR_CUDA, "paged_prefill_kv4 launch: %s", cudaGetErrorString(e));
   in.k_pool = ws + pl.off_k;
   in.v_pool = ws + pl.off_v;
   in.num_blocks = (int64_t)a.B * a.max_pages;
@@ -128,12 +117,12 @@ int launch_kv4_prefill(const AttnArgs& a, const Kv4PrefillPlan& pl, cudaStream_t
   in.workspace_bytes = pl.inner_bytes;
   int rc;
   switch (a.dtype) {
-    case B2PA_DTYPE_F32: rc = launch_paged_prefill_f32_on_halves(in, epoch, s); break;
+    case B2PA_DTYPE_F32: rc = launch_paged_prefill_f32_on_halves(in, flag, epoch, s); break;
     case B2PA_DTYPE_BF16: rc = launch_paged_prefill_bf16(in, s); break;
     default: rc = launch_paged_prefill_f16(in, s); break;
   }
   if (rc != B2PA_OK) return rc;
-  return launch_kv4_prefill_mma(a, reinterpret_cast<const uint32_t*>(ws + pl.off_flag), epoch, s);
+  return launch_kv4_prefill_mma(a, flag, epoch, s);
 }
 
 }  // namespace b2pa

@@ -1,7 +1,6 @@
-// kv4_prefill_mma.cu -- chunked prefill straight from 4-bit pages, for the
-// shapes that have no tcgen05 kernel to run on unpacked pages (head_dim 256,
-// and fp32 with head_dim 128), and for inputs that those kernels do not take:
-// see kv4_prefill.cu for which call takes which.
+// kv4_prefill_mma.cu -- chunked prefill straight from 4-bit pages, for shapes
+// that have no tcgen05 kernel to run on unpacked pages (head_dim 256) and for
+// inputs that it does not take: see kv4_prefill.cu for which call takes which.
 //
 // One CTA takes 64 queries of a (head, sequence); each of its 4 warps 16 of
 // them with all channels.  Tiles of keys are unpacked to fp16 (exact) into

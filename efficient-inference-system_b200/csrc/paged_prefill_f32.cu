@@ -45,11 +45,16 @@ int launch_paged_prefill_f32(const AttnArgs& a, cudaStream_t s) {
   return dispatch_prefill<float>(a, s);
 }
 
-int launch_paged_prefill_f32_on_halves(const AttnArgs& a, uint32_t epoch, cudaStream_t s) {
+template <int D>
+static int on_halves(const AttnArgs& a, uint32_t* flag, uint32_t epoch, cudaStream_t s) {
   switch (a.block_size) {
-    case 8: return launch_prefill_tc<float, 64, 8, true>(a, s, epoch);
-    case 16: return launch_prefill_tc<float, 64, 16, true>(a, s, epoch);
-    default: return launch_prefill_tc<float, 64, 32, true>(a, s, epoch);
+    case 8: return launch_prefill_tc<float, D, 8, true>(a, s, epoch, flag);
+    case 16: return launch_prefill_tc<float, D, 16, true>(a, s, epoch, flag);
+    default: return launch_prefill_tc<float, D, 32, true>(a, s, epoch, flag);
   }
+}
+
+int launch_paged_prefill_f32_on_halves(const AttnArgs& a, uint32_t* flag, uint32_t epoch, cudaStream_t s) {
+  return a.D == 64 ? on_halves<64>(a, flag, epoch, s) : on_halves<128>(a, flag, epoch, s);
 }
 }  // namespace b2pa

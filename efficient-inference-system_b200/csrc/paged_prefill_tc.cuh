@@ -140,11 +140,11 @@ struct PfTcCfg {
   // S/P buffers: two per group; one per group for the fp32 variant, whose
   // hi/lo operand tiles take twice the shared memory (its two groups still
   // alternate, so one group's softmax overlaps the other's Q.K^T).
-  static constexpr int NSLOT = SPLIT ? NG : 2 * NG;
+  static constexpr int NSLOT = SPLIT && D == 64 ? NG : 2 * NG;
   // Depth of the K ring and of the V ring.  A K stage is refilled once the
   // Q.K^T that read it is done, a V stage once its P.V is done, so each ring
   // loads up to STAGES tiles ahead of its consumer.
-  static constexpr int STAGES = SPLIT && !HALVES ? 3 : (D == 64 ? 6 : 4);
+  static constexpr int STAGES = SPLIT && !HALVES ? 3 : (D == 64 ? 6 : SPLIT ? 2 : 4);
   static constexpr int Q_TILE = BM * D * 2;   // one bf16 / fp16 tile
   static constexpr int KV_TILE = BN * D * 2;
   static constexpr int P_TILE = BM * BN * 2;
@@ -173,7 +173,7 @@ struct PfTcCfg {
   static constexpr int PV_WARP = 4 * NG + 3;  // issues O += P.V
   static constexpr int THREADS = SOFTMAX_THREADS + 128;
   static_assert(D == 64 || D == 128, "tcgen05 prefill is built for head_dim 64 and 128");
-  static_assert(!SPLIT || D == 64, "the fp32 variant fits shared memory for head_dim 64 only");
+  static_assert(!SPLIT || D == 64 || HALVES, "fp32 pages fit shared memory for head_dim 64 only");
   static_assert(BN % BS == 0 && 32 % PAGES == 0, "block size must divide the key tile");
   static_assert(TMEM_USED <= 512, "TMEM holds 512 columns");
   static_assert(SMEM_FIXED <= 200 * 1024, "shared-memory plan");
@@ -510,15 +510,22 @@ __global__ void __launch_bounds__(PfTcCfg<D, BS, kPfSplit<T>, HALVES>::THREADS, 
         tc::fence_after_sync();
         const uint32_t tS = tmem + (uint32_t)slot * C::BN;
         const uint64_t dKs = dK + (uint64_t)((st * C::KV_BYTES) >> 4);
+        if constexpr (HALVES) {  // q_lo . k, the smaller sums, first: fewer roundings of the larger
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const int kb = k >> 2, kk = k & 3;
+            tc::mma_f16_ss(tS, dQ + (uint64_t)((C::Q_TILE + kb * (C::BM * 128) + kk * 32) >> 4),
+                           dKs + (uint64_t)((kb * (C::BN * 128) + kk * 32) >> 4), idesc_s, k > 0);
+          }
+        }
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           const int kb = k >> 2, kk = k & 3;
           const uint64_t a = dQ + (uint64_t)((kb * (C::BM * 128) + kk * 32) >> 4);
           const uint64_t bd = dKs + (uint64_t)((kb * (C::BN * 128) + kk * 32) >> 4);
-          tc::mma_f16_ss(tS, a, bd, idesc_s, k > 0);
-          if constexpr (SPLIT) {
-            if constexpr (!HALVES)
-              tc::mma_f16_ss(tS, a, bd + (uint64_t)(C::KV_TILE >> 4), idesc_s, true);  // q_hi . k_lo
+          tc::mma_f16_ss(tS, a, bd, idesc_s, HALVES || k > 0);
+          if constexpr (SPLIT && !HALVES) {
+            tc::mma_f16_ss(tS, a, bd + (uint64_t)(C::KV_TILE >> 4), idesc_s, true);  // q_hi . k_lo
             tc::mma_f16_ss(tS, a + (uint64_t)(C::Q_TILE >> 4), bd, idesc_s, true);   // q_lo . k_hi
           }
         }
@@ -981,12 +988,14 @@ bool encode_q_tensor_map(CUtensorMap* map, const void* q, int B, int H, int T, i
                          int dim_of[3]);
 
 // epoch: the fp32 variant's number of this call (marks the range flag).
-// HALVES: a's pools are fp16, the table and the flag in place.
+// HALVES: a's pools are fp16, with the 16-bit types' plan, and the flag is the
+// caller's.
 template <typename T, int D, int BS, bool HALVES = false>
-int launch_prefill_tc(const AttnArgs& a, cudaStream_t stream, uint32_t epoch = 0) {
+int launch_prefill_tc(const AttnArgs& a, cudaStream_t stream, uint32_t epoch = 0, uint32_t* flag = nullptr) {
   constexpr bool SPLIT = kPfSplit<T>;
   using C = PfTcCfg<D, BS, SPLIT, HALVES>;
-  const PrefillPlan plan = make_prefill_plan(a.B, a.H, a.T, a.D, a.max_pages, BS, a.dtype);
+  const PrefillPlan plan =
+      make_prefill_plan(a.B, a.H, a.T, a.D, a.max_pages, BS, HALVES ? (int)B2PA_DTYPE_F16 : a.dtype);
   if (plan.bytes > 0 && (!a.workspace || a.workspace_bytes < plan.bytes))
     return set_error(B2PA_ERR_WORKSPACE, "paged_prefill: workspace of %zu bytes, %zu needed", a.workspace_bytes,
                      plan.bytes);
@@ -996,8 +1005,7 @@ int launch_prefill_tc(const AttnArgs& a, cudaStream_t stream, uint32_t epoch = 0
   int64_t pt_stride = a.pt_stride;
   int64_t num_blocks = a.num_blocks;
   if constexpr (HALVES) {
-    if (!plan.split_tc) return set_error(B2PA_ERR_UNSUPPORTED, "paged_prefill: fp32 split plan not applicable");
-    range_flag = reinterpret_cast<uint32_t*>(static_cast<char*>(a.workspace) + plan.off_flag);
+    range_flag = flag;
     const int64_t rows = a.num_blocks * a.H * BS;
     if (!encode_pool_tensor_map(&tmk, a.k_pool, rows, D, BS, B2PA_DTYPE_F16) ||
         !encode_pool_tensor_map(&tmv, a.v_pool, rows, D, BS, B2PA_DTYPE_F16))

@@ -403,10 +403,10 @@ B2PA_API int b2pa_paged_decode_kv4(const void* q, const int64_t q_strides[4],
 
 /*
  * Chunked-prefill paged attention over a 4-bit cache (any T >= 1):
- * b2pa_paged_prefill with 4-bit pools.  fp32 with head_dim 64 and 16-bit types
- * with 64 or 128: the workspace holds the pages of the call unpacked, 2 * B *
- * max_pages * H * block_size * D elements of q's type, and what
- * b2pa_paged_prefill needs.  The other shapes need none.
+ * b2pa_paged_prefill with 4-bit pools.  head_dim 64 and 128: the workspace
+ * holds the pages of the call unpacked, 2 * B * max_pages * H * block_size * D
+ * values of 16 bits, and what b2pa_paged_prefill needs for 16-bit types.
+ * head_dim 256 needs none.
  */
 B2PA_API size_t b2pa_paged_prefill_kv4_workspace_size(int B, int H, int T, int D, int max_pages,
                                              int block_size, int dtype);

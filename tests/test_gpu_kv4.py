@@ -495,8 +495,9 @@ def test_nothing_to_do(cuda_device):
         w = torch.ones(4, 2, 16, device=dev)
         assert b2pa.accumulate_key_weights(rows, kp, w, no_table, none, none).eq(1).all()
         # no pages at all
-        q = torch.ones(1, 2, T, 64, device=dev)
-        assert not fn(q, kp, vp, t[:, :0], _i32([0], dev), _i32([T], dev)).any()
+        for dtype in DTYPES:
+            q = torch.ones(1, 2, T, 64, dtype=dtype, device=dev)
+            assert not fn(q, kp, vp, t[:, :0], _i32([0], dev), _i32([T], dev)).any()
         assert b2pa.accumulate_key_weights(q, kp, w, t[:, :0], _i32([0], dev), _i32([T], dev)).eq(1).all()
     assert b2pa.evict_by_weight(kp, vp, w, no_table, none, 4).shape == (0, 2, 4)
     assert b2pa.evict_by_weight(kp, vp, w, t[:, :0], _i32([0], dev), 4).eq(-1).all()
