@@ -63,48 +63,61 @@ __device__ __forceinline__ uint32_t place(int r, int c) {
 }
 
 // Rows 32 warp .. 32 warp + 31 of a tile from fp32 or 16-bit values, as fp16 (or
-// bf16) operands; src_of(r): row r's values, null for zeros; done(r, back): the
-// factor that undoes its scaling.  D / 8 lanes read along a row.
+// bf16) operands; src_of(r): row r's values, null for zeros (read from `any`
+// then: no load hangs on a branch); done(r, back): the factor that undoes its
+// scaling.  D / 8 lanes read along a row, four rows' loads are under way at once.
 template <typename T, int D, bool SCALED, bool PERM, int PARTS, typename Src, typename Done>
-__device__ __forceinline__ void put_rows(int warp, uint8_t* tile, Src src_of, Done done) {
-  constexpr int LPR = D / 8, RPI = 32 / LPR, N = 16 / (int)sizeof(T);
+__device__ __forceinline__ void put_rows(int warp, uint8_t* tile, const void* any, Src src_of, Done done) {
+  constexpr int LPR = D / 8, RPI = 32 / LPR, N = 16 / (int)sizeof(T), W = 8 / N;
   const int lane = threadIdx.x & 31, c = lane % LPR;
-#pragma unroll 4
-  for (int it = 0; it < LPR; ++it) {
-    const int r = warp * 32 + it * RPI + lane / LPR;
-    const T* src = src_of(r);
-    uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
-    float back = 1.f;
-    if constexpr (SCALED) {
-      float x[8] = {}, top = 0.f;
-      if (src != nullptr) {
+#pragma unroll 1
+  for (int it0 = 0; it0 < LPR; it0 += 4) {
+    uint4 raw[4][W];
+    uint32_t there = 0;
 #pragma unroll
-        for (int i = 0; i < 8; i += N) {
+    for (int u = 0; u < 4; ++u) {
+      const T* src = src_of(warp * 32 + (it0 + u) * RPI + lane / LPR);
+      there |= (src != nullptr ? 1u : 0u) << u;
+      src = src != nullptr ? src : static_cast<const T*>(any);
+#pragma unroll
+      for (int i = 0; i < W; ++i) raw[u][i] = ld_global_nc<uint4>(src + 8 * c + i * N);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int r = warp * 32 + (it0 + u) * RPI + lane / LPR;
+      if (!(there >> u & 1u)) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) raw[u][i] = make_uint4(0, 0, 0, 0);
+      }
+      uint4 hi = raw[u][0], lo = make_uint4(0, 0, 0, 0);
+      float back = 1.f;
+      if constexpr (SCALED) {
+        float x[8], top = 0.f;
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
           Vec<T, N> v;
-          v.w = ld_global_nc<uint4>(src + 8 * c + i);
-          v.to_float(x + i);
+          v.w = raw[u][i];
+          v.to_float(x + i * N);
         }
-      }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
 #pragma unroll
-      for (int o = LPR / 2; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, o));
-      const float f = range_factor(top, back);
-      if constexpr (PERM) {
-        const float y[8] = {x[0], x[4], x[1], x[5], x[2], x[6], x[3], x[7]};
+        for (int o = LPR / 2; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, o));
+        const float f = range_factor(top, back);
+        if constexpr (PERM) {
+          const float y[8] = {x[0], x[4], x[1], x[5], x[2], x[6], x[3], x[7]};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = y[i];
-      }
-      split8(x, f, hi, lo);
-    } else {
-      if (src != nullptr) hi = ld_global_nc<uint4>(src + 8 * c);
-      if constexpr (PERM)
+          for (int i = 0; i < 8; ++i) x[i] = y[i];
+        }
+        split8(x, f, hi, lo);
+      } else if constexpr (PERM) {
         hi = make_uint4(__byte_perm(hi.x, hi.z, 0x5410), __byte_perm(hi.x, hi.z, 0x7632),
                         __byte_perm(hi.y, hi.w, 0x5410), __byte_perm(hi.y, hi.w, 0x7632));
+      }
+      *reinterpret_cast<uint4*>(tile + place(r, c)) = hi;
+      if constexpr (PARTS == 2) *reinterpret_cast<uint4*>(tile + kRows * D * 2 + place(r, c)) = lo;
+      if (c == 0) done(r, back);
     }
-    *reinterpret_cast<uint4*>(tile + place(r, c)) = hi;
-    if constexpr (PARTS == 2) *reinterpret_cast<uint4*>(tile + kRows * D * 2 + place(r, c)) = lo;
-    if (c == 0) done(r, back);
   }
 }
 
@@ -182,8 +195,12 @@ __global__ void __launch_bounds__(kTcThreads, 2) key_weights_tc_kernel(KeyWeight
   tc::fence_after_sync();
   const uint32_t tmem = tmem_slot;
 
-  pdl_wait();
-  pdl_launch_dependents();
+  // PASS 2 needs nothing of PASS 1 but its partial sums, and PASS 1 let it start
+  // after waiting for what was before: it waits where it reads them.
+  if (PASS == 1) {
+    pdl_wait();
+    pdl_launch_dependents();
+  }
   const Span s = span_of(a, b);
   const int32_t* table = a.page_table + (int64_t)b * a.pt_stride;
   const int64_t head = (int64_t)b * a.H + h;
@@ -228,12 +245,14 @@ __global__ void __launch_bounds__(kTcThreads, 2) key_weights_tc_kernel(KeyWeight
           copy_rows<T, D>(warp, qt, a.q, src);
           q_unit[tid] = qscale;
         } else {
-          put_rows<T, D, S::QSCALED, KV4, S::QP>(warp, qt, src, [&](int r, float back) { q_unit[r] = qscale * back; });
+          put_rows<T, D, S::QSCALED, KV4, S::QP>(warp, qt, a.q, src, [&](int r, float back) { q_unit[r] = qscale * back; });
         }
       }
       tc::fence_proxy_async_smem();
       mbar_arrive(&q_full);
       if constexpr (PASS == 2) {
+        pdl_wait();
+        pdl_launch_dependents();
         float lse = INFINITY;
         if (tid < n) {
           const float2* p = part + (head * a.T + c * kRows + tid) * nsplit;
@@ -429,7 +448,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) key_weights_tc_kernel(KeyWeight
             return reinterpret_cast<const T*>(pool + (uint32_t)blk * block_bytes) + (r & (bs - 1)) * D;
           };
           if constexpr (S::KSCALED)
-            put_rows<T, D, true, false, S::KP>(w, to, src, [&](int r, float back) { key_back[i % kLate][r] = back; });
+            put_rows<T, D, true, false, S::KP>(w, to, a.k_pool, src, [&](int r, float back) { key_back[i % kLate][r] = back; });
           else
             copy_rows<T, D>(w, to, a.k_pool, src);
         }
@@ -480,6 +499,10 @@ __global__ void __launch_bounds__(kTcThreads, 2) key_weights_tc_kernel(KeyWeight
   if (PASS == 1 && blockIdx.x == 0 && h == 0 && tid == 0 && (int64_t)a.seq_lens[b] > s.L)
     set_status(a.status, B2PA_ERR_BAD_BLOCK_ID);
   __syncwarp();
+  if (PASS == 2) {  // (and where a CTA had no keys)
+    pdl_wait();
+    pdl_launch_dependents();
+  }
   tc::fence_before_sync();
   __syncthreads();
   if (warp == 12) {
