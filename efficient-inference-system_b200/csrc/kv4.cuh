@@ -61,7 +61,7 @@ __device__ __forceinline__ uint32_t kv4_scale_code(uint32_t max_bits) {
 
 // Eight codes of one group, packed; s is the value of its scale code.
 template <typename T>
-__device__ __forceinline__ uint32_t kv4_pack8(const float* x, float s) {
+__device__ __forceinline__ uint32_t kv4_pack8(const float* x, uint32_t code, float s) {
   if (!(s > 0.f)) return 0x88888888u;  // a zero scale, or a NaN: zeros
   uint32_t w = 0;
   if constexpr (std::is_same<T, float>::value) {
@@ -72,22 +72,29 @@ __device__ __forceinline__ uint32_t kv4_pack8(const float* x, float s) {
       w |= (uint32_t)(c + 8) << (4 * i);
     }
   } else {
-    // 16-bit x: |x| times the two neighbours of 1 / s, each rounded to an
-    // integer in the addition to 1.5 * 2^23.  A neighbour is off by less than
-    // 2^-22 and x has at most 11 bits, so the two agree unless x lies on a
-    // border, where they differ by one: the even one is taken.  About 9
-    // instructions a value where the division takes over 16.
-    const float r = __frcp_rn(s), e = fmaf(s, r, -1.f);
-    const float up = e < 0.f ? __uint_as_float(__float_as_uint(r) + 1u) : r;
-    const float down = e > 0.f ? __uint_as_float(__float_as_uint(r) - 1u) : r;
+    // 16-bit x, without a division: x times 1 / s rounded (off by less than
+    // 2^-21) goes to a multiple of 2^-13 in the addition to 1536, then to an
+    // integer, ties to even.  x has at most 11 bits, so x / s lies on a border
+    // k + 1/2 or at least 0.49 / 2047 > 2^-12.1 away from it: the first
+    // rounding puts the former on the border and leaves the latter on its
+    // side.  Two packed additions for two values; their mantissas are the
+    // codes, summed up in place.
+    const float r = __frcp_rn(s);
+    const float2 r2 = make_float2(r, r), grid = make_float2(1536.f, 1536.f);
+    const float2 whole = make_float2(12582920.f - 1536.f, 12582920.f - 1536.f);  // 1.5 * 2^23 + 8
+    // |x| / s is at most 7 (1 + 1/16) unless the scale is subnormal or capped
+    const bool clamp = code < 8u || code >= kKv4MaxScale;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t u = __float_as_uint(fmaf(fabsf(x[i]), up, 12582912.f));
-      const uint32_t d = __float_as_uint(fmaf(fabsf(x[i]), down, 12582912.f));
-      uint32_t c = (u ^ ((u ^ d) & u & 1u)) & 15u;
-      c = c < 7u ? c : 7u;
-      w += (x[i] < 0.f ? 8u - c : 8u + c) << (4 * i);
+    for (int i = 0; i < 8; i += 2) {
+      float2 t = fma2(make_float2(x[i], x[i + 1]), r2, grid);
+      if (clamp) {
+        t.x = fminf(fmaxf(t.x, 1529.f), 1543.f);
+        t.y = fminf(fmaxf(t.y, 1529.f), 1543.f);
+      }
+      t = add2(t, whole);
+      w += (__float_as_uint(t.x) << (4 * i)) + (__float_as_uint(t.y) << (4 * i + 4));
     }
+    w -= 0x4b400000u * 0x11111111u;  // the bits of 1.5 * 2^23 in every place (mod 2^32)
   }
   return w;
 }

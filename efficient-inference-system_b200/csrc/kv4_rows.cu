@@ -126,9 +126,9 @@ __global__ void __launch_bounds__(128) kv4_append_kernel(AppendArgs a, int64_t* 
       float f[8];
       uint2 w;
       x.to_float(0, f);
-      w.x = kv4_pack8<T>(f, s);
+      w.x = kv4_pack8<T>(f, code, s);
       x.to_float(1, f);
-      w.y = kv4_pack8<T>(f, s);
+      w.y = kv4_pack8<T>(f, code, s);
       return w;
     };
 #pragma unroll

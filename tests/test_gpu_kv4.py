@@ -125,6 +125,35 @@ def test_append_borders(cuda_device):
     np.testing.assert_array_equal(_np(v)[0, 0], co.stored(-rows))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_append_borders_of_16_bits(cuda_device, dtype):
+    """Every border (k + 1/2) s of every scale s that the type holds with its neighbours, both signs; groups whose
+    largest value saturates, and all values of one sign and exponent against one scale."""
+    rows = []
+    up, down = torch.tensor(float("inf")), torch.tensor(float("-inf"))
+    for code in range(1, 226):
+        s = float(co.GRID[code])
+        x = torch.tensor([(k + 0.5) * s for k in range(7)]).to(dtype)
+        x = torch.cat([x, torch.nextafter(x, up.to(dtype)), torch.nextafter(x, down.to(dtype))])[None]
+        top = torch.full((1, 4), 7 * s, dtype=torch.float64).clamp(max=65504.0).to(dtype)
+        flat = torch.cat([x, -x], 1).flatten()
+        for i in range(0, 42, 14):
+            rows.append(torch.cat([top[0, :2], flat[i: i + 14]]))
+    for scale in (1e-7, 3e-6, 2e-5, 1.0, 1e4, 6e4):
+        steps = torch.linspace(-1, 1, 15 * 200, dtype=torch.float64).view(200, 15) * scale
+        rows += list(torch.cat([torch.full((200, 1), scale, dtype=torch.float64), steps], 1).to(dtype))
+    x = torch.stack(rows)
+    x = torch.cat([x, x.new_zeros(-len(x) % 4, 16)]).view(1, 1, -1, 64).to(cuda_device)
+    n = x.shape[2]
+    kp = torch.zeros(-(-n // 16), 1, 16, 36, dtype=torch.uint8, device=cuda_device)
+    vp, table = torch.zeros_like(kp), _i32(np.arange(len(kp))[None], cuda_device)
+    zero, cnt = _i32([0], cuda_device), _i32([n], cuda_device)
+    b2pa.kv4_append(x, -x, kp, vp, table, zero, cnt)
+    k, v = b2pa.kv4_read(kp, vp, table, zero, cnt, n, torch.float32)
+    np.testing.assert_array_equal(_np(k), co.stored(_np(x)))
+    np.testing.assert_array_equal(_np(v), co.stored(-_np(x)))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_append_takes_any_strides(cuda_device, dtype):
     """Channel-strided, misaligned and broadcast sources."""
