@@ -48,10 +48,20 @@ __device__ __forceinline__ float kv4_scale(uint32_t code) {
 }
 
 // Scale code of a group from the bits of its largest magnitude (a NaN's or
-// infinity's bits compare above every finite one's).
+// infinity's bits compare above every finite one's).  16-bit values T have at
+// most 11 bits, so top / 7 lies on a border of two scales or at least 2^-11 of
+// itself away from it: a product with 1 / 7 rounded, itself rounded to 13 bits
+// (2^-17 in the subnormal range: a border is an odd multiple of 2^-18), is on
+// the border with it, and a division can be spared.
+template <typename T>
 __device__ __forceinline__ uint32_t kv4_scale_code(uint32_t max_bits) {
   if (max_bits >= 0x7f800000u) return kKv4NanScale;
-  const float y = __fdiv_rn(__uint_as_float(max_bits), 7.0f);
+  const float top = __uint_as_float(max_bits);
+  float y;
+  if constexpr (std::is_same<T, float>::value)
+    y = __fdiv_rn(top, 7.0f);
+  else
+    y = __uint_as_float((__float_as_uint(top * (1.f / 7.f)) + 0x400u) & ~0x7ffu);
   if (y < 0x1p-14f) return (uint32_t)__float2int_rn(y * 0x1p17f);
   uint32_t u = __float_as_uint(y);
   u += 0x7ffffu + ((u >> 20) & 1u);
@@ -72,29 +82,31 @@ __device__ __forceinline__ uint32_t kv4_pack8(const float* x, uint32_t code, flo
       w |= (uint32_t)(c + 8) << (4 * i);
     }
   } else {
-    // 16-bit x, without a division: x times 1 / s rounded (off by less than
-    // 2^-21) goes to a multiple of 2^-13 in the addition to 1536, then to an
-    // integer, ties to even.  x has at most 11 bits, so x / s lies on a border
-    // k + 1/2 or at least 0.49 / 2047 > 2^-12.1 away from it: the first
-    // rounding puts the former on the border and leaves the latter on its
-    // side.  Two packed additions for two values; their mantissas are the
-    // codes, summed up in place.
-    const float r = __frcp_rn(s);
-    const float2 r2 = make_float2(r, r), grid = make_float2(1536.f, 1536.f);
-    const float2 whole = make_float2(12582920.f - 1536.f, 12582920.f - 1536.f);  // 1.5 * 2^23 + 8
+    // 16-bit x, without a division: x times 1 / s (off by less than 2^-18)
+    // goes to a multiple of 2^-13 in the addition to 1536, then to an integer,
+    // ties to even.  x has at most 11 bits, so x / s lies on a border k + 1/2
+    // or at least 0.49 / 2047 > 2^-12.1 away from it: the first rounding puts
+    // the former on the border and leaves the latter on its side.  Pairs of
+    // values, codes collected by multiplications: the other pipe unpacks x.
+    const float r = __fdividef(1.f, s);
+    auto both = [](float y) { return make_float2(y, y); };
     // |x| / s is at most 7 (1 + 1/16) unless the scale is subnormal or capped
     const bool clamp = code < 8u || code >= kKv4MaxScale;
+    float2 c[4];  // codes i and i + 4
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      float2 t = fma2(make_float2(x[i], x[i + 1]), r2, grid);
+    for (int i = 0; i < 4; ++i) {
+      c[i] = fma2(make_float2(x[i], x[i + 4]), both(r), both(1536.f));
       if (clamp) {
-        t.x = fminf(fmaxf(t.x, 1529.f), 1543.f);
-        t.y = fminf(fmaxf(t.y, 1529.f), 1543.f);
+        c[i].x = fminf(fmaxf(c[i].x, 1529.f), 1543.f);
+        c[i].y = fminf(fmaxf(c[i].y, 1529.f), 1543.f);
       }
-      t = add2(t, whole);
-      w += (__float_as_uint(t.x) << (4 * i)) + (__float_as_uint(t.y) << (4 * i + 4));
+      c[i] = add2(add2(c[i], both(12582912.f - 1536.f)), both(-12582912.f));
     }
-    w -= 0x4b400000u * 0x11111111u;  // the bits of 1.5 * 2^23 in every place (mod 2^32)
+    float2 v = fma2(c[3], both(16.f), c[2]);
+    v = fma2(v, both(16.f), c[1]);
+    v = fma2(v, both(16.f), c[0]);
+    v = add2(v, both(8388608.f + 0x8888));
+    w = __byte_perm(__float_as_uint(v.x), __float_as_uint(v.y), 0x5410);
   }
   return w;
 }

@@ -127,9 +127,11 @@ def test_append_borders(cuda_device):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_append_borders_of_16_bits(cuda_device, dtype):
-    """Every border (k + 1/2) s of every scale s that the type holds with its neighbours, both signs; groups whose
-    largest value saturates, and all values of one sign and exponent against one scale."""
-    rows = []
+    """Every finite value as a group's largest; every border (k + 1/2) s of every scale s that the type holds with its
+    neighbours, both signs; ranges of values against scales from subnormal to saturated."""
+    tops = torch.arange(2 ** 15, dtype=torch.int16).view(dtype)
+    tops = tops[torch.isfinite(tops)]
+    rows = list(torch.cat([tops[:, None], -tops[:, None] / 2, tops.new_zeros(len(tops), 14)], 1))
     up, down = torch.tensor(float("inf")), torch.tensor(float("-inf"))
     for code in range(1, 226):
         s = float(co.GRID[code])
