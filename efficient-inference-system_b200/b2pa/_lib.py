@@ -106,6 +106,32 @@ def load() -> ctypes.CDLL:
         return lib
 
 
+_calls = None
+
+
+def calls():
+    """The extension module of csrc/py_calls.cpp: the cache-compression calls on arguments that need no conversion
+    (it returns NotImplemented for others)."""
+    global _calls
+    if _calls is None:
+        import importlib.machinery
+        import importlib.util
+
+        path = LIB_PATH.with_name("b2pa_calls.so")
+        if not path.exists():
+            raise RuntimeError(f"b2pa_calls.so not found at {path}; build it with `python -m b2pa.build` "
+                               "(or __graft_entry__.build()).")
+        loader = importlib.machinery.ExtensionFileLoader("b2pa_calls", str(path))
+        module = importlib.util.module_from_spec(importlib.util.spec_from_file_location("b2pa_calls", path, loader=loader))
+        loader.exec_module(module)
+        lib = load()
+        module.set_functions(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+            "b2pa_kv4_append", "b2pa_kv4_read", "b2pa_paged_decode_kv4", "b2pa_paged_prefill_kv4_workspace_size",
+            "b2pa_paged_prefill_kv4", "b2pa_key_weights_workspace_size", "b2pa_key_weights", "b2pa_evict")))
+        _calls = module
+    return _calls
+
+
 def last_error() -> str:
     return load().b2pa_last_error_string().decode(errors="replace")
 

@@ -58,6 +58,9 @@ def accumulate_key_weights(q: torch.Tensor, k_pool: torch.Tensor, key_weights: t
     whose other slots stay as they are; returns it."""
     what = "accumulate_key_weights"
     out = key_weights if out is None else out
+    if _lib.calls().key_weights(q, k_pool, key_weights, page_table, seq_lens, current_lengths, window,
+                                out) is not NotImplemented:
+        return out
     dev = need_cuda(what, q=q, k_pool=k_pool, key_weights=key_weights, page_table=page_table, seq_lens=seq_lens,
                     current_lengths=current_lengths, out=out)
     if q.dim() != 4:
@@ -110,6 +113,9 @@ def evict_by_weight(k_pool: torch.Tensor, v_pool: torch.Tensor, key_weights: tor
     pools and their weights move, in order, to positions 0 .. k-1: in the same pages, or in those of ``out_table``
     ([B, >= ceil(keep / block_size)]; none of them in ``page_table``).  Slots behind the k-th row in its page are
     zeroed; pages behind it are left to the caller.  Returns the kept positions, int32 [B, H, keep], -1 behind k."""
+    kept = _lib.calls().evict(k_pool, v_pool, key_weights, page_table, seq_lens, keep, recent, out_table)
+    if kept is not NotImplemented:
+        return kept
     what = "evict_by_weight"
     dev = need_cuda(what, k_pool=k_pool, v_pool=v_pool, key_weights=key_weights, page_table=page_table,
                     seq_lens=seq_lens, out_table=page_table if out_table is None else out_table)

@@ -47,8 +47,9 @@ class Kv4BlockPool(LayerBlockPool):
 
 
 # ------------------------------------------------------------ argument checks
-# Small calls are bound by the host: these checks cost a microsecond or two in
-# all, so each reads what it needs once and converts nothing that fits.
+# Small calls are bound by the host, 13 us each with these checks and ctypes, so
+# arguments that need no conversion go through csrc/py_calls.cpp first; these
+# checks are for all others and for what has to be refused.
 _current_device = torch._C._cuda_getDevice
 _capturing = torch._C._cuda_isCurrentStreamCapturing
 _NO_GUARD = contextlib.nullcontext()
@@ -164,6 +165,7 @@ def status_at(index: int) -> int:
     got = _status_at.get(index)
     if got is None:
         got = _status_at[index] = _lib.status_buffer(torch.device("cuda", index)).data_ptr()
+        _lib.calls().set_status(index, got)
     return got
 
 
@@ -176,6 +178,9 @@ def kv4_append(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tensor, v
                seq_lens_out: torch.Tensor | None = None) -> None:
     """Quantises rows ``t < lengths[b]`` of ``k_new`` / ``v_new`` ([B, H, T, D]) into positions ``start_pos[b] + t``
     of the 4-bit pools.  ``seq_lens_out`` (int64 [B]) receives the lengths after the append."""
+    if _lib.calls().kv4_append(k_new, v_new, k_pool, v_pool, page_table, start_pos, lengths,
+                               seq_lens_out) is not NotImplemented:
+        return
     what = "kv4_append"
     dev = need_cuda(what, k_new=k_new, v_new=v_new, k_pool=k_pool, v_pool=v_pool, page_table=page_table,
                     start_pos=start_pos, lengths=lengths)
@@ -207,6 +212,9 @@ def kv4_read(k_pool: torch.Tensor, v_pool: torch.Tensor, page_table: torch.Tenso
              lengths: torch.Tensor, T: int, dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
     """The values stored at positions ``start_pos[b] + t``, t < lengths[b], as ``(k, v)`` of shape [B, H, T, D] in
     ``dtype`` (exact in fp32, bf16 and fp16); rows behind ``lengths[b]`` are zeros."""
+    out = _lib.calls().kv4_read(k_pool, v_pool, page_table, start_pos, lengths, T, dtype)
+    if out is not NotImplemented:
+        return out
     what = "kv4_read"
     dev = need_cuda(what, k_pool=k_pool, v_pool=v_pool, page_table=page_table, start_pos=start_pos, lengths=lengths)
     if T < 0:
@@ -231,6 +239,13 @@ def kv4_read(k_pool: torch.Tensor, v_pool: torch.Tensor, page_table: torch.Tenso
 
 
 def _attend(what: str, q, k_pool, v_pool, page_table, seq_lens, current_lengths, pages=None) -> torch.Tensor:
+    decode = what == "paged_attention_decode_kv4"
+    if pages is None:
+        calls = _lib.calls()
+        call = calls.decode_kv4 if decode else calls.prefill_kv4
+        out = call(q, k_pool, v_pool, page_table, seq_lens, current_lengths)
+        if out is not NotImplemented:
+            return out
     dev = need_cuda(what, q=q, k_pool=k_pool, v_pool=v_pool, page_table=page_table, seq_lens=seq_lens,
                     current_lengths=current_lengths)
     if q.dim() != 4:
@@ -239,7 +254,6 @@ def _attend(what: str, q, k_pool, v_pool, page_table, seq_lens, current_lengths,
     blocks, H, bs = pool_shape(what, D, k_pool, v_pool)
     check_heads(what, "q", q, H)
     code = _lib.dtype_code(q.dtype)
-    decode = what == "paged_attention_decode_kv4"
     if decode and T != 1:
         raise ValueError(f"b2pa.{what}: q has {T} tokens per sequence, not 1")
     table, pt_stride, width = table_args(what, "page_table", page_table, B)

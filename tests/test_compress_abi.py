@@ -180,3 +180,16 @@ def test_oracle_quantiser():
     bad[0, 5], bad[0, 40] = np.nan, np.inf
     r = co.stored(bad).reshape(8, 16)
     assert np.isnan(r[0]).all() and np.isnan(r[2]).all() and np.isfinite(np.delete(r, [0, 2], 0)).all()
+
+
+def test_short_calls_decline(lib):
+    """The extension module's functions launch nothing and raise nothing on what they do not take: CPU tensors, other
+    objects, missing arguments."""
+    calls = _lib.calls()
+    x = torch.zeros(1, 2, 1, 64)
+    for name in ("kv4_append", "kv4_read", "decode_kv4", "prefill_kv4", "key_weights", "evict"):
+        fn = getattr(calls, name)
+        for n in range(10):
+            assert fn(*[x] * n) is NotImplemented
+            assert fn(*[None] * n) is NotImplemented
+            assert fn(*["x", 3, x, None, 2 ** 70][:n]) is NotImplemented

@@ -355,6 +355,42 @@ def test_offsets_past_32_bits(cuda_device, kv4):
     assert b2pa.read_status(dev) == 0
 
 
+@pytest.mark.parametrize("T", [1, 9])
+def test_arguments_that_need_conversion(cuda_device, T):
+    """64-bit lengths, strided lengths, tables that are slices, columns or 64-bit, misaligned and channel-strided
+    queries: the same results as plain arguments, from every call."""
+    dev, H, D, bs, B = cuda_device, 2, 64, 16, 3
+    gen = torch.Generator().manual_seed(4)
+    k, v = (torch.randint(0, 200, (12, H, bs, 36), generator=gen, dtype=torch.uint8).to(dev) for _ in range(2))
+    w = torch.rand(12, H, bs, generator=gen).to(dev)
+    q = torch.randn(B, H, T, D, generator=gen).to(dev)
+    table = _i32(np.arange(12).reshape(3, 4), dev)
+    lens, cur, start = _i32([60, 33, 9], dev), _i32([T] * 3, dev), _i32([3, 0, 40], dev)
+    wide = torch.zeros(B, 9, dtype=torch.int32, device=dev)
+    wide[:, 2:6] = table
+    odd = torch.zeros(q.numel() + 1, device=dev)[1:].view(q.shape).copy_(q)
+    every = torch.zeros(*q.shape[:3], 2 * D, device=dev)[..., ::2].copy_(q)
+    strided = torch.stack([lens, lens], 1)[:, 0]
+    fn = b2pa.paged_attention_decode_kv4 if T == 1 else b2pa.paged_attention_prefill_kv4
+
+    def run(q, table, lens, cur, start):
+        pools = [t.clone() for t in (k, v, w)]
+        out = [fn(q, *pools[:2], table, lens, cur)]
+        b2pa.accumulate_key_weights(q, pools[0], pools[2], table, lens, cur)
+        b2pa.accumulate_key_weights(q, pools[0], pools[2], table, lens, cur, window=2)
+        out += b2pa.kv4_read(*pools[:2], table, start, cur, T, torch.float32)
+        b2pa.kv4_append(q, q, *pools[:2], table, start, cur)
+        out.append(b2pa.evict_by_weight(*pools, table, lens, 20, 3))
+        return out + pools
+
+    want = run(q, table, lens, cur, start)
+    for args in ((q, table.long(), lens.long(), cur.long(), start.long()), (q, wide[:, 2:6], strided, cur, start),
+                 (q, torch.stack([table, table], 2)[..., 0], lens, cur, start), (odd, table, lens, cur, start),
+                 (every, table, lens, cur, start)):
+        assert all(torch.equal(a, b) for a, b in zip(run(*args), want))
+    assert b2pa.read_status(dev) == 0
+
+
 def test_counts_past_32_bits(cuda_device):
     """``recent`` and ``window`` of any size mean all of them; a batch cut to any number keeps what it has."""
     dev = cuda_device
