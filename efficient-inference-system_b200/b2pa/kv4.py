@@ -240,12 +240,11 @@ def kv4_read(k_pool: torch.Tensor, v_pool: torch.Tensor, page_table: torch.Tenso
 
 def _attend(what: str, q, k_pool, v_pool, page_table, seq_lens, current_lengths, pages=None) -> torch.Tensor:
     decode = what == "paged_attention_decode_kv4"
-    if pages is None:
-        calls = _lib.calls()
-        call = calls.decode_kv4 if decode else calls.prefill_kv4
-        out = call(q, k_pool, v_pool, page_table, seq_lens, current_lengths)
-        if out is not NotImplemented:
-            return out
+    calls = _lib.calls()
+    call = calls.decode_kv4 if decode else calls.prefill_kv4
+    out = call(q, k_pool, v_pool, page_table, seq_lens, current_lengths, pages)
+    if out is not NotImplemented:
+        return out
     dev = need_cuda(what, q=q, k_pool=k_pool, v_pool=v_pool, page_table=page_table, seq_lens=seq_lens,
                     current_lengths=current_lengths)
     if q.dim() != 4:

@@ -182,10 +182,11 @@ at::Tensor scratch(size_t bytes, const at::Tensor& like) {
 }
 void* at_or_null(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
-// paged_attention_decode_kv4 (SINGLE) and _prefill_kv4(q, k_pool, v_pool, page_table, seq_lens, current_lengths)
+// paged_attention_decode_kv4 (SINGLE) and _prefill_kv4(q, k_pool, v_pool, page_table, seq_lens, current_lengths,
+// pages or None: how many of the table's columns count)
 template <bool SINGLE>
 PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != 6) return decline();
+  if (n != 7) return decline();
   Call c;
   const at::Tensor &q = c.take(a[0]), &kp = c.take(a[1]), &vp = c.take(a[2]), &t = c.take(a[3]), &len = c.take(a[4]),
                    &cur = c.take(a[5]);
@@ -197,6 +198,11 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
       vp.sizes() != kp.sizes() || !table.take(t, B) || !rows_of(len, B) || !rows_of(cur, B) || !aligned(q) ||
       !q.is_non_overlapping_and_dense())
     return decline();
+  if (a[6] != Py_None) {
+    const int64_t pages = count_of(a[6]);
+    if (pages < 0 || pages > table.pages) return decline();
+    table.pages = (int)pages;
+  }
   const at::Tensor out = at::detail::empty_strided_cuda(q.sizes(), q.strides(), q.scalar_type(), q.device());
   const int bs = (int)kp.size(2);
   const float scale = (float)(1.0 / std::sqrt((double)D));
