@@ -8,6 +8,8 @@
 // and the weights move, in order, to positions 0 .. k-1: in the same pages, or
 // in the pages of a second table.
 //
+//   evict_both_kernel    the two below in one CTA per (head, sequence), for
+//       short sequences;
 //   evict_select_kernel  one CTA per (head, sequence): radix selection of the
 //       smallest kept weight (digits of 11, 11 and 10 bits of order-preserving
 //       keys, which shared memory holds when they fit; it ends early once a
@@ -55,18 +57,15 @@ __device__ __forceinline__ Kept kept_of(const EvictArgs& a, int b) {
 
 constexpr int kBins = 2048;
 
+// The kept positions of head h of sequence b, by the whole CTA.
 template <int THREADS>
-__global__ void __launch_bounds__(THREADS) evict_select_kernel(EvictArgs a, int cached) {
+__device__ __forceinline__ void select_kept(const EvictArgs& a, int cached, uint32_t* keys, int h, int b, const Kept& s) {
   constexpr int WARPS = THREADS / 32;
-  extern __shared__ __align__(16) uint32_t keys[];
   __shared__ uint32_t hist[2][kBins];
   __shared__ uint32_t found[3];
   __shared__ uint32_t totals[8];
   __shared__ int2 warp_count[WARPS];
-  pdl_wait();
-  pdl_launch_dependents();
-  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const Kept s = kept_of(a, b);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (h == 0 && tid == 0 && a.seq_lens[b] > s.n) set_status(a.status, B2PA_ERR_BAD_BLOCK_ID);
   int32_t* out = a.kept + ((int64_t)b * a.H + h) * a.keep;
   for (int i = s.k + tid; i < a.keep; i += THREADS) out[i] = -1;
@@ -192,6 +191,14 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(EvictArgs a, int 
   }
 }
 
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) evict_select_kernel(EvictArgs a, int cached) {
+  extern __shared__ __align__(16) uint32_t keys[];
+  pdl_wait();
+  pdl_launch_dependents();
+  select_kept<THREADS>(a, cached, keys, blockIdx.x, blockIdx.y, kept_of(a, blockIdx.y));
+}
+
 // One slice of the rows: 1 << words_log2 words of VB bytes per row, at
 // page + offset + slot * row_stride + word * word_stride.
 struct Slice {
@@ -231,7 +238,7 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, const Slice& sl, i
 #pragma unroll
     for (int u = 0; u < kMoveWords; ++u) {
       const int r = r0 + row0 + u * step;
-      src[u] = __ldg(kept + (r < s.k ? r : s.k - 1));
+      src[u] = kept[r < s.k ? r : s.k - 1];  // (maybe this CTA's own writes)
     }
   };
   if (s.k > 0) positions(0);
@@ -271,13 +278,9 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, const Slice& sl, i
   if (bad) set_status(a.status, B2PA_ERR_BAD_BLOCK_ID);
 }
 
-__global__ void __launch_bounds__(kMoveThreads, 4) evict_move_kernel(EvictArgs a, int slices_log2) {
-  pdl_wait();
-  pdl_launch_dependents();
-  const int h = blockIdx.y, b = blockIdx.z;
-  const Kept s = kept_of(a, b);
-  if (!a.out_table && s.n == s.k) return;  // nothing leaves
-  int part = blockIdx.x;
+// Slice number `part` of the rows: K and V in 1 << slices_log2 parts each, the
+// weights, and the scales of 4-bit K and V.
+__device__ __forceinline__ void move_part(const EvictArgs& a, int part, int slices_log2, int h, int b, const Kept& s) {
   const bool kv4 = a.dtype == B2PA_DTYPE_KV4;
   const int row_bytes = kv4 ? a.D / 2 : a.D * a.elem;
   const uint32_t page_bytes = kv4 ? kv4_page_bytes(a.block_size, a.D) : a.block_size * row_bytes;
@@ -302,17 +305,38 @@ __global__ void __launch_bounds__(kMoveThreads, 4) evict_move_kernel(EvictArgs a
   }
 }
 
-template <int THREADS>
-int select_launch(const EvictArgs& a, cudaStream_t st) {
+__global__ void __launch_bounds__(kMoveThreads, 4) evict_move_kernel(EvictArgs a, int slices_log2) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int h = blockIdx.y, b = blockIdx.z;
+  const Kept s = kept_of(a, b);
+  if (!a.out_table && s.n == s.k) return;  // nothing leaves
+  move_part(a, blockIdx.x, slices_log2, h, b, s);
+}
+
+// Both at once: a CTA selects and then moves the rows of its head and sequence.
+__global__ void __launch_bounds__(kMoveThreads, 4) evict_both_kernel(EvictArgs a, int cached) {
+  extern __shared__ __align__(16) uint32_t keys[];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int h = blockIdx.x, b = blockIdx.y;
+  const Kept s = kept_of(a, b);
+  select_kept<kMoveThreads>(a, cached, keys, h, b, s);
+  if (!a.out_table && s.n == s.k) return;
+  __syncthreads();  // the positions are written; the weights have been read
+  const int parts = a.dtype == B2PA_DTYPE_KV4 ? 5 : 3;
+  for (int part = 0; part < parts; ++part) move_part(a, part, 0, h, b, s);
+}
+
+// `kern` with shared memory for the keys where they fit.
+int launch_with_keys(const EvictArgs& a, void (*kern)(EvictArgs, int), int threads, cudaStream_t st) {
   const int64_t longest = (int64_t)a.max_pages * a.block_size;
   constexpr int64_t kFixed = 2 * kBins * 4 + 1024;  // static shared memory
   const int cached = longest * 4 + kFixed <= device_max_smem_optin();
   const size_t smem = cached ? (size_t)longest * 4 : 0;
-  auto kern = evict_select_kernel<THREADS>;
   const int rc = set_max_dynamic_smem_cached(reinterpret_cast<const void*>(kern), (int)smem);
   if (rc != B2PA_OK) return rc;
-  const cudaError_t e =
-      launch_pdl(kern, dim3((unsigned)a.H, (unsigned)a.B), dim3(THREADS), smem, st, a, cached);
+  const cudaError_t e = launch_pdl(kern, dim3((unsigned)a.H, (unsigned)a.B), dim3(threads), smem, st, a, cached);
   if (e != cudaSuccess) return set_error(B2PA_ERR_CUDA, "evict launch: %s", cudaGetErrorString(e));
   return B2PA_OK;
 }
@@ -322,15 +346,23 @@ int select_launch(const EvictArgs& a, cudaStream_t st) {
 int launch_evict(const EvictArgs& a, cudaStream_t st) {
   if (a.keep <= 0) return B2PA_OK;
   const bool kv4 = a.dtype == B2PA_DTYPE_KV4;
-  // few keys a thread: a small CTA, so that an SM runs eight sequences at once
-  const int rc = (int64_t)a.max_pages * a.block_size <= 2048 ? select_launch<256>(a, st) : select_launch<1024>(a, st);
+  const int64_t pairs = (int64_t)a.B * a.H;
+  // few keys a thread: a small CTA, so that an SM runs several sequences at once
+  const bool few = (int64_t)a.max_pages * a.block_size <= 2048;
+  // One launch while a CTA's rows are few and most SMs have one: heads that are
+  // done selecting move while others select.  Two launches -> one, us: 64
+  // sequences of 128-1,024 to 200, 8 heads of 64, fp32 33 -> 29; of 1,024 to
+  // 300, heads of 128, bf16: 128 heads in all 21 -> 18, 256 30 -> 26, but 64 15
+  // -> 16 and 8 8 -> 13; of 2,000 to 1,500: 128 heads 55 -> 63, 512 158 -> 164.
+  if (few && a.keep <= 1024 && 4 * pairs >= 3 * device_sm_count())
+    return launch_with_keys(a, evict_both_kernel, kMoveThreads, st);
+  const int rc = few ? launch_with_keys(a, evict_select_kernel<256>, 256, st)
+                     : launch_with_keys(a, evict_select_kernel<1024>, 1024, st);
   if (rc != B2PA_OK) return rc;
   // rows in parts of 64 bytes or more while the parts are fewer than four CTAs per SM
   const int row_bytes = kv4 ? a.D / 2 : a.D * a.elem;
   int slices_log2 = 0;
-  while ((row_bytes >> slices_log2) > 64 &&
-         ((int64_t)a.B * a.H * 2 << slices_log2) < 4 * device_sm_count())
-    ++slices_log2;
+  while ((row_bytes >> slices_log2) > 64 && (pairs * 2 << slices_log2) < 4 * device_sm_count()) ++slices_log2;
   const cudaError_t e =
       launch_pdl(evict_move_kernel, dim3((unsigned)((2 << slices_log2) + (kv4 ? 3 : 1)), (unsigned)a.H, (unsigned)a.B),
                  dim3(kMoveThreads), 0, st, a, slices_log2);

@@ -31,12 +31,13 @@
 //     into fp16's range -- q by its own maximum, the weights by the largest V
 //     scale so far, which is tracked like the softmax maximum.
 //   * a lane fetches exactly the bytes that it consumes (its fragment of the
-//     tile) with asynchronous copies into its own slots of a 4-deep ring, so
-//     the ring needs no block-wide barrier; only a tile's 16 K scales rows and
-//     its visibility mask are read across the warp.
+//     tile) with asynchronous copies into its own slots of a ring of two
+//     stages, so the ring needs no block-wide barrier; only a tile's 16 K
+//     scales rows and its visibility mask are read across the warp.
 //
-// One warp works on tiles of 16 keys; the 8 warps of a CTA take turns over a
-// sequence's tiles, and a cluster of 1 to 8 CTAs splits a long sequence.  The
+// One warp works on steps of two tiles of 16 keys (head_dim 256: one); the 8 (4)
+// warps of a CTA take turns over a sequence's steps, and a cluster of 1 to 8
+// CTAs splits a long sequence.  The
 // partial softmaxes meet in shared memory, across the cluster through
 // distributed shared memory: one launch, no scratch.
 #include <cooperative_groups.h>

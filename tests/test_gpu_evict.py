@@ -259,6 +259,18 @@ def test_evict(cuda_device, fresh, dtype, kv4, D, bs, H):
                     dtype=dtype, kv4=kv4, seed=keep, fresh=fresh)
 
 
+@pytest.mark.parametrize("fresh", [False, True], ids=["in_place", "out_table"])
+@pytest.mark.parametrize("dtype,kv4,D", [(torch.float32, False, 64), (torch.bfloat16, False, 128), (None, True, 64),
+                                         (None, True, 256)])
+def test_evict_many_heads(cuda_device, fresh, dtype, kv4, D):
+    """Short sequences of many heads (one launch), to few tokens and to more than a chunk of rows."""
+    for keep, recent in ((5, 5), (150, 20), (400, 0)):
+        _evict_case(cuda_device, lens=[0, 3, 150, 151, 407, 512, 33, 260, 400, 401], keep=keep, recent=recent, H=16, D=D,
+                    bs=16, dtype=dtype, kv4=kv4, seed=keep, fresh=fresh)
+    _evict_case(cuda_device, lens=[300] * 10, keep=64, recent=0, H=16, D=D, bs=16, dtype=dtype, kv4=kv4, seed=1,
+                fresh=fresh, weights=_ties)
+
+
 def _ties(rng, shape):
     return np.floor(rng.random(shape) * 3).astype(np.float32)
 
