@@ -28,6 +28,7 @@
 // one launch.  4-bit keys take the product of the decode kernel (kv4_mma.cuh).
 #include <cooperative_groups.h>
 
+#include "by_length.cuh"
 #include "common.cuh"
 #include "kernels.h"
 #include "kv4.cuh"
@@ -503,7 +504,7 @@ struct StepRows {
 
 template <typename T, bool KV4, int D>
 __global__ void __launch_bounds__(kStepThreads, KV4 ? 3 : 0) key_weights_step_kernel(KeyWeightArgs a, float qscale, float* far,
-                                                                        int64_t far_stride) {
+                                                                        int64_t far_stride, int by_length) {
   using S = StepRows<T, KV4, D>;
   using O = Op<T, false>;
   constexpr int RB = S::RB, RW = S::RW, E = 16 / (int)sizeof(T);
@@ -512,7 +513,8 @@ __global__ void __launch_bounds__(kStepThreads, KV4 ? 3 : 0) key_weights_step_ke
   __shared__ float cta_m, cta_l;
   pdl_wait();
   pdl_launch_dependents();
-  const int ns = gridDim.x, rank = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+  const int ns = gridDim.x, rank = blockIdx.x, h = blockIdx.y;
+  const int b = by_length ? nth_longest(a.seq_lens, gridDim.z, blockIdx.z) : (int)blockIdx.z;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Span s = span_of(a, b);
   if (rank == 0 && h == 0 && tid == 0 && (int64_t)a.seq_lens[b] > s.L) set_status(a.status, B2PA_ERR_BAD_BLOCK_ID);
@@ -820,8 +822,10 @@ int step_launch(const KeyWeightArgs& a, cudaStream_t st) {
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
+  const int by_length = orders_by_length(a.B, (int64_t)ns * a.H * a.B, 2);
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a, a.scale * kLog2e,
-                                           far ? static_cast<float*>(a.workspace) : static_cast<float*>(nullptr), keys);
+                                           far ? static_cast<float*>(a.workspace) : static_cast<float*>(nullptr), keys,
+                                           by_length);
   if (e != cudaSuccess) return set_error(B2PA_ERR_CUDA, "key_weights launch: %s", cudaGetErrorString(e));
   return B2PA_OK;
 }

@@ -42,6 +42,7 @@
 // distributed shared memory: one launch, no scratch.
 #include <cooperative_groups.h>
 
+#include "by_length.cuh"
 #include "common.cuh"
 #include "kernels.h"
 #include "kv4.cuh"
@@ -111,6 +112,7 @@ struct DecodeKv4Params {
   int H;
   float qscale;  // scale * log2(e)
   int32_t* status;
+  int by_length;  // CTAs take the sequences longest first
 };
 
 }  // namespace
@@ -128,7 +130,7 @@ __global__ void __launch_bounds__(W * 32, D == 256 ? 8 / W : 16 / W) kv4_decode_
   constexpr int PAGE = kv4_page_bytes(BS, D), CODES = BS * (D / 2);
   extern __shared__ __align__(16) uint8_t ring_all[];
   __shared__ Smem<D, W> sm;
-  const int ns = gridDim.x, rank = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+  const int ns = gridDim.x, rank = blockIdx.x, h = blockIdx.y;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   uint8_t* ring = ring_all + warp * (kStages * C::BYTES);
   const uint32_t ring_at = smem_u32(ring);
@@ -138,6 +140,7 @@ __global__ void __launch_bounds__(W * 32, D == 256 ? 8 / W : 16 / W) kv4_decode_
   if (ns > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   pdl_wait();
   pdl_launch_dependents();
+  const int b = p.by_length ? nth_longest(p.seq_lens, gridDim.z, blockIdx.z) : (int)blockIdx.z;
   // Three loads that do not wait for one another: the lengths, q, and the
   // first block ids.  Steps go round the cluster's warps, so a warp's first
   // step does not depend on the length.
@@ -540,6 +543,7 @@ static int decode_launch(const AttnArgs& a, int ns, cudaStream_t s) {
   p.H = a.H;
   p.qscale = a.scale * kLog2e;
   p.status = a.status;
+  p.by_length = orders_by_length(a.B, (int64_t)ns * a.H * a.B, 2);
   constexpr int smem = C::WARPS * kStages * C::BYTES;
   auto kern = kv4_decode_kernel<T, D, BS, W>;
   const int rc = set_max_dynamic_smem_cached(reinterpret_cast<const void*>(kern), smem);
