@@ -122,19 +122,17 @@ class SharedStepMetadata:
         _rt_check(rt.cudaEventRecord(self.events[i], stream), "cudaEventRecord")
         self.recorded[i] = True
 
-    def ensure_workspace(self, H: int, D: int, block_size: int, dtype: torch.dtype,
-                         kv4: bool = False, weights: bool = False) -> torch.Tensor:
-        """Scratch for the decode of every layer (and, with ``weights``, for
-        the key weights' accumulation behind it); ``kv4``: 4-bit pools of rows
-        of ``dtype``."""
-        key = (H, D, block_size, dtype, kv4, weights)
-        if key == self._ws_key:
+    def ensure_workspace(self, kinds: set[tuple]) -> torch.Tensor:
+        """Scratch for the decode of every layer (and for the accumulation of
+        key weights behind it).  ``kinds``: the layers' (H, D, block size,
+        dtype of the rows, 4-bit pages, tracks key weights)."""
+        if kinds == self._ws_key:
             return self.workspace
-        self._ws_key = key
+        self._ws_key = kinds
         lib = _lib.load()
-        code = _lib.dtype_code(dtype)
 
-        def need_of(b: int) -> int:
+        def need_of(b: int, H: int, D: int, block_size: int, dtype: torch.dtype, kv4: bool, weights: bool) -> int:
+            code = _lib.dtype_code(dtype)
             n = 0 if kv4 else lib.b2pa_paged_decode_workspace_size(b, H, D, self.width, block_size, code)
             if weights:
                 n = max(n, lib.b2pa_key_weights_workspace_size(b, H, 1, D, self.width, block_size, code,
@@ -143,7 +141,7 @@ class SharedStepMetadata:
 
         # enough for every batch size the buffers serve (the split plan is not
         # monotone in B)
-        need = max(need_of(b) for b in range(1, self.capacity + 1))
+        need = max(need_of(b, *kind) for kind in kinds for b in range(1, self.capacity + 1))
         if self.workspace is None or self.workspace.numel() < need:
             self.workspace = torch.empty(max(need, 256), dtype=torch.uint8, device=self.device)
         return self.workspace
@@ -210,12 +208,7 @@ class DecodeStep:
         starts = reserve_lockstep(self.layer_states, self.pools)
         first = self.layer_states[0]
         self.meta.upload([s.block_ids for s in first], [s.seq_len for s in first], starts)
-        pool = self.pools[0]
-        kb = pool.k_blocks
-        kv4 = kb.dtype == torch.uint8
-        self.meta.ensure_workspace(kb.shape[1], pool.head_dim if kv4 else kb.shape[3], kb.shape[2],
-                                   pool.dtype if kv4 else kb.dtype, kv4,
-                                   any(getattr(p, "key_weights", None) is not None for p in self.pools))
+        self.meta.ensure_workspace({_kind_of(p) for p in self.pools})
         for pool in self.pools:
             pool._b2pa_step = self
         self.open = True
@@ -317,6 +310,14 @@ class DecodeStep:
                 tuple((p.k_blocks.data_ptr(), p.v_blocks.data_ptr(), p.k_blocks.shape[0]) for p in self.pools),
                 tuple((w.data_ptr(), p.key_weight_window) if (w := getattr(p, "key_weights", None)) is not None else None
                       for p in self.pools))
+
+
+def _kind_of(pool) -> tuple:
+    """What ``SharedStepMetadata.ensure_workspace`` has to know of a layer's pool."""
+    kb = pool.k_blocks
+    kv4 = kb.dtype == torch.uint8
+    return (kb.shape[1], pool.head_dim if kv4 else kb.shape[3], kb.shape[2], pool.dtype if kv4 else kb.dtype, kv4,
+            getattr(pool, "key_weights", None) is not None)
 
 
 def reserve_lockstep(layer_states: list[list], pools: list) -> list[int]:

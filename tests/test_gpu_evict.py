@@ -495,10 +495,12 @@ def test_run_of_steps(cuda_device, kv4, fused):
 
 
 def _model(dev, kv4):
-    def tracking_pool(*args):
-        pool = (b2pa.Kv4BlockPool if kv4 else b2pa.LayerBlockPool)(*args)
-        pool.track_key_weights()
-        return pool
+    made = []
+
+    def tracking_pool(*args):  # "mixed": the first layer's pages 4-bit, the second's plain
+        made.append((b2pa.Kv4BlockPool if kv4 is True or (kv4 == "mixed" and not made) else b2pa.LayerBlockPool)(*args))
+        made[-1].track_key_weights()
+        return made[-1]
 
     back = om.b2pa_backend()
     back.pool_cls = tracking_pool
@@ -508,7 +510,7 @@ def _model(dev, kv4):
 
 
 @torch.no_grad()
-@pytest.mark.parametrize("kv4", [False, True], ids=["plain", "kv4"])
+@pytest.mark.parametrize("kv4", [False, True, "mixed"], ids=["plain", "kv4", "mixed"])
 def test_decoder_graph_with_eviction(cuda_device, kv4):
     """FusedDecoder under DecodeGraph with tracking pools gives, bit for bit, the logits, pools and key weights of the
     same steps run eagerly in a DecodeStep, through an eviction of every layer between replays."""
