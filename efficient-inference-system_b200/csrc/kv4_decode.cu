@@ -572,7 +572,7 @@ static int decode_blocks(const AttnArgs& a, cudaStream_t s) {
   // every warp keeps a step of the longest sequence.  A CTA costs about 4 us
   // beside its keys (loads that depend on one another, the merge), so more
   // waves of smaller shares are slower: 64 sequences of 128-1,024 tokens and 8
-  // heads of 64 (fp32) take 16.9 us with 1 CTA each, 23.9 with 2; 64 of
+  // heads of 64 (fp32) take 16.9 us with 1 CTA each, 23.9 with 2 (in order); 64 of
   // 1,024-8,192 and 32 heads of 128 (bf16) 288 and 310; one sequence of 8,001
   // tokens and 32 heads of 128 44.6 us with 1, 24.5 with 2, 17.7 with 4, 13.1
   // with 8.  head_dim 256 takes half as many warps a CTA (registers).
