@@ -5,9 +5,10 @@
 //   kv4_read_kernel    reads rows back as the values they stand for.
 //
 // The bytes they move (D * element size in and 9/16 D out a row, or the
-// reverse) bound them from below: 18 us each for 9,186 rows of 32 heads of 128
-// in bf16, which take 30 and 37.  The append spends instructions, some 65 a
-// word of 8 codes.  There a thread takes whole groups (16
+// reverse) bound them from below: for 6,260 rows of 32 heads of 128 in bf16, in
+// 8 x 1,531 slots whose others are read back as zeros, 20 and 36 us at copy
+// bandwidth; they take about 30 and 37.  The append spends instructions, some
+// 65 a word of 8 codes.  There a thread takes whole groups (16
 // channels) of K and of V, so a group's scale and reciprocal are worked out once; the
 // group's maximum is taken on the bits of |x| (pairs of 16-bit values at a
 // time), so a NaN or an infinity wins it.  Prompts: a CTA takes two neighbouring
