@@ -55,7 +55,7 @@ def accumulate_key_weights(q: torch.Tensor, k_pool: torch.Tensor, key_weights: t
     """Adds to each cached key's sum in ``key_weights`` (fp32 [blocks, H, block_size]) the attention weights that the
     queries ``q`` [B, H, T, D] give it: those of ``t < current_lengths[b]``, or of the last ``window`` of them.
     ``k_pool`` is a plain pool of q's type or a 4-bit one.  The sums go to ``out`` (default: ``key_weights`` itself),
-    whose other slots stay as they are; returns it."""
+    whose other slots stay as they are; returns it.  A page belongs to one sequence of the call."""
     what = "accumulate_key_weights"
     out = key_weights if out is None else out
     if _lib.calls().key_weights(q, k_pool, key_weights, page_table, seq_lens, current_lengths, window,

@@ -434,7 +434,8 @@ B2PA_API int b2pa_paged_prefill_kv4(const void* q, const int64_t q_strides[4],
  * seq_lens[b] - cur_lens[b] + t + 1) - 1, as in the attention.  weights_out
  * may be weights_in; slots that hold no key are left as they are.  pool_dtype:
  * dtype, or B2PA_DTYPE_KV4 for a 4-bit K pool.  A key whose block id is out of
- * range is not seen.
+ * range is not seen.  A page belongs to one sequence of the call: one that
+ * several list receives the sums of one of them.
  */
 B2PA_API size_t b2pa_key_weights_workspace_size(int B, int H, int T, int D, int max_pages,
                                        int block_size, int dtype, int pool_dtype);
