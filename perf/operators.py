@@ -14,7 +14,6 @@ infinity stores the NaN scale 255.  A page of one head holds the codes [block_si
 nibble), then the scales: [block_size, D / 16] in the K pool, [D / 16, block_size] in the V pool.  Pools are uint8
 [blocks, H, block_size, D * 9 / 16].
 """
-import functools
 import math
 import os
 import sys
@@ -28,7 +27,6 @@ DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
 SIZE = {"f32": 4, "bf16": 2, "f16": 2}
 
 
-@functools.lru_cache(maxsize=None)
 def _b2pa():
     path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "efficient-inference-system_b200")
     if path not in sys.path:
