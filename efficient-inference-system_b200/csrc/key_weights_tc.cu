@@ -142,21 +142,6 @@ __device__ __forceinline__ bool wait_or_stop(uint64_t* bar, uint32_t parity, int
   }
 }
 
-// Waits for a tmem_ld32.  The values are operands: no arithmetic on them, and
-// no copy of them, can be placed before the wait, when their registers are
-// still to be written.
-__device__ __forceinline__ void wait_ld(float (&v)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-      : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]),
-        "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]),
-        "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]), "+f"(v[17]),
-        "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]),
-        "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]),
-        "+f"(v[30]), "+f"(v[31])
-      :
-      : "memory");
-}
-
 // Rows 32 warp .. 32 warp + 31 of a tile as they lie (16-bit values): copied
 // asynchronously, complete when it returns.
 template <typename T, int D, typename Src>
@@ -293,12 +278,11 @@ __global__ void __launch_bounds__(kTcThreads, 2) key_weights_tc_kernel(KeyWeight
             const int64_t seen = q0 + c * kRows + mine + 1 - j0;  // keys of the tile that this query sees
 #pragma unroll 1
             for (int k = 0; k < 4; ++k) {
-              float v[32];
-              tc::tmem_ld32(acc + 32 * k, v);
               const int64_t left = seen - 32 * k;
               uint32_t mask = left >= 32 ? kFullMask : left <= 0 ? 0u : (1u << left) - 1u;
               mask &= key_mask[i % kLate][k];
-              wait_ld(v);
+              float v[32];
+              tc::tmem_ld32(acc + 32 * k, v);
               if constexpr (S::KSCALED) {
                 const float4* kb = reinterpret_cast<const float4*>(&key_back[i % kLate][32 * k]);
 #pragma unroll
@@ -351,13 +335,12 @@ __global__ void __launch_bounds__(kTcThreads, 2) key_weights_tc_kernel(KeyWeight
           float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
 #pragma unroll 1
           for (int k = 0; 32 * k < lanes; ++k) {
-            float v[32];
-            tc::tmem_ld32(acc + 32 * k, v);
             const int64_t before = first - 32 * k;  // queries of these 32 that do not see the key
             uint32_t mask = before <= 0 ? kFullMask : before >= 32 ? 0u : kFullMask << before;
             if (lanes - 32 * k < 32) mask &= (1u << (lanes - 32 * k)) - 1u;
             const bool all = __all_sync(kFullMask, mask == kFullMask);
-            wait_ld(v);
+            float v[32];
+            tc::tmem_ld32(acc + 32 * k, v);
             const float4* ls = reinterpret_cast<const float4*>(&q_lse[32 * k]);
             const float4* un = reinterpret_cast<const float4*>(&q_unit[32 * k]);
             if constexpr (S::KSCALED) {

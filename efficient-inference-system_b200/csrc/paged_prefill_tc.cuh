@@ -619,17 +619,7 @@ __global__ void __launch_bounds__(PfTcCfg<D, BS, kPfSplit<T>, HALVES>::THREADS, 
       tc::fence_after_sync();
       float s[64];
       const uint32_t tS = tmem + (uint32_t)slot * C::BN + trow;
-      {
-        float a[32], c[32];
-        tc::tmem_ld32(tS, a);
-        tc::tmem_ld32(tS + 32, c);
-        tc::tmem_wait_ld();
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          s[e] = a[e];
-          s[32 + e] = c[e];
-        }
-      }
+      tc::tmem_ld64(tS, s);
       const int64_t k0 = (int64_t)(j0 + j) * C::BN;
       bool all_pages = true;
       bool page_ok[C::PAGES];
@@ -724,7 +714,6 @@ __global__ void __launch_bounds__(PfTcCfg<D, BS, kPfSplit<T>, HALVES>::THREADS, 
         for (int cb = 0; cb < D / 32; ++cb) {
           float ov[32];
           tc::tmem_ld32(tO + g * D + trow + cb * 32, ov);
-          tc::tmem_wait_ld();
 #pragma unroll
           for (int e = 0; e < 32; ++e) ov[e] *= alpha;
           tc::tmem_st32(tO + g * D + trow + cb * 32, ov);
@@ -783,7 +772,6 @@ __global__ void __launch_bounds__(PfTcCfg<D, BS, kPfSplit<T>, HALVES>::THREADS, 
           if (gg >= ntiles) break;  // group without tiles: its O was never written
           float ov[32];
           tc::tmem_ld32(tO + gg * D + trow + c0 + cb * 32, ov);
-          tc::tmem_wait_ld();
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = NG > 1 ? fmaf(wgt[gg], ov[e], o[e]) : ov[e];
         }
