@@ -259,4 +259,13 @@ __device__ __forceinline__ float warp_sum(float v) {
 
 constexpr int ilog2(int x) { return x <= 1 ? 0 : 1 + ilog2(x / 2); }
 
+// A power of two that brings magnitudes up to `top` near 2^10, and its
+// inverse; 0, tiny, infinite and NaN maxima keep a finite factor.
+__device__ __forceinline__ float range_factor(float top, float& back) {
+  int e = 137 - (int)(__float_as_uint(top) >> 23);
+  e = e > 100 ? 100 : e;
+  back = __uint_as_float((uint32_t)(127 - e) << 23);
+  return __uint_as_float((uint32_t)(127 + e) << 23);
+}
+
 }  // namespace b2pa

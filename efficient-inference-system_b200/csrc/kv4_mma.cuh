@@ -46,15 +46,6 @@ __device__ __forceinline__ void split8(const float* x, float f, uint4& hi, uint4
   }
 }
 
-// A power of two that brings magnitudes up to `top` near 2^10, and its
-// inverse; 0, tiny, infinite and NaN maxima keep a finite factor.
-__device__ __forceinline__ float range_factor(float top, float& back) {
-  int e = 137 - (int)(__float_as_uint(top) >> 23);
-  e = e > 100 ? 100 : e;
-  back = __uint_as_float((uint32_t)(127 - e) << 23);
-  return __uint_as_float((uint32_t)(127 + e) << 23);
-}
-
 // One 4-bit word (8 channels of scale s) as 4 operand registers, exact, in
 // the order 0 4 1 5 2 6 3 7: a masked nibble pair in the mantissa is 1024 + c,
 // or 16 (64 + c) for the upper nibbles.

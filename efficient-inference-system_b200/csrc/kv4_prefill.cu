@@ -3,17 +3,18 @@
 // A prompt chunk of T queries makes 4 T L D operations of every L keys, so
 // its time is the tensor cores' and not the cache's.  Where the tcgen05 kernel
 // of the plain pools can do the rest (head_dim 64 and 128; else
-// kv4_prefill_mma.cu does it all), the pages that the call reads are written out in the workspace, in q's type or, for fp32, in fp16 (exact
-// either way: a stored value has 7 significant bits, so fp32 q needs two
-// products where fp32 pages need three), as a pool of B * max_pages blocks with
-// a table of their own, and that kernel runs on it; rows past a sequence's
-// length are written as zeros.
-// Two kinds of inputs are not for that kernel: fp32 queries of 2^15 and more,
-// which it splits into fp16 halves as they are, and NaN groups of V at keys
-// that only some of the chunk's queries see (a zero weight times NaN).  They
-// leave the call's number in a flag, and the kernel of kv4_prefill_mma.cu,
-// launched behind it, redoes the call if it finds it there.  The number is part
-// of a captured graph: once a replay has set it, later ones redo the call too.
+// kv4_prefill_mma.cu does it all), the pages that the call reads are written out
+// in the workspace, in q's type or, for fp32, in fp16 (exact either way: a stored
+// value has 7 significant bits, so fp32 q needs two products where fp32 pages
+// need three), as a pool of B * max_pages blocks with a table of their own, and
+// that kernel runs on it; rows past a sequence's length are written as zeros.
+// The workspace is thus a 16-bit copy of the call's pages, by the width of the
+// table: 3.6 times the 4-bit pages' bytes, for one layer at a time.
+// One kind of input is not for that kernel: NaN groups of V at keys that only
+// some of the chunk's queries see (a zero weight times NaN).  They leave the
+// call's number in a flag, and the kernel of kv4_prefill_mma.cu, launched behind
+// it, redoes the call if it finds it there.  The number is part of a captured
+// graph: once a replay has set it, later ones redo the call too.
 #include <atomic>
 
 #include "common.cuh"

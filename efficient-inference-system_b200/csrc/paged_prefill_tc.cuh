@@ -122,7 +122,12 @@ __device__ __forceinline__ void prefill_tile_range(const PfTcParams& p, int b, i
 // does nothing otherwise.  The K/V pages are split into a workspace copy
 // beforehand (prefill_split_pages_kernel); q and P are split in the kernel.
 // HALVES: fp32 q on K/V pages whose values fp16 holds exactly (they are fp16
-// in memory): their lo tiles, and the products with them, drop out.
+// in memory): their lo tiles, and the products with them, drop out.  Rows of q
+// are brought near 2^10 by powers of two before they are split, undone in the
+// softmax's scale: an unscaled lo half is a subnormal for |x| < 2^-3, off by
+// up to 2^-25, which keys of up to 64,512 multiply (1,000 unit normal keys
+// times 2^12, queries times 2^-12: 7e-5 of the output -> 5e-8).  So no query is
+// out of range, and one that is not finite spoils its own row alone, as it should.
 template <int D, int BS, bool SPLIT = false, bool HALVES = false>
 struct PfTcCfg {
   static constexpr int BM = 128;         // query rows per CTA (UMMA M)
@@ -137,7 +142,7 @@ struct PfTcCfg {
   // softmax warps on every SM sub-partition, so one warp's exponentials
   // overlap the other's TMEM loads, barrier waits and P stores.
   static constexpr int NG = D == 64 ? 2 : 1;
-  // S/P buffers: two per group; one per group for the fp32 variant, whose
+  // S/P buffers: two per group; one per group for fp32 with head_dim 64, whose
   // hi/lo operand tiles take twice the shared memory (its two groups still
   // alternate, so one group's softmax overlaps the other's Q.K^T).
   static constexpr int NSLOT = SPLIT && D == 64 ? NG : 2 * NG;
@@ -281,6 +286,7 @@ __global__ void __launch_bounds__(PfTcCfg<D, BS, kPfSplit<T>, HALVES>::THREADS, 
   const int t0 = (blockIdx.x / p.nsplit_max) * C::BM;
   const int h = blockIdx.y;
   const int b = blockIdx.z;
+  __shared__ float q_back[HALVES ? C::BM : 1];  // undoes the scaling of a row of q
   // Q rows -> 128B-swizzled K-major tile, zeros past T, by the softmax
   // threads (the fp32 variant: hi tile, then lo tile, with the range check);
   // consecutive threads read consecutive 16-byte pieces of a row.
@@ -301,10 +307,23 @@ __global__ void __launch_bounds__(PfTcCfg<D, BS, kPfSplit<T>, HALVES>::THREADS, 
           const float4 x0 = src[0], x1 = src[1];
           f[0] = x0.x; f[1] = x0.y; f[2] = x0.z; f[3] = x0.w;
           f[4] = x1.x; f[5] = x1.y; f[6] = x1.z; f[7] = x1.w;
-          bool in_range = true;
+          if constexpr (!HALVES) {
+            bool in_range = true;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) in_range = in_range && fabsf(f[e]) < kSplitRange;
-          if (!in_range) *p.range_flag = p.epoch;
+            for (int e = 0; e < 8; ++e) in_range = in_range && fabsf(f[e]) < kSplitRange;
+            if (!in_range) *p.range_flag = p.epoch;
+          }
+        }
+        if constexpr (HALVES) {  // D / 8 neighbouring lanes hold a row
+          float top = 0.f, back;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[e]));
+#pragma unroll
+          for (int o = D / 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, o));
+          const float up = range_factor(top, back);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[e] *= up;
+          if (qc == 0) q_back[qr] = back;
         }
         uint4 hi, lo;
         split_f16x8(f, hi, lo);
@@ -331,9 +350,10 @@ __global__ void __launch_bounds__(PfTcCfg<D, BS, kPfSplit<T>, HALVES>::THREADS, 
   if (!p.early) pdl_wait();
   pdl_launch_dependents();
   if constexpr (SPLIT) {
-    // an input out of the split's range was seen (pre-pass or another CTA):
-    // the CUDA-core kernel that follows recomputes the call.  One read,
-    // shared, so the whole CTA takes the same branch.
+    // an input out of the split's range was seen (pre-pass or another CTA; with
+    // HALVES one that this kernel does not take, by the kernel before it): the
+    // kernel that follows recomputes the call.  One read, shared, so the whole
+    // CTA takes the same branch.
     __shared__ int stop;
     if (tid == 0) stop = *reinterpret_cast<volatile uint32_t*>(p.range_flag) == p.epoch;
     __syncthreads();
@@ -598,7 +618,7 @@ __global__ void __launch_bounds__(PfTcCfg<D, BS, kPfSplit<T>, HALVES>::THREADS, 
     // store) is rare.  Rescaling at the group's i-th tile j waits for the
     // group's previous P.V (tile j - NG): o_full[g] completes one phase per
     // P.V of the group; the p_free wait before it makes P.V(j - NSLOT) done
-    // (NSLOT is 2*NG, or NG for the fp32 variant: then that is the group's
+    // (NSLOT is 2*NG, or NG for fp32 with head_dim 64: then that is the group's
     // previous P.V itself), and P.V(j) cannot start before this warp releases
     // P(j), so o_full[g] has completed i-1 or i phases and the parity wait
     // is exact.
@@ -606,7 +626,8 @@ __global__ void __launch_bounds__(PfTcCfg<D, BS, kPfSplit<T>, HALVES>::THREADS, 
     // Row maxima are taken on unscaled scores and scaled once (sc > 0); a
     // scale that is not positive is applied to the scores first instead.
     const bool pre_scale = !(p.scale_log2 > 0.f);
-    const float sc = pre_scale ? 1.f : p.scale_log2;
+    const float row_scale = HALVES ? p.scale_log2 * q_back[r] : p.scale_log2;
+    const float sc = pre_scale ? 1.f : row_scale;
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int j = g; j < ntiles; j += NG) {
@@ -635,7 +656,7 @@ __global__ void __launch_bounds__(PfTcCfg<D, BS, kPfSplit<T>, HALVES>::THREADS, 
       // unless it is not positive; invisible keys become -inf.
       if (pre_scale) {
 #pragma unroll
-        for (int e = 0; e < 64; ++e) s[e] *= p.scale_log2;
+        for (int e = 0; e < 64; ++e) s[e] *= row_scale;
       }
       if (lim < C::BN || !all_pages) {
 #pragma unroll

@@ -253,6 +253,31 @@ def test_fp32_precision(cuda_device, D, T):
     assert np.linalg.norm(_np(out)[0] - ref) <= 2.0 ** -19 * np.linalg.norm(ref)
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("T", [1, 60, 200])
+@pytest.mark.parametrize("p", [-9, 6, 9, 12])
+@pytest.mark.parametrize("lost", [False, True])
+def test_fp32_precision_of_unlike_magnitudes(cuda_device, D, T, p, lost):
+    """Queries times 2^-p on keys times 2^p: powers of two, which leave codes, logits and so the bound of
+    test_fp32_precision as they are.  A query's low half that is a subnormal shows (7e-5 for p = 12).  With ``lost``
+    the last row, which is padding, is not finite and stays alone."""
+    rng = np.random.default_rng(D)
+    H, bs, n = 2, 16, 1000
+    NB = -(-n // bs)
+    k, v = rng.standard_normal((NB, H, bs, D)) * 2.0 ** p, rng.standard_normal((NB, H, bs, D))
+    q = torch.from_numpy(rng.standard_normal((1, H, T, D)) * 2.0 ** -p).float().to(cuda_device)
+    live = T - 1 if lost and T > 1 else T
+    q[:, :, live:, 3] = float("inf")
+    fn = b2pa.paged_attention_decode_kv4 if T == 1 else b2pa.paged_attention_prefill_kv4
+    out = fn(q, torch.from_numpy(co.pack_pages(k, False)).to(cuda_device),
+             torch.from_numpy(co.pack_pages(v, True)).to(cuda_device), _i32(np.arange(NB)[None], cuda_device),
+             _i32([n], cuda_device), _i32([live], cuda_device))
+    w, _ = co.softmax_rows(_np(q)[0, :, :live], co.rows_of(co.stored(k), range(NB), n), live, D ** -0.5)
+    ref = np.einsum("htn,nhd->htd", w, co.rows_of(co.stored(v), range(NB), n))
+    assert np.linalg.norm(_np(out)[0, :, :live] - ref) <= 2.0 ** -19 * np.linalg.norm(ref)
+    assert torch.isnan(out[:, :, live:]).all()
+
+
 @pytest.mark.parametrize("dtype,D", [(torch.float32, 64), (torch.float32, 128), (torch.bfloat16, 256),
                                      (torch.float16, 128)])
 def test_prefill_long(cuda_device, dtype, D):
