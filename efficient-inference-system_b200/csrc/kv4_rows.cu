@@ -152,8 +152,10 @@ __global__ void __launch_bounds__(128) kv4_read_kernel(Kv4ReadArgs a) {
   pdl_wait();
   pdl_launch_dependents();
   const int t0 = blockIdx.x * TOKENS, b = blockIdx.y;
-  const Places<TOKENS> at(a.page_table + (int64_t)b * a.pt_stride, a.start_pos[b], t0, a.lengths[b], a.bs_log2,
-                          a.max_pages, a.num_blocks, a.status);
+  int len = a.lengths[b];
+  len = len < a.T ? len : a.T;
+  const Places<TOKENS> at(a.page_table + (int64_t)b * a.pt_stride, a.start_pos[b], t0, len, a.bs_log2, a.max_pages,
+                          a.num_blocks, a.status);
   // a thread reads one word of K and of V per token, so that a warp's stores
   // are contiguous (whole groups per thread: 61 us where this takes 40)
   const int wpr_log2 = 31 - __clz(a.D / 8);

@@ -313,6 +313,22 @@ def test_append_many_is_append_one_by_one(cuda_device, dtype, D, bs, H):
         assert np.array_equal(_np(got), np.where(live, co.stored(_np(x)), 0))
 
 
+@pytest.mark.parametrize("B", [2, 9])
+def test_read_of_lengths_past_its_slots(cuda_device, B):
+    """Lengths above T are T, for an odd number of slots whose table ends with the last one; one or two tokens a CTA."""
+    rng = np.random.default_rng(B)
+    T, D, bs, H, pages = 143, 64, 16, 2, 9  # positions 1 .. 143
+    kp, vp, k, v = _pools(rng, B * pages, H, bs, D)
+    table = np.arange(B * pages).reshape(B, pages)
+    out = b2pa.kv4_read(torch.from_numpy(kp).to(cuda_device), torch.from_numpy(vp).to(cuda_device),
+                        _i32(table, cuda_device), _i32([1] * B, cuda_device), _i32([T + 1, 500] + [T] * (B - 2), cuda_device),
+                        T, torch.float32)
+    for got, x in zip(out, (k, v)):
+        want = [co.rows_of(x, ids, pages * bs)[1:].transpose(1, 0, 2) for ids in table]
+        assert np.array_equal(_np(got), np.stack(want))
+    assert b2pa.read_status(cuda_device) == 0
+
+
 def test_decode_offsets_past_32_bits(cuda_device):
     """Pages at byte offsets past 2^32 of the pool."""
     H, D, bs = 8, 128, 32
