@@ -143,6 +143,14 @@ def note_released_rows(cache, device: torch.device) -> None:
         mark_shrunk_rows(ent)
 
 
+def device_lengths(t: torch.Tensor, B: int) -> torch.Tensor:
+    """Lengths that the caller holds on the device as the kernels read them: ``B`` int32 values in a row, whatever the
+    tensor's type and strides (a column, one expanded value)."""
+    if t.numel() != B:
+        raise ValueError(f"b2pa: {B} lengths are needed, not a tensor of shape {tuple(t.shape)}")
+    return t.to(torch.int32).contiguous()
+
+
 def block_table_and_lengths(cache, device: torch.device, extra: list[list[int]] | None = None,
                             transient: bool = False):
     """Returns ``(page_table, seq_lens, *extras, max_pages)`` as int32 device

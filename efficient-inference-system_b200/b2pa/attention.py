@@ -21,7 +21,7 @@ import math
 import torch
 
 from . import _lib
-from ._metadata import block_table_and_lengths
+from ._metadata import block_table_and_lengths, device_lengths
 from .eviction import accumulate_from
 from .kv4 import _attend as _attend_kv4
 from .paged_kv import _kv_append, flush_pending, take_pending
@@ -46,8 +46,8 @@ def _attn_call(fn_name: str, q, k_pool, v_pool, page_table, seq_lens, current_le
     if page_table.numel() and page_table.stride(1) != 1:
         page_table = page_table.contiguous()
     pt_stride = page_table.stride(0) if page_table.dim() == 2 and page_table.numel() else max(max_pages, 1)
-    seq_lens = seq_lens.to(dtype=torch.int32)
-    cur = current_lengths.to(dtype=torch.int32)
+    seq_lens = device_lengths(seq_lens, B)
+    cur = device_lengths(current_lengths, B)
     dev = q.device
     dt = _lib.dtype_code(q.dtype)
     lib = _lib.load()
@@ -130,7 +130,7 @@ def paged_attention(backend: str, q: torch.Tensor, kv_cache, current_lengths) ->
 def _attention_now(q: torch.Tensor, kv_cache, current_lengths, host_cur, pool, pend) -> torch.Tensor:
     """paged_attention outside a DecodeStep."""
     dev = q.device
-    T = q.shape[2]
+    B, _, T, _ = q.shape
     if pend is not None:
         if (pend.cache is kv_cache and pend.k_new.shape[2] == T and pend.k_new.device == dev
                 and pool.k_blocks.dtype == q.dtype):
@@ -146,7 +146,7 @@ def _attention_now(q: torch.Tensor, kv_cache, current_lengths, host_cur, pool, p
         page_table, seq_lens, cur, max_pages = block_table_and_lengths(kv_cache, dev, [host_cur], transient=True)
     else:
         page_table, seq_lens, max_pages = block_table_and_lengths(kv_cache, dev, transient=True)
-        cur = current_lengths.to(dtype=torch.int32)
+        cur = device_lengths(current_lengths, B)
     if pool.k_blocks.dtype == torch.uint8:
         name = "paged_attention_decode_kv4" if T == 1 else "paged_attention_prefill_kv4"
         return _attend_kv4(name, q, pool.k_blocks, pool.v_blocks, page_table, seq_lens, cur, max_pages)
@@ -168,7 +168,7 @@ def _decode_with_append(q, kv_cache, current_lengths, host_cur, pend) -> torch.T
     else:
         page_table, seq_lens, start_t, len_t, max_pages = block_table_and_lengths(
             kv_cache, dev, [pend.starts, pend.lengths], transient=True)
-        cur = current_lengths.to(dtype=torch.int32)
+        cur = device_lengths(current_lengths, B)
     out = torch.empty_like(q)
     dt = _lib.dtype_code(q.dtype)
     lib = _lib.load()
@@ -212,7 +212,7 @@ def _prefill_with_append(q, kv_cache, current_lengths, host_cur, pend) -> torch.
     else:
         page_table, seq_lens, start_t, len_t, max_pages = block_table_and_lengths(
             kv_cache, dev, [pend.starts, pend.lengths], transient=True)
-        cur = current_lengths.to(dtype=torch.int32)
+        cur = device_lengths(current_lengths, B)
     out = torch.empty_like(q)
     dt = _lib.dtype_code(q.dtype)
     lib = _lib.load()

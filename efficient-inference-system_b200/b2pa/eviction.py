@@ -148,14 +148,14 @@ def evict_by_weight(k_pool: torch.Tensor, v_pool: torch.Tensor, key_weights: tor
 # ------------------------------------------------------------- cache objects
 def accumulate_from(kv_cache, q: torch.Tensor, current_lengths) -> None:
     """Adds the weights of ``q`` to the sums of ``kv_cache``'s pool, which tracks them (paged_attention calls this)."""
-    from ._metadata import block_table_and_lengths
+    from ._metadata import block_table_and_lengths, device_lengths
 
     pool = kv_cache.pool
     dev = q.device
-    T = q.shape[2]
+    B, _, T, _ = q.shape
     if isinstance(current_lengths, torch.Tensor) and current_lengths.is_cuda:
         table, seq_lens, pages = block_table_and_lengths(kv_cache, dev, transient=True)
-        cur = current_lengths.to(torch.int32)
+        cur = device_lengths(current_lengths, B)
     else:
         if current_lengths is None:
             row = T

@@ -494,6 +494,40 @@ def test_run_of_steps(cuda_device, kv4, fused):
     assert b2pa.read_status(dev) == 0
 
 
+@pytest.mark.parametrize("kv4", [False, True], ids=["plain", "kv4"])
+@pytest.mark.parametrize("fused", [False, True])
+@pytest.mark.parametrize("T", [1, 6])
+def test_device_lengths_of_any_layout(cuda_device, kv4, fused, T):
+    """Current lengths on the device as a column, as one expanded value and in 64 bits: outputs and key weights are
+    those of the plain tensor."""
+    dev, H, D, B = cuda_device, 2, 64, 3
+    rng = np.random.default_rng(T)
+    prompt, q, k, v = (torch.from_numpy(rng.standard_normal((B, H, n, D))).float().to(dev) for n in (9, T, T, T))
+    base = torch.full((B,), max(1, T - 2), dtype=torch.int32, device=dev)
+    column = torch.stack([base, torch.full_like(base, 77)], 1)[:, 0]
+    expanded = base[:1].expand(B)
+    got = []
+    prev = b2pa.set_fused_append(fused)
+    try:
+        for lengths in (base, column, expanded, base.long(), column.long()):
+            pool = (b2pa.Kv4BlockPool if kv4 else b2pa.LayerBlockPool)(16, 8, 2.0)
+            pool.track_key_weights()
+            cache = b2pa.BatchedPagedKVCache([b2pa.PagedKVCacheState(pool) for _ in range(B)], pool)
+            cache.append_batch(prompt, prompt, [9, 5, 7])
+            b2pa.paged_attention("b200_paged", prompt, cache, [9, 5, 7])
+            cache.append_batch(k, v, lengths)
+            got.append((b2pa.paged_attention("b200_paged", q, cache, lengths), pool.key_weights))
+    finally:
+        b2pa.set_fused_append(prev)
+    for out, weights in got[1:]:
+        assert torch.equal(out, got[0][0]) and torch.equal(weights, got[0][1])
+    with pytest.raises(ValueError, match="lengths"):
+        b2pa.paged_attention("b200_paged", q, cache, base[:2])
+    with pytest.raises(ValueError):
+        b2pa.paged_attention("b200_paged", q, cache, base[:1].expand(B, B))
+    assert b2pa.read_status(dev) == 0
+
+
 def _model(dev, kv4):
     made = []
 

@@ -300,3 +300,16 @@ def test_install_into_reference_rebinds_and_restores(tmp_path, monkeypatch):
         assert pk._fused_append is False
     finally:
         b2pa.set_fused_append(prev)
+
+
+def test_device_lengths_are_values_in_a_row():
+    """A column and an expanded value come as the values that they stand for, in int32 and contiguous."""
+    from b2pa._metadata import device_lengths
+
+    x = torch.tensor([[3, 9], [4, 9], [5, 9]], dtype=torch.int32)
+    for t, want in ((x[:, 0], [3, 4, 5]), (x[0, :1].expand(3), [3, 3, 3]), (x[:, 0].long(), [3, 4, 5]),
+                    (x[:, :1], [3, 4, 5])):
+        got = device_lengths(t, 3)
+        assert got.is_contiguous() and got.dtype == torch.int32 and got.flatten().tolist() == want
+    with pytest.raises(ValueError):
+        device_lengths(x[0], 3)
