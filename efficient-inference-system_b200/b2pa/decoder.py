@@ -181,6 +181,11 @@ class FusedDecodeExecutor:
         M = len(requests)
         n_layers = len(self.decoder.layers)
         layer_states = [[r.kv_caches[l] for r in requests] for l in range(n_layers)]
+        if self.evict_keep is not None and any(getattr(states[0].pool, "key_weights", None) is None
+                                               for states in layer_states):
+            # (before anything moves: layers evicted without the others would be out of step for good)
+            raise RuntimeError("b2pa.FusedDecodeExecutor: evict_keep needs pools that track key weights in every layer "
+                               "(pool.track_key_weights())")
         batches = [BatchedPagedKVCache(states=states, pool=states[0].pool) for states in layer_states]
         torch.cuda.synchronize(self.device)
         t0 = time.perf_counter()

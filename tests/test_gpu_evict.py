@@ -612,3 +612,34 @@ def test_executor_bounds_every_cache(cuda_device):
     assert len(done) == 4 and all(len(r.generated_token_ids) == 40 for r in done)
     assert longest and max(longest) < 48 + 8
     assert b2pa.read_status(dev) == 0
+
+
+@torch.no_grad()
+def test_executor_refuses_layers_that_do_not_track(cuda_device):
+    """A layer that does not track key weights is refused before the step: nothing has moved, and with the layers in
+    step the same requests go on without eviction."""
+    from oracle import serving as osv
+
+    dev = cuda_device
+    model = _model(dev, False)
+    ex = osv.ModelExecutors(model, dev)
+    reqs = osv.generate_requests(2, 1000.0, 300, [osv.WorkloadProfile("x", 60, 60, 20, 20, 1.0)], seed=2)
+    bounded = b2pa.FusedDecodeExecutor(model, dev, max_batch=2, evict_keep=32, evict_slack=1)
+    free = b2pa.FusedDecodeExecutor(model, dev, max_batch=2)
+    refused = []
+
+    def step(requests, *args, **kw):
+        pool = requests[0].kv_caches[1].pool
+        pool.key_weights = None  # the second layer stops tracking
+        before = [(s.seq_len, list(s.block_ids)) for r in requests for s in r.kv_caches]
+        tokens = [list(r.generated_token_ids) for r in requests]
+        with pytest.raises(RuntimeError, match="track"):
+            bounded(requests, *args, **kw)
+        assert before == [(s.seq_len, list(s.block_ids)) for r in requests for s in r.kv_caches]
+        assert tokens == [list(r.generated_token_ids) for r in requests]
+        refused.append(1)
+        return free(requests, *args, **kw)
+
+    done, _ = osv.ContinuousScheduler(2, 128, 512).run(reqs, ex.prefill, step, ex.release)
+    assert refused and len(done) == 2 and all(len(r.generated_token_ids) == 20 for r in done)
+    assert b2pa.read_status(dev) == 0
