@@ -184,8 +184,10 @@ def evict_batch(cache, keep: int, recent: int = 0) -> torch.Tensor:
         raise RuntimeError("b2pa: a batch cannot be evicted inside an open DecodeStep")
     if keep < 1 or recent < 0:
         raise ValueError(f"b2pa: keep must be at least 1 and recent not negative, got {keep} and {recent}")
-    if getattr(pool, "key_weights", None) is None:
+    if not getattr(pool, "_tracks_weights", False):
         raise RuntimeError("b2pa: the pool does not track key weights (call pool.track_key_weights() first)")
+    if pool.k_blocks is None:
+        raise RuntimeError("b2pa: nothing to evict from: the pool has no blocks before its first append")
     states = cache.states
     if any(s.pool is not pool for s in states):
         raise ValueError("b2pa: all states of a BatchedPagedKVCache must share its pool")

@@ -163,6 +163,19 @@ def test_kv4_pool_bookkeeping_on_meta():
     assert cache.live_bytes() == 40 * 3 * 72 * 2
 
 
+def test_evicting_before_the_first_append():
+    """A pool that tracks and holds nothing is told from one that does not track."""
+    import b2pa
+
+    pool = b2pa.LayerBlockPool(16, 2, 2.0)
+    cache = b2pa.BatchedPagedKVCache([b2pa.PagedKVCacheState(pool)], pool)
+    with pytest.raises(RuntimeError, match="does not track"):
+        cache.evict(4)
+    pool.track_key_weights()
+    with pytest.raises(RuntimeError, match="before its first append"):
+        cache.evict(4)
+
+
 def test_oracle_quantiser():
     rng = np.random.default_rng(0)
     x = (rng.standard_normal((64, 128)) * np.exp(rng.uniform(-12, 12, (64, 1)))).astype(np.float32)
