@@ -294,9 +294,10 @@ __global__ void __launch_bounds__(kTcThreads, 2) key_weights_tc_kernel(KeyWeight
                   v[4 * x + 3] *= y.w;
                 }
               }
-              if (unit < 0.f) {  // (a negative scale: so that the largest product is the largest logit)
+              if (!(unit > 0.f)) {  // (a scale that is not positive: the largest product shall be the largest logit)
+                const float sign = unit < 0.f ? -1.f : 0.f;
 #pragma unroll
-                for (int x = 0; x < 32; ++x) v[x] = -v[x];
+                for (int x = 0; x < 32; ++x) v[x] *= sign;
               }
               if (__any_sync(kFullMask, mask != kFullMask)) {
 #pragma unroll
@@ -309,9 +310,8 @@ __global__ void __launch_bounds__(kTcThreads, 2) key_weights_tc_kernel(KeyWeight
                 top2 = fmax3(v[x + 2], v[x + 3], top2);
               }
               top = fmax3(v[30], v[31], fmaxf(top, top2));
-              // m, in logits; a product of -inf (hidden) times a unit of 0 stays hidden
-              const float size = fabsf(unit);
-              top = fmaxf(m, top == -INFINITY ? -INFINITY : top * size);
+              const float size = unit != 0.f ? fabsf(unit) : 1.f;  // (hidden ones, at -inf, stay so)
+              top = fmaxf(m, top * size);  // m, in logits
               const float ref = top == -INFINITY ? 0.f : top;
               const float2 u2 = make_float2(size, size), r2 = make_float2(-ref, -ref);
               float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;

@@ -643,3 +643,57 @@ def test_executor_refuses_layers_that_do_not_track(cuda_device):
     done, _ = osv.ContinuousScheduler(2, 128, 512).run(reqs, ex.prefill, step, ex.release)
     assert refused and len(done) == 2 and all(len(r.generated_token_ids) == 20 for r in done)
     assert b2pa.read_status(dev) == 0
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 0.2])
+@pytest.mark.parametrize("T", [1, 5, 140])
+@pytest.mark.parametrize("kind,D", [("f32", 64), ("f32", 128), ("bf16", 64), ("f16", 128), ("f32", 32), ("bf16", 16),
+                                    ("kv4", 64), ("kv4", 128), ("kv4", 256)])
+def test_any_scale(cuda_device, scale, T, kind, D):
+    """The C entries' scale may be zero (every visible key counts alike) or negative: key weights, and on 4-bit pools
+    the attention."""
+    dev, H, bs, n = cuda_device, 2, 16, 173
+    rng = np.random.default_rng(D + T)
+    NB = -(-n // bs)
+    dtype = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16, "kv4": torch.float32}[kind]
+    k, v = rng.standard_normal((2, NB, H, bs, D))
+    if kind == "kv4":
+        pool, vpool = (torch.from_numpy(co.pack_pages(x, y)).to(dev) for x, y in ((k, False), (v, True)))
+        k, v = co.stored(k), co.stored(v)
+    else:
+        pool = torch.from_numpy(k).to(dtype).to(dev)
+        k = _np(pool)
+    q = torch.from_numpy(rng.standard_normal((1, H, T, D))).to(dtype).to(dev)
+    w = torch.zeros(NB, H, bs, device=dev)
+    table, lens, cur = _i32(np.arange(NB)[None], dev), _i32([n], dev), _i32([T], dev)
+    code = b2pa._lib.dtype_code(dtype)
+    pool_code = b2pa._lib.DTYPE_KV4 if kind == "kv4" else code
+    lib, status, stream = b2pa._lib.load(), b2pa._lib.status_buffer(dev).data_ptr(), b2pa._lib.stream_handle(dev)
+    ws = torch.empty(lib.b2pa_key_weights_workspace_size(1, H, T, D, NB, bs, code, pool_code) + 256, dtype=torch.uint8,
+                     device=dev)
+    strides = b2pa._lib.strides4(q)
+    assert 0 == lib.b2pa_key_weights(q.data_ptr(), strides, pool.data_ptr(), pool_code, NB, table.data_ptr(), NB, NB,
+                                     lens.data_ptr(), cur.data_ptr(), 0, w.data_ptr(), w.data_ptr(), 1, H, T, D, bs,
+                                     scale, code, ws.data_ptr(), ws.numel(), status, stream)
+    K = co.rows_of(k, range(NB), n)
+    p, _ = co.softmax_rows(_np(q)[0] * np.sign(scale), K, T, abs(scale))
+    size = abs(scale) * float(np.einsum("htd,nhd->htn", np.abs(_np(q)[0]), np.abs(K)).max())
+    got = co.rows_of(_np(w)[..., None], range(NB), n)[..., 0].T
+    want = p.sum(1)
+    assert (np.abs(got - want) <= want * (co.weight_error(D, size, n) + (T + 2) * 2.0 ** -23) + 2.0 ** -30).all()
+    if kind != "kv4":
+        return
+    out = torch.empty_like(q)
+    if T == 1:
+        assert 0 == lib.b2pa_paged_decode_kv4(
+            q.data_ptr(), strides, pool.data_ptr(), vpool.data_ptr(), NB, table.data_ptr(), NB, NB, lens.data_ptr(),
+            cur.data_ptr(), out.data_ptr(), strides, 1, H, D, bs, scale, code, status, stream)
+    else:
+        ws = torch.empty(lib.b2pa_paged_prefill_kv4_workspace_size(1, H, T, D, NB, bs, code) + 256, dtype=torch.uint8,
+                         device=dev)
+        assert 0 == lib.b2pa_paged_prefill_kv4(
+            q.data_ptr(), strides, pool.data_ptr(), vpool.data_ptr(), NB, table.data_ptr(), NB, NB, lens.data_ptr(),
+            cur.data_ptr(), out.data_ptr(), strides, 1, H, T, D, bs, scale, code, ws.data_ptr(), ws.numel(), status, stream)
+    V = co.rows_of(v, range(NB), n)
+    ref = np.einsum("htn,nhd->htd", p, V)
+    assert (np.abs(_np(out)[0] - ref) <= co.output_bound(ref, 2.0 ** -24, D, size, n, np.abs(V).max())).all()
