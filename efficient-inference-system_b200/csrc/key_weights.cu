@@ -500,6 +500,7 @@ struct StepRows {
   static constexpr int LPR = RB / 16 < 32 ? RB / 16 : 32, CPL = RB / 16 / LPR, RP = 32 / LPR, R = 8 / CPL;
   static constexpr int PACKED = D == 256 ? 1 : 2;  // 16-row tiles of 4-bit rows per turn
   static constexpr int RW = KV4 ? 16 * PACKED : MMA ? 16 * TILES : RP * R;  // rows per warp and turn
+  static constexpr bool ORDERS = KV4 || !MMA || D != 256;  // by length, where that pays (by_length.cuh)
 };
 
 template <typename T, bool KV4, int D>
@@ -514,7 +515,7 @@ __global__ void __launch_bounds__(kStepThreads, KV4 ? 3 : 0) key_weights_step_ke
   pdl_wait();
   pdl_launch_dependents();
   const int ns = gridDim.x, rank = blockIdx.x, h = blockIdx.y;
-  const int b = by_length ? nth_longest(a.seq_lens, gridDim.z, blockIdx.z) : (int)blockIdx.z;
+  const int b = S::ORDERS && by_length ? nth_longest(a.seq_lens, gridDim.z, blockIdx.z) : (int)blockIdx.z;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Span s = span_of(a, b);
   if (rank == 0 && h == 0 && tid == 0 && (int64_t)a.seq_lens[b] > s.L) set_status(a.status, B2PA_ERR_BAD_BLOCK_ID);
@@ -822,7 +823,15 @@ int step_launch(const KeyWeightArgs& a, cudaStream_t st) {
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  const int by_length = orders_by_length(a.B, (int64_t)ns * a.H * a.B, 2);
+  // CTAs on an SM: by registers (64 a thread, else 80)
+  using S = StepRows<T, KV4, D>;
+  constexpr bool ROWS32 = !KV4 && sizeof(T) == 4, ROWS16 = !KV4 && !ROWS32;
+  const int by_length = S::ORDERS && orders_by_length(a.B, (int64_t)ns * a.H * a.B, ROWS32 && D != 128 ? 4 : 3, keys / ns,
+                                                      ROWS32 ? 256 : 512,
+                                                      ROWS32                ? 150
+                                                      : !ROWS16 || D == 128 ? 800
+                                                      : D == 64             ? 2600
+                                                                            : 1200);
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a, a.scale * kLog2e,
                                            far ? static_cast<float*>(a.workspace) : static_cast<float*>(nullptr), keys,
                                            by_length);

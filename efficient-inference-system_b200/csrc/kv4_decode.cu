@@ -543,7 +543,8 @@ static int decode_launch(const AttnArgs& a, int ns, cudaStream_t s) {
   p.H = a.H;
   p.qscale = a.scale * kLog2e;
   p.status = a.status;
-  p.by_length = orders_by_length(a.B, (int64_t)ns * a.H * a.B, 2);
+  p.by_length = orders_by_length(a.B, (int64_t)ns * a.H * a.B, 2, (int64_t)a.max_pages * BS / ns, 512,
+                                 D == 64 ? 900 : D == 128 ? 650 : 350);
   constexpr int smem = C::WARPS * kStages * C::BYTES;
   auto kern = kv4_decode_kernel<T, D, BS, W>;
   const int rc = set_max_dynamic_smem_cached(reinterpret_cast<const void*>(kern), smem);

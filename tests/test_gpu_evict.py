@@ -127,6 +127,19 @@ def test_key_weights_many_queries(cuda_device, dtype, kv4, D):
                       dtype=dtype, kv4=kv4, window=window, seed=T + window)
 
 
+@pytest.mark.parametrize("longest", [200, 600])
+@pytest.mark.parametrize("dtype,kv4,D", [(torch.float32, False, 64), (torch.bfloat16, True, 64),
+                                         (torch.bfloat16, False, 128), (torch.float16, False, 256),
+                                         (torch.float16, False, 32)])
+def test_key_weights_of_many(cuda_device, dtype, kv4, D, longest):
+    """More CTAs than the GPU holds at once, with and without the order by length; equal lengths and empty ones."""
+    rng = np.random.default_rng(longest)
+    lens = rng.integers(longest // 8, longest, 64).tolist()
+    lens[5:9] = [longest] * 4
+    lens[20:23], lens[63] = [0, 1, 0], longest
+    _weights_case(cuda_device, lens=lens, cur=[1] * 64, T=1, H=10, D=D, bs=16, dtype=dtype, kv4=kv4, window=0, seed=7)
+
+
 @pytest.mark.parametrize("kv4", [False, True])
 @pytest.mark.parametrize("T", [1, 3])
 def test_key_weights_wide_table(cuda_device, kv4, T):

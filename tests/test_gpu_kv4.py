@@ -231,6 +231,19 @@ def test_decode_long(cuda_device, dtype, B, L):
     _check(out, ref, bound)
 
 
+@pytest.mark.parametrize("dtype,D,H,longest", [(torch.float32, 64, 8, 1040), (torch.bfloat16, 128, 8, 700),
+                                               (torch.float16, 256, 6, 600), (torch.bfloat16, 64, 8, 500)])
+def test_decode_of_many(cuda_device, dtype, D, H, longest):
+    """More CTAs than the GPU holds at once, with and without the order by length; equal lengths and empty ones."""
+    rng = np.random.default_rng(longest)
+    lens = rng.integers(longest // 8, longest, 64).tolist()
+    lens[5:9] = [longest] * 4
+    lens[20:23], lens[63] = [0, 1, 0], longest
+    out, ref, bound, _ = _attend_case(cuda_device, lens=lens, cur=[1] * 64, H=H, D=D, bs=16, dtype=dtype, T=1, seed=D)
+    _check(out, ref, bound)
+    assert b2pa.read_status(cuda_device) == 0
+
+
 @pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("T", [1, 60])
 def test_fp32_precision(cuda_device, D, T):
