@@ -109,18 +109,38 @@ def load() -> ctypes.CDLL:
 _calls = None
 
 
+def calls_path() -> Path:
+    """Where the extension module for the running PyTorch and Python lies: it uses PyTorch's C++ classes, so one built
+    for another version must not be loaded."""
+    import sysconfig
+
+    import torch
+
+    return LIB_PATH.with_name(f"b2pa_calls.torch-{torch.__version__}.{sysconfig.get_config_var('SOABI')}.so")
+
+
+class _NoCalls:
+    """In the extension module's place: takes no call."""
+
+    def __getattr__(self, name):
+        return lambda *args: NotImplemented
+
+
 def calls():
     """The extension module of csrc/py_calls.cpp: the cache-compression calls on arguments that need no conversion
-    (it returns NotImplemented for others)."""
+    (it returns NotImplemented for others).  Without it every call goes the longer way through ctypes."""
     global _calls
     if _calls is None:
         import importlib.machinery
         import importlib.util
+        import warnings
 
-        path = LIB_PATH.with_name("b2pa_calls.so")
+        path = calls_path()
         if not path.exists():
-            raise RuntimeError(f"b2pa_calls.so not found at {path}; build it with `python -m b2pa.build` "
-                               "(or __graft_entry__.build()).")
+            warnings.warn(f"b2pa: {path.name} is not built; 4-bit and eviction calls cost some 10 us more of host time "
+                          "each (build it with `python -m b2pa.build`)", RuntimeWarning, stacklevel=2)
+            _calls = _NoCalls()
+            return _calls
         loader = importlib.machinery.ExtensionFileLoader("b2pa_calls", str(path))
         module = importlib.util.module_from_spec(importlib.util.spec_from_file_location("b2pa_calls", path, loader=loader))
         loader.exec_module(module)

@@ -1,5 +1,6 @@
 """Builds libb2pa.so in-tree with nvcc for sm_100a, and the Python extension
-b2pa_calls.so (csrc/py_calls.cpp) with the host compiler.
+b2pa_calls (csrc/py_calls.cpp) with the host compiler, for the PyTorch and
+Python that run the build: its file is named after both.
 
 Usage: ``python -m b2pa.build [--force] [-j N]`` (with the package directory on
 ``sys.path``) or ``b2pa.build.build()``.  Objects go to ``<pkg>/build/``, the
@@ -23,7 +24,6 @@ INCLUDE = REPO_DIR / "include"
 BUILD_DIR = PKG_DIR / "build"
 LIB_DIR = PKG_DIR / "lib"
 LIB_PATH = LIB_DIR / "libb2pa.so"
-CALLS_PATH = LIB_DIR / "b2pa_calls.so"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 CFLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-O3",
@@ -69,13 +69,16 @@ def _build_calls(force: bool) -> None:
 
     import torch
 
+    from . import _lib
+
+    path = _lib.calls_path()
     src = CSRC / "py_calls.cpp"
     newest = max(src.stat().st_mtime, (INCLUDE / "b2pa.h").stat().st_mtime)
-    if not force and CALLS_PATH.exists() and CALLS_PATH.stat().st_mtime > newest:
+    if not force and path.exists() and path.stat().st_mtime > newest:
         return
     torch_dir = Path(torch.__file__).resolve().parent
     cuda_home = Path(_nvcc()).parent.parent
-    tmp = CALLS_PATH.with_suffix(".so.tmp")
+    tmp = path.with_suffix(".so.tmp")
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{torch_dir}/include",
            f"-I{torch_dir}/include/torch/csrc/api/include", f"-I{sysconfig.get_paths()['include']}",
@@ -84,14 +87,15 @@ def _build_calls(force: bool) -> None:
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError(f"{src.name} failed:\n{' '.join(cmd)}\n{proc.stdout}\n{proc.stderr}")
-    os.replace(tmp, CALLS_PATH)
+    for old in LIB_DIR.glob("b2pa_calls*.so"):  # of another PyTorch or Python
+        old.unlink()
+    os.replace(tmp, path)
 
 
 def build(force: bool = False, jobs: int | None = None, verbose: bool = False, ptxas_info: bool = False) -> Path:
-    """Compiles every csrc/*.cu for sm_100a and links lib/libb2pa.so; builds lib/b2pa_calls.so."""
+    """Compiles every csrc/*.cu for sm_100a and links lib/libb2pa.so; then builds lib/b2pa_calls.*.so."""
     BUILD_DIR.mkdir(exist_ok=True)
     LIB_DIR.mkdir(exist_ok=True)
-    _build_calls(force)
     srcs = _sources()
     newest_header = max((h.stat().st_mtime for h in _headers()), default=0.0)
     extra = ["-Xptxas", "-v"] if ptxas_info else []
@@ -114,6 +118,7 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False, p
         if proc.returncode != 0:
             raise RuntimeError(f"link failed:\n{' '.join(cmd)}\n{proc.stdout}\n{proc.stderr}")
         os.replace(tmp, LIB_PATH)
+    _build_calls(force)
     return LIB_PATH
 
 

@@ -195,6 +195,18 @@ def test_oracle_quantiser():
     assert np.isnan(r[0]).all() and np.isnan(r[2]).all() and np.isfinite(np.delete(r, [0, 2], 0)).all()
 
 
+def test_extension_module_is_the_running_pytorchs(lib, monkeypatch):
+    """A module built for another PyTorch is not loaded: a warning, and every call is declined to the longer way."""
+    assert torch.__version__ in _lib.calls_path().name and _lib.calls_path().exists()
+    assert _lib.calls().__file__ == str(_lib.calls_path())
+    monkeypatch.setattr(torch, "__version__", "0.0.1")
+    monkeypatch.setattr(_lib, "_calls", None)
+    with pytest.warns(RuntimeWarning, match="not built"):
+        calls = _lib.calls()
+    assert calls.kv4_append(1, 2) is NotImplemented and calls.set_status(0, 0) is NotImplemented
+    assert _lib.calls() is calls
+
+
 def test_short_calls_decline(lib):
     """The extension module's functions launch nothing and raise nothing on what they do not take: CPU tensors, other
     objects, missing arguments."""
