@@ -11,7 +11,7 @@ import b2pa
 from oracle import model as om
 from tests import _compress_oracle as co
 from tests._helpers import random_tables
-from tests.test_gpu_kv4 import DTYPES, _i32, _np, _rows, _table
+from tests.test_gpu_kv4 import DTYPES, HALF_STEP, _i32, _np, _rows, _table
 
 pytestmark = pytest.mark.gpu
 
@@ -538,6 +538,85 @@ def test_device_lengths_of_any_layout(cuda_device, kv4, fused, T):
         b2pa.paged_attention("b200_paged", q, cache, base[:2])
     with pytest.raises(ValueError):
         b2pa.paged_attention("b200_paged", q, cache, base[:1].expand(B, B))
+    assert b2pa.read_status(dev) == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,bs", [(64, 8), (128, 16), (256, 32)])
+def test_run_on_4_bit_pools_of_every_type(cuda_device, dtype, D, bs):
+    """The cache objects on 4-bit pools for rows of every type and width: a ragged prompt, decode steps with and
+    without a DecodeStep, an eviction, a second chunk; outputs and key weights against 64-bit bookkeeping."""
+    dev, H, B = cuda_device, 2, 3
+    rng = np.random.default_rng(D)
+    pool = b2pa.Kv4BlockPool(bs, 4, 1.5)
+    pool.track_key_weights()
+    states = [b2pa.PagedKVCacheState(pool) for _ in range(B)]
+    K = [np.zeros((0, H, D)) for _ in range(B)]
+    V = [np.zeros((0, H, D)) for _ in range(B)]
+    W = [np.zeros((H, 0)) for _ in range(B)]
+    err = [0.0] * B
+
+    def step(lengths, T):
+        cache = b2pa.BatchedPagedKVCache(states, pool)
+        q, k, v = (torch.from_numpy(rng.standard_normal((B, T, H, D))).to(dtype).to(dev).transpose(1, 2)
+                   for _ in range(3))
+        cache.append_batch(k, v, lengths)
+        out = b2pa.paged_attention("b200_paged", q, cache, lengths)
+        assert out.dtype == dtype and pool.k_blocks.dtype == torch.uint8
+        for b, m in enumerate(lengths):
+            new = [co.stored(_np(t)[b, :, :m].transpose(1, 0, 2)) for t in (k, v)]
+            K[b], V[b] = np.concatenate([K[b], new[0]]), np.concatenate([V[b], new[1]])
+            n = len(K[b])
+            assert n == states[b].seq_len
+            p, size = co.softmax_rows(_np(q)[b], K[b], m, D ** -0.5)
+            ref = np.einsum("htn,nhd->htd", p, V[b])
+            bound = co.output_bound(ref, HALF_STEP[dtype], D, size, n, np.abs(V[b]).max())
+            if T > 1 and dtype != torch.float32:  # weights rounded to the operand type, as in test_prefill
+                bound = bound + HALF_STEP[dtype] * np.abs(ref).max()
+            assert (np.abs(_np(out)[b, :, :m] - ref[:, :m]) <= bound[:, :m]).all()
+            W[b] = np.concatenate([W[b], np.zeros((H, n - W[b].shape[1]))], 1) + p[:, :m].sum(1)
+            err[b] += m * co.weight_error(D, size, n) + 2.0 ** -20
+            mine = co.rows_of(_np(pool.key_weights)[..., None], states[b].block_ids, n)[..., 0].T
+            assert (np.abs(mine - W[b]) <= err[b] * np.maximum(W[b], 2.0 ** -10)).all()
+
+    step([37, 5, 22], 37)
+    plan = None
+    for i in range(4):
+        if i % 2 == 0:
+            step([1] * B, 1)
+        else:
+            grown = [s.seq_len for s in states]
+            plan = b2pa.DecodeStep([states], plan)
+            with plan:
+                q, k, v = (torch.from_numpy(rng.standard_normal((B, H, 1, D))).to(dtype).to(dev) for _ in range(3))
+                cache = b2pa.BatchedPagedKVCache(states, pool)
+                cache.append_batch(k, v, 1)
+                out = b2pa.paged_attention("b200_paged", q, cache, 1)
+            plan = plan.meta
+            for b in range(B):
+                K[b], V[b] = (np.concatenate([x[b], co.stored(_np(t)[b].transpose(1, 0, 2))]) for x, t in ((K, k), (V, v)))
+                assert len(K[b]) == grown[b] + 1 == states[b].seq_len
+                p, size = co.softmax_rows(_np(q)[b], K[b], 1, D ** -0.5)
+                ref = np.einsum("htn,nhd->htd", p, V[b])
+                assert (np.abs(_np(out)[b] - ref) <= co.output_bound(ref, HALF_STEP[dtype], D, size, len(K[b]),
+                                                                     np.abs(V[b]).max())).all()
+                W[b] = np.concatenate([W[b], np.zeros((H, 1))], 1) + p.sum(1)
+                err[b] += co.weight_error(D, size, len(K[b])) + 2.0 ** -20
+    kept = b2pa.BatchedPagedKVCache(states, pool).evict(16, recent=5).cpu().numpy()
+    for b in range(B):
+        n = min(16, len(K[b]))
+        sel = kept[b][:, :n]
+        assert (np.diff(sel) > 0).all() and states[b].seq_len == n
+        # the best by the sums, within their error
+        for h in range(H):
+            gone = np.setdiff1d(np.arange(len(K[b])), sel[h])
+            old = sel[h][sel[h] < len(K[b]) - 5]
+            if len(gone) and len(old):
+                assert W[b][h, gone].max() <= W[b][h, old].min() * (1 + 4 * err[b]) + 2.0 ** -10 * err[b]
+        K[b], V[b] = (np.stack([x[sel[h], h] for h in range(H)], 1) for x in (K[b], V[b]))
+        W[b] = np.stack([W[b][h, sel[h]] for h in range(H)])
+    step([3, 9, 1], 9)
+    step([1] * B, 1)
     assert b2pa.read_status(dev) == 0
 
 
