@@ -620,6 +620,22 @@ def test_run_on_4_bit_pools_of_every_type(cuda_device, dtype, D, bs):
     assert b2pa.read_status(dev) == 0
 
 
+@pytest.mark.parametrize("kv4", [False, True], ids=["plain", "kv4"])
+def test_device_lengths_of_any_shape(cuda_device, kv4):
+    """One request's length as a scalar, and a column of lengths as [B, 1]."""
+    dev, H, D, B = cuda_device, 2, 64, 2
+    x = torch.randn(B, H, 7, D, generator=torch.Generator().manual_seed(1)).to(dev)
+    pool = (b2pa.Kv4BlockPool if kv4 else b2pa.LayerBlockPool)(16, 8, 2.0)
+    states = [b2pa.PagedKVCacheState(pool) for _ in range(B)]
+    both = b2pa.BatchedPagedKVCache(states, pool)
+    both.append_batch(x, x, [7, 4])
+    want = b2pa.paged_attention("b200_paged", x, both, [7, 4])
+    lens = torch.tensor([[7], [4]], device=dev)
+    assert torch.equal(b2pa.paged_attention("b200_paged", x, both, lens), want)
+    one = b2pa.BatchedPagedKVCache(states[:1], pool)
+    assert torch.equal(b2pa.paged_attention("b200_paged", x[:1], one, lens[0, 0]), want[:1])
+
+
 def _model(dev, kv4):
     made = []
 
