@@ -10,11 +10,12 @@
 // that kernel runs on it; rows past a sequence's length are written as zeros.
 // The workspace is thus a 16-bit copy of the call's pages, by the width of the
 // table: 3.6 times the 4-bit pages' bytes, for one layer at a time.
-// One kind of input is not for that kernel: NaN groups of V at keys that only
-// some of the chunk's queries see (a zero weight times NaN).  They leave the
-// call's number in a flag, and the kernel of kv4_prefill_mma.cu, launched behind
-// it, redoes the call if it finds it there.  The number is part of a captured
-// graph: once a replay has set it, later ones redo the call too.
+// Two kinds of inputs are not for that kernel: NaN groups of V at keys that only
+// some of the chunk's queries see (a zero weight times NaN), and scores whose own
+// rounding shows (past 2^24).  They leave the call's number in a flag, and the kernel of
+// kv4_prefill_mma.cu, launched behind it, redoes the call if it finds it there.
+// The number is part of a captured graph: once a replay has set it, later ones
+// redo the call too.
 #include <atomic>
 
 #include "common.cuh"
@@ -119,8 +120,8 @@ int launch_kv4_prefill(const AttnArgs& a, const Kv4PrefillPlan& pl, cudaStream_t
   int rc;
   switch (a.dtype) {
     case B2PA_DTYPE_F32: rc = launch_paged_prefill_f32_on_halves(in, flag, epoch, s); break;
-    case B2PA_DTYPE_BF16: rc = launch_paged_prefill_bf16(in, s); break;
-    default: rc = launch_paged_prefill_f16(in, s); break;
+    case B2PA_DTYPE_BF16: rc = launch_paged_prefill_bf16(in, s, flag, epoch); break;
+    default: rc = launch_paged_prefill_f16(in, s, flag, epoch); break;
   }
   if (rc != B2PA_OK) return rc;
   return launch_kv4_prefill_mma(a, flag, epoch, s);

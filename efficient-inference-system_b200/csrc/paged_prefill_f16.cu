@@ -4,10 +4,10 @@
 #include "paged_prefill_tc.cuh"
 
 namespace b2pa {
-int launch_paged_prefill_f16(const AttnArgs& a, cudaStream_t s) {
+int launch_paged_prefill_f16(const AttnArgs& a, cudaStream_t s, uint32_t* far_flag, uint32_t epoch) {
   if (prefill_uses_tensor_cores(a.D, a.block_size, a.dtype, a.num_blocks * a.H * a.block_size)) {
 #define B2PA_TC_CASE(DD, BB) \
-    if (a.D == DD && a.block_size == BB) return launch_prefill_tc<__half, DD, BB>(a, s);
+    if (a.D == DD && a.block_size == BB) return launch_prefill_tc<__half, DD, BB>(a, s, epoch, far_flag);
     B2PA_TC_CASE(64, 8) B2PA_TC_CASE(64, 16) B2PA_TC_CASE(64, 32)
     B2PA_TC_CASE(128, 8) B2PA_TC_CASE(128, 16) B2PA_TC_CASE(128, 32)
 #undef B2PA_TC_CASE

@@ -76,6 +76,10 @@ struct PfTcParams {
   // and the fp32 CUDA-core kernel launched after it recomputes the call.
   // Marking with the call's number needs no reset between calls.
   uint32_t* range_flag;
+  // May be null.  Set to `epoch` when scores are so far from zero that their own
+  // rounding shows (2^24 in base-2 units): a kernel behind this one redoes the
+  // call.
+  uint32_t* far_flag;
   uint32_t epoch;
   // 1: the kernel before this one is b2pa's append kernel (see
   // AttnArgs::after_append): only the K/V producers wait for it, before
@@ -127,7 +131,8 @@ __device__ __forceinline__ void prefill_tile_range(const PfTcParams& p, int b, i
 // softmax's scale: an unscaled lo half is a subnormal for |x| < 2^-3, off by
 // up to 2^-25, which keys of up to 64,512 multiply (1,000 unit normal keys
 // times 2^12, queries times 2^-12: 7e-5 of the output -> 5e-8).  So no query is
-// out of range, and one that is not finite spoils its own row alone, as it should.
+// out of range, and one that is not finite spoils its own row alone, as it
+// should.
 template <int D, int BS, bool SPLIT = false, bool HALVES = false>
 struct PfTcCfg {
   static constexpr int BM = 128;         // query rows per CTA (UMMA M)
@@ -748,6 +753,10 @@ __global__ void __launch_bounds__(PfTcCfg<D, BS, kPfSplit<T>, HALVES>::THREADS, 
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[slot]);
     }
+    // Far scores: the fma's product is not rounded as the reference was, and the
+    // difference, half a unit of its last place, is a factor of every weight.
+    constexpr float kFar = 0x1p24f;
+    if (p.far_flag != nullptr && fabsf(m) >= kFar && fabsf(m) < INFINITY) *p.far_flag = p.epoch;
     // ---------------------------------------------------------- epilogue
     // Merge the groups' (m, l, O) for this row: weights 2^(m_g - M).  Group g
     // writes columns [g*D/NG, (g+1)*D/NG) of the row.
@@ -996,9 +1005,9 @@ bool encode_pool_tensor_map(CUtensorMap* map, const void* pool, int64_t rows, in
 bool encode_q_tensor_map(CUtensorMap* map, const void* q, int B, int H, int T, int D, const int64_t sq[3], int dtype,
                          int dim_of[3]);
 
-// epoch: the fp32 variant's number of this call (marks the range flag).
-// HALVES: a's pools are fp16, with the 16-bit types' plan, and the flag is the
-// caller's.
+// epoch: the number of this call (marks the flags; plain 16-bit pools have none).
+// flag: PfTcParams::far_flag.  HALVES: a's pools are fp16, with the 16-bit types'
+// plan, and the caller's flag is the range flag too.
 template <typename T, int D, int BS, bool HALVES = false>
 int launch_prefill_tc(const AttnArgs& a, cudaStream_t stream, uint32_t epoch = 0, uint32_t* flag = nullptr) {
   constexpr bool SPLIT = kPfSplit<T>;
@@ -1090,6 +1099,7 @@ int launch_prefill_tc(const AttnArgs& a, cudaStream_t stream, uint32_t epoch = 0
   p.part_o = nullptr;
   p.part_ml = nullptr;
   p.range_flag = range_flag;
+  p.far_flag = flag;
   p.epoch = epoch;
   p.early = (!SPLIT && a.after_append) ? 1 : 0;
   if (plan.nsplit_max > 1) {
