@@ -158,7 +158,7 @@ bool prefill_uses_tensor_cores(int D, int block_size, int dtype, int64_t pool_ro
 
 int launch_paged_prefill_f32(const AttnArgs& a, cudaStream_t s);
 // fp32 q with head_dim 64 or 128 on fp16 pages (make_prefill_plan for fp16).
-// Scores past 2^24 leave `epoch` in *flag, and so may a kernel before it; the
+// Scores past 2^18 leave `epoch` in *flag, and so may a kernel before it; the
 // result is then the caller's next kernel's to make.
 int launch_paged_prefill_f32_on_halves(const AttnArgs& a, uint32_t* flag, uint32_t epoch, cudaStream_t s);
 // far_flag (may be null): scores past 2^24 leave `epoch` there, and the result is

@@ -12,7 +12,7 @@
 // table: 3.6 times the 4-bit pages' bytes, for one layer at a time.
 // Two kinds of inputs are not for that kernel: NaN groups of V at keys that only
 // some of the chunk's queries see (a zero weight times NaN), and scores whose own
-// rounding shows (past 2^24).  They leave the call's number in a flag, and the kernel of
+// rounding shows (past 2^24, for fp32 2^18).  They leave the call's number in a flag, and the kernel of
 // kv4_prefill_mma.cu, launched behind it, redoes the call if it finds it there.
 // The number is part of a captured graph: once a replay has set it, later ones
 // redo the call too.

@@ -58,6 +58,12 @@ __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[VL]) 
     w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
 }
 
+// What the weights of a row are taken relative to: 15 below its maximum, so that
+// they go up to 2^15 (the division by their sum takes that out again) and one of
+// 2^-29 of the largest is still a normal fp16 number.  A far maximum, whose own
+// rounding would carry the largest past fp16's range, is taken as it is.
+__device__ __forceinline__ float reference(float m) { return fabsf(m) < 0x1p20f ? m - 15.f : m; }
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 2)
     kv4_prefill_kernel(AttnArgs a, float qscale, const uint32_t* flag, uint32_t epoch) {
@@ -243,7 +249,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       top[r] = fmaxf(top[r], __shfl_xor_sync(kFullMask, top[r], 1));
       top[r] = fmaxf(top[r], __shfl_xor_sync(kFullMask, top[r], 2));
       const float up = fmaxf(m[r], top[r]);
-      f[r] = m[r] == up ? 1.f : fast_exp2(m[r] - up);
+      f[r] = m[r] == up ? 1.f : fast_exp2(reference(m[r]) - reference(up));
       move = move || m[r] != up;
       m[r] = up;
       l[r] *= f[r];
@@ -257,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         o[n][3] *= f[1];
       }
     }
-    const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+    const float ref[2] = {m[0] == -INFINITY ? 0.f : reference(m[0]), m[1] == -INFINITY ? 0.f : reference(m[1])};
     // ---- O += P . V, 16 keys at a time
 #pragma unroll
     for (int ks = 0; ks < KT / 16; ++ks) {
@@ -330,7 +336,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       for (int n = 0; n < NC; n += 4)
         *reinterpret_cast<float4*>(mine + row * D + (2 * t + e) * NC + n) =
             make_float4(o[n][2 * r + e], o[n + 1][2 * r + e], o[n + 2][2 * r + e], o[n + 3][2 * r + e]);
-    if (t == 0) row_ml[row] = make_float2(m[r], l[r]);
+    if (t == 0) row_ml[row] = make_float2(reference(m[r]), l[r]);
   }
   cluster.sync();
   const int share = kRows / ns;

@@ -77,8 +77,8 @@ struct PfTcParams {
   // Marking with the call's number needs no reset between calls.
   uint32_t* range_flag;
   // May be null.  Set to `epoch` when scores are so far from zero that their own
-  // rounding shows (2^24 in base-2 units): a kernel behind this one redoes the
-  // call.
+  // rounding shows (2^24 in base-2 units; 2^18 with HALVES, whose weights use all
+  // of fp16's range): a kernel behind this one redoes the call.
   uint32_t* far_flag;
   uint32_t epoch;
   // 1: the kernel before this one is b2pa's append kernel (see
@@ -627,7 +627,12 @@ __global__ void __launch_bounds__(PfTcCfg<D, BS, kPfSplit<T>, HALVES>::THREADS, 
     // previous P.V itself), and P.V(j) cannot start before this warp releases
     // P(j), so o_full[g] has completed i-1 or i phases and the parity wait
     // is exact.
-    constexpr float kRescale = 8.f;
+    // HALVES: the reference is set kShift below the maximum, so weights go up to
+    // 2^kRescale, just below fp16's largest number (the division by their sum
+    // takes the factor out again).  With weights up to 1, a low half that is a
+    // subnormal leaves 2^-25 of the largest: over 1 % of the output where one key
+    // without a value draws e^14 times the others' weight (so: 3e-6).
+    constexpr float kShift = HALVES ? 13.f : 0.f, kRescale = HALVES ? 15.9f : 8.f;
     // Row maxima are taken on unscaled scores and scaled once (sc > 0); a
     // scale that is not positive is applied to the scores first instead.
     const bool pre_scale = !(p.scale_log2 > 0.f);
@@ -692,7 +697,7 @@ __global__ void __launch_bounds__(PfTcCfg<D, BS, kPfSplit<T>, HALVES>::THREADS, 
         break;
       }
       const bool need = mt > m + kRescale;
-      const float m_new = need ? mt : m;
+      const float m_new = need ? mt - kShift : m;
       const bool scale_o = need && m != -INFINITY;
       const float alpha = scale_o ? fast_exp2(m - m_new) : 1.f;
       m = m_new;
@@ -755,7 +760,7 @@ __global__ void __launch_bounds__(PfTcCfg<D, BS, kPfSplit<T>, HALVES>::THREADS, 
     }
     // Far scores: the fma's product is not rounded as the reference was, and the
     // difference, half a unit of its last place, is a factor of every weight.
-    constexpr float kFar = 0x1p24f;
+    constexpr float kFar = HALVES ? 0x1p18f : 0x1p24f;
     if (p.far_flag != nullptr && fabsf(m) >= kFar && fabsf(m) < INFINITY) *p.far_flag = p.epoch;
     // ---------------------------------------------------------- epilogue
     // Merge the groups' (m, l, O) for this row: weights 2^(m_g - M).  Group g

@@ -291,6 +291,45 @@ def test_fp32_precision_of_unlike_magnitudes(cuda_device, D, T, p, lost):
     assert torch.isnan(out[:, :, live:]).all()
 
 
+@pytest.mark.parametrize("dtype,D,most", [(torch.float32, 64, 2.0 ** -17), (torch.float32, 128, 2.0 ** -17),
+                                          (torch.float32, 256, 2.0 ** -17), (torch.bfloat16, 64, 2.0 ** -7),
+                                          (torch.bfloat16, 128, 2.0 ** -7), (torch.bfloat16, 256, 2.0 ** -8),
+                                          (torch.float16, 256, 2.0 ** -10)])
+@pytest.mark.parametrize("T", [1, 60])
+@pytest.mark.parametrize("at", [0, 700])
+def test_one_key_draws_nearly_all(cuda_device, dtype, D, most, T, at):
+    """One key with a logit 10 to 14 above the others' and a value of zero, so that the output is made of weights of
+    about 2^-20 of the largest; the output as a whole.
+
+    fp32: those weights are split with a rounding of 2^-38 of the largest, 2^-18.6 of themselves in the mean square; the
+    far logit's own roundings (14 log2 e in fp32, and the scale's) are 2^-19.3 of every weight, the others' logits 2^-20,
+    the exponential 2^-22, and the sums over 1,000 keys 2^-19 as in test_fp32_precision: 2^-17.1 together.  16-bit
+    outputs round to half a step, and the prefill weights before that: to the operand type (head_dim 64 and 128), or to
+    11 bits."""
+    rng = np.random.default_rng(D)
+    H, bs, n = 2, 16, 1000
+    NB = -(-n // bs)
+    k, v = rng.standard_normal((NB, H, bs, D)) / 4, rng.standard_normal((NB, H, bs, D))
+    q = rng.standard_normal((1, H, T, D))
+    k[..., :16] = 0                      # a group of its own, with the far key's 2^a in channel 0
+    q[..., :16] = 0
+    a = 4
+    k[at // bs, :, at % bs] = 0
+    k[at // bs, :, at % bs, 0] = 7 * 2.0 ** a   # code 7 of scale 2^a: exact
+    q[..., 0] = 2.0 ** round(np.log2(12 * D ** 0.5 / (7 * 2.0 ** a)))
+    far = 7 * 2.0 ** a * q[0, 0, 0, 0] * D ** -0.5
+    assert 9 < far < 16
+    v[at // bs, :, at % bs] = 0
+    q = torch.from_numpy(q).to(dtype).to(cuda_device)
+    fn = b2pa.paged_attention_decode_kv4 if T == 1 else b2pa.paged_attention_prefill_kv4
+    out = fn(q, torch.from_numpy(co.pack_pages(k, False)).to(cuda_device),
+             torch.from_numpy(co.pack_pages(v, True)).to(cuda_device), _i32(np.arange(NB)[None], cuda_device),
+             _i32([n], cuda_device), _i32([T], cuda_device))
+    p, _ = co.softmax_rows(_np(q)[0], co.rows_of(co.stored(k), range(NB), n), T, D ** -0.5)
+    ref = np.einsum("htn,nhd->htd", p, co.rows_of(co.stored(v), range(NB), n))
+    assert np.linalg.norm(_np(out)[0] - ref) <= most * np.linalg.norm(ref)
+
+
 @pytest.mark.parametrize("dtype,D", [(torch.float32, 64), (torch.float32, 128), (torch.bfloat16, 256),
                                      (torch.float16, 128)])
 def test_prefill_long(cuda_device, dtype, D):
