@@ -238,7 +238,7 @@ PrefillPlan make_prefill_plan_f32_tiled(int B, int H, int T, int D, int max_page
   return pl;
 }
 
-PrefillPlan make_prefill_plan(int B, int H, int T, int D, int max_pages, int block_size, int dtype) {
+PrefillPlan make_prefill_plan(int B, int H, int T, int D, int max_pages, int block_size, int dtype, int kt_cap) {
   const int64_t ktmax = ((int64_t)max_pages * block_size + 63) / 64;
   PrefillPlan pl = empty_prefill_plan(ktmax);
   if (dtype == B2PA_DTYPE_F32 && B > 0 && T > 0 &&
@@ -247,7 +247,7 @@ PrefillPlan make_prefill_plan(int B, int H, int T, int D, int max_pages, int blo
     // pages (B * max_pages slots of H pages, K and V, 2 * D halves per row),
     // after the partials of its key-range split; then the range flag.
     pl.split_tc = 1;
-    const size_t part = tc_key_split(pl, B, H, T, D, ktmax, 148, 1024);
+    const size_t part = tc_key_split(pl, B, H, T, D, ktmax, 148, kt_cap);
     const size_t slot_bytes = (size_t)H * block_size * 2 * D * 2;
     const size_t nslots = (size_t)B * max_pages;
     pl.off_split_k = align_up(part, 256);
@@ -260,7 +260,7 @@ PrefillPlan make_prefill_plan(int B, int H, int T, int D, int max_pages, int blo
   if (dtype == B2PA_DTYPE_F32 && (D == 64 || D == 128))
     return make_prefill_plan_f32_tiled(B, H, T, D, max_pages, block_size);
   if (!prefill_uses_tensor_cores(D, block_size, dtype, 0)) return pl;
-  pl.bytes = tc_key_split(pl, B, H, T, D, ktmax, 148, 1024);
+  pl.bytes = tc_key_split(pl, B, H, T, D, ktmax, 148, kt_cap);
   return pl;
 }
 

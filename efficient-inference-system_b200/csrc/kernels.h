@@ -151,13 +151,15 @@ struct PrefillPlan {
   // split_tc: split pages, slot table and the out-of-range flag
   size_t off_part_ml, off_part_o, off_split_k, off_split_v, off_slots, off_flag, bytes;
 };
-PrefillPlan make_prefill_plan(int B, int H, int T, int D, int max_pages, int block_size, int dtype);
+// kt_cap: key tiles of one CTA at most, whose block ids it keeps in shared memory.
+PrefillPlan make_prefill_plan(int B, int H, int T, int D, int max_pages, int block_size, int dtype, int kt_cap = 1024);
+constexpr int kHalvesKtCap = 960;  // of launch_paged_prefill_f32_on_halves, whose tiles leave less room
 // The fp32 register-tiled kernel's plan (its workspace offsets from 0).
 PrefillPlan make_prefill_plan_f32_tiled(int B, int H, int T, int D, int max_pages, int block_size);
 bool prefill_uses_tensor_cores(int D, int block_size, int dtype, int64_t pool_rows);
 
 int launch_paged_prefill_f32(const AttnArgs& a, cudaStream_t s);
-// fp32 q with head_dim 64 or 128 on fp16 pages (make_prefill_plan for fp16).
+// fp32 q with head_dim 64 or 128 on fp16 pages (make_prefill_plan for fp16, kHalvesKtCap).
 // Scores past 2^18 leave `epoch` in *flag, and so may a kernel before it; the
 // result is then the caller's next kernel's to make.
 int launch_paged_prefill_f32_on_halves(const AttnArgs& a, uint32_t* flag, uint32_t epoch, cudaStream_t s);

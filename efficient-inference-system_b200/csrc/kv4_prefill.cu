@@ -83,7 +83,8 @@ Kv4PrefillPlan make_kv4_prefill_plan(int B, int H, int T, int D, int max_pages, 
   const int type = dtype == B2PA_DTYPE_F32 ? (int)B2PA_DTYPE_F16 : dtype;  // of the unpacked pages
   if (!takes_unpacked(B, H, D, max_pages, block_size, type)) return pl;
   pl.unpack = 1;
-  pl.inner_bytes = make_prefill_plan(B, H, T, D, max_pages, block_size, type).bytes;
+  pl.inner_bytes = dtype == B2PA_DTYPE_F32 ? make_prefill_plan(B, H, T, D, max_pages, block_size, type, kHalvesKtCap).bytes
+                                           : make_prefill_plan(B, H, T, D, max_pages, block_size, type).bytes;
   const size_t pool = up256((size_t)B * max_pages * H * block_size * D * 2);
   pl.off_v = pool;
   pl.off_table = 2 * pool;

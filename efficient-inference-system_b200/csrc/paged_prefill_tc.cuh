@@ -1017,8 +1017,9 @@ template <typename T, int D, int BS, bool HALVES = false>
 int launch_prefill_tc(const AttnArgs& a, cudaStream_t stream, uint32_t epoch = 0, uint32_t* flag = nullptr) {
   constexpr bool SPLIT = kPfSplit<T>;
   using C = PfTcCfg<D, BS, SPLIT, HALVES>;
-  const PrefillPlan plan =
-      make_prefill_plan(a.B, a.H, a.T, a.D, a.max_pages, BS, HALVES ? (int)B2PA_DTYPE_F16 : a.dtype);
+  const PrefillPlan plan = HALVES ? make_prefill_plan(a.B, a.H, a.T, a.D, a.max_pages, BS, B2PA_DTYPE_F16, kHalvesKtCap)
+                                  : make_prefill_plan(a.B, a.H, a.T, a.D, a.max_pages, BS, a.dtype);
+  static_assert(!HALVES || C::SMEM_FIXED + 4 * kHalvesKtCap * C::PAGES + 1024 <= 227 * 1024, "block ids of a CTA");
   if (plan.bytes > 0 && (!a.workspace || a.workspace_bytes < plan.bytes))
     return set_error(B2PA_ERR_WORKSPACE, "paged_prefill: workspace of %zu bytes, %zu needed", a.workspace_bytes,
                      plan.bytes);

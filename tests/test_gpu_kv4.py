@@ -593,6 +593,14 @@ def test_prefill(cuda_device, dtype, D, bs, H):
     assert b2pa.read_status(cuda_device) == 0
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_prefill_on_a_wide_table(cuda_device, dtype):
+    """Tables for 65,000 tokens in pages of 8, with CTAs enough that none shares its keys."""
+    out, ref, bound, _ = _attend_case(cuda_device, lens=[90], cur=[3], H=160, D=64, bs=8, dtype=dtype, T=3, seed=2,
+                                      width=8120)
+    _check(out, ref, bound + (0 if dtype == torch.float32 else HALF_STEP[dtype] * np.abs(ref).max()))
+
+
 def test_streams_layouts_and_capture(cuda_device):
     """Strided q, a wide table, a non-current stream, and two graphs replayed after the inputs changed."""
     args = dict(lens=[50, 333], cur=[1, 1], H=4, D=128, bs=16, dtype=torch.bfloat16, T=1)
