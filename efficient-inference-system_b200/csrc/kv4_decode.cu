@@ -570,12 +570,13 @@ static int decode_launch(const AttnArgs& a, int ns, cudaStream_t s) {
 template <typename T, int D>
 static int decode_blocks(const AttnArgs& a, cudaStream_t s) {
   // CTAs per sequence and head: one wave of the two CTAs an SM holds, while
-  // every warp keeps a step of the longest sequence.  A CTA costs about 4 us
+  // every warp keeps a step of the longest sequence that the table has room for
+  // (the host does not know the lengths).  A CTA costs about 4 us
   // beside its keys (loads that depend on one another, the merge), so more
   // waves of smaller shares are slower: 64 sequences of 128-1,024 tokens and 8
-  // heads of 64 (fp32) take 16.9 us with 1 CTA each, 23.9 with 2 (in order); 64 of
-  // 1,024-8,192 and 32 heads of 128 (bf16) 288 and 310; one sequence of 8,001
-  // tokens and 32 heads of 128 44.6 us with 1, 24.5 with 2, 17.7 with 4, 13.1
+  // heads of 64 (fp32) take 16.8 us with 1 CTA each, 24.8 with 2; 64 of
+  // 1,024-8,192 and 32 heads of 128 (bf16) 273 and 312; one sequence of 8,001
+  // tokens and 32 heads of 128 46.0 us with 1, 25.9 with 2, 18.7 with 4, 14.3
   // with 8.  head_dim 256 takes half as many warps a CTA (registers).
   constexpr int W = D == 256 ? 4 : 8;
   const int64_t pairs = (int64_t)a.B * a.H;

@@ -192,7 +192,7 @@ struct KeyQuery {
   // numbers c.  The former costs a few 2^-20 of a logit: the sums are larger
   // than the result, and the product aligns subnormal operands by an exponent
   // up to 10 too large.  (Key weights of a 16-bit q, in fp32: 5e-7 off with the
-  // former and 3e-7 with the latter, which takes 152 us where it takes 132.)
+  // former and 3e-7 with the latter, which took 152 us where it took 132.)
   static constexpr bool SIGNED = std::is_same<T, float>::value;
   uint4 raw[C::KW][sizeof(T) / 2];  // the channels of this lane's column, 8 per word
   uint32_t qh[C::KW][4], ql[QLO ? C::KW : 1][4];

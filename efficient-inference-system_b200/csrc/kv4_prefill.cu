@@ -71,9 +71,9 @@ __global__ void __launch_bounds__(256) kv4_unpack_kernel(AttnArgs a, T* k_out, T
 static size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
 // Whether the tcgen05 kernel takes the shape.  Unpacking and that kernel -> straight
-// from the pages (us; 2 sequences, 32 heads, 1,021 queries on 1,024 to 7,168
-// keys): fp32 head_dim 64 271 -> 918, 128 417 -> 1,406; bf16 64 205 -> 753, 128
-// 305 -> 1,107; head_dim 256 only straight, 2,507 and 1,745.
+// from the pages (us; 2 sequences, 32 heads, 1,021 queries behind prefixes of 1,024
+// and 7,168): fp32 head_dim 64 265 -> 974, 128 409 -> 1,344; bf16 64 196 -> 791, 128
+// 293 -> 1,088; head_dim 256 only straight, 2,390 and 1,676.
 static bool takes_unpacked(int B, int H, int D, int max_pages, int block_size, int type) {
   return max_pages > 0 && prefill_uses_tensor_cores(D, block_size, type, (int64_t)B * max_pages * H * block_size);
 }

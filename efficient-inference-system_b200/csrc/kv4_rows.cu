@@ -7,12 +7,13 @@
 // The bytes they move (D * element size in and 9/16 D out a row, or the
 // reverse) bound them from below: for 6,260 rows of 32 heads of 128 in bf16, in
 // 8 x 1,531 slots whose others are read back as zeros, 20 and 36 us at copy
-// bandwidth; they take about 30 and 37.  The append spends instructions, some
-// 65 a word of 8 codes.  There a thread takes whole groups (16
-// channels) of K and of V, so a group's scale and reciprocal are worked out once; the
-// group's maximum is taken on the bits of |x| (pairs of 16-bit values at a
-// time), so a NaN or an infinity wins it.  Prompts: a CTA takes two neighbouring
-// tokens, all of whose loads are under way at once.
+// bandwidth; they take 26 and 42 (fp32 append: 60 for 36, with 17 divisions a
+// group).  The append spends instructions, some 65 a word of 8 codes.  There a
+// thread takes whole groups (16 channels) of K and of V, so a group's scale and
+// reciprocal are worked out once; the group's maximum is taken on the bits of
+// |x| (pairs of 16-bit values at a time), so a NaN or an infinity wins it.
+// Prompts: a CTA takes two neighbouring tokens, all of whose loads are under way
+// at once.
 #include "common.cuh"
 #include "kernels.h"
 #include "kv4.cuh"
@@ -157,7 +158,7 @@ __global__ void __launch_bounds__(128) kv4_read_kernel(Kv4ReadArgs a) {
   const Places<TOKENS> at(a.page_table + (int64_t)b * a.pt_stride, a.start_pos[b], t0, len, a.bs_log2, a.max_pages,
                           a.num_blocks, a.status);
   // a thread reads one word of K and of V per token, so that a warp's stores
-  // are contiguous (whole groups per thread: 61 us where this takes 40)
+  // are contiguous (whole groups per thread: 61 us where this took 40)
   const int wpr_log2 = 31 - __clz(a.D / 8);
   const int page_bytes = kv4_page_bytes(a.block_size, a.D);
   const int codes = a.block_size * (a.D / 2);
