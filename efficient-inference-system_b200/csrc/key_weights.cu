@@ -12,15 +12,18 @@
 // queries, so every key's sum stays in one thread and needs no atomics: results
 // do not depend on the order of anything.  The product is computed twice
 // because the alternative, keeping T x L logits, costs more bytes than the
-// product costs time.  Operands: 16-bit types as they are; 4-bit keys unpacked
-// (exactly) to fp16; fp32 as two fp16 halves each (22 bits, three products),
-// rows scaled by powers of two into fp16's range.
+// product costs time.  Both passes round a logit before they subtract from it: a
+// fused product would leave the rounded reference by up to half a unit of its
+// last place, a factor of every weight (2 % at logits of 500,000).
+// Operands: 16-bit types as they are; 4-bit keys unpacked (exactly) to fp16;
+// fp32 as two fp16 halves each (22 bits, three products), rows scaled by powers
+// of two into fp16's range.
 //   head_dim 64 and 128: key_weights_tc.cu (tcgen05).
 //   head_dim 16, 32 and 256: key_weights_tile_kernel here (mma.sync), whose key
 //   rows go from global memory to registers -- each is used by one warp only --
 //   with 64 queries in shared memory as columns; the first launch keeps, per
 //   lane and column, a maximum and a sum over the rows that the lane sees.
-//   Bound by instruction issue, about four instructions a logit.
+//   Bound by instruction issue, about five instructions a logit.
 //
 // One query (key_weights_step_kernel): bound by reading K once.
 // A cluster of CTAs shares a sequence, each keeps its logits in shared
@@ -306,17 +309,24 @@ __global__ void __launch_bounds__(kTileThreads, Shape<T, KV4, D>::KPARTS == 2 &&
 #pragma unroll
             for (int x = 0; x < S::MT; ++x)
 #pragma unroll
-              for (int i = 0; i < 2; ++i) z[e][x][i] = fmaf(acc[x][2 * i + e], unit_of(n * 8 + 2 * t + e, x, i), -m[n][e]);
+              for (int i = 0; i < 2; ++i) z[e][x][i] = __fsub_rn(acc[x][2 * i + e] * unit_of(n * 8 + 2 * t + e, x, i), m[n][e]);
             top[e] = highest(z[e]);
           }
           if (__any_sync(kFullMask, fmaxf(top[0], top[1]) > 8.f)) {
 #pragma unroll
             for (int e = 0; e < 2; ++e)
               if (top[e] > 8.f) {
-                l[n][e] *= fast_exp2(-top[e]);
-                m[n][e] += top[e];
+                const int col = n * 8 + 2 * t + e;
+                float up = -INFINITY;  // (the logit itself: a reference plus a difference would be rounded)
 #pragma unroll
-                for (int x = 0; x < S::MT; ++x) z[e][x][0] -= top[e], z[e][x][1] -= top[e];
+                for (int x = 0; x < S::MT; ++x)
+                  up = fmaxf(up, fmaxf(acc[x][e] * unit_of(col, x, 0), acc[x][2 + e] * unit_of(col, x, 1)));
+                l[n][e] *= fast_exp2(m[n][e] - up);
+                m[n][e] = up;
+#pragma unroll
+                for (int x = 0; x < S::MT; ++x)
+#pragma unroll
+                  for (int i = 0; i < 2; ++i) z[e][x][i] = __fsub_rn(acc[x][2 * i + e] * unit_of(col, x, i), up);
               }
           }
 #pragma unroll
@@ -445,7 +455,8 @@ __global__ void __launch_bounds__(kTileThreads, Shape<T, KV4, D>::KPARTS == 2 &&
               for (int i = 0; i < 2; ++i) {
                 float u0 = unit.x, u1 = unit.y;
                 if constexpr (S::KPARTS == 2) u0 *= keys.back[x][i], u1 *= keys.back[x][i];
-                float p0 = fast_exp2(fmaf(acc[x][2 * i], u0, -lse.x)), p1 = fast_exp2(fmaf(acc[x][2 * i + 1], u1, -lse.y));
+                float p0 = fast_exp2(__fsub_rn(acc[x][2 * i] * u0, lse.x));
+                float p1 = fast_exp2(__fsub_rn(acc[x][2 * i + 1] * u1, lse.y));
                 if constexpr (decltype(masked)::value) {
                   const int64_t r = base + 16 * x + 8 * i + g;
                   if (r > col || col >= left) p0 = 0.f;

@@ -4,7 +4,7 @@
 // Two launches over one product, as in key_weights.cu, but on the 5th
 // generation tensor cores: tiles of 128 keys x up to 128 queries, fp32
 // accumulators in TMEM, so that the warps are left with the softmax -- about
-// five instructions a logit -- and with putting key rows in place.
+// six instructions a logit -- and with putting key rows in place.
 //   PASS 1: queries are the product's rows.  A thread owns one query, reads its
 //     logits from TMEM and keeps the running maximum and sum in two registers.
 //   PASS 2: keys are the rows.  A thread owns one key and adds
@@ -314,10 +314,12 @@ __global__ void __launch_bounds__(kTcThreads, 2) key_weights_tc_kernel(KeyWeight
               top = fmaxf(m, top * size);  // m, in logits
               const float ref = top == -INFINITY ? 0.f : top;
               const float2 u2 = make_float2(size, size), r2 = make_float2(-ref, -ref);
-              float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
+              const float2 zero = make_float2(0.f, 0.f);
+              float2 sum0 = zero, sum1 = zero;
 #pragma unroll
               for (int x = 0; x < 32; x += 4) {
-                const float2 y = fma2(make_float2(v[x], v[x + 1]), u2, r2), z = fma2(make_float2(v[x + 2], v[x + 3]), u2, r2);
+                const float2 y = add2(fma2(make_float2(v[x], v[x + 1]), u2, zero), r2),
+                             z = add2(fma2(make_float2(v[x + 2], v[x + 3]), u2, zero), r2);
                 sum0 = add2(sum0, make_float2(fast_exp2(y.x), fast_exp2(y.y)));
                 sum1 = add2(sum1, make_float2(fast_exp2(z.x), fast_exp2(z.y)));
               }
@@ -352,8 +354,9 @@ __global__ void __launch_bounds__(kTcThreads, 2) key_weights_tc_kernel(KeyWeight
               const float4 z = ls[x];
               float4 u = make_float4(qscale, qscale, qscale, qscale);
               if constexpr (S::QSCALED) u = un[x];
-              float2 p = fma2(make_float2(v[4 * x], v[4 * x + 1]), make_float2(u.x, u.y), make_float2(z.x, z.y));
-              float2 r = fma2(make_float2(v[4 * x + 2], v[4 * x + 3]), make_float2(u.z, u.w), make_float2(z.z, z.w));
+              const float2 zero = make_float2(0.f, 0.f);
+              float2 p = add2(fma2(make_float2(v[4 * x], v[4 * x + 1]), make_float2(u.x, u.y), zero), make_float2(z.x, z.y));
+              float2 r = add2(fma2(make_float2(v[4 * x + 2], v[4 * x + 3]), make_float2(u.z, u.w), zero), make_float2(z.z, z.w));
               p = make_float2(fast_exp2(p.x), fast_exp2(p.y));
               r = make_float2(fast_exp2(r.x), fast_exp2(r.y));
               if (!all) {

@@ -805,3 +805,42 @@ def test_any_scale(cuda_device, scale, T, kind, D):
     V = co.rows_of(v, range(NB), n)
     ref = np.einsum("htn,nhd->htd", p, V)
     assert (np.abs(_np(out)[0] - ref) <= co.output_bound(ref, 2.0 ** -24, D, size, n, np.abs(V).max())).all()
+
+
+@pytest.mark.parametrize("dtype,kv4,D", [
+    (torch.float32, False, 32), (torch.float32, False, 64), (torch.float32, True, 64), (torch.float32, False, 128),
+    (torch.bfloat16, False, 64), (torch.bfloat16, True, 128), (torch.float16, False, 128), (torch.float16, True, 256),
+    (torch.bfloat16, False, 256), (torch.bfloat16, False, 16)])
+@pytest.mark.parametrize("T", [1, 50])
+@pytest.mark.parametrize("far", [1e5, 5e5, 2e6, 3e7])
+def test_key_weights_of_far_logits(cuda_device, dtype, kv4, D, T, far):
+    """Logits whose own rounding is of the size of usual logits: a query whose largest is far ahead gives that key a
+    weight of one, whatever the size of the logit."""
+    dev, H, bs, n = cuda_device, 6, 16, 500
+    rng = np.random.default_rng(D)
+    NB = -(-n // bs)
+    big = 64.0 if dtype == torch.float16 and not kv4 else 4096.0
+    k = rng.standard_normal((NB, H, bs, D)) * big
+    if kv4:
+        pool, k = torch.from_numpy(co.pack_pages(k, False)).to(dev), co.stored(k)
+    else:
+        pool = torch.from_numpy(k).to(dtype).to(dev)
+        k = _np(pool)
+    far = min(far, 1e4 * big) if dtype == torch.float16 else far
+    q = torch.from_numpy(rng.standard_normal((1, H, T, D)) * far / big).to(dtype).to(dev)
+    w = torch.zeros(NB, H, bs, device=dev)
+    b2pa.accumulate_key_weights(q, pool, w, _i32(np.arange(NB)[None], dev), _i32([n], dev), _i32([T], dev))
+    K = co.rows_of(k, range(NB), n)
+    z = np.einsum("htd,nhd->htn", _np(q)[0], K) * D ** -0.5
+    z = np.where(np.arange(n) < n - T + 1 + np.arange(T)[:, None], z, -np.inf)
+    first, second = np.sort(z, -1)[..., -1], np.sort(z, -1)[..., -2]
+    clear = first - second > 40 + 2.0 ** -16 * np.abs(_np(q)[0]).max() * np.abs(K).max() * D ** 0.5
+    assert clear.mean() > 0.6
+    got = co.rows_of(_np(w)[..., None], range(NB), n)[..., 0].T          # [H, n]
+    least = np.zeros((H, n))
+    for h in range(H):
+        np.add.at(least[h], z[h].argmax(-1)[clear[h]], 1.0)
+    unclear = (~clear).sum(1)[:, None]
+    # a weight is 2^0 over a sum of it alone: exact but for the exponential's 2^-22 and a rounding per addend
+    assert (got >= least * (1 - (T + 4) * 2.0 ** -22)).all()
+    assert (got <= least + unclear + (T + 4) * 2.0 ** -22 * (least + 1)).all()
