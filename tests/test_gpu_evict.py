@@ -11,7 +11,8 @@ import b2pa
 from oracle import model as om
 from tests import _compress_oracle as co
 from tests._helpers import random_tables
-from tests.test_gpu_kv4 import DTYPES, HALF_STEP, _i32, _np, _rows, _table
+from tests.test_gpu_kv4 import DTYPES, _i32, _np, _rows, _table
+from tests.test_gpu_kv4 import HALF_STEP
 
 pytestmark = pytest.mark.gpu
 
